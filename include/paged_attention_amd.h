@@ -38,8 +38,11 @@ enum {
     PA_ERR_LAUNCH = 4            /* the HIP runtime refused a launch       */
 };
 
-/* Element type tags for K/V/query/output buffers. */
-enum { PA_DTYPE_F32 = 0, PA_DTYPE_BF16 = 1, PA_DTYPE_F16 = 2 };
+/* Element type tags for K/V/query/output buffers.  PA_DTYPE_E4M3 (8-bit codes
+ * with a scale per block and KV head, section (g)) names a cache only: in
+ * PaRowDims.cache_dtype, pa_plan_step_for, pa_decode_workgroups_per_item and
+ * pa_decode_workgroups_per_cu. */
+enum { PA_DTYPE_F32 = 0, PA_DTYPE_BF16 = 1, PA_DTYPE_F16 = 2, PA_DTYPE_E4M3 = 3 };
 
 /* Default split-K partition of the decode kernel, in context tokens, and the
  * largest one its fast path takes (larger or non-multiple-of-32 partitions
@@ -641,6 +644,148 @@ enum { PA_STEP_PREFILL_WRITE = 1, PA_STEP_NO_APPEND = 2 };
 int pa_attention_step(const PaStepCall *call, const void *query, void *key_cache, void *value_cache,
                       int32_t layer_idx, const PaNewRows *new_rows, float scaling, void *output,
                       int32_t flags, int32_t *declined, void *stream);
+
+/* ---- (g) rotated rows, and the 8-bit cache -------------------------------- */
+
+/*
+ * The 8-bit cache.  key_cache / value_cache hold e4m3 codes (OCP: four
+ * significant bits, +-448, NaN, no infinities) in the layout of the other
+ * caches, and key_scales / value_scales float [num_layers, total_blocks,
+ * num_kv_heads]; an element is code * scale.  Scales are powers of two: of any
+ * other the exponent alone is read.  The write entry points keep them so:
+ *
+ *  - A block's scale is the smallest power of two >= (largest finite magnitude
+ *    of its rows) / 448, at least 2^-64, per KV head and tensor.
+ *  - A call that writes a block's first row starts the block afresh: what it
+ *    held counts for nothing.  So a block is filled from its first row on.
+ *  - A call that writes other rows of a block keeps the larger of its scale
+ *    and the one the new rows need.  If that is larger, the block's other rows
+ *    are re-coded with it (rounded to nearest even): their values stay but
+ *    where they fall among the subnormal codes.
+ *  - Rows are coded as the 16-bit cache would hold them, rounded to their type
+ *    first; fp16 ones are limited to +-61440, the largest four-bit value below
+ *    fp16's maximum.  Infinities and NaN become NaN and count for no scale.
+ *  - The tokens of one block follow each other in the call's slot_mapping (as
+ *    pa_pack's scatter_slots have them), and no slot occurs twice.  (A mapping
+ *    that breaks this reads and writes inside the caches, but leaves blocks
+ *    whose scale does not fit all of their codes.)
+ *  - block_size is at most 256.
+ *
+ * pa_copy_blocks / pa_swap_blocks move codes and scales alike (a block of
+ * scales is num_kv_heads floats).
+ */
+
+/* Sizes of a step's rows and of the cache they go to. */
+typedef struct {
+    int32_t num_tokens;      /* T                                          */
+    int32_t num_query_heads; /* H_q                                        */
+    int32_t num_kv_heads;    /* H_kv                                       */
+    int32_t head_dim;        /* D, at most 256                             */
+    int32_t block_size;
+    int32_t total_blocks;
+    int32_t num_layers;
+    int32_t dtype;           /* PA_DTYPE_* of the rows                     */
+    int32_t cache_dtype;     /* the rows' type, or PA_DTYPE_E4M3           */
+} PaRowDims;
+
+/* The projections' rows, [T, H_q, D] and [T, H_kv, D] with element strides
+ * between tokens and heads and unit stride along D, and where the rotated ones
+ * go (query_out may be query, and key_out key). */
+typedef struct {
+    const void *query;
+    const void *key;
+    const void *value;
+    int64_t query_token_stride;
+    int64_t query_head_stride;
+    int64_t key_token_stride;
+    int64_t key_head_stride;
+    int64_t value_token_stride;
+    int64_t value_head_stride;
+    void *query_out;
+    int64_t query_out_token_stride;
+    int64_t query_out_head_stride;
+    void *key_out;                 /* pa_rotate only */
+    int64_t key_out_token_stride;
+    int64_t key_out_head_stride;
+} PaRotateRows;
+
+/* The rotation, and the norm ahead of it. */
+typedef struct {
+    const int64_t *positions;  /* [T], device                                 */
+    const float *cos_sin;      /* [num_positions, rotary_dim], device: a
+                                  position's cosines, then its sines          */
+    int64_t num_positions;
+    int32_t rotary_dim;        /* R: even, at most D; 0: no rotation (the two
+                                  pointers may then be NULL)                  */
+    int32_t interleaved;       /* pairs (2i, 2i + 1) instead of (i, i + R/2)  */
+    const void *query_weight;  /* [D], or NULL: not normalised                */
+    const void *key_weight;
+    int32_t weight_dtype;      /* the rows' type or PA_DTYPE_F32              */
+    float eps;
+} PaRotation;
+
+/*
+ * No counterpart in the reference, whose models rotate before they hand rows
+ * over.  Each Q and K row of a token is normalised (x * rsqrt(mean(x^2) + eps)
+ * * weight, where a weight is given) and rotated: the pair (a, b) becomes
+ * (a cos - b sin, b cos + a sin) with the position's cosine and sine, the
+ * elements past R stay.  All of it in fp32, rounded once.  A token whose
+ * position lies outside [0, num_positions) gets NaN rows.  rows.value is not
+ * read.  Asynchronous on `stream`, as every entry point here.
+ */
+int pa_rotate(PaRotateRows rows, PaRotation rotation, PaRowDims dims, void *stream);
+
+/*
+ * pa_rotate, with K and V going into the paged cache at slot_mapping (int64
+ * [T]) in the same launch: bit for bit pa_rotate followed by
+ * pa_reshape_and_cache (or _8bit) where all rows start at multiples of four
+ * elements or none does.  Slots outside [0, N * bs) are skipped, and
+ * so is the K row of a token whose position lies outside the table.
+ * key_scales / value_scales: for PA_DTYPE_E4M3 caches, NULL otherwise.
+ */
+int pa_rotate_and_cache(PaRotateRows rows, PaRotation rotation, PaRowDims dims,
+                        void *key_cache, void *value_cache, float *key_scales,
+                        float *value_scales, const int64_t *slot_mapping,
+                        int32_t layer_idx, void *stream);
+
+/* pa_reshape_and_cache into an 8-bit cache; dtype is the rows'. */
+int pa_reshape_and_cache_8bit(const void *key, const void *value,
+                              int64_t key_token_stride, int64_t key_head_stride,
+                              int64_t value_token_stride, int64_t value_head_stride,
+                              void *key_cache, void *value_cache,
+                              float *key_scales, float *value_scales,
+                              const int64_t *slot_mapping, int32_t num_tokens,
+                              int32_t num_kv_heads, int32_t head_dim,
+                              int32_t block_size, int32_t total_blocks,
+                              int32_t num_layers, int32_t layer_idx,
+                              int32_t dtype, void *stream);
+
+/* The scales of an 8-bit cache, device. */
+typedef struct {
+    const float *key;
+    const float *value;
+} PaCacheScales;
+
+/*
+ * pa_decode_phases and pa_prefill over an 8-bit cache: dims.dtype is the
+ * query's and the output's.  Same work lists, workspace (of dims), phases and
+ * results for missing blocks and empty rows.
+ */
+int pa_decode_8bit(int32_t phases, const void *query, const void *key_cache,
+                   const void *value_cache, PaCacheScales scales,
+                   int32_t layer_idx, PaStepDims dims,
+                   const int32_t *block_tables, const int32_t *context_lens,
+                   const int64_t *cu_seqlens, const int32_t *decode_items,
+                   int64_t num_decode_items, const int32_t *merge_items,
+                   int64_t num_merge_items, float scaling, void *output,
+                   void *workspace, size_t workspace_bytes, void *stream);
+int pa_prefill_8bit(const void *query, const void *key_cache,
+                    const void *value_cache, PaCacheScales scales,
+                    int32_t layer_idx, PaStepDims dims,
+                    const int32_t *block_tables, const int32_t *context_lens,
+                    const int64_t *cu_seqlens, const int32_t *prefill_items,
+                    int64_t num_prefill_items, int32_t prefill_tile,
+                    float scaling, void *output, void *stream);
 
 #ifdef __cplusplus
 }

@@ -26,6 +26,7 @@ PA_ERR_LAUNCH = 4
 PA_DTYPE_F32 = 0
 PA_DTYPE_BF16 = 1
 PA_DTYPE_F16 = 2
+PA_DTYPE_E4M3 = 3  # a cache of 8-bit codes with scales
 
 PA_DECODE_PARTITION = 2048
 PA_DECODE_MAX_PARTITION = 4096
@@ -62,6 +63,11 @@ EXPORTED_SYMBOLS = (
     "pa_prefill",
     "pa_prefill_append",
     "pa_attention_step",
+    "pa_rotate",
+    "pa_rotate_and_cache",
+    "pa_reshape_and_cache_8bit",
+    "pa_decode_8bit",
+    "pa_prefill_8bit",
     "pa_map_host_memory",
     "pa_calibrate_mfma",
     "pa_calibrate_mfma_flops",
@@ -115,6 +121,61 @@ class PaNewRows(ctypes.Structure):
         ("key_head_stride", ctypes.c_int64),
         ("value_token_stride", ctypes.c_int64),
         ("value_head_stride", ctypes.c_int64),
+    ]
+
+
+class PaRowDims(ctypes.Structure):
+    _fields_ = [
+        ("num_tokens", ctypes.c_int32),
+        ("num_query_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("total_blocks", ctypes.c_int32),
+        ("num_layers", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("cache_dtype", ctypes.c_int32),
+    ]
+
+
+class PaRotateRows(ctypes.Structure):
+    _fields_ = [
+        ("query", ctypes.c_void_p),
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("query_token_stride", ctypes.c_int64),
+        ("query_head_stride", ctypes.c_int64),
+        ("key_token_stride", ctypes.c_int64),
+        ("key_head_stride", ctypes.c_int64),
+        ("value_token_stride", ctypes.c_int64),
+        ("value_head_stride", ctypes.c_int64),
+        ("query_out", ctypes.c_void_p),
+        ("query_out_token_stride", ctypes.c_int64),
+        ("query_out_head_stride", ctypes.c_int64),
+        ("key_out", ctypes.c_void_p),
+        ("key_out_token_stride", ctypes.c_int64),
+        ("key_out_head_stride", ctypes.c_int64),
+    ]
+
+
+class PaRotation(ctypes.Structure):
+    _fields_ = [
+        ("positions", ctypes.c_void_p),
+        ("cos_sin", ctypes.c_void_p),
+        ("num_positions", ctypes.c_int64),
+        ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("query_weight", ctypes.c_void_p),
+        ("key_weight", ctypes.c_void_p),
+        ("weight_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class PaCacheScales(ctypes.Structure):
+    _fields_ = [
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
     ]
 
 
@@ -247,6 +308,25 @@ _SIGNATURES = {
     "pa_prefill_append": (
         ctypes.c_int,
         [_vp, _vp, _vp, _i32, PaStepDims, PaNewRows, _vp, _vp, _vp, _vp, _i64, _i32, _f32, _vp, _vp],
+    ),
+    "pa_rotate": (ctypes.c_int, [PaRotateRows, PaRotation, PaRowDims, _vp]),
+    "pa_rotate_and_cache": (
+        ctypes.c_int,
+        [PaRotateRows, PaRotation, PaRowDims, _vp, _vp, _vp, _vp, _vp, _i32, _vp],
+    ),
+    "pa_reshape_and_cache_8bit": (
+        ctypes.c_int,
+        [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+         _vp],
+    ),
+    "pa_decode_8bit": (
+        ctypes.c_int,
+        [_i32, _vp, _vp, _vp, PaCacheScales, _i32, PaStepDims, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _f32, _vp, _vp,
+         _sz, _vp],
+    ),
+    "pa_prefill_8bit": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, PaCacheScales, _i32, PaStepDims, _vp, _vp, _vp, _vp, _i64, _i32, _f32, _vp, _vp],
     ),
     "pa_map_host_memory": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_void_p)]),
     "pa_error_string": (ctypes.c_char_p, [ctypes.c_int]),

@@ -80,10 +80,13 @@ int require(const char* who, std::initializer_list<Required> list) {
   return PA_OK;
 }
 
-const char* layer_base(const void* cache, const PaStepDims& d, int32_t layer_idx) {
-  const int64_t span = static_cast<int64_t>(d.total_blocks) * d.block_size * d.num_kv_heads *
-                       d.head_dim * elem_bytes(d.dtype);
+// (eb: bytes of a cache element)
+const char* layer_base(const void* cache, const PaStepDims& d, int32_t layer_idx, int eb) {
+  const int64_t span = static_cast<int64_t>(d.total_blocks) * d.block_size * d.num_kv_heads * d.head_dim * eb;
   return reinterpret_cast<const char*>(cache) + span * layer_idx;
+}
+const float* layer_scales(const float* scales, const PaStepDims& d, int32_t layer_idx) {
+  return scales + static_cast<int64_t>(d.total_blocks) * d.num_kv_heads * layer_idx;
 }
 
 }  // namespace
@@ -494,7 +497,7 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
                   const int64_t* cu_seqlens, const int32_t* decode_items,
                   int64_t num_decode_items, const int32_t* merge_items, int64_t num_merge_items,
                   float scaling, void* output, void* workspace, size_t workspace_bytes,
-                  void* stream, const PaNewRows* new_rows = nullptr) {
+                  void* stream, const PaNewRows* new_rows = nullptr, const PaCacheScales* scales = nullptr) {
   if (phases <= 0 || (phases & ~(PA_DECODE_PHASE_PARTITIONS | PA_DECODE_PHASE_MERGE)) != 0)
     return fail(PA_ERR_INVALID_ARGUMENT, "%s: phases must be a non-empty mask of "
                 "PA_DECODE_PHASE_PARTITIONS and PA_DECODE_PHASE_MERGE, got %d", who, phases);
@@ -519,8 +522,10 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int group = dims.num_query_heads / dims.num_kv_heads;
   const int eb = elem_bytes(dims.dtype);
+  const int cache_eb = scales != nullptr ? 1 : eb;
   const int log2_bs = log2_exact(dims.block_size);
   const bool fast =
+      scales == nullptr &&
       pa::decode_fast_path_supported(dims.dtype, dims.head_dim, group, dims.block_size,
                                      dims.partition_size) &&
       aligned16(query) && aligned16(key_cache) && aligned16(value_cache) &&
@@ -568,8 +573,8 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
     a.query = query;
     a.q_token_stride = dims.q_token_stride;
     a.q_head_stride = dims.q_head_stride;
-    a.key_cache = layer_base(key_cache, dims, layer_idx);
-    a.value_cache = layer_base(value_cache, dims, layer_idx);
+    a.key_cache = layer_base(key_cache, dims, layer_idx, cache_eb);
+    a.value_cache = layer_base(value_cache, dims, layer_idx, cache_eb);
     a.block_tables = block_tables;
     a.rows = dims.block_table_rows;
     a.num_table_rows = dims.num_table_rows > 0 ? dims.num_table_rows : dims.num_seqs;
@@ -614,8 +619,8 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
   a.query = query;
   a.q_token_stride = dims.q_token_stride;
   a.q_head_stride = dims.q_head_stride;
-  a.key_cache = layer_base(key_cache, dims, layer_idx);
-  a.value_cache = layer_base(value_cache, dims, layer_idx);
+  a.key_cache = layer_base(key_cache, dims, layer_idx, cache_eb);
+  a.value_cache = layer_base(value_cache, dims, layer_idx, cache_eb);
   a.block_tables = block_tables;
   a.rows = dims.block_table_rows;
   a.num_table_rows = dims.num_table_rows > 0 ? dims.num_table_rows : dims.num_seqs;
@@ -632,6 +637,10 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
   a.num_kv_heads = dims.num_kv_heads;
   a.head_dim = dims.head_dim;
   a.scale_log2e = scaling * pa::kLog2e;
+  if (scales != nullptr) {
+    a.key_scales = layer_scales(scales->key, dims, layer_idx);
+    a.value_scales = layer_scales(scales->value, dims, layer_idx);
+  }
   return from_hip(pa::launch_generic(a, dims.dtype, s), who);
 }
 
@@ -688,7 +697,7 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
                  int32_t layer_idx, PaStepDims dims, const int32_t* block_tables,
                  const int32_t* context_lens, const int64_t* cu_seqlens, const int32_t* prefill_items,
                  int64_t num_prefill_items, int32_t prefill_tile, float scaling, void* output,
-                 void* stream, const PaNewRows* new_rows) {
+                 void* stream, const PaNewRows* new_rows, const PaCacheScales* scales = nullptr) {
   int rc = check_step(dims, who);
   if (rc != PA_OK) return rc;
   if (layer_idx < 0 || layer_idx >= dims.num_layers)
@@ -706,7 +715,9 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int group = dims.num_query_heads / dims.num_kv_heads;
   const int eb = elem_bytes(dims.dtype);
+  const int cache_eb = scales != nullptr ? 1 : eb;
   const bool fast =
+      scales == nullptr &&
       pa::prefill_fast_path_supported(dims.dtype, dims.head_dim, group, dims.block_size) &&
       prefill_tile == pa::prefill_tile_for(group) && dims.max_blocks_per_seq > 0 &&
       static_cast<int64_t>(dims.block_size) * dims.num_kv_heads * dims.head_dim * eb <= 0xffffffffLL &&
@@ -732,8 +743,8 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
     a.query = query;
     a.q_token_stride = dims.q_token_stride;
     a.q_head_stride = dims.q_head_stride;
-    a.key_cache = layer_base(key_cache, dims, layer_idx);
-    a.value_cache = layer_base(value_cache, dims, layer_idx);
+    a.key_cache = layer_base(key_cache, dims, layer_idx, cache_eb);
+    a.value_cache = layer_base(value_cache, dims, layer_idx, cache_eb);
     a.block_tables = block_tables;
     a.rows = dims.block_table_rows;
     a.num_table_rows = dims.num_table_rows > 0 ? dims.num_table_rows : dims.num_seqs;
@@ -765,8 +776,8 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
   a.query = query;
   a.q_token_stride = dims.q_token_stride;
   a.q_head_stride = dims.q_head_stride;
-  a.key_cache = layer_base(key_cache, dims, layer_idx);
-  a.value_cache = layer_base(value_cache, dims, layer_idx);
+  a.key_cache = layer_base(key_cache, dims, layer_idx, cache_eb);
+  a.value_cache = layer_base(value_cache, dims, layer_idx, cache_eb);
   a.block_tables = block_tables;
   a.rows = dims.block_table_rows;
   a.num_table_rows = dims.num_table_rows > 0 ? dims.num_table_rows : dims.num_seqs;
@@ -783,6 +794,10 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
   a.num_kv_heads = dims.num_kv_heads;
   a.head_dim = dims.head_dim;
   a.scale_log2e = scaling * pa::kLog2e;
+  if (scales != nullptr) {
+    a.key_scales = layer_scales(scales->key, dims, layer_idx);
+    a.value_scales = layer_scales(scales->value, dims, layer_idx);
+  }
   return from_hip(pa::launch_generic(a, dims.dtype, s), who);
 }
 
@@ -865,6 +880,183 @@ int pa_attention_step(const PaStepCall* call, const void* query, void* key_cache
                      c.decode_items, c.num_decode_items, c.merge_items, c.num_merge_items, scaling, output,
                      c.workspace, c.workspace_bytes, stream);
   return PA_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+// Whether `dims` and `rotation` describe rows the kernels take.
+int check_rows(const char* who, const PaRowDims& d, const PaRotation& r, bool query) {
+  if (elem_bytes(d.dtype) == 0) return fail(PA_ERR_INVALID_ARGUMENT, "%s: unknown dtype %d", who, d.dtype);
+  if (d.num_tokens < 0 || (query ? d.num_query_heads <= 0 : d.num_query_heads != 0) || d.num_kv_heads <= 0 ||
+      d.head_dim <= 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: bad geometry", who);
+  if (d.head_dim > 256) return fail(PA_ERR_UNSUPPORTED, "%s: head_dim %d is above 256", who, d.head_dim);
+  // (row ids are 32 bits)
+  if (static_cast<int64_t>(d.num_tokens) * (static_cast<int64_t>(d.num_query_heads) + 2 * d.num_kv_heads) >
+      0x3fffffffLL)
+    return fail(PA_ERR_UNSUPPORTED, "%s: too many rows in one call", who);
+  if (r.rotary_dim < 0 || r.rotary_dim % 2 != 0 || r.rotary_dim > d.head_dim)
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: rotary_dim must be even and at most head_dim (%d), got %d", who,
+                d.head_dim, r.rotary_dim);
+  if (r.rotary_dim > 0 && r.num_positions <= 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: the table needs at least one position", who);
+  if ((r.query_weight != nullptr || r.key_weight != nullptr) && r.weight_dtype != d.dtype &&
+      r.weight_dtype != PA_DTYPE_F32)
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: weight_dtype must be the rows' or PA_DTYPE_F32", who);
+  return PA_OK;
+}
+
+pa::RotateArgs rotate_args(const PaRotateRows& w, const PaRotation& r, const PaRowDims& d) {
+  pa::RotateArgs a{};
+  a.query = w.query;
+  a.key = w.key;
+  a.value = w.value;
+  a.q_token_stride = w.query_token_stride;
+  a.q_head_stride = w.query_head_stride;
+  a.k_token_stride = w.key_token_stride;
+  a.k_head_stride = w.key_head_stride;
+  a.v_token_stride = w.value_token_stride;
+  a.v_head_stride = w.value_head_stride;
+  a.query_out = w.query_out;
+  a.q_out_token_stride = w.query_out_token_stride;
+  a.q_out_head_stride = w.query_out_head_stride;
+  a.positions = r.positions;
+  a.cos_sin = r.cos_sin;
+  a.num_positions = r.num_positions;
+  a.query_weight = r.query_weight;
+  a.key_weight = r.key_weight;
+  a.eps = r.eps;
+  a.weight_f32 = r.weight_dtype == PA_DTYPE_F32;
+  a.rotary_dim = r.rotary_dim;
+  a.interleaved = r.interleaved != 0;
+  a.num_tokens = d.num_tokens;
+  a.num_query_heads = d.num_query_heads;
+  a.num_kv_heads = d.num_kv_heads;
+  a.head_dim = d.head_dim;
+  a.block_size = d.block_size;
+  return a;
+}
+
+// Points `a` at the layer's cache (and scales) after checking its geometry.
+int bind_cache(const char* who, const PaRowDims& d, int32_t layer_idx, void* key_cache, void* value_cache,
+               float* key_scales, float* value_scales, const int64_t* slot_mapping, pa::RotateArgs* a) {
+  if (d.block_size <= 0 || d.total_blocks < 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: bad cache geometry", who);
+  if (layer_idx < 0 || layer_idx >= d.num_layers)
+    return fail(PA_ERR_INVALID_ARGUMENT, "Layer index %d out of range (num_layers=%d)", layer_idx, d.num_layers);
+  const bool codes = d.cache_dtype == PA_DTYPE_E4M3;
+  if (!codes && d.cache_dtype != d.dtype)
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: cache_dtype must be the rows' type or PA_DTYPE_E4M3", who);
+  if (codes != (key_scales != nullptr) || codes != (value_scales != nullptr))
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: scales are given with an 8-bit cache, and only with one", who);
+  if (codes && d.block_size > pa::kMaxCache8Block)
+    return fail(PA_ERR_UNSUPPORTED, "%s: 8-bit caches have blocks of at most %d tokens, got %d", who,
+                pa::kMaxCache8Block, d.block_size);
+  if (d.num_tokens == 0) return PA_OK;
+  const int rc = require(who, {{key_cache, "key_cache"}, {value_cache, "value_cache"}, {slot_mapping, "slot_mapping"}});
+  if (rc != PA_OK) return rc;
+  const int64_t slots = static_cast<int64_t>(d.total_blocks) * d.block_size;
+  const int64_t span = slots * d.num_kv_heads * d.head_dim * (codes ? 1 : elem_bytes(d.dtype)) * layer_idx;
+  a->key_cache = static_cast<char*>(key_cache) + span;
+  a->value_cache = static_cast<char*>(value_cache) + span;
+  if (codes) {
+    const int64_t at = static_cast<int64_t>(d.total_blocks) * d.num_kv_heads * layer_idx;
+    a->key_scales = key_scales + at;
+    a->value_scales = value_scales + at;
+  }
+  a->slot_mapping = slot_mapping;
+  a->num_slots = slots;
+  return PA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pa_rotate(PaRotateRows rows, PaRotation rotation, PaRowDims dims, void* stream) {
+  int rc = check_rows("pa_rotate", dims, rotation, true);
+  if (rc != PA_OK || dims.num_tokens == 0) return rc;
+  rc = require("pa_rotate", {{rows.query, "rows.query"}, {rows.key, "rows.key"}, {rows.query_out, "rows.query_out"},
+                             {rows.key_out, "rows.key_out"}});
+  if (rc == PA_OK && rotation.rotary_dim > 0)
+    rc = require("pa_rotate", {{rotation.positions, "positions"}, {rotation.cos_sin, "cos_sin"}});
+  if (rc != PA_OK) return rc;
+  pa::RotateArgs a = rotate_args(rows, rotation, dims);
+  a.value = nullptr;
+  a.v_token_stride = a.v_head_stride = 0;
+  a.key_out = rows.key_out;
+  a.k_out_token_stride = rows.key_out_token_stride;
+  a.k_out_head_stride = rows.key_out_head_stride;
+  return from_hip(pa::launch_rotate(a, dims.dtype, static_cast<hipStream_t>(stream)), "pa_rotate");
+}
+
+int pa_rotate_and_cache(PaRotateRows rows, PaRotation rotation, PaRowDims dims, void* key_cache, void* value_cache,
+                        float* key_scales, float* value_scales, const int64_t* slot_mapping, int32_t layer_idx,
+                        void* stream) {
+  const char* who = "pa_rotate_and_cache";
+  int rc = check_rows(who, dims, rotation, true);
+  if (rc != PA_OK) return rc;
+  pa::RotateArgs a = rotate_args(rows, rotation, dims);
+  rc = bind_cache(who, dims, layer_idx, key_cache, value_cache, key_scales, value_scales, slot_mapping, &a);
+  if (rc != PA_OK || dims.num_tokens == 0) return rc;
+  rc = require(who, {{rows.query, "rows.query"}, {rows.key, "rows.key"}, {rows.value, "rows.value"},
+                     {rows.query_out, "rows.query_out"}});
+  if (rc == PA_OK && rotation.rotary_dim > 0)
+    rc = require(who, {{rotation.positions, "positions"}, {rotation.cos_sin, "cos_sin"}});
+  if (rc != PA_OK) return rc;
+  return from_hip(pa::launch_rotate(a, dims.dtype, static_cast<hipStream_t>(stream)), who);
+}
+
+int pa_reshape_and_cache_8bit(const void* key, const void* value, int64_t key_token_stride, int64_t key_head_stride,
+                              int64_t value_token_stride, int64_t value_head_stride, void* key_cache,
+                              void* value_cache, float* key_scales, float* value_scales,
+                              const int64_t* slot_mapping, int32_t num_tokens, int32_t num_kv_heads,
+                              int32_t head_dim, int32_t block_size, int32_t total_blocks, int32_t num_layers,
+                              int32_t layer_idx, int32_t dtype, void* stream) {
+  const char* who = "pa_reshape_and_cache_8bit";
+  const PaRowDims dims{num_tokens,   0,          num_kv_heads, head_dim,     block_size,
+                       total_blocks, num_layers, dtype,        PA_DTYPE_E4M3};
+  const PaRotation none{};
+  int rc = check_rows(who, dims, none, false);
+  if (rc != PA_OK) return rc;
+  PaRotateRows rows{};
+  rows.key = key;
+  rows.value = value;
+  rows.key_token_stride = key_token_stride;
+  rows.key_head_stride = key_head_stride;
+  rows.value_token_stride = value_token_stride;
+  rows.value_head_stride = value_head_stride;
+  pa::RotateArgs a = rotate_args(rows, none, dims);
+  rc = bind_cache(who, dims, layer_idx, key_cache, value_cache, key_scales, value_scales, slot_mapping, &a);
+  if (rc != PA_OK || num_tokens == 0) return rc;
+  rc = require(who, {{key, "key"}, {value, "value"}});
+  if (rc != PA_OK) return rc;
+  return from_hip(pa::launch_rotate(a, dtype, static_cast<hipStream_t>(stream)), who);
+}
+
+int pa_decode_8bit(int32_t phases, const void* query, const void* key_cache, const void* value_cache,
+                   PaCacheScales scales, int32_t layer_idx, PaStepDims dims, const int32_t* block_tables,
+                   const int32_t* context_lens, const int64_t* cu_seqlens, const int32_t* decode_items,
+                   int64_t num_decode_items, const int32_t* merge_items, int64_t num_merge_items, float scaling,
+                   void* output, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = require("pa_decode_8bit", {{scales.key, "scales.key"}, {scales.value, "scales.value"}});
+  if (rc != PA_OK) return rc;
+  return decode_phases("pa_decode_8bit", false, phases, query, key_cache, value_cache, layer_idx, dims, block_tables,
+                       context_lens, cu_seqlens, decode_items, num_decode_items, merge_items, num_merge_items,
+                       scaling, output, workspace, workspace_bytes, stream, nullptr, &scales);
+}
+
+int pa_prefill_8bit(const void* query, const void* key_cache, const void* value_cache, PaCacheScales scales,
+                    int32_t layer_idx, PaStepDims dims, const int32_t* block_tables, const int32_t* context_lens,
+                    const int64_t* cu_seqlens, const int32_t* prefill_items, int64_t num_prefill_items,
+                    int32_t prefill_tile, float scaling, void* output, void* stream) {
+  const int rc = require("pa_prefill_8bit", {{scales.key, "scales.key"}, {scales.value, "scales.value"}});
+  if (rc != PA_OK) return rc;
+  return prefill_impl("pa_prefill_8bit", query, key_cache, value_cache, layer_idx, dims, block_tables, context_lens,
+                      cu_seqlens, prefill_items, num_prefill_items, prefill_tile, scaling, output, stream, nullptr,
+                      &scales);
 }
 
 }  // extern "C"

@@ -13,12 +13,21 @@
 // slot (from the mask + gather list, or from the block table), a ballot
 // keeps the attended ones, and the wave then walks them in ascending order,
 // the lanes splitting the head dimension.
+// C: the caches' elements, T or the 8-bit cache's codes (block tables only);
+// a lane then resolves its token's two scales with its slot.
+#include "cache8.hpp"
 #include "pa_common.hpp"
 #include "pa_launch.hpp"
 
 namespace pa {
 
-template <typename T, int EPL, bool kMasked>
+template <typename C>
+__device__ __forceinline__ float cache_value(const C* p, float scale) {
+  if constexpr (sizeof(C) == 1) return code_to_f32<0>(p->bits) * scale;
+  else return load_scalar<C>(p);
+}
+
+template <typename T, int EPL, bool kMasked, typename C = T>
 __global__ __launch_bounds__(kWave) void generic_attention_kernel(GenericArgs a) {
   const int lane = threadIdx.x;
   const int hq = a.num_query_heads;
@@ -59,8 +68,8 @@ __global__ __launch_bounds__(kWave) void generic_attention_kernel(GenericArgs a)
     const int d = lane + e * kWave;
     q[e] = d < D ? load_scalar<T>(qrow + d) : 0.f;
   }
-  const T* kbase = reinterpret_cast<const T*>(a.key_cache) + kvh * D;
-  const T* vbase = reinterpret_cast<const T*>(a.value_cache) + kvh * D;
+  const C* kbase = reinterpret_cast<const C*>(a.key_cache) + kvh * D;
+  const C* vbase = reinterpret_cast<const C*>(a.value_cache) + kvh * D;
 
   float m = kScoreFloor, l = 0.f;
   float acc[EPL];
@@ -70,6 +79,7 @@ __global__ __launch_bounds__(kWave) void generic_attention_kernel(GenericArgs a)
   for (int c0 = 0; c0 < n_ctx; c0 += kWave) {
     const int c = c0 + lane;
     int64_t slot = -1;
+    float kscale = 1.f, vscale = 1.f;
     if (c < n_ctx) {
       if constexpr (kMasked) {
         if (a.mask[static_cast<int64_t>(t) * n_ctx + c] != 0) {
@@ -80,8 +90,13 @@ __global__ __launch_bounds__(kWave) void generic_attention_kernel(GenericArgs a)
         const int col = c / a.block_size;
         if (trow >= 0 && trow < a.num_table_rows && col < a.block_table_stride) {
           const int b = a.block_tables[trow * a.block_table_stride + col];
-          if (b >= 0 && b < a.total_blocks)
+          if (b >= 0 && b < a.total_blocks) {
             slot = static_cast<int64_t>(b) * a.block_size + (c - col * a.block_size);
+            if constexpr (sizeof(C) == 1) {
+              kscale = scale_pow2(a.key_scales[static_cast<int64_t>(b) * a.num_kv_heads + kvh]);
+              vscale = scale_pow2(a.value_scales[static_cast<int64_t>(b) * a.num_kv_heads + kvh]);
+            }
+          }
         }
       }
     }
@@ -90,16 +105,18 @@ __global__ __launch_bounds__(kWave) void generic_attention_kernel(GenericArgs a)
       const int src = __builtin_ctzll(live);
       live &= live - 1;
       const int64_t s = __shfl(slot, src, kWave);
-      const T* krow = kbase + s * row_stride;
-      const T* vrow = vbase + s * row_stride;
+      const C* krow = kbase + s * row_stride;
+      const C* vrow = vbase + s * row_stride;
+      const float ks = sizeof(C) == 1 ? __shfl(kscale, src, kWave) : 1.f;
+      const float vs = sizeof(C) == 1 ? __shfl(vscale, src, kWave) : 1.f;
       float part = 0.f;
       float v[EPL];
 #pragma unroll
       for (int e = 0; e < EPL; ++e) {
         const int d = lane + e * kWave;
         const bool in = d < D;
-        part = fmaf(q[e], in ? load_scalar<T>(krow + d) : 0.f, part);
-        v[e] = in ? load_scalar<T>(vrow + d) : 0.f;
+        part = fmaf(q[e], in ? cache_value<C>(krow + d, ks) : 0.f, part);
+        v[e] = in ? cache_value<C>(vrow + d, vs) : 0.f;
       }
       const float score = wave_sum(part) * a.scale_log2e;
       const float m_new = fmaxf(m, score);
@@ -318,17 +335,17 @@ bool generic_supported(int dtype, int head_dim) {
   return head_dim >= 1 && head_dim <= 256;
 }
 
-template <typename T, bool kMasked>
+template <typename T, bool kMasked, typename C = T>
 static hipError_t launch_generic_t(const GenericArgs& a, hipStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.num_query_tokens) * a.num_query_heads;
   if (rows <= 0) return hipSuccess;
   const dim3 grid(static_cast<uint32_t>(rows));
   if (a.head_dim <= 64)
-    hipLaunchKernelGGL((generic_attention_kernel<T, 1, kMasked>), grid, dim3(kWave), 0, s, a);
+    hipLaunchKernelGGL((generic_attention_kernel<T, 1, kMasked, C>), grid, dim3(kWave), 0, s, a);
   else if (a.head_dim <= 128)
-    hipLaunchKernelGGL((generic_attention_kernel<T, 2, kMasked>), grid, dim3(kWave), 0, s, a);
+    hipLaunchKernelGGL((generic_attention_kernel<T, 2, kMasked, C>), grid, dim3(kWave), 0, s, a);
   else
-    hipLaunchKernelGGL((generic_attention_kernel<T, 4, kMasked>), grid, dim3(kWave), 0, s, a);
+    hipLaunchKernelGGL((generic_attention_kernel<T, 4, kMasked, C>), grid, dim3(kWave), 0, s, a);
   return hipGetLastError();
 }
 
@@ -377,13 +394,14 @@ hipError_t launch_flat(const GenericArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_generic(const GenericArgs& a, int dtype, hipStream_t s) {
+  const bool codes = a.key_scales != nullptr;
   switch (dtype) {
     case PA_DTYPE_F32:
-      return launch_generic_t<float, false>(a, s);
+      return codes ? launch_generic_t<float, false, code8_t>(a, s) : launch_generic_t<float, false>(a, s);
     case PA_DTYPE_BF16:
-      return launch_generic_t<bf16_t, false>(a, s);
+      return codes ? launch_generic_t<bf16_t, false, code8_t>(a, s) : launch_generic_t<bf16_t, false>(a, s);
     case PA_DTYPE_F16:
-      return launch_generic_t<f16_t, false>(a, s);
+      return codes ? launch_generic_t<f16_t, false, code8_t>(a, s) : launch_generic_t<f16_t, false>(a, s);
     default:
       return hipErrorNotSupported;
   }

@@ -94,6 +94,9 @@ struct GenericArgs {
   int32_t num_kv_heads;
   int32_t head_dim;
   float scale_log2e;
+  // 8-bit caches (else null): base of the layer, [blocks, H_kv]
+  const float* key_scales;
+  const float* value_scales;
 };
 
 // Packing of one step (pack.hip): a one-workgroup scan and a per-sequence
@@ -153,6 +156,55 @@ struct CacheWriteArgs {
   int32_t num_tokens;
   int32_t num_kv_heads;
   int32_t head_dim;
+};
+
+// Largest block size of the 8-bit cache (its write keeps a run index per token
+// of a chunk and one block more in LDS).
+constexpr int kMaxCache8Block = 256;
+
+// rotate_and_cache (rotate.hip).  key_scales not null: the caches hold e4m3
+// codes.  key_cache null: K goes to key_out and V is not read.
+struct RotateArgs {
+  const void* query;
+  const void* key;
+  const void* value;
+  int64_t q_token_stride;
+  int64_t q_head_stride;
+  int64_t k_token_stride;
+  int64_t k_head_stride;
+  int64_t v_token_stride;
+  int64_t v_head_stride;
+  void* query_out;
+  int64_t q_out_token_stride;
+  int64_t q_out_head_stride;
+  void* key_out;
+  int64_t k_out_token_stride;
+  int64_t k_out_head_stride;
+  const int64_t* positions;
+  const float* cos_sin;      // [num_positions, rotary_dim]: cosines, then sines
+  int64_t num_positions;
+  const void* query_weight;  // [head_dim], or null: not normalised
+  const void* key_weight;
+  float eps;
+  int32_t weight_f32;        // the weights are fp32 (else of the rows' type)
+  int32_t rotary_dim;        // 0: not rotated
+  int32_t interleaved;
+  void* key_cache;           // base of the layer
+  void* value_cache;
+  float* key_scales;         // base of the layer, [blocks, H_kv]
+  float* value_scales;
+  const int64_t* slot_mapping;
+  int64_t num_slots;
+  int32_t num_tokens;
+  int32_t num_query_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t block_size;
+  // The launch's: (2^32 - 1) / d of the divisors that map its workgroups, and
+  // the workgroups of the 8-bit cache's rows.
+  uint32_t heads_rcp;
+  uint32_t kv_rcp;
+  uint32_t kv_groups;
 };
 
 // KV block copy (copy_blocks).
@@ -232,6 +284,7 @@ size_t pack_workspace_size(int64_t num_seqs);
 bool pack_fusable(const PackArgs& a, int32_t max_new_tokens, int32_t max_context);
 hipError_t launch_pack(const PackArgs& a, hipStream_t stream);
 
+hipError_t launch_rotate(const RotateArgs& a, int dtype, hipStream_t stream);
 hipError_t launch_cache_write(const CacheWriteArgs& a, int dtype, hipStream_t stream);
 hipError_t launch_copy_blocks(const CopyBlocksArgs& a, bool vec16, hipStream_t stream);
 

@@ -14,6 +14,9 @@ path's own:
     host checks a step once, vectorised, from the pool's token counts;
   * on a CPU store (the reference's CPU path) the same slot formula runs
     vectorised in NumPy over the pool's host rows;
+  * a GPU store of ``torch.float8_e4m3fn`` holds 8-bit codes, with the scales
+    of its blocks in ``key_scales`` / ``value_scales`` (None otherwise); the
+    new K/V come in the model's own dtype;
   * preempted sequences swap their blocks to a pinned host pool and back in
     one launch per cache (:meth:`swap_out` / :meth:`swap_in`).
 """
@@ -84,9 +87,18 @@ class PagedKVCacheManager:
         self.allocator = PageAllocator(total_blocks, self.block_size, token_bytes, total_cpu_blocks)
         self.key_cache, self.value_cache = strategy.allocate_cache(
             total_blocks, self.block_size, self.num_layers, self.num_heads, self.head_dim, dtype)
+        self.key_scales: Optional[torch.Tensor] = None
+        self.value_scales: Optional[torch.Tensor] = None
+        if dtype == paged_ops.CODE_DTYPE:
+            if not self.on_gpu:
+                raise ValueError(f"a cache of {dtype} needs a store in device memory")
+            shape = (self.num_layers, int(total_blocks), self.num_heads)
+            self.key_scales, self.value_scales = (
+                torch.zeros(shape, dtype=torch.float32, device=self.key_cache.device) for _ in range(2))
         self.tables = BlockTablePool(width=max(1, min(int(total_blocks), 64)))
         self._device_table: Optional[torch.Tensor] = None
         self._host_pool: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+        self._host_scales: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
 
     # -- pool bookkeeping ---------------------------------------------------------
     @property
@@ -245,12 +257,15 @@ class PagedKVCacheManager:
     def checked_layer_kv(self, layer_idx: int, keys: torch.Tensor, values: torch.Tensor,
                          num_tokens: int) -> Tuple[torch.Tensor, torch.Tensor]:
         """One layer's new K/V ([T, H, D]) checked as scatter_layer_kv checks
-        them, on the cache's device and in its dtype: what the GPU backend
-        writes itself."""
+        them, on the cache's device and in its dtype (rows for 8-bit codes keep
+        theirs): what the GPU backend writes itself."""
         self._validate_layer_idx(layer_idx)
         self._validate_token_tensors(keys, values, (num_tokens, self.num_heads, self.head_dim))
-        dev = self.key_cache.device
-        return keys.to(dev, self.dtype), values.to(dev, self.dtype)
+        return self._as_rows(keys), self._as_rows(values)
+
+    def _as_rows(self, rows: torch.Tensor) -> torch.Tensor:
+        """``rows`` on the cache's device, in the dtype its write takes."""
+        return rows.to(self.key_cache.device, rows.dtype if self.key_scales is not None else self.dtype)
 
     def scatter_layer_kv(self, layer_idx: int, keys: torch.Tensor, values: torch.Tensor,
                          slot_mapping: torch.Tensor) -> None:
@@ -262,25 +277,33 @@ class PagedKVCacheManager:
         if slot_mapping.numel() == 0:
             return
         if self.on_gpu:
-            dev = self.key_cache.device
-            paged_ops.reshape_and_cache(keys.to(dev, self.dtype), values.to(dev, self.dtype), self.key_cache,
-                                        self.value_cache, slot_mapping.to(dev, torch.int64), layer_idx)
+            paged_ops.reshape_and_cache(self._as_rows(keys), self._as_rows(values), self.key_cache, self.value_cache,
+                                        slot_mapping.to(self.key_cache.device, torch.int64), layer_idx,
+                                        self.key_scales, self.value_scales)
             return
         flat = (-1, self.num_heads, self.head_dim)
         slots = slot_mapping.to(torch.int64)
         self.key_cache[layer_idx].view(flat).index_copy_(0, slots, keys.to(self.dtype))
         self.value_cache[layer_idx].view(flat).index_copy_(0, slots, values.to(self.dtype))
 
-    def _gather_layer(self, cache: torch.Tensor, layer_idx: int, slot_indices: torch.Tensor) -> torch.Tensor:
+    def _gather_layer(self, cache: torch.Tensor, scales: Optional[torch.Tensor], layer_idx: int,
+                      slot_indices: torch.Tensor) -> torch.Tensor:
+        """Rows [n, H, D] at the slots, in the cache's dtype; the values of
+        8-bit codes in bf16, which holds each of them exactly."""
         self._validate_layer_idx(layer_idx)
         flat = cache[layer_idx].view(-1, self.num_heads, self.head_dim)
-        return flat.index_select(0, slot_indices.to(cache.device, torch.int64))
+        slots = slot_indices.to(cache.device, torch.int64)
+        if scales is None:
+            return flat.index_select(0, slots)
+        codes = flat.view(torch.uint8).index_select(0, slots).view(cache.dtype)
+        factors = scales[layer_idx].index_select(0, slots // self.block_size).unsqueeze(-1)
+        return (codes.float() * factors).to(torch.bfloat16)
 
     def gather_layer_keys(self, layer_idx: int, slot_indices: torch.Tensor) -> torch.Tensor:
-        return self._gather_layer(self.key_cache, layer_idx, slot_indices)
+        return self._gather_layer(self.key_cache, self.key_scales, layer_idx, slot_indices)
 
     def gather_layer_values(self, layer_idx: int, slot_indices: torch.Tensor) -> torch.Tensor:
-        return self._gather_layer(self.value_cache, layer_idx, slot_indices)
+        return self._gather_layer(self.value_cache, self.value_scales, layer_idx, slot_indices)
 
     def write_prefix_kv(self, seq, keys: torch.Tensor, values: torch.Tensor) -> torch.Tensor:
         """K/V of a whole prompt ([L, T, H, D]) into the sequence's first T
@@ -326,6 +349,20 @@ class PagedKVCacheManager:
                 self.head_dim, self.dtype)
         return self._host_pool
 
+    def _swap(self, mapping, out: bool) -> None:
+        """The blocks of ``mapping`` between the caches and the host pool,
+        with the scales of 8-bit codes."""
+        hk, hv = self.host_pool()
+        pairs = [(self.key_cache, hk), (self.value_cache, hv)]
+        if self.key_scales is not None:
+            if self._host_scales is None:
+                shape = (self.num_layers, self.allocator.get_total_cpu_blocks(), self.num_heads)
+                self._host_scales = tuple(torch.zeros(shape, dtype=torch.float32, pin_memory=True) for _ in range(2))
+            pairs += [(paged_ops.scales_as_blocks(device), paged_ops.scales_as_blocks(host)) for device, host in
+                      zip((self.key_scales, self.value_scales), self._host_scales)]
+        for device, host in pairs:
+            paged_ops.swap_blocks(device, host, mapping, out=out)
+
     def swap_out(self, seq) -> List[int]:
         """Move a sequence's blocks to the host pool: host blocks are taken
         (PageAllocator.swap_out), one launch per cache copies every layer's
@@ -339,10 +376,7 @@ class PagedKVCacheManager:
         table = seq.block_table
         blocks = table.get_physical_blocks()
         host_ids = [self.allocator.swap_out(b) for b in blocks]
-        hk, hv = self.host_pool()
-        mapping = list(zip(blocks, host_ids))
-        paged_ops.swap_blocks(self.key_cache, hk, mapping, out=True)
-        paged_ops.swap_blocks(self.value_cache, hv, mapping, out=True)
+        self._swap(list(zip(blocks, host_ids)), out=True)
         table.take_blocks()
         table.swapped_blocks = host_ids
         return host_ids
@@ -355,10 +389,7 @@ class PagedKVCacheManager:
         if not host_ids:
             raise RuntimeError(f"Sequence {seq.seq_id} is not swapped out")
         blocks = [self.allocator.swap_in(h) for h in host_ids]
-        hk, hv = self.host_pool()
-        mapping = list(zip(host_ids, blocks))
-        paged_ops.swap_blocks(self.key_cache, hk, mapping, out=False)
-        paged_ops.swap_blocks(self.value_cache, hv, mapping, out=False)
+        self._swap(list(zip(host_ids, blocks)), out=False)
         table.put_blocks(blocks)
         table.swapped_blocks = None
         return blocks

@@ -18,11 +18,13 @@ from typing import Tuple, Union
 
 import torch
 
-# Names accepted for LLM_DTYPE / a dtype argument (strategies.py:14-32).
+# Names accepted for LLM_DTYPE / a dtype argument (strategies.py:14-32; "fp8",
+# the 8-bit cache, is this path's own).
 _DTYPE_NAMES = {
     torch.float16: ("fp16", "float16"),
     torch.bfloat16: ("bf16", "bfloat16"),
     torch.float32: ("fp32", "float32"),
+    torch.float8_e4m3fn: ("fp8", "float8_e4m3fn"),
 }
 _DTYPE_BY_NAME = {name: dtype for dtype, names in _DTYPE_NAMES.items() for name in names}
 

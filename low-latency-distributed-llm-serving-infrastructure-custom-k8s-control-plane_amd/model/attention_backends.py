@@ -114,15 +114,18 @@ class NativePagedBackend(AttentionBackend):
                 )
             raise RuntimeError("the native backend needs a step packed on the GPU store")
         step = context.packed_for(int(query.shape[1]))
+        scales = {}
+        if getattr(store, "key_scales", None) is not None:
+            scales = {"key_scales": store.key_scales, "value_scales": store.value_scales}
         recorder = metrics.current()
         if recorder is None:
             out = paged_ops.attention(query, store.key_cache, store.value_cache, layer_idx, step, scaling,
-                                      new_key=new_key, new_value=new_value)
+                                      new_key=new_key, new_value=new_value, **scales)
             return out.unsqueeze(0)
         stream = torch.cuda.current_stream(query.device)
         start = recorder.begin(stream)
         out = paged_ops.attention(query, store.key_cache, store.value_cache, layer_idx, step, scaling,
-                                  new_key=new_key, new_value=new_value)
+                                  new_key=new_key, new_value=new_value, **scales)
         nbytes = getattr(context, "_attention_bytes", None)
         if nbytes is None:
             nbytes = metrics.step_bytes(context.context_lens, context.num_query_tokens, int(query.shape[1]),

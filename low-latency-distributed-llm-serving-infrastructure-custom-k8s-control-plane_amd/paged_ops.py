@@ -12,10 +12,21 @@ The four jobs of the path:
   (d) :func:`prefill`            causal chunked prefill (MFMA)
 plus :func:`attention` (decode + prefill of one flattened step) and
 :func:`paged_attention_flat`, the reference C-ABI call over device tensors.
+
+Models that leave the position rotation to the serving path hand over their
+projections' rows: :func:`rotate_and_cache` normalises and rotates Q and K and
+does (b) in the same launch (:func:`rotate` without a cache, :func:`rope_table`
+for the table).
+
+A cache of ``torch.float8_e4m3fn`` holds 8-bit codes, with fp32 scales
+[layers, blocks, H_kv] beside it (``key_scales`` / ``value_scales`` of (b), (c),
+(d) and :func:`attention`; see :func:`reshape_and_cache` for its rules).  Rows,
+query and output are then of any of the other types.
 """
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 from typing import Optional, Sequence, Tuple
@@ -32,12 +43,27 @@ _DTYPES = {
     torch.float16: _native.PA_DTYPE_F16,
 }
 
+# The 8-bit cache's codes.
+CODE_DTYPE = torch.float8_e4m3fn
+
 
 def dtype_code(dtype: torch.dtype) -> int:
     try:
         return _DTYPES[dtype]
     except KeyError as exc:
         raise ValueError(f"unsupported dtype for the HIP path: {dtype}") from exc
+
+
+def cache_dtype_code(dtype: torch.dtype) -> int:
+    """dtype_code of a cache, which may also hold 8-bit codes."""
+    return _native.PA_DTYPE_E4M3 if dtype == CODE_DTYPE else dtype_code(dtype)
+
+
+def _current(device: torch.device):
+    """Makes ``device`` current for a launch where it is not."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def _stream(device: torch.device) -> int:
@@ -423,7 +449,7 @@ def decode_workgroups_per_item(dtype: torch.dtype, head_dim: int, num_kv_heads: 
     counts).  16-bit heads of 64, 80, 96 and 128 run two sub-groups in one
     workgroup, which counts as two here and in
     :func:`decode_workgroups_per_cu`."""
-    return _workgroups_per_item(dtype_code(dtype), int(head_dim), int(num_kv_heads), int(num_query_heads))
+    return _workgroups_per_item(cache_dtype_code(dtype), int(head_dim), int(num_kv_heads), int(num_query_heads))
 
 
 @functools.lru_cache(maxsize=256)
@@ -450,7 +476,7 @@ def decode_workgroups_per_cu(dtype: torch.dtype, head_dim: int, num_kv_heads: in
     key = (id(lib), torch.cuda.current_device(), dtype, int(head_dim), int(num_kv_heads), int(num_query_heads))
     per_cu = _OCCUPANCY_CACHE.get(key)
     if per_cu is None:
-        per_cu = int(lib.pa_decode_workgroups_per_cu(dtype_code(dtype), int(head_dim), int(num_kv_heads),
+        per_cu = int(lib.pa_decode_workgroups_per_cu(cache_dtype_code(dtype), int(head_dim), int(num_kv_heads),
                                                      int(num_query_heads)))
         _OCCUPANCY_CACHE[key] = per_cu
     return per_cu
@@ -669,7 +695,8 @@ def pack_step(
         per_cu = _occupancy_on(device, dtype, head_dim, num_kv_heads, hq)
     allocated = None if allocated_tokens is None else _int64_array(allocated_tokens)
     plan = _plan(starts, counts, block_size, prefill_tile, partition_size or 0, num_kv_heads, hq, per_item,
-                 per_cu, _compute_units(device), allocated, dtype_code(dtype) if per_cu else -1, int(head_dim or 0))
+                 per_cu, _compute_units(device), allocated, cache_dtype_code(dtype) if per_cu else -1,
+                 int(head_dim or 0))
     pooled = rows is not None
     n_upd = 0 if updates is None else int(updates.shape[0])
 
@@ -697,7 +724,7 @@ def pack_step(
         # An unknown cache dtype is sized as fp32, whose unpaired KV heads
         # need the most merge records.
         ws_dims = _native.PaStepDims(num_seqs=b, num_query_heads=hq, num_kv_heads=int(num_kv_heads),
-                                     head_dim=int(head_dim), dtype=dtype_code(dtype or torch.float32))
+                                     head_dim=int(head_dim), dtype=cache_dtype_code(dtype or torch.float32))
         ws_bytes = int(lib.pa_decode_workspace_size(ws_dims, int(plan.num_decode_items)))
         # (the records follow the partials)
         state_bytes = ws_bytes - decode_workspace_bytes(int(plan.num_decode_items), hq, int(head_dim))
@@ -726,11 +753,22 @@ def reshape_and_cache(
     value_cache: torch.Tensor,
     slot_mapping: torch.Tensor,
     layer_idx: int,
+    key_scales: Optional[torch.Tensor] = None,
+    value_scales: Optional[torch.Tensor] = None,
 ) -> None:
     """key_cache[layer].view(-1, H_kv, D)[slot_mapping] = key (and value), on the GPU.
 
     ``key`` / ``value``: [T, H_kv, D] (any token / head strides, unit stride on D);
     caches: (L, N, bs, H_kv, D) contiguous; ``slot_mapping``: int64 [T].
+
+    An 8-bit cache (``torch.float8_e4m3fn``) takes rows of any type and its
+    scales, fp32 [L, N, H_kv], which the call keeps: a block's scale is the
+    smallest power of two that is at least its rows' largest magnitude / 448
+    (and 2^-64), a call that writes a block's first row starts the block
+    afresh, and one that writes later rows re-codes the block's others where
+    its scale grows.  The tokens of a block follow each other in
+    ``slot_mapping``, no slot occurs twice, and blocks have at most 256
+    tokens.  fp16 rows are limited to +-61440; infinities become NaN.
     """
     device = _require_device(key, value, key_cache, value_cache, slot_mapping)
     if key_cache.dim() != 5 or value_cache.shape != key_cache.shape:
@@ -740,8 +778,11 @@ def reshape_and_cache(
     num_layers, total_blocks, block_size, num_kv_heads, head_dim = key_cache.shape
     if key.shape != value.shape or key.dim() != 3 or tuple(key.shape[1:]) != (num_kv_heads, head_dim):
         raise ValueError(f"Expected keys shape (T, {num_kv_heads}, {head_dim}), got {tuple(key.shape)}")
-    if key.dtype != key_cache.dtype or value.dtype != key_cache.dtype:
+    scales = _cache_scales(key_cache, value_cache, key_scales, value_scales)
+    if scales is None and (key.dtype != key_cache.dtype or value.dtype != key_cache.dtype):
         raise ValueError("key/value dtype must match the cache dtype")
+    if value.dtype != key.dtype:
+        raise ValueError("key and value must have the same dtype")
     if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != key.shape[0]:
         raise ValueError("slot_mapping must be int64 with one entry per token")
     if key.stride(2) != 1:
@@ -750,6 +791,15 @@ def reshape_and_cache(
         value = value.contiguous()
     slot_mapping = slot_mapping.contiguous()
     lib = _native.load_library()
+    if scales is not None:
+        with _current(device):
+            status = lib.pa_reshape_and_cache_8bit(
+                key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), value.stride(0), value.stride(1),
+                key_cache.data_ptr(), value_cache.data_ptr(), scales.key, scales.value, slot_mapping.data_ptr(),
+                int(key.shape[0]), num_kv_heads, head_dim, block_size, total_blocks, num_layers, int(layer_idx),
+                dtype_code(key.dtype), _stream(device))
+        _native.check(status, "pa_reshape_and_cache_8bit")
+        return
     status = lib.pa_reshape_and_cache(
         key.data_ptr(),
         value.data_ptr(),
@@ -771,6 +821,201 @@ def reshape_and_cache(
         _stream(device),
     )
     _native.check(status, "pa_reshape_and_cache")
+
+
+def _cache_scales(key_cache: torch.Tensor, value_cache: torch.Tensor, key_scales: Optional[torch.Tensor],
+                  value_scales: Optional[torch.Tensor]) -> Optional[_native.PaCacheScales]:
+    """The scales of an 8-bit cache as the library takes them, None for a
+    cache of another type; ValueError for scales that do not go with the
+    caches."""
+    if key_cache.dtype != CODE_DTYPE and value_cache.dtype != CODE_DTYPE:
+        if key_scales is not None or value_scales is not None:
+            raise ValueError(f"scales go with a cache of {CODE_DTYPE}, not {key_cache.dtype}")
+        return None
+    if key_cache.dtype != value_cache.dtype:
+        raise ValueError("key and value cache must have the same dtype")
+    if key_scales is None or value_scales is None:
+        raise ValueError(f"a cache of {CODE_DTYPE} needs key_scales and value_scales")
+    shape = (key_cache.shape[0], key_cache.shape[1], key_cache.shape[3])
+    for t in (key_scales, value_scales):
+        if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"scales must be contiguous float32 tensors of shape {shape} (layers, blocks, heads)")
+        if t.device != key_cache.device:
+            raise ValueError(f"scales are on {t.device}, the cache on {key_cache.device}")
+    return _native.PaCacheScales(key_scales.data_ptr(), value_scales.data_ptr())
+
+
+def scales_as_blocks(scales: torch.Tensor) -> torch.Tensor:
+    """The scales of an 8-bit cache as a cache of blocks, for
+    :func:`copy_blocks` and :func:`swap_blocks` (which a copy of its codes
+    needs as well)."""
+    return scales[:, :, None, None, :]
+
+
+# ---------------------------------------------------------------------------
+# rows that come without their rotation
+
+
+def rope_table(num_positions: int, rotary_dim: int, theta: float = 10000.0,
+               device: Optional[torch.device] = None) -> torch.Tensor:
+    """fp32 [num_positions, rotary_dim]: the cosines, then the sines, of
+    position * theta^(-2i / rotary_dim), i < rotary_dim / 2.  The angles are
+    taken in fp64: in fp32 that of position 100000 is off by up to 0.004."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if num_positions <= 0:
+        raise ValueError(f"num_positions must be positive, got {num_positions}")
+    freq = float(theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
+    angle = torch.arange(num_positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], dim=1).float()
+
+
+def _rotate_inputs(query, key, positions, cos_sin, query_weight, key_weight, eps, interleaved):
+    """(query, key, positions, PaRotation) after the checks both rotations
+    share; rows without unit stride along D are copied."""
+    if query.dim() != 3 or key.dim() != 3 or query.shape[0] != key.shape[0] or query.shape[2] != key.shape[2]:
+        raise ValueError(f"query and key must be (T, H_q, D) and (T, H_kv, D), got {tuple(query.shape)} and "
+                         f"{tuple(key.shape)}")
+    if key.dtype != query.dtype:
+        raise ValueError(f"query dtype {query.dtype} differs from key dtype {key.dtype}")
+    code = dtype_code(query.dtype)
+    tokens, dim = int(query.shape[0]), int(query.shape[2])
+    if positions.dtype != torch.int64 or positions.numel() != tokens:
+        raise ValueError("positions must be int64 with one entry per token")
+    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
+        raise ValueError("cos_sin must be a contiguous float32 (positions, rotary_dim) tensor (rope_table)")
+    rotary = int(cos_sin.shape[1])
+    if rotary % 2 or rotary > dim or rotary == 0 or cos_sin.shape[0] == 0:
+        raise ValueError(f"cos_sin must have an even rotary_dim of at most the head dim ({dim}) and a position, got "
+                         f"{tuple(cos_sin.shape)}")
+    weight_dtype = None
+    for w in (query_weight, key_weight):
+        if w is None:
+            continue
+        if tuple(w.shape) != (dim,) or not w.is_contiguous() or w.dtype not in (query.dtype, torch.float32):
+            raise ValueError(f"norm weights must be contiguous ({dim},) tensors of the rows' dtype or float32")
+        if weight_dtype is not None and w.dtype != weight_dtype:
+            raise ValueError("query_weight and key_weight must have the same dtype")
+        weight_dtype = w.dtype
+    query = query if query.stride(2) == 1 else query.contiguous()
+    key = key if key.stride(2) == 1 else key.contiguous()
+    positions = positions.contiguous()
+    rotation = _native.PaRotation(
+        positions.data_ptr(), cos_sin.data_ptr(), int(cos_sin.shape[0]), rotary, int(bool(interleaved)),
+        _ptr(query_weight), _ptr(key_weight), code if weight_dtype is None else dtype_code(weight_dtype), float(eps))
+    return query, key, positions, rotation
+
+
+def _rows_out(out: Optional[torch.Tensor], like: torch.Tensor, name: str) -> torch.Tensor:
+    """``out`` checked against the rows it gets (any token / head strides), or
+    a new contiguous tensor."""
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if tuple(out.shape) != tuple(like.shape) or out.dtype != like.dtype or out.device != like.device:
+        raise ValueError(f"{name} must have shape {tuple(like.shape)}, dtype {like.dtype} and be on {like.device}")
+    if out.stride(2) != 1 or any(out.shape[i] > 1 and out.stride(i) < out.shape[2] for i in (0, 1)):
+        raise ValueError(f"{name} needs unit stride along D and rows of its own")
+    return out
+
+
+def rotate(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    positions: torch.Tensor,
+    cos_sin: torch.Tensor,
+    *,
+    query_weight: Optional[torch.Tensor] = None,
+    key_weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+    out_query: Optional[torch.Tensor] = None,
+    out_key: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Per-head RMS norm (where a weight is given) and rotation of Q and K rows.
+
+    ``query`` / ``key``: [T, H_q, D] / [T, H_kv, D] of fp32, bf16 or fp16, D up
+    to 256, any token / head strides (views of one projection's output);
+    ``positions``: int64 [T] (``PackedStep.position_ids``); ``cos_sin``: fp32
+    [P, R] (:func:`rope_table`), R <= D elements of a head rotate.  Pairs are
+    (i, i + R/2), or (2i, 2i + 1) with ``interleaved``.  Weights: [D], of the
+    rows' dtype or fp32.  fp32 arithmetic, rounded once.  A position outside
+    the table gives NaN rows.  ``out_query`` / ``out_key`` may be the inputs.
+    """
+    device = _require_device(query, key, positions, cos_sin, query_weight, key_weight)
+    query, key, positions, rotation = _rotate_inputs(query, key, positions, cos_sin, query_weight, key_weight, eps,
+                                                     interleaved)
+    out_query = _rows_out(out_query, query, "out_query")
+    out_key = _rows_out(out_key, key, "out_key")
+    rows = _native.PaRotateRows(
+        query.data_ptr(), key.data_ptr(), None, query.stride(0), query.stride(1), key.stride(0), key.stride(1), 0, 0,
+        out_query.data_ptr(), out_query.stride(0), out_query.stride(1), out_key.data_ptr(), out_key.stride(0),
+        out_key.stride(1))
+    dims = _native.PaRowDims(int(query.shape[0]), int(query.shape[1]), int(key.shape[1]), int(query.shape[2]), 1, 0, 1,
+                             dtype_code(query.dtype), dtype_code(query.dtype))
+    with _current(device):
+        status = _native.load_library().pa_rotate(rows, rotation, dims, _stream(device))
+    _native.check(status, "pa_rotate")
+    return out_query, out_key
+
+
+def rotate_and_cache(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    layer_idx: int,
+    positions: torch.Tensor,
+    cos_sin: torch.Tensor,
+    *,
+    query_weight: Optional[torch.Tensor] = None,
+    key_weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+    key_scales: Optional[torch.Tensor] = None,
+    value_scales: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """:func:`rotate` with K and V written into the paged cache at
+    ``slot_mapping`` (:func:`reshape_and_cache`) in the same launch, bit for
+    bit the two calls (on rows that start at multiples of four elements);
+    returns (or fills) the rotated query [T, H_q, D].
+
+    ``out`` may be ``query``.  A token whose position lies outside the table
+    gets a NaN query row and no K row.
+    """
+    device = _require_device(query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin, query_weight,
+                             key_weight)
+    if key_cache.dim() != 5 or value_cache.shape != key_cache.shape:
+        raise ValueError("caches must be 5-D (layers, blocks, block_size, heads, dim) and alike")
+    if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+        raise ValueError("caches must be contiguous")
+    num_layers, total_blocks, block_size, num_kv_heads, head_dim = key_cache.shape
+    if key.shape != value.shape or key.dim() != 3 or tuple(key.shape[1:]) != (num_kv_heads, head_dim):
+        raise ValueError(f"Expected keys shape (T, {num_kv_heads}, {head_dim}), got {tuple(key.shape)}")
+    scales = _cache_scales(key_cache, value_cache, key_scales, value_scales)
+    if value.dtype != key.dtype or (scales is None and (key.dtype != key_cache.dtype or key.dtype != value_cache.dtype)):
+        raise ValueError("key/value dtype must match the cache dtype")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != key.shape[0]:
+        raise ValueError("slot_mapping must be int64 with one entry per token")
+    query, key, positions, rotation = _rotate_inputs(query, key, positions, cos_sin, query_weight, key_weight, eps,
+                                                     interleaved)
+    value = value if value.stride(2) == 1 else value.contiguous()
+    slot_mapping = slot_mapping.contiguous()
+    out = _rows_out(out, query, "out")
+    rows = _native.PaRotateRows(
+        query.data_ptr(), key.data_ptr(), value.data_ptr(), query.stride(0), query.stride(1), key.stride(0),
+        key.stride(1), value.stride(0), value.stride(1), out.data_ptr(), out.stride(0), out.stride(1), None, 0, 0)
+    dims = _native.PaRowDims(int(query.shape[0]), int(query.shape[1]), num_kv_heads, head_dim, block_size, total_blocks,
+                             num_layers, dtype_code(query.dtype), cache_dtype_code(key_cache.dtype))
+    with _current(device):
+        status = _native.load_library().pa_rotate_and_cache(
+            rows, rotation, dims, key_cache.data_ptr(), value_cache.data_ptr(),
+            None if scales is None else scales.key, None if scales is None else scales.value,
+            slot_mapping.data_ptr(), int(layer_idx), _stream(device))
+    _native.check(status, "pa_rotate_and_cache")
+    return out
 
 
 # ---------------------------------------------------------------------------
@@ -862,6 +1107,11 @@ def decode_workspace_bytes(num_decode_items: int, num_query_heads: int, head_dim
     return acc + ml
 
 
+def _row_dtype(query: torch.Tensor, key_cache: torch.Tensor) -> torch.dtype:
+    """The dtype of the query and the output: the cache's, but for 8-bit codes."""
+    return query.dtype if key_cache.dtype == CODE_DTYPE else key_cache.dtype
+
+
 def _step_dims(query_t: torch.Tensor, key_cache: torch.Tensor, step: PackedStep) -> _native.PaStepDims:
     """query_t is the [T, H_q, D] view of the query."""
     num_layers, total_blocks, block_size, num_kv_heads, head_dim = key_cache.shape
@@ -876,7 +1126,7 @@ def _step_dims(query_t: torch.Tensor, key_cache: torch.Tensor, step: PackedStep)
         num_layers=int(num_layers),
         max_blocks_per_seq=step.table_width,
         partition_size=step.partition_size,
-        dtype=dtype_code(key_cache.dtype),
+        dtype=dtype_code(_row_dtype(query_t, key_cache)),
         num_table_rows=step._source_rows,
         q_token_stride=query_t.stride(0),
         q_head_stride=query_t.stride(1),
@@ -904,7 +1154,7 @@ def _check_attention_inputs(q: torch.Tensor, key_cache: torch.Tensor, value_cach
         raise ValueError("caches must be 5-D (layers, blocks, block_size, heads, dim) and alike")
     if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
         raise ValueError("caches must be contiguous")
-    if q.dtype != key_cache.dtype or value_cache.dtype != key_cache.dtype:
+    if q.dtype != _row_dtype(q, key_cache) or value_cache.dtype != key_cache.dtype:
         raise ValueError(f"query dtype {q.dtype} differs from cache dtype {key_cache.dtype}")
     num_kv_heads, head_dim = key_cache.shape[3], key_cache.shape[4]
     if q.shape[2] != head_dim:
@@ -917,15 +1167,17 @@ def _check_attention_inputs(q: torch.Tensor, key_cache: torch.Tensor, value_cach
 
 def _output_for(q: torch.Tensor, key_cache: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
     """``out`` checked against what the kernels write ([T, H_q, D] contiguous rows
-    of the cache dtype on the query's device; a [1, T, H_q, D] tensor is taken
-    as the same rows), or a new such tensor when ``out`` is None."""
+    of the cache dtype (over 8-bit codes, the query's) on the query's device; a
+    [1, T, H_q, D] tensor is taken as the same rows), or a new such tensor when
+    ``out`` is None."""
+    dtype = _row_dtype(q, key_cache)
     if out is None:
-        return torch.empty(q.shape, dtype=key_cache.dtype, device=q.device)
+        return torch.empty(q.shape, dtype=dtype, device=q.device)
     rows = out[0] if out.dim() == 4 and out.shape[0] == 1 else out
     if tuple(rows.shape) != tuple(q.shape):
         raise ValueError(f"out must have shape {tuple(q.shape)} (or (1, *that)), got {tuple(out.shape)}")
-    if out.dtype != key_cache.dtype:
-        raise ValueError(f"out dtype {out.dtype} differs from the cache dtype {key_cache.dtype}")
+    if out.dtype != dtype:
+        raise ValueError(f"out dtype {out.dtype} differs from the cache dtype {dtype}")
     if out.device != q.device:
         raise ValueError(f"out is on {out.device}, the query on {q.device}")
     if not out.is_contiguous():
@@ -933,27 +1185,45 @@ def _output_for(q: torch.Tensor, key_cache: torch.Tensor, out: Optional[torch.Te
     return rows
 
 
-def _checked(query, key_cache, value_cache, step: PackedStep):
-    """([T, H_q, D] query view, launch dims) after the input checks.  The
+def _checked(query, key_cache, value_cache, step: PackedStep, key_scales=None, value_scales=None):
+    """([T, H_q, D] query view, launch dims, scales of an 8-bit cache or None)
+    after the input checks.  The
     checks and dims of the last call on ``step`` are kept, keyed by
     everything they depend on, so the layers of a step after the first skip
     them."""
     q = _query_view(query)
     key = (tuple(q.shape), q.stride(), q.dtype, q.device, key_cache.data_ptr(), value_cache.data_ptr(),
-           tuple(key_cache.shape), key_cache.dtype, value_cache.dtype)
+           tuple(key_cache.shape), key_cache.dtype, value_cache.dtype, _scales_key(key_scales),
+           _scales_key(value_scales))
     cached = step.__dict__.get("_launch_key")
     if cached is not None and cached[0] == key:
-        return q, cached[1]
+        return q, cached[1], cached[2]
     _require_device(q, key_cache, value_cache, step.buffer)
     _check_attention_inputs(q, key_cache, value_cache, step)
+    scales = _cache_scales(key_cache, value_cache, key_scales, value_scales)
     dims = _step_dims(q, key_cache, step)
-    step.__dict__["_launch_key"] = (key, dims)
-    return q, dims
+    step.__dict__["_launch_key"] = (key, dims, scales)
+    return q, dims, scales
 
 
-def _launch_decode(q, key_cache, value_cache, layer_idx, step, scaling, out, dims, phases) -> None:
+def _scales_key(scales: Optional[torch.Tensor]):
+    """What the checks of a cache's scales depend on."""
+    return None if scales is None else (scales.data_ptr(), scales.shape, scales.stride(), scales.dtype, scales.device)
+
+
+def _launch_decode(q, key_cache, value_cache, layer_idx, step, scaling, out, dims, phases, scales=None) -> None:
     ws_ptr, ws_bytes = step.workspace_ptr(dims)
     lib = _native.load_library()
+    if scales is not None:
+        with _current(q.device):
+            status = lib.pa_decode_8bit(
+                int(phases), q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), scales, int(layer_idx), dims,
+                step.ptr("block_tables"), step.ptr("context_lens"), step.ptr("cu_seqlens"),
+                step.ptr("decode_items") if step.num_decode_items else None, step.num_decode_items,
+                step.ptr("merge_items") if step.num_merge_items else None, step.num_merge_items, float(scaling),
+                out.data_ptr(), ws_ptr, ws_bytes, _stream(q.device))
+        _native.check(status, "pa_decode_8bit")
+        return
     status = lib.pa_decode_phases(
         int(phases),
         q.data_ptr(),
@@ -977,8 +1247,17 @@ def _launch_decode(q, key_cache, value_cache, layer_idx, step, scaling, out, dim
     _native.check(status, "pa_decode")
 
 
-def _launch_prefill(q, key_cache, value_cache, layer_idx, step, scaling, out, dims) -> None:
+def _launch_prefill(q, key_cache, value_cache, layer_idx, step, scaling, out, dims, scales=None) -> None:
     lib = _native.load_library()
+    if scales is not None:
+        with _current(q.device):
+            status = lib.pa_prefill_8bit(
+                q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), scales, int(layer_idx), dims,
+                step.ptr("block_tables"), step.ptr("context_lens"), step.ptr("cu_seqlens"),
+                step.ptr("prefill_items") if step.num_prefill_items else None, step.num_prefill_items,
+                step.prefill_tile, float(scaling), out.data_ptr(), _stream(q.device))
+        _native.check(status, "pa_prefill_8bit")
+        return
     status = lib.pa_prefill(
         q.data_ptr(),
         key_cache.data_ptr(),
@@ -1007,16 +1286,19 @@ def decode(
     scaling: float,
     out: Optional[torch.Tensor] = None,
     phases: int = _native.PA_DECODE_PHASE_PARTITIONS | _native.PA_DECODE_PHASE_MERGE,
+    key_scales: Optional[torch.Tensor] = None,
+    value_scales: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Split-K paged decode for the single-token sequences of ``step``.
 
     Returns (or fills) ``out`` [T, H_q, D]; rows of other tokens are untouched.
     ``phases`` launches only the partition and/or the merge phase (a merge
     call must follow a partition call of the same step and workspace).
+    ``key_scales`` / ``value_scales``: of an 8-bit cache.
     """
-    q, dims = _checked(query, key_cache, value_cache, step)
+    q, dims, scales = _checked(query, key_cache, value_cache, step, key_scales, value_scales)
     out = _output_for(q, key_cache, out)
-    _launch_decode(q, key_cache, value_cache, layer_idx, step, scaling, out, dims, phases)
+    _launch_decode(q, key_cache, value_cache, layer_idx, step, scaling, out, dims, phases, scales)
     return out
 
 
@@ -1028,11 +1310,14 @@ def prefill(
     step: PackedStep,
     scaling: float,
     out: Optional[torch.Tensor] = None,
+    key_scales: Optional[torch.Tensor] = None,
+    value_scales: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
-    """Causal chunked prefill for the multi-token sequences of ``step``."""
-    q, dims = _checked(query, key_cache, value_cache, step)
+    """Causal chunked prefill for the multi-token sequences of ``step``
+    (``key_scales`` / ``value_scales``: of an 8-bit cache)."""
+    q, dims, scales = _checked(query, key_cache, value_cache, step, key_scales, value_scales)
     out = _output_for(q, key_cache, out)
-    _launch_prefill(q, key_cache, value_cache, layer_idx, step, scaling, out, dims)
+    _launch_prefill(q, key_cache, value_cache, layer_idx, step, scaling, out, dims, scales)
     return out
 
 
@@ -1045,7 +1330,11 @@ def _new_rows(new_key: torch.Tensor, new_value: torch.Tensor, key_cache: torch.T
     if tuple(new_key.shape) != shape or tuple(new_value.shape) != shape:
         raise ValueError(f"new_key / new_value must have shape {shape}, got {tuple(new_key.shape)} "
                          f"and {tuple(new_value.shape)}")
-    if new_key.dtype != key_cache.dtype or new_value.dtype != key_cache.dtype:
+    if key_cache.dtype == CODE_DTYPE:
+        if new_key.dtype != new_value.dtype:
+            raise ValueError("new_key and new_value must have the same dtype")
+        dtype_code(new_key.dtype)
+    elif new_key.dtype != key_cache.dtype or new_value.dtype != key_cache.dtype:
         raise ValueError("new_key / new_value dtype must match the cache dtype")
     if new_key.stride(2) != 1:
         new_key = new_key.contiguous()
@@ -1120,7 +1409,7 @@ def _attention_step(query, key_cache, value_cache, layer_idx, step, scaling, out
            new_key.shape, ks, new_key.dtype, new_key.device, new_value.shape, vs, new_value.dtype, new_value.device)
     cached = step.__dict__.get("_layer_call")
     if cached is None or cached[0] != key:
-        q, dims = _checked(query, key_cache, value_cache, step)
+        q, dims, _ = _checked(query, key_cache, value_cache, step)
         k, v = _new_rows(new_key, new_value, key_cache, step)
         call = _step_call(step, dims)
         # (the step's workspace of other head counts stays alive with the call)
@@ -1157,6 +1446,8 @@ def attention(
     new_key: Optional[torch.Tensor] = None,
     new_value: Optional[torch.Tensor] = None,
     fused_prefill_write: Optional[bool] = None,
+    key_scales: Optional[torch.Tensor] = None,
+    value_scales: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Attention of a whole flattened step (decode + prefill sequences) -> [T, H_q, D].
 
@@ -1176,25 +1467,31 @@ def attention(
     prefill reads its chunks' new rows more slowly than the same rows from the
     cache, and the cache-write kernel and plain launches are faster.  A
     decode-only step writes its rows inside the decode launches.
+
+    ``key_scales`` / ``value_scales``: of an 8-bit cache, whose rows the
+    cache-write kernel writes ahead of the attention (a block's scale has to
+    be settled before anything reads the block).
     """
     if (new_key is None) != (new_value is None):
         raise ValueError("new_key and new_value are given together")
     need_prefill = step.num_prefill_items > 0
     need_decode = step.num_decode_items > 0
-    if new_key is not None and (need_prefill or need_decode):
+    if new_key is not None and (need_prefill or need_decode) and key_cache.dtype != CODE_DTYPE:
+        if key_scales is not None or value_scales is not None:
+            raise ValueError(f"scales go with a cache of {CODE_DTYPE}, not {key_cache.dtype}")
         return _attention_step(query, key_cache, value_cache, layer_idx, step, scaling, out, new_key, new_value,
                                fused_prefill_write)
-    q, dims = _checked(query, key_cache, value_cache, step)
+    q, dims, scales = _checked(query, key_cache, value_cache, step, key_scales, value_scales)
     out = _output_for(q, key_cache, out)
     if new_key is not None:
         k, v = _new_rows(new_key, new_value, key_cache, step)
         if step.num_query_tokens > 0:
-            reshape_and_cache(k, v, key_cache, value_cache, step.scatter_slots, layer_idx)
+            reshape_and_cache(k, v, key_cache, value_cache, step.scatter_slots, layer_idx, key_scales, value_scales)
     if need_prefill:
-        _launch_prefill(q, key_cache, value_cache, layer_idx, step, scaling, out, dims)
+        _launch_prefill(q, key_cache, value_cache, layer_idx, step, scaling, out, dims, scales)
     if need_decode:
         _launch_decode(q, key_cache, value_cache, layer_idx, step, scaling, out, dims,
-                       _native.PA_DECODE_PHASE_PARTITIONS | _native.PA_DECODE_PHASE_MERGE)
+                       _native.PA_DECODE_PHASE_PARTITIONS | _native.PA_DECODE_PHASE_MERGE, scales)
     if step.num_query_tokens > 0 and step.num_decode_items == 0 and step.num_prefill_items == 0:
         out.zero_()
     return out
