@@ -525,9 +525,9 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
   const int cache_eb = scales != nullptr ? 1 : eb;
   const int log2_bs = log2_exact(dims.block_size);
   const bool fast =
-      scales == nullptr &&
-      pa::decode_fast_path_supported(dims.dtype, dims.head_dim, group, dims.block_size,
-                                     dims.partition_size) &&
+      pa::decode_fast_path_supported(scales == nullptr ? dims.dtype : PA_DTYPE_E4M3, dims.head_dim, group,
+                                     dims.block_size, dims.partition_size) &&
+      (scales == nullptr || dims.dtype != PA_DTYPE_F32) &&
       aligned16(query) && aligned16(key_cache) && aligned16(value_cache) &&
       (dims.q_token_stride * eb) % 16 == 0 && (dims.q_head_stride * eb) % 16 == 0;
   if (new_rows != nullptr) {
@@ -598,6 +598,10 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
     // A record's fields hold counts and items below 65535.
     a.merge_state = num_decode_items < 65535 ? merge_state : nullptr;
     a.num_seqs = dims.num_seqs;
+    if (scales != nullptr) {
+      a.key_scales = layer_scales(scales->key, dims, layer_idx);
+      a.value_scales = layer_scales(scales->value, dims, layer_idx);
+    }
     if (new_rows != nullptr) {
       a.new_key = new_rows->key;
       a.new_value = new_rows->value;

@@ -964,10 +964,15 @@ int decode_workgroups_per_head(int dtype, int head_dim, int group) {
 
 bool decode_fast_path_supported(int dtype, int head_dim, int group, int block_size,
                                 int partition) {
-  if (dtype != PA_DTYPE_F32 && dtype != PA_DTYPE_BF16 && dtype != PA_DTYPE_F16) return false;
+  if (dtype == PA_DTYPE_E4M3) {
+    // (two tokens of a V operand's pair share a block, hence a scale)
+    if (!decode_uses_mfma(dtype, head_dim) || block_size < 2) return false;
+  } else if (dtype != PA_DTYPE_F32 && dtype != PA_DTYPE_BF16 && dtype != PA_DTYPE_F16) {
+    return false;
+  }
   // Rows of up to 512 bytes: heads of 64 and 128, and of 256 in 16-bit types;
   // heads of 80 and 96 on the lane layout of 128.
-  const bool wide16 = dtype != PA_DTYPE_F32 && head_dim == 256;
+  const bool wide16 = dtype != PA_DTYPE_F32 && dtype != PA_DTYPE_E4M3 && head_dim == 256;
   if (head_dim != 64 && head_dim != 128 && head_dim != 80 && head_dim != 96 && !wide16) return false;
   if (group < 1 || group > kMaxDecodeQueryGroup) return false;
   if (block_size <= 0 || (block_size & (block_size - 1)) != 0) return false;
@@ -981,7 +986,9 @@ hipError_t launch_decode(const DecodeArgs& a, int dtype, int head_dim, int group
   if (decode_uses_mfma(dtype, head_dim)) {
     if (phases & PA_DECODE_PHASE_PARTITIONS) {
       const int heads = decode_unit_heads(dtype, head_dim, a.num_kv_heads, group);
-      const hipError_t err = launch_decode_mfma(a, dtype, head_dim, heads, num_items, stream);
+      const hipError_t err = a.key_scales != nullptr
+                                 ? launch_decode8(a, dtype, head_dim, heads, num_items, stream)
+                                 : launch_decode_mfma(a, dtype, head_dim, heads, num_items, stream);
       if (err != hipSuccess) return err;
     }
     return launch_merge(a, dtype, head_dim, phases, stream);
@@ -993,8 +1000,10 @@ hipError_t decode_workgroups_per_cu(int dtype, int head_dim, int num_kv_heads, i
   *per_cu = 0;
   if (!decode_uses_mfma(dtype, head_dim)) return visit_decode(dtype, head_dim, group, OccupancyOp{per_cu});
   const int wgs = decode_workgroups_per_head(dtype, head_dim, group);
-  const hipError_t err = decode_mfma_workgroups_per_cu(
-      dtype, head_dim, wgs > 1, decode_unit_heads(dtype, head_dim, num_kv_heads, group), per_cu);
+  const int heads = decode_unit_heads(dtype, head_dim, num_kv_heads, group);
+  const hipError_t err = dtype == PA_DTYPE_E4M3
+                             ? decode8_workgroups_per_cu(head_dim, wgs > 1, heads, per_cu)
+                             : decode_mfma_workgroups_per_cu(dtype, head_dim, wgs > 1, heads, per_cu);
   *per_cu *= decode_sub_groups(group) / wgs;
   return err;
 }

@@ -164,4 +164,8 @@ __device__ __forceinline__ void merge_in_launch(const DecodeArgs& a, int G, int 
 hipError_t launch_decode_mfma(const DecodeArgs& a, int dtype, int head_dim, int unit_heads, int64_t num_items, hipStream_t stream);
 hipError_t decode_mfma_workgroups_per_cu(int dtype, int head_dim, bool shared, int unit_heads, int* per_cu);
 
+// decode8.hip (the occupancy of bf16 queries)
+hipError_t launch_decode8(const DecodeArgs& a, int dtype, int head_dim, int unit_heads, int64_t num_items, hipStream_t stream);
+hipError_t decode8_workgroups_per_cu(int head_dim, bool shared, int unit_heads, int* per_cu);
+
 }  // namespace pa

@@ -66,29 +66,11 @@
 #include <type_traits>
 
 #include "decode_common.hpp"
+#include "decode_mfma_common.hpp"
 
 namespace pa {
 
 constexpr int kMfmaTile = 32;   // context tokens per wave iteration
-
-typedef float f32x4m __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8m __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8m __attribute__((ext_vector_type(8)));
-typedef unsigned int u32x4m __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x2m __attribute__((ext_vector_type(2)));
-
-template <typename T>
-__device__ __forceinline__ f32x4m mfma16(u32x4m a, u32x4m b, f32x4m c);
-template <>
-__device__ __forceinline__ f32x4m mfma16<bf16_t>(u32x4m a, u32x4m b, f32x4m c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8m, a), __builtin_bit_cast(bf16x8m, b), c,
-                                                 0, 0, 0);
-}
-template <>
-__device__ __forceinline__ f32x4m mfma16<f16_t>(u32x4m a, u32x4m b, f32x4m c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8m, a), __builtin_bit_cast(f16x8m, b), c, 0,
-                                                0, 0);
-}
 
 // A lane's piece of a V row: D / 16 elements.
 template <int D>
@@ -101,13 +83,6 @@ template <>
 struct VPiece<128> {
   using type = u32x4m;
 };
-
-// NT: streaming loads, for rows no other workgroup reads.
-template <typename V, bool NT>
-__device__ __forceinline__ V row_load(const void* p) {
-  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
-  return *reinterpret_cast<const V*>(p);
-}
 
 // The K operands of a tile from the wave's LDS rows, at[j] the LDS address of
 // piece 4j + c of token r and the second half of the tile HALF bytes further.
@@ -147,14 +122,6 @@ __device__ __forceinline__ void read_k(const uint32_t (&at)[KJ], u32x4m (&k)[2][
           "=&v"(k[1][2]), "=&v"(k[1][3])
         : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(HALF), "n"(VM)
         : "memory");
-}
-
-// n / d, with rcp = (2^32 - 1) / d from the host: the product's high half is
-// the quotient or one less.  (A division by a runtime value is a chain of some
-// 30 dependent instructions, and the prologue's stood in front of every load.)
-__device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t d, uint32_t rcp) {
-  const uint32_t q = __umulhi(n, rcp);
-  return n - q * d >= d ? q + 1 : q;
 }
 
 template <typename T, int D, int DM, bool SHARED, int HEADS>
@@ -558,7 +525,7 @@ decode_mfma_kernel(DecodeArgs a) {
 }
 
 bool decode_uses_mfma(int dtype, int head_dim) {
-  return (dtype == PA_DTYPE_BF16 || dtype == PA_DTYPE_F16) &&
+  return (dtype == PA_DTYPE_BF16 || dtype == PA_DTYPE_F16 || dtype == PA_DTYPE_E4M3) &&
          (head_dim == 64 || head_dim == 80 || head_dim == 96 || head_dim == 128);
 }
 

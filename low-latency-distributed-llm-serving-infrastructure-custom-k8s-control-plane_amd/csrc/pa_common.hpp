@@ -230,6 +230,14 @@ __device__ __forceinline__ float wave_sum(float x) {
   return x;
 }
 
+// n / d, with rcp = (2^32 - 1) / d from the host: the product's high half is
+// the quotient or one less.  (A division by a runtime value is a chain of some
+// 30 dependent instructions, and the prologue's stood in front of every load.)
+__device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t d, uint32_t rcp) {
+  const uint32_t q = __umulhi(n, rcp);
+  return n - q * d >= d ? q + 1 : q;
+}
+
 // 16-byte global load / store.
 __device__ __forceinline__ uint4 ld16(const void* p) {
   return *reinterpret_cast<const uint4*>(p);

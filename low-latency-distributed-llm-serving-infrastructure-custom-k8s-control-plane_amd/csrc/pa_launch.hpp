@@ -60,6 +60,9 @@ struct DecodeArgs {
   // workgroups.
   uint32_t unit_rcp;
   uint32_t run_rcp;
+  // 8-bit caches (else null): base of the layer, [blocks, H_kv].
+  const float* key_scales;
+  const float* value_scales;
 };
 
 // Generic one-wave-per-(query token, head) attention: any head_dim <= 256,

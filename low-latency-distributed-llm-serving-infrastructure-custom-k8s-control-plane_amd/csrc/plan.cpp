@@ -112,23 +112,43 @@ constexpr MfmaModel kMfmaModel64 = {1.19, 0.26, 0.0007, 0.63, 2.0};
 // at 1024, 47.4 at 256); 15 of 990-2801, 12/12, 30.3 at its 512 (35.4 at 4096).
 constexpr MfmaModel kMfmaModelPadded = {1.68, 0.3, 0.00019, 2.2, 1.9};
 
+// The 8-bit cache's kernel (decode8.hip): half the bytes a token, 6.5 TB/s, and
+// a launch that fills the chip stops at 2048 (256 sequences of 32-8192 tokens,
+// 32/8 heads of 128: 154 us at 4096, 144 at 2048).  Fitted to 44 steps of 1-150
+// sequences of 16-25000 tokens over ten head shapes, at seven partitions each:
+// the picks take 0.4 % (heads of 128) and 1 % (of 64) longer than the best power
+// of two on average and 6 % at most (the 16-bit kernel's constants: 2 % and 17 %).
+constexpr double kHbmBytesPerUs8 = 6.5e6;
+constexpr int64_t kMaxFullChip8 = 2048;
+constexpr MfmaModel kModel8Of128 = {0.75, 0.068, 0.000065, 0.27, 1.46};
+constexpr MfmaModel kModel8Of64 = {0.81, 0.58, 0.00022, 1.24, 2.65};
+constexpr MfmaModel kModel8Padded = {0.61, 0.51, 0.0017, 1.02, 1.54};
+
 int64_t choose_partition_mfma(const DecodeContexts& d, const PaPlanParams& p, int dtype, int head_dim,
                               int64_t longest) {
-  const int64_t rule = choose_partition(d, p, longest);
+  const bool codes = dtype == PA_DTYPE_E4M3;
+  int64_t rule = choose_partition(d, p, longest);
+  if (codes && rule > kMaxFullChip8) rule = kMaxFullChip8;
   const int64_t hkv = p.num_kv_heads > 0 ? p.num_kv_heads : 1;
   const int64_t hq = p.num_query_heads > 0 ? p.num_query_heads : 4 * hkv;
   const int group = static_cast<int>(hq / hkv > 0 ? hq / hkv : 1);
   const int64_t width = p.workgroups_per_item > 0 ? p.workgroups_per_item : hkv;
   const int64_t unit_slots = (p.compute_units > 0 ? p.compute_units : 256) *
                              (p.workgroups_per_cu > 0 ? p.workgroups_per_cu : 3);
-  const MfmaModel& model = head_dim == 128 ? kMfmaModel128 : head_dim == 64 ? kMfmaModel64 : kMfmaModelPadded;
+  const MfmaModel& model = codes ? (head_dim == 128  ? kModel8Of128
+                                    : head_dim == 64 ? kModel8Of64
+                                                     : kModel8Padded)
+                                 : (head_dim == 128  ? kMfmaModel128
+                                    : head_dim == 64 ? kMfmaModel64
+                                                     : kMfmaModelPadded);
   if (rule >= kMinFullChipMfmaPartition && d.workgroups(rule, width) >= 3 * unit_slots / 2) return rule;
   const int64_t tokens = d.workgroups(1, 1);
   if (tokens == 0) return rule;
   // Units that one workgroup serves (sub-groups of 8 heads run two to one).
   const int64_t per_wg = pa::decode_sub_groups(group) / pa::decode_workgroups_per_head(dtype, head_dim, group);
   const int heads = pa::decode_unit_heads(dtype, head_dim, static_cast<int>(hkv), group);
-  const double total_us = static_cast<double>(tokens) * 4.0 * head_dim * static_cast<double>(hkv) / kHbmBytesPerUs;
+  const double total_us = static_cast<double>(tokens) * head_dim * static_cast<double>(hkv) *
+                          (codes ? 2.0 / kHbmBytesPerUs8 : 4.0 / kHbmBytesPerUs);
   int64_t best = kMinPartition;
   double best_us = -1.0;
   for (int64_t part = kMinPartition; part <= kMaxPartition; part *= 2) {

@@ -23,13 +23,6 @@ namespace pa {
 
 constexpr int kRotateThreads = 256;
 
-// n / d, with rcp = (2^32 - 1) / d: the product's high half is the quotient or
-// one less.
-__device__ __forceinline__ uint32_t div_by(uint32_t n, uint32_t d, uint32_t rcp) {
-  const uint32_t q = __umulhi(n, rcp);
-  return n - q * d >= d ? q + 1 : q;
-}
-
 // Four elements at p as floats, and back (rounded to nearest even).
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, float* x) {
@@ -210,7 +203,7 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs a) {
   constexpr int kRows = kRotateThreads / L;
   const uint32_t heads = a.num_query_heads + (a.key_cache != nullptr ? 2 : 1) * a.num_kv_heads;
   const uint32_t id = blockIdx.x * kRows + threadIdx.x / L;
-  const uint32_t tok = div_by(id, heads, a.heads_rcp);
+  const uint32_t tok = quotient(id, heads, a.heads_rcp);
   if (tok >= static_cast<uint32_t>(a.num_tokens)) return;
   const int64_t t = tok;
   int h = static_cast<int>(id - tok * heads);
@@ -265,7 +258,7 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
   float x[kN];
   if (blockIdx.x >= a.kv_groups) {
     const uint32_t id = (blockIdx.x - a.kv_groups) * C + group;
-    const uint32_t tok = div_by(id, a.num_query_heads, a.heads_rcp);
+    const uint32_t tok = quotient(id, a.num_query_heads, a.heads_rcp);
     if (tok >= static_cast<uint32_t>(a.num_tokens)) return;
     const int64_t t = tok;
     const int h = static_cast<int>(id - tok * a.num_query_heads);
@@ -285,7 +278,7 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
   __shared__ int16_t s_run[C + kMaxCache8Block];
 
   const uint32_t units = 2 * a.num_kv_heads;
-  const uint32_t chunk = div_by(blockIdx.x, units, a.kv_rcp);
+  const uint32_t chunk = quotient(blockIdx.x, units, a.kv_rcp);
   const int u = static_cast<int>(blockIdx.x - chunk * units);
   const bool is_v = u >= a.num_kv_heads;
   const int h = is_v ? u - a.num_kv_heads : u;

@@ -69,11 +69,12 @@ def rotated(x, weight, positions, cos_sin, eps, interleaved):
 
 def attention(q, keys, vals, table, starts, counts, scale):
     """Causal attention of each sequence's new tokens over its blocks in fp64:
-    the result and the weighted mean of |v| beside it.  Positions whose block
-    is missing are skipped; a row that attends nothing is zero."""
+    the result, the weighted mean of |v| beside it, and the largest weight times
+    the sum of |v|.  Positions whose block is missing are skipped; a row that
+    attends nothing is zero."""
     total, bs, hkv, dim = keys.shape
     group = q.shape[1] // hkv
-    out, size = [], []
+    out, size, peak = [], [], []
     at = 0
     for row, start, count in zip(table, starts, counts):
         end = start + count
@@ -90,5 +91,7 @@ def attention(q, keys, vals, table, starts, counts, scale):
         w = torch.nan_to_num(torch.softmax(w.masked_fill(later, -float("inf")), dim=-1)) if p.numel() else w
         out.append(torch.matmul(w, v).transpose(0, 1))
         size.append(torch.matmul(w, v.abs()).transpose(0, 1))
+        most = w.amax(-1, keepdim=True) if p.numel() else w.sum(-1, keepdim=True)
+        peak.append(torch.matmul((w > 0).double() * most, v.abs()).transpose(0, 1))
         at += count
-    return torch.cat(out), torch.cat(size)
+    return torch.cat(out), torch.cat(size), torch.cat(peak)

@@ -202,18 +202,22 @@ def attend(heads, kv_heads, dim, bs, starts, counts, dtype, device, partition=No
     out = torch.full((q.shape[0], heads, dim), 77.0, dtype=dtype, device=device)
     ops.attention(q.to(device), dev[0], dev[1], 0, step, scale, out=out, key_scales=dev[2], value_scales=dev[3])
     vals = [oracle.values(c[0], torch.nan_to_num(s[0])) for c, s in zip(codes, scales)]
-    ref, size = oracle.attention(q, *vals, table, starts, counts, scale)
+    ref, size, peak = oracle.attention(q, *vals, table, starts, counts, scale)
     out = out.cpu().double()
     assert torch.isfinite(out).all()
     # One rounding of the result (u); a probability enters its product rounded
     # to the query's type, by u of itself at most, in the sum as in the
     # product (prefill) or one of the two (2 u in all; the decode takes two
     # terms, u^2); scores and sums in fp32, 1.5e-5 of a probability.  fp16's
-    # steps below 2^-14 are 2^-24, of V and of the result.
+    # steps below 2^-14 are 2^-24: of V, of the result, and of probabilities,
+    # which count there from 2^14 (decode) or 2^6 (prefill) at the row's largest,
+    # so that one is off by 2^-25 / 2^6 of the largest at most.
     u = oracle.ROW_EPS[dtype]
     several = torch.from_numpy(np.repeat(np.asarray(counts) > 1, counts))[:, None, None]
     each = torch.where(several, torch.tensor(2 * u), torch.tensor(u * u)) + 1.5e-5
-    bound = (1 + 2 * u) * u * ref.abs() + each * size + (2.0**-24 if dtype == torch.float16 else 0)
+    bound = (1 + 2 * u) * u * ref.abs() + each * size
+    if dtype == torch.float16:
+        bound = bound + 2.0**-24 + 2.0**-31 * peak
     excess = ((out - ref).abs() - bound).max().item()
     assert excess <= 0, f"{excess:.3e} over the bound"
 
@@ -300,7 +304,7 @@ def test_steps_of_a_sequence(device):
                                   query_weight=w, key_weight=w, key_scales=mine[2], value_scales=mine[3])
         out = ops.attention(rq, mine[0], mine[1], 1, step, dim**-0.5, key_scales=mine[2], value_scales=mine[3])
         same(mine, want, 1)
-        ref, size = oracle.attention(rq.cpu(), oracle.values(want[0], want[1]), oracle.values(want[2], want[3]), table,
+        ref, size, _ = oracle.attention(rq.cpu(), oracle.values(want[0], want[1]), oracle.values(want[2], want[3]), table,
                                      starts, counts, dim**-0.5)
         u = 2.0**-8
         assert ((out.cpu().double() - ref).abs() <= 1.01 * u * ref.abs() + (2 * u + 1.5e-5) * size).all()
@@ -323,6 +327,11 @@ def test_phases_streams_and_graphs(device):
     out = torch.full_like(want, 7.0)
     ops.decode(q, kc, vc, 0, step, 0.1, out=out, **args)
     assert torch.equal(out[:3], want[:3]) and bool((out[3:] == 7).all())
+    ops.decode(q, kc, vc, 0, step, 0.1, out=out, phases=1, **args)
+    out[:3] = 5
+    ops.decode(q, kc, vc, 0, step, 0.1, out=out, phases=2, **args)
+    multi = [0, 2]  # one-partition rows belong to the first phase
+    assert torch.equal(out[multi], want[multi])
     out = torch.full_like(want, 7.0)
     ops.prefill(q, kc, vc, 0, step, 0.1, out=out, **args)
     assert torch.equal(out[3:], want[3:]) and bool((out[:3] == 7).all())
