@@ -721,10 +721,10 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
   const int eb = elem_bytes(dims.dtype);
   const int cache_eb = scales != nullptr ? 1 : eb;
   const bool fast =
-      scales == nullptr &&
       pa::prefill_fast_path_supported(dims.dtype, dims.head_dim, group, dims.block_size) &&
+      (scales == nullptr || pa::prefill_codes_supported(dims.dtype, dims.head_dim)) &&
       prefill_tile == pa::prefill_tile_for(group) && dims.max_blocks_per_seq > 0 &&
-      static_cast<int64_t>(dims.block_size) * dims.num_kv_heads * dims.head_dim * eb <= 0xffffffffLL &&
+      static_cast<int64_t>(dims.block_size) * dims.num_kv_heads * dims.head_dim * cache_eb <= 0xffffffffLL &&
       aligned16(query) && aligned16(key_cache) &&
       aligned16(value_cache) && aligned16(output) && (dims.q_token_stride * eb) % 16 == 0 &&
       (dims.q_head_stride * eb) % 16 == 0;
@@ -770,6 +770,10 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
       a.new_key_head_stride = new_rows->key_head_stride;
       a.new_value_token_stride = new_rows->value_token_stride;
       a.new_value_head_stride = new_rows->value_head_stride;
+    }
+    if (scales != nullptr) {
+      a.key_scales = layer_scales(scales->key, dims, layer_idx);
+      a.value_scales = layer_scales(scales->value, dims, layer_idx);
     }
     return from_hip(pa::launch_prefill(a, dims.dtype, dims.head_dim, group, num_prefill_items, s), who);
   }

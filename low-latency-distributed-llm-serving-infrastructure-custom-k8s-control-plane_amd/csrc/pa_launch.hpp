@@ -259,6 +259,9 @@ struct PrefillArgs {
   int64_t new_key_head_stride;
   int64_t new_value_token_stride;
   int64_t new_value_head_stride;
+  // 8-bit caches (else null): base of the layer, [blocks, H_kv].
+  const float* key_scales;
+  const float* value_scales;
 };
 
 bool decode_fast_path_supported(int dtype, int head_dim, int group, int block_size,
@@ -294,6 +297,8 @@ hipError_t launch_copy_blocks(const CopyBlocksArgs& a, bool vec16, hipStream_t s
 bool prefill_fast_path_supported(int dtype, int head_dim, int group, int block_size);
 // Whether the fast path of this shape also takes new rows (PrefillArgs::new_key).
 bool prefill_append_supported(int dtype, int head_dim);
+// Whether the fast path of this shape also reads an 8-bit cache.
+bool prefill_codes_supported(int dtype, int head_dim);
 // Compute units of the current device (cached per device; 0 if unknown): the
 // width of the persistent prefill launches.
 int device_compute_units();

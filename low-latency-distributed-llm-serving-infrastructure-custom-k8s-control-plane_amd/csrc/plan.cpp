@@ -147,8 +147,8 @@ int64_t choose_partition_mfma(const DecodeContexts& d, const PaPlanParams& p, in
   // Units that one workgroup serves (sub-groups of 8 heads run two to one).
   const int64_t per_wg = pa::decode_sub_groups(group) / pa::decode_workgroups_per_head(dtype, head_dim, group);
   const int heads = pa::decode_unit_heads(dtype, head_dim, static_cast<int>(hkv), group);
-  const double total_us = static_cast<double>(tokens) * head_dim * static_cast<double>(hkv) *
-                          (codes ? 2.0 / kHbmBytesPerUs8 : 4.0 / kHbmBytesPerUs);
+  const double total_us = static_cast<double>(tokens) * (codes ? 2.0 : 4.0) * head_dim * static_cast<double>(hkv) /
+                          (codes ? kHbmBytesPerUs8 : kHbmBytesPerUs);
   int64_t best = kMinPartition;
   double best_us = -1.0;
   for (int64_t part = kMinPartition; part <= kMaxPartition; part *= 2) {

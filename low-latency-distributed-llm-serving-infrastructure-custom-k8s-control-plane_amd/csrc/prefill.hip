@@ -64,6 +64,16 @@
 // rescaled only when some row's maximum grew by more than 2^8 over the
 // reference maximum in use.
 //
+// CODES (the 8-bit cache): the rings hold 16-bit rows as above, so everything
+// after them is the same; only the copies differ.  A thread takes one 16-byte
+// piece (16 codes) of one row of K and of V a stage, converts it on its way
+// (v_cvt_scalef32_pk_*_fp8, the block's scale in the same instruction) and
+// writes two chunks.  The pieces are loaded two steps before the step that
+// writes them, into registers of that step's parity: K of stage st+5 and V of
+// st+3 go out in step st, which writes K of st+3 and V of st+1; the block id
+// comes one step earlier still.  All eight waves share the conversions (16 a
+// thread and step, against its 16 exponentials).
+//
 // Reference: the block-diagonal causal mask of app/model/paged_attention.py:
 // 92-118 applied by SDPA (paged_attention.py:170-178); query token j of a
 // sequence at position start + j attends context positions [0, start + j].
@@ -71,6 +81,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "cache8.hpp"
 #include "pa_common.hpp"
 #include "pa_launch.hpp"
 #include "prefill_common.hpp"
@@ -99,12 +110,13 @@ constexpr int kIdAhead = 8;      // stages between an id slot's copy and the sta
 // the rings into the cache (the rings then hold the last four stages, which
 // cover the tile's at most 128 tokens), so no unit reads a row another one
 // writes.
-template <typename T, int D, int DM, bool LANE_IDS, bool APPEND>
+template <typename T, int D, int DM, bool LANE_IDS, bool APPEND, bool CODES = false>
 __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a) {
-  static_assert(Elem<T>::kBytes == 2, "16-bit caches (bf16 or fp16)");
+  static_assert(Elem<T>::kBytes == 2, "16-bit rows (bf16 or fp16)");
+  static_assert(!CODES || (!LANE_IDS && !APPEND), "8-bit copies take any block size; their rows are written before");
   static_assert(DM <= D && DM % 16 == 0, "memory head dim: a multiple of 16 up to D");
   constexpr bool MASKD = DM < D;
-  constexpr int MEM_ROW = DM * 2;         // bytes of a head's row in memory
+  constexpr int MEM_ROW = CODES ? DM : DM * 2;  // bytes of a head's row in the cache
   constexpr int KS = D / 16;              // MFMA k-steps of QK^T
   constexpr int DB = D / 32;              // 32-wide d blocks of the output
   constexpr int CHUNKS = D / 8;           // 16-byte pieces per row
@@ -242,6 +254,21 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
     return r;
   };
   auto tile_max = [&](const f32x16& s) {
+    if constexpr (CODES) {
+      // The compiler keeps a vector instruction that reads a product's result
+      // the product's latency behind it, but does not look into assembly (in
+      // the other instances 60 and more instructions lie between, here a
+      // v_max3 came right after): so each of these depends on one of its own.
+      const float ready = __builtin_amdgcn_fmed3f(s[15], s[15], s[15]);
+      auto first3 = [&](float x, float y, float z) {
+        float r;
+        asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z), "v"(ready));
+        return r;
+      };
+      const float a0 = first3(s[0], s[1], s[2]), a1 = first3(s[3], s[4], s[5]), a2 = first3(s[6], s[7], s[8]);
+      const float a3 = first3(s[9], s[10], s[11]), a4 = first3(s[12], s[13], s[14]);
+      return max_halves(max3(max3(a0, a1, a2), max3(a3, a4, ready), ready));
+    }
     const float a0 = max3(s[0], s[1], s[2]), a1 = max3(s[3], s[4], s[5]), a2 = max3(s[6], s[7], s[8]);
     const float a3 = max3(s[9], s[10], s[11]), a4 = max3(s[12], s[13], s[14]);
     const float b0 = max3(a0, a1, a2), b1 = max3(a3, a4, s[15]);
@@ -511,6 +538,43 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
       float m = kScoreFloor, l = 0.f;  // l: this lane's half of the row sum
+
+      // ---- copies of 8-bit rows ------------------------------------------------
+      // This thread's piece: codes [16 c8, 16 c8 + 16) of row r8 of a stage.
+      constexpr int kPieces8 = D / 16;
+      [[maybe_unused]] uint4 kr8[2], vr8[2];      // pieces in flight, by the parity of the step that loads them
+      [[maybe_unused]] float ks8[2], vs8[2];      // their scales
+      [[maybe_unused]] uint32_t id8[4] = {0, 0, 0, 0};  // block of the row in stage x, at x % 4
+      [[maybe_unused]] uint32_t first8[3] = {0, 0, 0};  // ... and in stages 0-2
+      int tid8 = tid;
+      if constexpr (CODES) asm volatile("" : "+v"(tid8));  // (kept inside the unit loop)
+      const int r8 = tid8 / kPieces8, c8 = tid8 % kPieces8;
+      const bool on8 = CODES && r8 < kStage && (!MASKD || c8 * 16 < DM);
+      auto pos8 = [&](int x) { return min(x * kStage + r8, kv_last); };
+      auto load_id8 = [&](int x) { return on8 ? static_cast<uint32_t>(btg[pos8(x) >> log2_bs]) : 0u; };
+      // (rows of a block outside the pool are zeros: a NaN there would reach the
+      // product, whose weight of zero it outlives)
+      auto load8 = [&](int x, uint32_t b, const char* base, const float* scales, uint4& piece, float& sc) {
+        piece = make_uint4(0, 0, 0, 0);
+        sc = 1.f;
+        if (on8 && b < static_cast<uint32_t>(a.total_blocks)) {
+          piece = ld16(base + (static_cast<uint64_t>(b) * block_bytes +
+                               static_cast<uint32_t>(pos8(x) & bs_mask) * row_bytes + c8 * 16));
+          sc = scales[static_cast<int64_t>(b) * hkv + kvh];
+        }
+      };
+      auto write8 = [&](uint32_t region, const uint4& piece, float sc) {
+        if (on8) {
+          char* row = s_lds + region + r8 * ROW_BYTES;
+          const int sw = chunk_swizzle<CHUNKS>(r8);
+          st16(row + (((2 * c8) ^ sw) * 16),
+               make_uint4(codes_to_half2<T, false>(piece.x, sc), codes_to_half2<T, true>(piece.x, sc),
+                          codes_to_half2<T, false>(piece.y, sc), codes_to_half2<T, true>(piece.y, sc)));
+          st16(row + (((2 * c8 + 1) ^ sw) * 16),
+               make_uint4(codes_to_half2<T, false>(piece.z, sc), codes_to_half2<T, true>(piece.z, sc),
+                          codes_to_half2<T, false>(piece.w, sc), codes_to_half2<T, true>(piece.w, sc)));
+        }
+      };
       // Lazy rescale: the reference maximum m of a row moves only when a tile's
       // maximum exceeds it by more than kLazyRescale (log2 units), so
       // p <= 2^kLazyRescale; l and acc use the same m, and the result is the
@@ -568,7 +632,24 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
           qtok += kRowsPerDma;
           if (qtok >= MTOK) { qtok -= MTOK; ++qg; }
         }
-        if (wave == 0) {
+        if constexpr (CODES) {
+          // Stages 0-2 of K and 0 of V, through registers to LDS.
+#pragma unroll
+          for (int x = 0; x < 3; ++x) first8[x] = load_id8(x);
+#pragma unroll
+          for (int x = 3; x < 6; ++x) id8[x % 4] = load_id8(x);
+          uint4 piece[4];
+          float sc[4];
+#pragma unroll
+          for (int x = 0; x < 3; ++x)
+            if (x < nstages) load8(x, first8[x], kbase, a.key_scales, piece[x], sc[x]);
+          load8(0, first8[0], vbase, a.value_scales, piece[3], sc[3]);
+#pragma unroll
+          for (int x = 0; x < 3; ++x)
+            if (x < nstages) write8(x * kRegion, piece[x], sc[x]);
+          write8(kVBase, piece[3], sc[3]);
+        }
+        if (!CODES && wave == 0) {
 #pragma unroll
           for (int x = 0; x < kIdAhead; ++x)
             if (x < nstages) dma_ids(x);
@@ -578,7 +659,7 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
           wait_vmcnt<0>();
           __syncthreads();
         }
-        if (wave < kCopyWaves) {
+        if (!CODES && wave < kCopyWaves) {
           // The block of this wave's rows in each of stages 0-3, all loaded
           // before the first copy (one round trip, not one per copy).
           int pid[4];
@@ -595,6 +676,13 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
         }
       }
       __syncthreads();  // the query tile, K of stage 0 and the id ring
+      if constexpr (CODES) {
+        // What steps 0 and 1 write.
+        if (nstages > 3) load8(3, id8[3], kbase, a.key_scales, kr8[0], ks8[0]);
+        if (nstages > 1) load8(1, first8[1], vbase, a.value_scales, vr8[0], vs8[0]);
+        if (nstages > 4) load8(4, id8[0], kbase, a.key_scales, kr8[1], ks8[1]);
+        if (nstages > 2) load8(2, first8[2], vbase, a.value_scales, vr8[1], vs8[1]);
+      }
       f32x16 s0, s1;
       uint4 ka[KS];
 #pragma unroll
@@ -608,20 +696,20 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
       int bad_local = static_cast<uint32_t>(scan0) >= static_cast<uint32_t>(a.total_blocks) ? 1 : 0;
       for (int c = tid + kPrefillThreads; c < ncols; c += kPrefillThreads)
         bad_local |= static_cast<uint32_t>(btg[c]) >= static_cast<uint32_t>(a.total_blocks) ? 1 : 0;
-      wait_vmcnt<0>();
+      if constexpr (!CODES) wait_vmcnt<0>();
       // (also publishes K of stages 1-2 and V of stage 0, and tells that every
       // wave has read K of stage 0 before step 0 refills its slot)
       bad_ids = __syncthreads_or(bad_local) != 0;
       // Tiles below this index need no mask for any row of the unit.
       const int first_masked = bad_ids ? 0 : min(start + tok0 + 1, kv_read) / kKvTile;
-      if (wave < kCopyWaves) {
+      if (!CODES && wave < kCopyWaves) {
         if (nstages > 3) copy_step(3, 3 * kRegion, kbase, nkbase, nkstride, ring_fast(3), ring_ids(3));
         if (nstages > 1) copy_step(1, kVBase + kRegion, vbase, nvbase, nvstride, ring_fast(1), ring_ids(1));
       }
       // Ids of step 0's copies (K of stage 4, V of stage 2), from the ring.
       int idk = 0, idv = 0;
       auto prefetch_ids = [&](int st) {
-        if (wave < kCopyWaves) {
+        if (!CODES && wave < kCopyWaves) {
           idk = ring_fast(st + 4);
           idv = ring_fast(st + 2);
         }
@@ -642,13 +730,23 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
         // Copies of this step: K of stage st+4, V of stage st+2 and (wave 0)
         // the id slot of stage st+8, each only if that stage exists.
         const bool cpk = st + 4 < nstages, cpv = st + 2 < nstages, cpi = st + kIdAhead < nstages;
-        if (wave < kCopyWaves && cpk)
+        if constexpr (CODES) {
+          constexpr int P = SLOT & 1;
+          if (st + 3 < nstages) write8(((SLOT + 3) & 3) * kRegion, kr8[P], ks8[P]);
+          if (st + 1 < nstages) write8(kVBase + ((SLOT + 1) & 3) * kRegion, vr8[P], vs8[P]);
+          if (st + 5 < nstages) load8(st + 5, id8[(SLOT + 5) & 3], kbase, a.key_scales, kr8[P], ks8[P]);
+          if (st + 3 < nstages) load8(st + 3, id8[(SLOT + 3) & 3], vbase, a.value_scales, vr8[P], vs8[P]);
+          if (st + 6 < nstages) id8[(SLOT + 6) & 3] = load_id8(st + 6);
+        }
+        if (!CODES && wave < kCopyWaves && cpk)
           copy_step(st + 4, slot * kRegion, kbase, nkbase, nkstride, idk, ring_ids(st + 4));
         const int idv_cur = idv;  // (the prefetch below replaces idv)
         if (bad_ids) mask_bad(2 * st + kh, s_cur);
 
         // ---- A: S_next = K_next Q^T | P = exp2(S - m) | V^T reads
-        const float msc = m * scale;
+        // (fp16 over 8-bit rows: probabilities, of up to 2^8, times 2^6, in the
+        // sums as well, which keeps small ones out of fp16's subnormals)
+        const float msc = CODES && Elem<T>::kDtype == PA_DTYPE_F16 ? fmaf(m, scale, -6.f) : m * scale;
         f32x16 sn;
 #pragma unroll
         for (int i = 0; i < 16; ++i) sn[i] = 0.f;
@@ -700,18 +798,20 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
         s_nxt = sn;
         // The V copies and the id slot go out after the math, so that a copying
         // wave issues its copies in two short runs rather than one long one.
-        if (wave < kCopyWaves && cpv)
+        if (!CODES && wave < kCopyWaves && cpv)
           copy_step(st + 2, kVBase + ((slot + 2) & (kKBufs - 1)) * kRegion, vbase, nvbase, nvstride, idv_cur,
                     ring_ids(st + 2));
-        if (wave == 0 && cpi) dma_ids(st + kIdAhead);
+        if (!CODES && wave == 0 && cpi) dma_ids(st + kIdAhead);
         // K of stage st+3, V of stage st+1 and (wave 0) the id slot of stage
         // st+7, copied last step, must have landed before the barrier
         // publishes them; this step's copies may stay in flight (copies
         // complete in issue order, so their count is the wait).
-        if (wave < kCopyWaves) {
+        if (!CODES && wave < kCopyWaves) {
           const int n = (cpk ? kDmaPerWave : 0) + (cpv ? kDmaPerWave : 0) + (wave == 0 && cpi ? 1 : 0);
           wait_vmcnt_at_most<2 * kDmaPerWave + 1>(n);
         }
+        // (8-bit rows: this step's LDS writes)
+        if constexpr (CODES) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         stage_barrier();
       };
 
@@ -906,6 +1006,11 @@ bool prefill_append_supported(int dtype, int head_dim) {
          (head_dim == 64 || head_dim == 80 || head_dim == 96 || head_dim == 128);
 }
 
+bool prefill_codes_supported(int dtype, int head_dim) {
+  // The kernel of this file.
+  return (dtype == PA_DTYPE_BF16 || dtype == PA_DTYPE_F16) && head_dim <= 128;
+}
+
 // Query tokens per work item: 128 rows over the heads of one workgroup (a
 // sub-group of at most 8 when the group is larger).
 int prefill_tile_for(int group) {
@@ -939,6 +1044,11 @@ static hipError_t launch_prefill_d(const PrefillArgs& args, int group, int64_t n
   const int cus = device_compute_units();
   const int64_t wgs = cus > 0 ? std::min<int64_t>(a.num_units, cus) : a.num_units;
   const dim3 grid(static_cast<uint32_t>(wgs));
+  if (a.key_scales != nullptr) {
+    if constexpr (!APPEND)
+      hipLaunchKernelGGL((prefill_kernel<T, D, DM, false, false, true>), grid, dim3(kPrefillThreads), 0, s, a);
+    return APPEND ? hipErrorNotSupported : hipGetLastError();
+  }
   // A copying wave's 16 rows of a stage share one block from blocks of 16
   // up; smaller blocks take the per-lane copy addresses (ids read per lane
   // from the ring), which beat one scalar base per copy with its id read
