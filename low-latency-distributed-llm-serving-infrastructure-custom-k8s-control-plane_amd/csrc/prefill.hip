@@ -772,6 +772,11 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
             rsum1 = dot2_half<T>(pb[c].w, kOnes, rsum1);
           }
         }
+        // (8-bit rows: the conversions ahead of A leave the scheduler one region
+        // for both phases, in which it drew the maxima of S_next up against its
+        // last product and waited: 2048 tokens at 6000, 32/8 heads of 128, 298
+        // -> 285 us; four chunks of 512 at 4096, 16/4 of 96, 107 -> 99.)
+        if constexpr (CODES) __builtin_amdgcn_sched_barrier(0);
         // ---- B: O^T += V^T P^T | row maxima of S_next | K reads of stage st+2
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
