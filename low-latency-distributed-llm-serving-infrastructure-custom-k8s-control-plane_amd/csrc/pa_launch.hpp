@@ -208,6 +208,7 @@ struct RotateArgs {
   uint32_t heads_rcp;
   uint32_t kv_rcp;
   uint32_t kv_groups;
+  int32_t log2_block;  // of the block size, -1 if it is no power of two
 };
 
 // KV block copy (copy_blocks).

@@ -13,8 +13,14 @@
 // its sum of squares is a few DPP additions, a lane holds both elements of its
 // pairs, and the cosines and sines a lane needs are one 16-byte load each.
 //
-// What bounds it is memory once a step has some thousand rows, and before that
-// the launch and two dependent reads (position, then table).
+// What bounds it is memory once a step has some ten thousand rows, and before
+// that the launch and two dependent reads (position, then table).  bf16 rows,
+// cold caches: 8 tokens of 32/8 heads of 128 2.4 us; 2176 tokens with norms
+// (54.6 MB) 17.6 us, 3.1 TB/s; 4096 tokens 28.9 us, 3.5 TB/s.  The 8-bit write:
+// 256 decode tokens 6.0 us; 1400 tokens of 32/32 heads of 128, fp16 with norms
+// (58 MB) 28 us; 15000 tokens of 9/3 heads of 64 (75 MB) 27 us, 2.8 TB/s: there
+// each chunk reads the rows that may belong to its last run, which the next one
+// reads again, and waits for slots, rows and scales one after the other.
 #include "cache8.hpp"
 #include "pa_common.hpp"
 #include "pa_launch.hpp"
@@ -23,23 +29,31 @@ namespace pa {
 
 constexpr int kRotateThreads = 256;
 
-// Four elements at p as floats, and back (rounded to nearest even).
+// Four elements in memory, as floats, and back (rounded to nearest even).
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, float* x) {
+struct Four {
+  using type = uint2;
+};
+template <>
+struct Four<float> {
+  using type = float4;
+};
+template <typename T>
+__device__ __forceinline__ typename Four<T>::type load4(const T* p) {
+  return *reinterpret_cast<const typename Four<T>::type*>(p);
+}
+template <typename T>
+__device__ __forceinline__ void unpack4(typename Four<T>::type v, float* x) {
   if constexpr (sizeof(T) == 4) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
     x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
   } else {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
     x[0] = half_lo<T>(v.x), x[1] = half_hi<T>(v.x), x[2] = half_lo<T>(v.y), x[3] = half_hi<T>(v.y);
   }
 }
 template <typename T>
-__device__ __forceinline__ void store4(T* p, const float* x) {
-  if constexpr (sizeof(T) == 4)
-    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-  else
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_half2<T>(x[0], x[1]), pack_half2<T>(x[2], x[3]));
+__device__ __forceinline__ typename Four<T>::type pack4(const float* x) {
+  if constexpr (sizeof(T) == 4) return make_float4(x[0], x[1], x[2], x[3]);
+  else return make_uint2(pack_half2<T>(x[0], x[1]), pack_half2<T>(x[2], x[3]));
 }
 // x as its type holds it.
 template <typename T>
@@ -69,11 +83,16 @@ __device__ __forceinline__ float row_max(float x) {
 
 // What a lane of a row's group does with its row.  VEC: 8 elements, in two
 // runs of 4 at `a` and `b` (the two halves of its pairs, or 8 in a row);
-// needs D and R in multiples of 8 and rows at multiples of 4 elements.  Else
-// elements lane + 64 e, each with its partner read again; any D up to 256.
+// needs D and R in multiples of 8 and rows at multiples of 4 elements.  Lanes
+// past the row load its first pieces, so that no load waits behind a branch.
+// Else elements lane + 64 e, each with its partner read again; any D up to 256.
 template <typename T, int L, bool VEC>
 struct RowLane {
   static constexpr int kN = VEC ? 8 : 4;
+  using Piece = typename Four<T>::type;
+  struct Raw {
+    Piece lo, hi;  // VEC: as they are in memory
+  };
   const RotateArgs& args;
   int lane;  // in the row's group
   int a, b;  // VEC
@@ -81,25 +100,32 @@ struct RowLane {
 
   __device__ __forceinline__ RowLane(const RotateArgs& r, int l) : args(r), lane(l) {
     if constexpr (VEC) {
-      const int pairs = r.rotary_dim / 8;  // lanes that rotate
-      turns = l < pairs;
+      turns = 8 * l < r.rotary_dim;
       live = 8 * l < r.head_dim;
       const bool halves = turns && !r.interleaved;
       a = halves ? 4 * l : 8 * l;
       b = halves ? r.rotary_dim / 2 + 4 * l : 8 * l + 4;
+      if (!live) a = b = 0;
     } else {
       turns = live = true;
       a = b = 0;
     }
   }
-  __device__ __forceinline__ void load(const T* row, float* x) const {
+  __device__ __forceinline__ Raw load_raw(const T* row) const {
+    Raw v{};
     if constexpr (VEC) {
+      v.lo = load4<T>(row + a);
+      v.hi = load4<T>(row + b);
+    }
+    return v;
+  }
+  // The row as floats (zeros past its end).
+  __device__ __forceinline__ void unpack(const Raw& v, const T* row, float* x) const {
+    if constexpr (VEC) {
+      unpack4<T>(v.lo, x);
+      unpack4<T>(v.hi, x + 4);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.f;
-      if (live) {
-        load4<T>(row + a, x);
-        load4<T>(row + b, x + 4);
-      }
+      for (int i = 0; i < 8; ++i) x[i] = live ? x[i] : 0.f;
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -108,11 +134,17 @@ struct RowLane {
       }
     }
   }
-  __device__ __forceinline__ void store(T* row, const float* x) const {
+  // Stores x, or (`copy`) the raw row.
+  __device__ __forceinline__ void store(T* row, const float* x, const Raw& v, bool copy) const {
     if constexpr (VEC) {
+      Piece lo = pack4<T>(x), hi = pack4<T>(x + 4);
+      if (copy) {
+        lo = v.lo;
+        hi = v.hi;
+      }
       if (live) {
-        store4<T>(row + a, x);
-        store4<T>(row + b, x + 4);
+        *reinterpret_cast<Piece*>(row + a) = lo;
+        *reinterpret_cast<Piece*>(row + b) = hi;
       }
     } else {
 #pragma unroll
@@ -123,117 +155,176 @@ struct RowLane {
   __device__ __forceinline__ float weight(const void* w, int d) const {
     return args.weight_f32 ? static_cast<const float*>(w)[d] : load_scalar<T>(static_cast<const T*>(w) + d);
   }
-  // Normalise (w not null) and rotate the row x holds.
-  // (No contraction but the fmaf written here: the kernels below give the
-  // same bits.)
-  __device__ __forceinline__ void apply(const T* row, float* x, const void* w, int64_t pos) const {
-#pragma clang fp contract(off)
-    float r = 1.f;
-    if (w != nullptr) {
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < kN; ++i) ss = fmaf(x[i], x[i], ss);
-      r = rsqrtf(row_sum<L>(ss) / static_cast<float>(args.head_dim) + args.eps);
+  // VEC: the lane's cosines and sines at a position of the table.
+  __device__ __forceinline__ void angles(int64_t pos, float4* c, float4* s) const {
+    *c = *s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (args.rotary_dim > 0) {
+      const float* cs = args.cos_sin + pos * args.rotary_dim + (turns ? 4 * lane : 0);
+      *c = *reinterpret_cast<const float4*>(cs);
+      *s = *reinterpret_cast<const float4*>(cs + args.rotary_dim / 2);
     }
+  }
+  // VEC: the lane's norm weights.
+  __device__ __forceinline__ void weights(const void* w, float* g) const {
+    if (args.weight_f32) {
+      unpack4<float>(load4<float>(static_cast<const float*>(w) + a), g);
+      unpack4<float>(load4<float>(static_cast<const float*>(w) + b), g + 4);
+    } else {
+      unpack4<T>(load4<T>(static_cast<const T*>(w) + a), g);
+      unpack4<T>(load4<T>(static_cast<const T*>(w) + b), g + 4);
+    }
+  }
+  // The norm's factor of the row x holds.  (No contraction but the fmaf
+  // written here, in these three: the kernels below give the same bits.)
+  __device__ __forceinline__ float norm(const float* x) const {
+#pragma clang fp contract(off)
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) ss = fmaf(x[i], x[i], ss);
+    return rsqrtf(row_sum<L>(ss) / static_cast<float>(args.head_dim) + args.eps);
+  }
+  // VEC: normalise (`normed`, with the weights g) and rotate the row x holds.
+  __device__ __forceinline__ void apply(float* x, bool normed, const float* g, const float4& c4, const float4& s4) const {
+#pragma clang fp contract(off)
+    if (normed) {
+      const float r = norm(x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = x[i] * r * g[i];
+    }
+    if (turns) {
+      auto turn = [](float& p, float& q, float c, float s) {
+        const float u = p, v = q;
+        p = fmaf(u, c, -(v * s));
+        q = fmaf(v, c, u * s);
+      };
+      if (args.interleaved) {
+        turn(x[0], x[1], c4.x, s4.x);
+        turn(x[2], x[3], c4.y, s4.y);
+        turn(x[4], x[5], c4.z, s4.z);
+        turn(x[6], x[7], c4.w, s4.w);
+      } else {
+        turn(x[0], x[4], c4.x, s4.x);
+        turn(x[1], x[5], c4.y, s4.y);
+        turn(x[2], x[6], c4.z, s4.z);
+        turn(x[3], x[7], c4.w, s4.w);
+      }
+    }
+  }
+  // Not VEC: the same, each partner read again from the row.
+  __device__ __forceinline__ void apply_any(const T* row, float* x, const void* w, int64_t pos) const {
+#pragma clang fp contract(off)
+    const float r = w != nullptr ? norm(x) : 1.f;
     const int rot = args.rotary_dim;
     const float* cs = args.cos_sin + pos * rot;  // (not read without rotation)
-    if constexpr (VEC) {
-      if (w != nullptr && live) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = x[i] * r * weight(w, a + i);
-          x[4 + i] = x[4 + i] * r * weight(w, b + i);
-        }
+    for (int e = 0; e < 4; ++e) {
+      const int d = lane + 64 * e;
+      if (d >= args.head_dim) continue;
+      float u = x[e];
+      if (w != nullptr) u = u * r * weight(w, d);
+      if (d < rot) {
+        const bool second = args.interleaved ? d & 1 : d >= rot / 2;
+        const int o = args.interleaved ? d ^ 1 : second ? d - rot / 2 : d + rot / 2;
+        const int k = args.interleaved ? d / 2 : second ? o : d;
+        float v = load_scalar<T>(row + o);
+        if (w != nullptr) v = v * r * weight(w, o);
+        const float vs = v * cs[rot / 2 + k];
+        u = fmaf(u, cs[k], second ? vs : -vs);
       }
-      if (turns && rot > 0) {
-        const float4 c4 = *reinterpret_cast<const float4*>(cs + 4 * lane);
-        const float4 s4 = *reinterpret_cast<const float4*>(cs + rot / 2 + 4 * lane);
-        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float& p = args.interleaved ? x[2 * i] : x[i];
-          float& q = args.interleaved ? x[2 * i + 1] : x[4 + i];
-          const float u = p, v = q;
-          p = fmaf(u, c[i], -(v * s[i]));
-          q = fmaf(v, c[i], u * s[i]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = lane + 64 * e;
-        if (d >= args.head_dim) continue;
-        float u = x[e];
-        if (w != nullptr) u = u * r * weight(w, d);
-        if (d < rot) {
-          const bool second = args.interleaved ? d & 1 : d >= rot / 2;
-          const int o = args.interleaved ? d ^ 1 : second ? d - rot / 2 : d + rot / 2;
-          const int k = args.interleaved ? d / 2 : second ? o : d;
-          float v = load_scalar<T>(row + o);
-          if (w != nullptr) v = v * r * weight(w, o);
-          const float vs = v * cs[rot / 2 + k];
-          u = fmaf(u, cs[k], second ? vs : -vs);
-        }
-        x[e] = u;
-      }
+      x[e] = u;
     }
+  }
+  __device__ __forceinline__ void invalidate(float* x) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) x[i] = __builtin_nanf("");
   }
 };
 
-// A row of Q (head < H_q) or K, rotated; a position outside the table makes
-// it NaN, so that no such call passes for a result.
-template <typename T, int L, bool VEC>
-__device__ __forceinline__ bool rotated_row(const RotateArgs& a, const RowLane<T, L, VEC>& ln, const T* row, int64_t t,
-                                            const void* w, float* x) {
+// A token's position, 0 (and not ok) where it lies outside the table: its Q
+// rows are NaN then, so that no such call passes for a result, and its K rows
+// are not cached.
+__device__ __forceinline__ int64_t position_of(const RotateArgs& a, int64_t t, bool* ok) {
   const int64_t pos = a.rotary_dim > 0 ? a.positions[t] : 0;
-  ln.load(row, x);
-  const bool ok = a.rotary_dim == 0 || (pos >= 0 && pos < a.num_positions);
-  ln.apply(row, x, w, ok ? pos : 0);
-  if (!ok) {
-#pragma unroll
-    for (int i = 0; i < RowLane<T, L, VEC>::kN; ++i) x[i] = __builtin_nanf("");
-  }
-  return ok;
+  *ok = a.rotary_dim == 0 || (pos >= 0 && pos < a.num_positions);
+  return *ok ? pos : 0;
 }
 
-// Every row of the step in turn, (token, head) with the heads of Q, K, V in
-// this order; K and V go to the cache's slots, or (no cache) K to key_out.
-template <typename T, int L, bool VEC>
+// Heads h0 .. h0 + NR - 1 of token t, of the heads of Q, K, V in this order
+// (`heads` of them): K and V go to the cache's slot, or (no cache) K to
+// key_out.  Every load is issued before the first row is finished, and the
+// rows share the token's angles.
+template <typename T, int L, bool VEC, int NR>
+__device__ __forceinline__ void rotate_rows(const RotateArgs& a, const RowLane<T, L, VEC>& ln, int64_t t, int h0,
+                                            int heads) {
+  const T* src[NR];
+  typename RowLane<T, L, VEC>::Raw raw[NR];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    int h = min(h0 + i, heads - 1);
+    const bool is_q = h < a.num_query_heads;
+    if (!is_q) h -= a.num_query_heads;
+    const bool is_v = !is_q && h >= a.num_kv_heads;
+    if (is_v) h -= a.num_kv_heads;
+    src[i] = reinterpret_cast<const T*>(is_q ? a.query : is_v ? a.value : a.key) +
+             t * (is_q ? a.q_token_stride : is_v ? a.v_token_stride : a.k_token_stride) +
+             h * (is_q ? a.q_head_stride : is_v ? a.v_head_stride : a.k_head_stride);
+    raw[i] = ln.load_raw(src[i]);
+  }
+  const int64_t slot = a.slot_mapping != nullptr ? a.slot_mapping[t] : 0;
+  bool ok;
+  const int64_t pos = position_of(a, t, &ok);
+  const bool any_norm = a.query_weight != nullptr || a.key_weight != nullptr;
+  float qg[8] = {}, kg[8] = {};  // the weights of Q rows and of K rows
+  float4 c, s;
+  if constexpr (VEC) {
+    if (any_norm) {
+      ln.weights(a.query_weight != nullptr ? a.query_weight : a.key_weight, qg);
+      ln.weights(a.key_weight != nullptr ? a.key_weight : a.query_weight, kg);
+    }
+    ln.angles(pos, &c, &s);
+  }
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int h = h0 + i;
+    const bool is_q = h < a.num_query_heads;
+    const bool is_v = h >= a.num_query_heads + a.num_kv_heads;
+    const void* w = is_q ? a.query_weight : a.key_weight;
+    float x[RowLane<T, L, VEC>::kN];
+    ln.unpack(raw[i], src[i], x);
+    if constexpr (VEC) {
+      float g[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[k] = is_q ? qg[k] : kg[k];
+      ln.apply(x, any_norm && w != nullptr, g, c, s);
+    } else {
+      if (!is_v && h < heads) ln.apply_any(src[i], x, w, pos);
+    }
+    if (!is_v && !ok) ln.invalidate(x);
+    T* out;
+    bool keep = h < heads;
+    if (is_q) {
+      out = reinterpret_cast<T*>(a.query_out) + t * a.q_out_token_stride + h * a.q_out_head_stride;
+    } else if (a.key_cache != nullptr) {
+      keep = keep && slot >= 0 && slot < a.num_slots && (is_v || ok);
+      const int kv = h - a.num_query_heads - (is_v ? a.num_kv_heads : 0);
+      out = reinterpret_cast<T*>(is_v ? a.value_cache : a.key_cache) + (slot * a.num_kv_heads + kv) * a.head_dim;
+    } else {
+      out = reinterpret_cast<T*>(a.key_out) + t * a.k_out_token_stride + (h - a.num_query_heads) * a.k_out_head_stride;
+    }
+    if (keep) ln.store(out, x, raw[i], is_v);
+  }
+}
+
+// Every row of the step, NR heads of a token to a group of lanes.
+template <typename T, int L, bool VEC, int NR>
 __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs a) {
-  constexpr int kRows = kRotateThreads / L;
-  const uint32_t heads = a.num_query_heads + (a.key_cache != nullptr ? 2 : 1) * a.num_kv_heads;
-  const uint32_t id = blockIdx.x * kRows + threadIdx.x / L;
-  const uint32_t tok = quotient(id, heads, a.heads_rcp);
+  const int heads = a.num_query_heads + (a.key_cache != nullptr ? 2 : 1) * a.num_kv_heads;
+  const uint32_t units = (heads + NR - 1) / NR;  // per token
+  const uint32_t id = blockIdx.x * (kRotateThreads / L) + threadIdx.x / L;
+  const uint32_t tok = quotient(id, units, a.heads_rcp);
   if (tok >= static_cast<uint32_t>(a.num_tokens)) return;
-  const int64_t t = tok;
-  int h = static_cast<int>(id - tok * heads);
   const RowLane<T, L, VEC> ln(a, threadIdx.x % L);
-  float x[RowLane<T, L, VEC>::kN];
-  if (h < a.num_query_heads) {
-    const T* row = reinterpret_cast<const T*>(a.query) + t * a.q_token_stride + h * a.q_head_stride;
-    rotated_row<T, L, VEC>(a, ln, row, t, a.query_weight, x);
-    ln.store(reinterpret_cast<T*>(a.query_out) + t * a.q_out_token_stride + h * a.q_out_head_stride, x);
-    return;
-  }
-  h -= a.num_query_heads;
-  const bool is_v = h >= a.num_kv_heads;
-  if (is_v) h -= a.num_kv_heads;
-  T* out;
-  if (a.key_cache != nullptr) {
-    const int64_t slot = a.slot_mapping[t];
-    if (slot < 0 || slot >= a.num_slots) return;
-    out = reinterpret_cast<T*>(is_v ? a.value_cache : a.key_cache) + (slot * a.num_kv_heads + h) * a.head_dim;
-  } else {
-    out = reinterpret_cast<T*>(a.key_out) + t * a.k_out_token_stride + h * a.k_out_head_stride;
-  }
-  if (is_v) {
-    ln.load(reinterpret_cast<const T*>(a.value) + t * a.v_token_stride + h * a.v_head_stride, x);
-  } else {
-    const T* row = reinterpret_cast<const T*>(a.key) + t * a.k_token_stride + h * a.k_head_stride;
-    // (a K row without a position is not cached)
-    if (!rotated_row<T, L, VEC>(a, ln, row, t, a.key_weight, x) && a.key_cache != nullptr) return;
-  }
-  ln.store(out, x);
+  rotate_rows<T, L, VEC, NR>(a, ln, tok, static_cast<int>(id - tok * units) * NR, heads);
 }
 
 // The 8-bit cache's write.  The first a.kv_groups workgroups take (chunk of C
@@ -243,39 +334,38 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs a) {
 // every row the step brings for the block.  Those follow each other in the
 // step: a chunk owns the runs (tokens of one block) that begin in it, and so
 // looks at up to block_size - 1 tokens past its end and leaves the first ones
-// to the chunk before where their run began there.  It goes over them twice,
-// for the runs' largest magnitudes (kept in LDS by an integer maximum of the
-// floats' bits, which no order changes) and then to write the codes, the rows
-// coming from the L2 the second time.  A run that holds its block's first row
-// starts the block afresh; the other rows of any other block are re-coded if
-// its scale grows.
-template <typename T, int L, bool VEC>
+// to the chunk before where their run began there.  It takes the rows' largest
+// magnitudes (kept in LDS by an integer maximum of the floats' bits, which no
+// order changes), settles the scales, and writes the codes.  KEEP: the span is
+// at most two rows a group, which are loaded first of all, beside the slots,
+// and stay in registers; else the rows are read (and rotated) again.  A run
+// that holds its block's first row starts the block afresh; the other rows of
+// any other block are re-coded if its scale grows.
+template <typename T, int L, bool VEC, bool KEEP, int NR>
 __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs a) {
   constexpr int C = kRotateThreads / L;  // tokens a chunk owns, rows at once
   constexpr int kN = RowLane<T, L, VEC>::kN;
   const RowLane<T, L, VEC> ln(a, threadIdx.x % L);
   const int group = threadIdx.x / L;
-  float x[kN];
   if (blockIdx.x >= a.kv_groups) {
+    const uint32_t units = (a.num_query_heads + NR - 1) / NR;
     const uint32_t id = (blockIdx.x - a.kv_groups) * C + group;
-    const uint32_t tok = quotient(id, a.num_query_heads, a.heads_rcp);
+    const uint32_t tok = quotient(id, units, a.heads_rcp);
     if (tok >= static_cast<uint32_t>(a.num_tokens)) return;
-    const int64_t t = tok;
-    const int h = static_cast<int>(id - tok * a.num_query_heads);
-    const T* row = reinterpret_cast<const T*>(a.query) + t * a.q_token_stride + h * a.q_head_stride;
-    rotated_row<T, L, VEC>(a, ln, row, t, a.query_weight, x);
-    ln.store(reinterpret_cast<T*>(a.query_out) + t * a.q_out_token_stride + h * a.q_out_head_stride, x);
+    rotate_rows<T, L, VEC, NR>(a, ln, tok, static_cast<int>(id - tok * units) * NR, a.num_query_heads);
     return;
   }
-  // Per run that begins in the chunk (at token C c + i): its block, its first
-  // and one past its last token, whether it holds the block's first row, its
-  // largest magnitude's bits, the block's scales.
+  // Per run that begins in the chunk (at token C c + i): its block, whether it
+  // holds the block's first row, its largest magnitude's bits, the scale the
+  // block has (0 if it starts afresh); and one past the last run's last token.
   __shared__ int64_t s_block[C];
-  __shared__ int s_end[C], s_fresh[C];
+  __shared__ int s_fresh[C], s_end;
   __shared__ uint32_t s_amax[C];
-  __shared__ float s_new[C], s_ratio[C];
-  // Per token of the span: the run it belongs to (< 0: none of the chunk's).
+  __shared__ float s_old[C];
+  // Per token of the span: the run it belongs to (< 0: none of the chunk's),
+  // and its row of the cache.
   __shared__ int16_t s_run[C + kMaxCache8Block];
+  __shared__ int64_t s_slot[C + kMaxCache8Block];
 
   const uint32_t units = 2 * a.num_kv_heads;
   const uint32_t chunk = quotient(blockIdx.x, units, a.kv_rcp);
@@ -284,137 +374,242 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
   const int h = is_v ? u - a.num_kv_heads : u;
   const int64_t t0 = static_cast<int64_t>(chunk) * C;
   const int span = static_cast<int>(min<int64_t>(C + a.block_size - 1, a.num_tokens - t0));
-  auto block_of = [&](int64_t t) -> int64_t {
-    if (t < 0 || t >= a.num_tokens) return -1;
-    const int64_t slot = a.slot_mapping[t];
-    if (slot < 0 || slot >= a.num_slots) return -1;
-    return slot / a.block_size;
+  const T* src = reinterpret_cast<const T*>(is_v ? a.value : a.key) + h * (is_v ? a.v_head_stride : a.k_head_stride);
+  const int64_t tok_stride = is_v ? a.v_token_stride : a.k_token_stride;
+  const void* w = is_v ? nullptr : a.key_weight;
+  // Row j as it is given, with what turning it takes; then as the 16-bit cache
+  // would hold it (false if it is not cached).
+  using Raw = typename RowLane<T, L, VEC>::Raw;
+  float g[8] = {};
+  if constexpr (VEC)
+    if (w != nullptr) ln.weights(w, g);
+  auto load_row = [&](int j, Raw* raw, int64_t* pos, bool* ok, float4* c, float4* s) {
+    *ok = true;
+    *pos = 0;
+    *raw = ln.load_raw(src + (t0 + j) * tok_stride);
+    if (!is_v) {
+      *pos = position_of(a, t0 + j, ok);
+      if constexpr (VEC) ln.angles(*pos, c, s);
+    }
   };
+  auto finish_row = [&](int j, const Raw& raw, float* x, int64_t pos, const float4& c, const float4& s) {
+    ln.unpack(raw, src + (t0 + j) * tok_stride, x);
+    if (!is_v) {
+      if constexpr (VEC) ln.apply(x, w != nullptr, g, c, s);
+      else ln.apply_any(src + (t0 + j) * tok_stride, x, w, pos);
+    }
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      x[i] = rounded<T>(x[i]);
+      if constexpr (Elem<T>::kDtype == PA_DTYPE_F16)
+        if (fabsf(x[i]) < INFINITY) x[i] = fminf(fmaxf(x[i], -kMaxF16Row), kMaxF16Row);
+    }
+  };
+  constexpr int kKept = KEEP ? 2 : 1;
+  float x[kKept][kN];
+  Raw raw[kKept];
+  float4 cs[kKept], sn[kKept];
+  int64_t pos[kKept];
+  bool ok[kKept];
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      load_row(min(group + k * C, span - 1), &raw[k], &pos[k], &ok[k], &cs[k], &sn[k]);
+  }
+
+  float* scales = (is_v ? a.value_scales : a.key_scales) + h;
+  float old = 0.f;  // lane i < C of the first wave: the scale of run i's block
   if (threadIdx.x < C) {
     s_block[threadIdx.x] = -1;
-    s_end[threadIdx.x] = 0;
+    s_end = 0;
     s_fresh[threadIdx.x] = 0;
     s_amax[threadIdx.x] = 0;
   }
-  __syncthreads();
   if (threadIdx.x < kWave) {
-    int last = -1;  // the run the tokens before this batch end in
+    // A slot's block, -1 outside the pool.
+    auto split = [&](int64_t slot, int* row) -> int64_t {
+      if (slot < 0 || slot >= a.num_slots) {
+        *row = 0;
+        return -1;
+      }
+      if (a.log2_block >= 0) {
+        *row = static_cast<int>(slot) & (a.block_size - 1);
+        return slot >> a.log2_block;
+      }
+      const int64_t b = slot / a.block_size;
+      *row = static_cast<int>(slot - b * a.block_size);
+      return b;
+    };
+    int row;
+    int64_t before = t0 > 0 ? split(a.slot_mapping[t0 - 1], &row) : -1;  // the block of the token ahead of the batch
+    int last = -1;                                                       // the run that token ends
     for (int base = 0; base < span; base += kWave) {
       const int j = base + threadIdx.x;
-      const int64_t blk = j < span ? block_of(t0 + j) : -1;
-      const bool starts = j < span && blk != block_of(t0 + j - 1);
+      const int64_t slot = j < span ? a.slot_mapping[t0 + j] : -1;
+      const int64_t blk = split(slot, &row);
+      int64_t prev = __shfl_up(blk, 1, kWave);
+      if (threadIdx.x == 0) prev = before;
+      before = __shfl(blk, kWave - 1, kWave);
+      const bool starts = blk != prev;
       const uint64_t mask = __ballot(starts);
       const uint64_t upto = mask & (~uint64_t{0} >> (kWave - 1 - threadIdx.x));
       const int lead = upto != 0 ? base + 63 - __builtin_clzll(upto) : last;
-      const bool ours = lead >= 0 && lead < C && blk >= 0 && j < span;
-      if (j < span) s_run[j] = static_cast<int16_t>(ours ? lead : -1);
+      const bool ours = lead >= 0 && lead < C && blk >= 0;
+      if (j < span) {
+        s_run[j] = static_cast<int16_t>(ours ? lead : -1);
+        s_slot[j] = slot;
+      }
       if (ours) {
         if (starts) s_block[lead] = blk;
-        atomicMax(&s_end[lead], j + 1);
-        if (a.slot_mapping[t0 + j] % a.block_size == 0) s_fresh[lead] = 1;
+        atomicMax(&s_end, j + 1);
+        if (row == 0) s_fresh[lead] = 1;
       }
       if (mask != 0) last = base + 63 - __builtin_clzll(mask);
+      // (run i begins at token i, so its lane holds its block)
+      if (base == 0 && threadIdx.x < C && ours && starts) old = scale_pow2(scales[blk * a.num_kv_heads]);
     }
   }
   __syncthreads();
-  const T* src = reinterpret_cast<const T*>(is_v ? a.value : a.key) + h * (is_v ? a.v_head_stride : a.k_head_stride);
-  const int64_t tok_stride = is_v ? a.v_token_stride : a.k_token_stride;
-  // Row j as the 16-bit cache would hold it; false if it is not cached.
-  auto read_row = [&](int j) {
-    const int64_t t = t0 + j;
-    const T* row = src + t * tok_stride;
-    bool ok = true;
-    if (is_v) ln.load(row, x);
-    else ok = rotated_row<T, L, VEC>(a, ln, row, t, a.key_weight, x);
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      if constexpr (Elem<T>::kDtype == PA_DTYPE_F16) {
-        if (fabsf(x[i]) < INFINITY) x[i] = fminf(fmaxf(rounded<T>(x[i]), -kMaxF16Row), kMaxF16Row);
-      } else {
-        x[i] = rounded<T>(x[i]);
-      }
-    }
-    return ok;
-  };
-  // The run past whose end no token is the chunk's.
-  int end = 0;
-  for (int i = 0; i < C; ++i) end = max(end, s_end[i]);
-  for (int j = group; j < end; j += C) {
-    const int run = s_run[j];
-    if (run < 0 || !read_row(j)) continue;
+  // Rows past the last run that begins in the chunk are not the chunk's.
+  const int end = s_end;
+  auto note = [&](int run, const float* y) {
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const float v = fabsf(x[i]);
+      const float v = fabsf(y[i]);
       m = fmaxf(m, v < INFINITY ? v : 0.f);
     }
     m = row_max<L>(m);
     if (ln.lane == 0) atomicMax(&s_amax[run], __float_as_uint(m));
+  };
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int j = group + k * C;
+      const int run = j < end ? s_run[j] : -1;
+      ok[k] = run >= 0 && ok[k];
+      if (ok[k]) {
+        finish_row(j, raw[k], x[k], pos[k], cs[k], sn[k]);
+        note(run, x[k]);
+      }
+    }
+  } else {
+    for (int j = group; j < end; j += C) {
+      if (s_run[j] < 0) continue;
+      load_row(j, &raw[0], &pos[0], &ok[0], &cs[0], &sn[0]);
+      finish_row(j, raw[0], x[0], pos[0], cs[0], sn[0]);
+      if (ok[0]) note(s_run[j], x[0]);
+    }
   }
+  if (threadIdx.x < C) s_old[threadIdx.x] = s_fresh[threadIdx.x] ? 0.f : old;
   __syncthreads();
-  float* scales = is_v ? a.value_scales : a.key_scales;
-  if (threadIdx.x < C && s_block[threadIdx.x] >= 0) {
-    float* at = scales + s_block[threadIdx.x] * a.num_kv_heads + h;
-    const float need = scale_for(__uint_as_float(s_amax[threadIdx.x]));
-    const float was = s_fresh[threadIdx.x] ? 0.f : scale_pow2(*at);
-    const float now = fmaxf(was, need);
-    s_new[threadIdx.x] = now;
-    s_ratio[threadIdx.x] = s_fresh[threadIdx.x] ? 1.f : was * inverse_pow2(now);
-    *at = now;
-  }
-  __syncthreads();
+  auto new_scale = [&](int run) { return fmaxf(s_old[run], scale_for(__uint_as_float(s_amax[run]))); };
+  // What the other rows of a run's block are re-coded by (1: not at all).
+  auto recode = [&](int run) {
+    return s_block[run] < 0 || s_fresh[run] ? 1.f : s_old[run] * inverse_pow2(new_scale(run));
+  };
+  if (threadIdx.x < C && s_block[threadIdx.x] >= 0)
+    scales[s_block[threadIdx.x] * a.num_kv_heads] = new_scale(threadIdx.x);
   uint8_t* cache = reinterpret_cast<uint8_t*>(is_v ? a.value_cache : a.key_cache) + h * a.head_dim;
   const int64_t row_codes = static_cast<int64_t>(a.num_kv_heads) * a.head_dim;
   // Blocks whose scale grew: all of their rows; the run's own follow below.
-  for (int i = 0; i < C; ++i) {
-    if (s_block[i] < 0 || s_ratio[i] == 1.f) continue;
-    const float ratio = s_ratio[i];
-    uint8_t* rows = cache + s_block[i] * a.block_size * row_codes;
-    for (int k = threadIdx.x; k < a.block_size * a.head_dim; k += kRotateThreads) {
-      const int r = k / a.head_dim;
-      uint8_t* p = rows + r * row_codes + (k - r * a.head_dim);
-      *p = static_cast<uint8_t>(pack_codes2(code_to_f32<0>(*p) * ratio, 0.f));
+  const int lane = threadIdx.x % kWave;
+  if (__any(lane < C && recode(min(lane, C - 1)) != 1.f)) {  // (alike in every wave)
+    for (int i = 0; i < C; ++i) {
+      const float ratio = recode(i);
+      if (ratio == 1.f) continue;
+      uint8_t* rows = cache + s_block[i] * a.block_size * row_codes;
+      if constexpr (VEC) {
+        const int words = a.head_dim / 4;
+        for (int k = threadIdx.x; k < a.block_size * words; k += kRotateThreads) {
+          const int r = k / words;
+          uint32_t* p = reinterpret_cast<uint32_t*>(rows + r * row_codes) + (k - r * words);
+          const uint32_t v = *p;
+          *p = pack_codes4(code_to_f32<0>(v) * ratio, code_to_f32<1>(v) * ratio, code_to_f32<2>(v) * ratio,
+                           code_to_f32<3>(v) * ratio);
+        }
+      } else {
+        for (int k = threadIdx.x; k < a.block_size * a.head_dim; k += kRotateThreads) {
+          const int r = k / a.head_dim;
+          uint8_t* p = rows + r * row_codes + (k - r * a.head_dim);
+          *p = static_cast<uint8_t>(pack_codes2(code_to_f32<0>(*p) * ratio, 0.f));
+        }
+      }
     }
+    __syncthreads();  // (orders the stores of a row's two writes)
   }
-  __syncthreads();  // (orders the stores of a row's two writes)
-  for (int j = group; j < end; j += C) {
-    const int run = s_run[j];
-    if (run < 0 || !read_row(j)) continue;
-    const float inv = inverse_pow2(s_new[run]);
-    uint8_t* out = cache + a.slot_mapping[t0 + j] * row_codes;
+  auto write = [&](int j, const float* y) {
+    const float inv = inverse_pow2(new_scale(s_run[j]));
+    uint8_t* out = cache + s_slot[j] * row_codes;
     if constexpr (VEC) {
       if (ln.live) {
-        *reinterpret_cast<uint32_t*>(out + ln.a) = pack_codes4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-        *reinterpret_cast<uint32_t*>(out + ln.b) = pack_codes4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+        *reinterpret_cast<uint32_t*>(out + ln.a) = pack_codes4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+        *reinterpret_cast<uint32_t*>(out + ln.b) = pack_codes4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv);
       }
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (ln.lane + 64 * e < a.head_dim)
-          out[ln.lane + 64 * e] = static_cast<uint8_t>(pack_codes2(x[e] * inv, 0.f));
+          out[ln.lane + 64 * e] = static_cast<uint8_t>(pack_codes2(y[e] * inv, 0.f));
+    }
+  };
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (ok[k]) write(group + k * C, x[k]);
+  } else {
+    for (int j = group; j < end; j += C) {
+      if (s_run[j] < 0) continue;
+      load_row(j, &raw[0], &pos[0], &ok[0], &cs[0], &sn[0]);
+      finish_row(j, raw[0], x[0], pos[0], cs[0], sn[0]);
+      if (ok[0]) write(j, x[0]);
     }
   }
 }
 
-template <typename T, int L, bool VEC>
-static hipError_t launch_rotate_l(const RotateArgs& args, hipStream_t s) {
+template <typename T, int L, bool VEC, int NR>
+static hipError_t launch_rotate_n(const RotateArgs& args, hipStream_t s) {
   constexpr int kRows = kRotateThreads / L;
   RotateArgs a = args;
-  if (a.key_scales == nullptr) {
-    const uint32_t heads = a.num_query_heads + (a.key_cache != nullptr ? 2 : 1) * a.num_kv_heads;
-    a.heads_rcp = 0xffffffffu / heads;
-    const int64_t rows = static_cast<int64_t>(a.num_tokens) * heads;
-    const dim3 grid(static_cast<uint32_t>((rows + kRows - 1) / kRows));
-    hipLaunchKernelGGL((rotate_kernel<T, L, VEC>), grid, dim3(kRotateThreads), 0, s, a);
+  const bool codes = a.key_scales != nullptr;
+  const uint32_t heads =
+      codes ? a.num_query_heads : a.num_query_heads + (a.key_cache != nullptr ? 2 : 1) * a.num_kv_heads;
+  const uint32_t units = (heads + NR - 1) / NR;
+  const int64_t groups = static_cast<int64_t>(a.num_tokens) * units;
+  const uint32_t grid = static_cast<uint32_t>((groups + kRows - 1) / kRows);
+  a.heads_rcp = units > 0 ? 0xffffffffu / units : 0;
+  if (!codes) {
+    hipLaunchKernelGGL((rotate_kernel<T, L, VEC, NR>), dim3(grid), dim3(kRotateThreads), 0, s, a);
     return hipGetLastError();
   }
-  a.heads_rcp = a.num_query_heads > 0 ? 0xffffffffu / a.num_query_heads : 0;
   a.kv_rcp = 0xffffffffu / (2 * a.num_kv_heads);
   a.kv_groups = static_cast<uint32_t>((a.num_tokens + kRows - 1) / kRows * (2 * a.num_kv_heads));
-  const int64_t q_rows = static_cast<int64_t>(a.num_tokens) * a.num_query_heads;
-  const dim3 grid(a.kv_groups + static_cast<uint32_t>((q_rows + kRows - 1) / kRows));
-  hipLaunchKernelGGL((cache8_write_kernel<T, L, VEC>), grid, dim3(kRotateThreads), 0, s, a);
+  a.log2_block = -1;
+  for (int i = 0; i <= 8; ++i)
+    if (1 << i == a.block_size) a.log2_block = i;
+  if (a.block_size <= kRows + 1)
+    hipLaunchKernelGGL((cache8_write_kernel<T, L, VEC, true, NR>), dim3(a.kv_groups + grid), dim3(kRotateThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL((cache8_write_kernel<T, L, VEC, false, NR>), dim3(a.kv_groups + grid), dim3(kRotateThreads), 0, s, a);
   return hipGetLastError();
+}
+
+// Two heads to a group of lanes once one each would take more lanes than the
+// chip holds at a time (2048 on each of 256 CUs): from there on loads in
+// flight are what counts, and below it the depth of one row's work.  One
+// against two, bf16, 32/8 heads of 128 with norms: 256 tokens 4.6 / 4.9 us,
+// 512 6.7 / 6.7, 768 9.7 / 8.7, 4096 36.3 / 28.9; 9/3 heads of 64: 1024 tokens
+// 3.9 / 4.2 us, 4096 7.2 / 7.2; fp32, 8/8 heads of 64: 1024 5.6 / 6.2 us, 4096
+// 13.3 / 13.4.  Four: 18.2 us where two took 17.9 and one 21.3.
+constexpr int64_t kResidentLanes = 256 * 2048;
+
+template <typename T, int L, bool VEC>
+static hipError_t launch_rotate_l(const RotateArgs& a, hipStream_t s) {
+  if constexpr (VEC) {
+    const int64_t rows = static_cast<int64_t>(a.num_tokens) * (a.num_query_heads + 2 * a.num_kv_heads);
+    if (rows * L > kResidentLanes) return launch_rotate_n<T, L, VEC, 2>(a, s);
+  }
+  return launch_rotate_n<T, L, VEC, 1>(a, s);
 }
 
 template <typename T>
@@ -438,7 +633,9 @@ hipError_t launch_rotate(const RotateArgs& a, int dtype, hipStream_t s) {
   const bool vec = a.head_dim % 8 == 0 && a.rotary_dim % 8 == 0 && q && fits(a.key, a.k_token_stride, a.k_head_stride) &&
                    fits(a.value, a.v_token_stride, a.v_head_stride) &&
                    fits(a.key_out, a.k_out_token_stride, a.k_out_head_stride) && fits(a.key_cache, 0, 0) &&
-                   fits(a.value_cache, 0, 0) && reinterpret_cast<uintptr_t>(a.cos_sin) % 16 == 0;
+                   fits(a.value_cache, 0, 0) && reinterpret_cast<uintptr_t>(a.cos_sin) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(a.query_weight) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(a.key_weight) % 16 == 0;
   switch (dtype) {
     case PA_DTYPE_F32: return launch_rotate_t<float>(a, vec, s);
     case PA_DTYPE_BF16: return launch_rotate_t<bf16_t>(a, vec, s);
