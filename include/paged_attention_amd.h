@@ -40,7 +40,7 @@ enum {
 
 /* Element type tags for K/V/query/output buffers.  PA_DTYPE_E4M3 (8-bit codes
  * with a scale per block and KV head, section (g)) names a cache only: in
- * PaRowDims.cache_dtype, pa_plan_step_for, pa_decode_workgroups_per_item and
+ * PaRotateDims.cache_dtype, pa_plan_step_for, pa_decode_workgroups_per_item and
  * pa_decode_workgroups_per_cu. */
 enum { PA_DTYPE_F32 = 0, PA_DTYPE_BF16 = 1, PA_DTYPE_F16 = 2, PA_DTYPE_E4M3 = 3 };
 
@@ -675,75 +675,65 @@ int pa_attention_step(const PaStepCall *call, const void *query, void *key_cache
  * scales is num_kv_heads floats).
  */
 
-/* Sizes of a step's rows and of the cache they go to. */
+/* What a rotation's calls share: sizes, element strides between tokens and
+ * heads (unit stride along D) and the rotation itself. */
 typedef struct {
     int32_t num_tokens;      /* T                                          */
     int32_t num_query_heads; /* H_q                                        */
     int32_t num_kv_heads;    /* H_kv                                       */
     int32_t head_dim;        /* D, at most 256                             */
-    int32_t block_size;
-    int32_t total_blocks;
-    int32_t num_layers;
     int32_t dtype;           /* PA_DTYPE_* of the rows                     */
+    int32_t weight_dtype;    /* of the norm weights: the rows' or F32      */
+    int32_t rotary_dim;      /* R: even, at most D; 0: no rotation (then no
+                                positions and no table)                    */
+    int32_t interleaved;     /* pairs (2i, 2i + 1) instead of (i, i + R/2) */
+    int64_t num_positions;   /* rows of the table                          */
+    float eps;
     int32_t cache_dtype;     /* the rows' type, or PA_DTYPE_E4M3           */
-} PaRowDims;
-
-/* The projections' rows, [T, H_q, D] and [T, H_kv, D] with element strides
- * between tokens and heads and unit stride along D, and where the rotated ones
- * go (query_out may be query, and key_out key). */
-typedef struct {
-    const void *query;
-    const void *key;
-    const void *value;
+    int32_t block_size;      /* of the cache (pa_rotate reads none of the  */
+    int32_t total_blocks;    /* cache's sizes)                             */
+    int32_t num_layers;
+    int32_t reserved;        /* 0 */
     int64_t query_token_stride;
     int64_t query_head_stride;
     int64_t key_token_stride;
     int64_t key_head_stride;
     int64_t value_token_stride;
     int64_t value_head_stride;
-    void *query_out;
     int64_t query_out_token_stride;
     int64_t query_out_head_stride;
-    void *key_out;                 /* pa_rotate only */
     int64_t key_out_token_stride;
     int64_t key_out_head_stride;
-} PaRotateRows;
-
-/* The rotation, and the norm ahead of it. */
-typedef struct {
-    const int64_t *positions;  /* [T], device                                 */
-    const float *cos_sin;      /* [num_positions, rotary_dim], device: a
-                                  position's cosines, then its sines          */
-    int64_t num_positions;
-    int32_t rotary_dim;        /* R: even, at most D; 0: no rotation (the two
-                                  pointers may then be NULL)                  */
-    int32_t interleaved;       /* pairs (2i, 2i + 1) instead of (i, i + R/2)  */
-    const void *query_weight;  /* [D], or NULL: not normalised                */
-    const void *key_weight;
-    int32_t weight_dtype;      /* the rows' type or PA_DTYPE_F32              */
-    float eps;
-} PaRotation;
+} PaRotateDims;
 
 /*
  * No counterpart in the reference, whose models rotate before they hand rows
- * over.  Each Q and K row of a token is normalised (x * rsqrt(mean(x^2) + eps)
- * * weight, where a weight is given) and rotated: the pair (a, b) becomes
- * (a cos - b sin, b cos + a sin) with the position's cosine and sine, the
- * elements past R stay.  All of it in fp32, rounded once.  A token whose
- * position lies outside [0, num_positions) gets NaN rows.  rows.value is not
- * read.  Asynchronous on `stream`, as every entry point here.
+ * over.  query [T, H_q, D] and key [T, H_kv, D] rows are normalised (x *
+ * rsqrt(mean(x^2) + eps) * weight, query_weight / key_weight [D]; NULL: not
+ * normalised) and rotated: the pair (a, b) becomes (a cos - b sin, b cos + a
+ * sin) with the cosine and sine of the token's position (positions int64 [T];
+ * cos_sin float [num_positions, rotary_dim]: a position's cosines, then its
+ * sines), the elements past R stay.  All of it in fp32, rounded once.  A token
+ * whose position lies outside [0, num_positions) gets NaN rows.  query_out may
+ * be query, and key_out key.  `dims` is read before the call returns.
  */
-int pa_rotate(PaRotateRows rows, PaRotation rotation, PaRowDims dims, void *stream);
+int pa_rotate(const PaRotateDims *dims, const void *query, const void *key,
+              const int64_t *positions, const float *cos_sin,
+              const void *query_weight, const void *key_weight,
+              void *query_out, void *key_out, void *stream);
 
 /*
- * pa_rotate, with K and V going into the paged cache at slot_mapping (int64
- * [T]) in the same launch: bit for bit pa_rotate followed by
- * pa_reshape_and_cache (or _8bit) where all rows start at multiples of four
- * elements or none does.  Slots outside [0, N * bs) are skipped, and
- * so is the K row of a token whose position lies outside the table.
- * key_scales / value_scales: for PA_DTYPE_E4M3 caches, NULL otherwise.
+ * pa_rotate, with K and V (value [T, H_kv, D]) going into the paged cache at
+ * slot_mapping (int64 [T]) in the same launch: bit for bit pa_rotate followed
+ * by pa_reshape_and_cache (or _8bit) where all rows start at multiples of four
+ * elements or none does.  Slots outside [0, N * bs) are skipped, and so is the
+ * K row of a token whose position lies outside the table.  key_scales /
+ * value_scales: for PA_DTYPE_E4M3 caches, NULL otherwise.
  */
-int pa_rotate_and_cache(PaRotateRows rows, PaRotation rotation, PaRowDims dims,
+int pa_rotate_and_cache(const PaRotateDims *dims, const void *query, const void *key,
+                        const void *value, const int64_t *positions,
+                        const float *cos_sin, const void *query_weight,
+                        const void *key_weight, void *query_out,
                         void *key_cache, void *value_cache, float *key_scales,
                         float *value_scales, const int64_t *slot_mapping,
                         int32_t layer_idx, void *stream);
@@ -786,6 +776,16 @@ int pa_prefill_8bit(const void *query, const void *key_cache,
                     const int64_t *cu_seqlens, const int32_t *prefill_items,
                     int64_t num_prefill_items, int32_t prefill_tile,
                     float scaling, void *output, void *stream);
+
+/*
+ * One layer of a packed step over an 8-bit cache: with new_rows (of dims.dtype;
+ * may be NULL) pa_reshape_and_cache_8bit at call->scatter_slots, then
+ * pa_prefill_8bit and pa_decode_8bit, as the step has work items for them.
+ */
+int pa_attention_step_8bit(const PaStepCall *call, const void *query, void *key_cache,
+                           void *value_cache, float *key_scales, float *value_scales,
+                           int32_t layer_idx, const PaNewRows *new_rows, float scaling,
+                           void *output, void *stream);
 
 #ifdef __cplusplus
 }

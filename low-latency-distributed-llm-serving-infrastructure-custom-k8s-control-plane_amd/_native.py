@@ -68,6 +68,7 @@ EXPORTED_SYMBOLS = (
     "pa_reshape_and_cache_8bit",
     "pa_decode_8bit",
     "pa_prefill_8bit",
+    "pa_attention_step_8bit",
     "pa_map_host_memory",
     "pa_calibrate_mfma",
     "pa_calibrate_mfma_flops",
@@ -124,51 +125,33 @@ class PaNewRows(ctypes.Structure):
     ]
 
 
-class PaRowDims(ctypes.Structure):
+class PaRotateDims(ctypes.Structure):
     _fields_ = [
         ("num_tokens", ctypes.c_int32),
         ("num_query_heads", ctypes.c_int32),
         ("num_kv_heads", ctypes.c_int32),
         ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("num_positions", ctypes.c_int64),
+        ("eps", ctypes.c_float),
+        ("cache_dtype", ctypes.c_int32),
         ("block_size", ctypes.c_int32),
         ("total_blocks", ctypes.c_int32),
         ("num_layers", ctypes.c_int32),
-        ("dtype", ctypes.c_int32),
-        ("cache_dtype", ctypes.c_int32),
-    ]
-
-
-class PaRotateRows(ctypes.Structure):
-    _fields_ = [
-        ("query", ctypes.c_void_p),
-        ("key", ctypes.c_void_p),
-        ("value", ctypes.c_void_p),
+        ("reserved", ctypes.c_int32),
         ("query_token_stride", ctypes.c_int64),
         ("query_head_stride", ctypes.c_int64),
         ("key_token_stride", ctypes.c_int64),
         ("key_head_stride", ctypes.c_int64),
         ("value_token_stride", ctypes.c_int64),
         ("value_head_stride", ctypes.c_int64),
-        ("query_out", ctypes.c_void_p),
         ("query_out_token_stride", ctypes.c_int64),
         ("query_out_head_stride", ctypes.c_int64),
-        ("key_out", ctypes.c_void_p),
         ("key_out_token_stride", ctypes.c_int64),
         ("key_out_head_stride", ctypes.c_int64),
-    ]
-
-
-class PaRotation(ctypes.Structure):
-    _fields_ = [
-        ("positions", ctypes.c_void_p),
-        ("cos_sin", ctypes.c_void_p),
-        ("num_positions", ctypes.c_int64),
-        ("rotary_dim", ctypes.c_int32),
-        ("interleaved", ctypes.c_int32),
-        ("query_weight", ctypes.c_void_p),
-        ("key_weight", ctypes.c_void_p),
-        ("weight_dtype", ctypes.c_int32),
-        ("eps", ctypes.c_float),
     ]
 
 
@@ -309,10 +292,14 @@ _SIGNATURES = {
         ctypes.c_int,
         [_vp, _vp, _vp, _i32, PaStepDims, PaNewRows, _vp, _vp, _vp, _vp, _i64, _i32, _f32, _vp, _vp],
     ),
-    "pa_rotate": (ctypes.c_int, [PaRotateRows, PaRotation, PaRowDims, _vp]),
+    "pa_rotate": (ctypes.c_int, [ctypes.POINTER(PaRotateDims), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "pa_rotate_and_cache": (
         ctypes.c_int,
-        [PaRotateRows, PaRotation, PaRowDims, _vp, _vp, _vp, _vp, _vp, _i32, _vp],
+        [ctypes.POINTER(PaRotateDims), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp],
+    ),
+    "pa_attention_step_8bit": (
+        ctypes.c_int,
+        [ctypes.POINTER(PaStepCall), _vp, _vp, _vp, _vp, _vp, _i32, ctypes.POINTER(PaNewRows), _f32, _vp, _vp],
     ),
     "pa_reshape_and_cache_8bit": (
         ctypes.c_int,

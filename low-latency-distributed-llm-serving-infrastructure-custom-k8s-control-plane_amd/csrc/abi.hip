@@ -894,8 +894,8 @@ int pa_attention_step(const PaStepCall* call, const void* query, void* key_cache
 
 namespace {
 
-// Whether `dims` and `rotation` describe rows the kernels take.
-int check_rows(const char* who, const PaRowDims& d, const PaRotation& r, bool query) {
+// Whether `d` describes rows the kernels take.
+int check_rows(const char* who, const PaRotateDims& d, bool query, bool weights) {
   if (elem_bytes(d.dtype) == 0) return fail(PA_ERR_INVALID_ARGUMENT, "%s: unknown dtype %d", who, d.dtype);
   if (d.num_tokens < 0 || (query ? d.num_query_heads <= 0 : d.num_query_heads != 0) || d.num_kv_heads <= 0 ||
       d.head_dim <= 0)
@@ -905,50 +905,50 @@ int check_rows(const char* who, const PaRowDims& d, const PaRotation& r, bool qu
   if (static_cast<int64_t>(d.num_tokens) * (static_cast<int64_t>(d.num_query_heads) + 2 * d.num_kv_heads) >
       0x3fffffffLL)
     return fail(PA_ERR_UNSUPPORTED, "%s: too many rows in one call", who);
-  if (r.rotary_dim < 0 || r.rotary_dim % 2 != 0 || r.rotary_dim > d.head_dim)
+  if (d.rotary_dim < 0 || d.rotary_dim % 2 != 0 || d.rotary_dim > d.head_dim)
     return fail(PA_ERR_INVALID_ARGUMENT, "%s: rotary_dim must be even and at most head_dim (%d), got %d", who,
-                d.head_dim, r.rotary_dim);
-  if (r.rotary_dim > 0 && r.num_positions <= 0)
+                d.head_dim, d.rotary_dim);
+  if (d.rotary_dim > 0 && d.num_positions <= 0)
     return fail(PA_ERR_INVALID_ARGUMENT, "%s: the table needs at least one position", who);
-  if ((r.query_weight != nullptr || r.key_weight != nullptr) && r.weight_dtype != d.dtype &&
-      r.weight_dtype != PA_DTYPE_F32)
+  if (weights && d.weight_dtype != d.dtype && d.weight_dtype != PA_DTYPE_F32)
     return fail(PA_ERR_INVALID_ARGUMENT, "%s: weight_dtype must be the rows' or PA_DTYPE_F32", who);
   return PA_OK;
 }
 
-pa::RotateArgs rotate_args(const PaRotateRows& w, const PaRotation& r, const PaRowDims& d) {
-  pa::RotateArgs a{};
-  a.query = w.query;
-  a.key = w.key;
-  a.value = w.value;
-  a.q_token_stride = w.query_token_stride;
-  a.q_head_stride = w.query_head_stride;
-  a.k_token_stride = w.key_token_stride;
-  a.k_head_stride = w.key_head_stride;
-  a.v_token_stride = w.value_token_stride;
-  a.v_head_stride = w.value_head_stride;
-  a.query_out = w.query_out;
-  a.q_out_token_stride = w.query_out_token_stride;
-  a.q_out_head_stride = w.query_out_head_stride;
-  a.positions = r.positions;
-  a.cos_sin = r.cos_sin;
-  a.num_positions = r.num_positions;
-  a.query_weight = r.query_weight;
-  a.key_weight = r.key_weight;
-  a.eps = r.eps;
-  a.weight_f32 = r.weight_dtype == PA_DTYPE_F32;
-  a.rotary_dim = r.rotary_dim;
-  a.interleaved = r.interleaved != 0;
-  a.num_tokens = d.num_tokens;
-  a.num_query_heads = d.num_query_heads;
-  a.num_kv_heads = d.num_kv_heads;
-  a.head_dim = d.head_dim;
-  a.block_size = d.block_size;
-  return a;
+// The arguments of `d`, after the checks (needs: pointers that must be there).
+int rotate_args(const char* who, const PaRotateDims& d, bool query, const int64_t* positions, const float* cos_sin,
+                const void* query_weight, const void* key_weight, pa::RotateArgs* a) {
+  int rc = check_rows(who, d, query, query_weight != nullptr || key_weight != nullptr);
+  if (rc == PA_OK && d.num_tokens > 0 && d.rotary_dim > 0)
+    rc = require(who, {{positions, "positions"}, {cos_sin, "cos_sin"}});
+  if (rc != PA_OK) return rc;
+  a->q_token_stride = d.query_token_stride;
+  a->q_head_stride = d.query_head_stride;
+  a->k_token_stride = d.key_token_stride;
+  a->k_head_stride = d.key_head_stride;
+  a->v_token_stride = d.value_token_stride;
+  a->v_head_stride = d.value_head_stride;
+  a->q_out_token_stride = d.query_out_token_stride;
+  a->q_out_head_stride = d.query_out_head_stride;
+  a->positions = positions;
+  a->cos_sin = cos_sin;
+  a->num_positions = d.num_positions;
+  a->query_weight = query_weight;
+  a->key_weight = key_weight;
+  a->eps = d.eps;
+  a->weight_f32 = d.weight_dtype == PA_DTYPE_F32;
+  a->rotary_dim = d.rotary_dim;
+  a->interleaved = d.interleaved != 0;
+  a->num_tokens = d.num_tokens;
+  a->num_query_heads = d.num_query_heads;
+  a->num_kv_heads = d.num_kv_heads;
+  a->head_dim = d.head_dim;
+  a->block_size = d.block_size;
+  return PA_OK;
 }
 
 // Points `a` at the layer's cache (and scales) after checking its geometry.
-int bind_cache(const char* who, const PaRowDims& d, int32_t layer_idx, void* key_cache, void* value_cache,
+int bind_cache(const char* who, const PaRotateDims& d, int32_t layer_idx, void* key_cache, void* value_cache,
                float* key_scales, float* value_scales, const int64_t* slot_mapping, pa::RotateArgs* a) {
   if (d.block_size <= 0 || d.total_blocks < 0)
     return fail(PA_ERR_INVALID_ARGUMENT, "%s: bad cache geometry", who);
@@ -983,38 +983,47 @@ int bind_cache(const char* who, const PaRowDims& d, int32_t layer_idx, void* key
 
 extern "C" {
 
-int pa_rotate(PaRotateRows rows, PaRotation rotation, PaRowDims dims, void* stream) {
-  int rc = check_rows("pa_rotate", dims, rotation, true);
-  if (rc != PA_OK || dims.num_tokens == 0) return rc;
-  rc = require("pa_rotate", {{rows.query, "rows.query"}, {rows.key, "rows.key"}, {rows.query_out, "rows.query_out"},
-                             {rows.key_out, "rows.key_out"}});
-  if (rc == PA_OK && rotation.rotary_dim > 0)
-    rc = require("pa_rotate", {{rotation.positions, "positions"}, {rotation.cos_sin, "cos_sin"}});
+int pa_rotate(const PaRotateDims* dims, const void* query, const void* key, const int64_t* positions,
+              const float* cos_sin, const void* query_weight, const void* key_weight, void* query_out, void* key_out,
+              void* stream) {
+  const char* who = "pa_rotate";
+  int rc = require(who, {{dims, "dims"}});
   if (rc != PA_OK) return rc;
-  pa::RotateArgs a = rotate_args(rows, rotation, dims);
-  a.value = nullptr;
+  pa::RotateArgs a{};
+  rc = rotate_args(who, *dims, true, positions, cos_sin, query_weight, key_weight, &a);
+  if (rc != PA_OK || dims->num_tokens == 0) return rc;
+  rc = require(who, {{query, "query"}, {key, "key"}, {query_out, "query_out"}, {key_out, "key_out"}});
+  if (rc != PA_OK) return rc;
+  a.query = query;
+  a.key = key;
   a.v_token_stride = a.v_head_stride = 0;
-  a.key_out = rows.key_out;
-  a.k_out_token_stride = rows.key_out_token_stride;
-  a.k_out_head_stride = rows.key_out_head_stride;
-  return from_hip(pa::launch_rotate(a, dims.dtype, static_cast<hipStream_t>(stream)), "pa_rotate");
+  a.query_out = query_out;
+  a.key_out = key_out;
+  a.k_out_token_stride = dims->key_out_token_stride;
+  a.k_out_head_stride = dims->key_out_head_stride;
+  return from_hip(pa::launch_rotate(a, dims->dtype, static_cast<hipStream_t>(stream)), who);
 }
 
-int pa_rotate_and_cache(PaRotateRows rows, PaRotation rotation, PaRowDims dims, void* key_cache, void* value_cache,
+int pa_rotate_and_cache(const PaRotateDims* dims, const void* query, const void* key, const void* value,
+                        const int64_t* positions, const float* cos_sin, const void* query_weight,
+                        const void* key_weight, void* query_out, void* key_cache, void* value_cache,
                         float* key_scales, float* value_scales, const int64_t* slot_mapping, int32_t layer_idx,
                         void* stream) {
   const char* who = "pa_rotate_and_cache";
-  int rc = check_rows(who, dims, rotation, true);
+  int rc = require(who, {{dims, "dims"}});
   if (rc != PA_OK) return rc;
-  pa::RotateArgs a = rotate_args(rows, rotation, dims);
-  rc = bind_cache(who, dims, layer_idx, key_cache, value_cache, key_scales, value_scales, slot_mapping, &a);
-  if (rc != PA_OK || dims.num_tokens == 0) return rc;
-  rc = require(who, {{rows.query, "rows.query"}, {rows.key, "rows.key"}, {rows.value, "rows.value"},
-                     {rows.query_out, "rows.query_out"}});
-  if (rc == PA_OK && rotation.rotary_dim > 0)
-    rc = require(who, {{rotation.positions, "positions"}, {rotation.cos_sin, "cos_sin"}});
+  pa::RotateArgs a{};
+  rc = rotate_args(who, *dims, true, positions, cos_sin, query_weight, key_weight, &a);
   if (rc != PA_OK) return rc;
-  return from_hip(pa::launch_rotate(a, dims.dtype, static_cast<hipStream_t>(stream)), who);
+  rc = bind_cache(who, *dims, layer_idx, key_cache, value_cache, key_scales, value_scales, slot_mapping, &a);
+  if (rc != PA_OK || dims->num_tokens == 0) return rc;
+  rc = require(who, {{query, "query"}, {key, "key"}, {value, "value"}, {query_out, "query_out"}});
+  if (rc != PA_OK) return rc;
+  a.query = query;
+  a.key = key;
+  a.value = value;
+  a.query_out = query_out;
+  return from_hip(pa::launch_rotate(a, dims->dtype, static_cast<hipStream_t>(stream)), who);
 }
 
 int pa_reshape_and_cache_8bit(const void* key, const void* value, int64_t key_token_stride, int64_t key_head_stride,
@@ -1024,23 +1033,28 @@ int pa_reshape_and_cache_8bit(const void* key, const void* value, int64_t key_to
                               int32_t head_dim, int32_t block_size, int32_t total_blocks, int32_t num_layers,
                               int32_t layer_idx, int32_t dtype, void* stream) {
   const char* who = "pa_reshape_and_cache_8bit";
-  const PaRowDims dims{num_tokens,   0,          num_kv_heads, head_dim,     block_size,
-                       total_blocks, num_layers, dtype,        PA_DTYPE_E4M3};
-  const PaRotation none{};
-  int rc = check_rows(who, dims, none, false);
+  PaRotateDims dims{};
+  dims.num_tokens = num_tokens;
+  dims.num_kv_heads = num_kv_heads;
+  dims.head_dim = head_dim;
+  dims.dtype = dtype;
+  dims.cache_dtype = PA_DTYPE_E4M3;
+  dims.block_size = block_size;
+  dims.total_blocks = total_blocks;
+  dims.num_layers = num_layers;
+  dims.key_token_stride = key_token_stride;
+  dims.key_head_stride = key_head_stride;
+  dims.value_token_stride = value_token_stride;
+  dims.value_head_stride = value_head_stride;
+  pa::RotateArgs a{};
+  int rc = rotate_args(who, dims, false, nullptr, nullptr, nullptr, nullptr, &a);
   if (rc != PA_OK) return rc;
-  PaRotateRows rows{};
-  rows.key = key;
-  rows.value = value;
-  rows.key_token_stride = key_token_stride;
-  rows.key_head_stride = key_head_stride;
-  rows.value_token_stride = value_token_stride;
-  rows.value_head_stride = value_head_stride;
-  pa::RotateArgs a = rotate_args(rows, none, dims);
   rc = bind_cache(who, dims, layer_idx, key_cache, value_cache, key_scales, value_scales, slot_mapping, &a);
   if (rc != PA_OK || num_tokens == 0) return rc;
   rc = require(who, {{key, "key"}, {value, "value"}});
   if (rc != PA_OK) return rc;
+  a.key = key;
+  a.value = value;
   return from_hip(pa::launch_rotate(a, dtype, static_cast<hipStream_t>(stream)), who);
 }
 
@@ -1065,6 +1079,35 @@ int pa_prefill_8bit(const void* query, const void* key_cache, const void* value_
   return prefill_impl("pa_prefill_8bit", query, key_cache, value_cache, layer_idx, dims, block_tables, context_lens,
                       cu_seqlens, prefill_items, num_prefill_items, prefill_tile, scaling, output, stream, nullptr,
                       &scales);
+}
+
+int pa_attention_step_8bit(const PaStepCall* call, const void* query, void* key_cache, void* value_cache,
+                           float* key_scales, float* value_scales, int32_t layer_idx, const PaNewRows* new_rows,
+                           float scaling, void* output, void* stream) {
+  int rc = require("pa_attention_step_8bit", {{call, "call"}});
+  if (rc != PA_OK) return rc;
+  const PaStepCall& c = *call;
+  const PaCacheScales scales{key_scales, value_scales};
+  if (new_rows != nullptr) {
+    rc = pa_reshape_and_cache_8bit(new_rows->key, new_rows->value, new_rows->key_token_stride,
+                                   new_rows->key_head_stride, new_rows->value_token_stride,
+                                   new_rows->value_head_stride, key_cache, value_cache, key_scales, value_scales,
+                                   c.scatter_slots, c.dims.num_query_tokens, c.dims.num_kv_heads, c.dims.head_dim,
+                                   c.dims.block_size, c.dims.total_blocks, c.dims.num_layers, layer_idx, c.dims.dtype,
+                                   stream);
+    if (rc != PA_OK) return rc;
+  }
+  if (c.num_prefill_items > 0) {
+    rc = pa_prefill_8bit(query, key_cache, value_cache, scales, layer_idx, c.dims, c.block_tables, c.context_lens,
+                         c.cu_seqlens, c.prefill_items, c.num_prefill_items, c.prefill_tile, scaling, output, stream);
+    if (rc != PA_OK) return rc;
+  }
+  if (c.num_decode_items > 0)
+    return pa_decode_8bit(PA_DECODE_PHASE_PARTITIONS | PA_DECODE_PHASE_MERGE, query, key_cache, value_cache, scales,
+                          layer_idx, c.dims, c.block_tables, c.context_lens, c.cu_seqlens, c.decode_items,
+                          c.num_decode_items, c.merge_items, c.num_merge_items, scaling, output, c.workspace,
+                          c.workspace_bytes, stream);
+  return PA_OK;
 }
 
 }  // extern "C"

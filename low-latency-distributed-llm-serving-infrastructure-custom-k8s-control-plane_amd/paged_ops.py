@@ -59,10 +59,13 @@ def cache_dtype_code(dtype: torch.dtype) -> int:
     return _native.PA_DTYPE_E4M3 if dtype == CODE_DTYPE else dtype_code(dtype)
 
 
+_NO_CONTEXT = contextlib.nullcontext()
+
+
 def _current(device: torch.device):
     """Makes ``device`` current for a launch where it is not."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        return _NO_CONTEXT
     return torch.cuda.device(device)
 
 
@@ -870,9 +873,9 @@ def rope_table(num_positions: int, rotary_dim: int, theta: float = 10000.0,
     return torch.cat([angle.cos(), angle.sin()], dim=1).float()
 
 
-def _rotate_inputs(query, key, positions, cos_sin, query_weight, key_weight, eps, interleaved):
-    """(query, key, positions, PaRotation) after the checks both rotations
-    share; rows without unit stride along D are copied."""
+def _rotate_dims(query, key, positions, cos_sin, query_weight, key_weight, eps, interleaved) -> _native.PaRotateDims:
+    """What both rotations hand to the library, after the checks they share
+    (the output's strides and the cache's sizes are the caller's to fill in)."""
     if query.dim() != 3 or key.dim() != 3 or query.shape[0] != key.shape[0] or query.shape[2] != key.shape[2]:
         raise ValueError(f"query and key must be (T, H_q, D) and (T, H_kv, D), got {tuple(query.shape)} and "
                          f"{tuple(key.shape)}")
@@ -897,25 +900,43 @@ def _rotate_inputs(query, key, positions, cos_sin, query_weight, key_weight, eps
         if weight_dtype is not None and w.dtype != weight_dtype:
             raise ValueError("query_weight and key_weight must have the same dtype")
         weight_dtype = w.dtype
-    query = query if query.stride(2) == 1 else query.contiguous()
-    key = key if key.stride(2) == 1 else key.contiguous()
-    positions = positions.contiguous()
-    rotation = _native.PaRotation(
-        positions.data_ptr(), cos_sin.data_ptr(), int(cos_sin.shape[0]), rotary, int(bool(interleaved)),
-        _ptr(query_weight), _ptr(key_weight), code if weight_dtype is None else dtype_code(weight_dtype), float(eps))
-    return query, key, positions, rotation
+    return _native.PaRotateDims(
+        num_tokens=tokens, num_query_heads=int(query.shape[1]), num_kv_heads=int(key.shape[1]), head_dim=dim, dtype=code,
+        weight_dtype=code if weight_dtype is None else dtype_code(weight_dtype), rotary_dim=rotary,
+        interleaved=int(interleaved), num_positions=int(cos_sin.shape[0]), eps=eps, cache_dtype=code,
+        query_token_stride=query.stride(0), query_head_stride=query.stride(1), key_token_stride=key.stride(0),
+        key_head_stride=key.stride(1))
 
 
-def _rows_out(out: Optional[torch.Tensor], like: torch.Tensor, name: str) -> torch.Tensor:
-    """``out`` checked against the rows it gets (any token / head strides), or
-    a new contiguous tensor."""
-    if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+def _check_rows_out(out: torch.Tensor, like: torch.Tensor, name: str) -> None:
+    """ValueError unless ``out`` can take the rows of ``like`` (any token /
+    head strides)."""
     if tuple(out.shape) != tuple(like.shape) or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} must have shape {tuple(like.shape)}, dtype {like.dtype} and be on {like.device}")
     if out.stride(2) != 1 or any(out.shape[i] > 1 and out.stride(i) < out.shape[2] for i in (0, 1)):
         raise ValueError(f"{name} needs unit stride along D and rows of its own")
-    return out
+
+
+def _kind(t: Optional[torch.Tensor]):
+    """What a call's checks depend on of one of its tensors."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+# The checked dims of the last rotation calls, by everything the checks depend
+# on: a model's layers repeat the same call, whose checks took longer than its
+# launch (15 us a call, 10 with this).
+_ROTATE_CALLS: dict = {}
+_MAX_ROTATE_CALLS = 256
+
+
+def _kept(key, build):
+    cached = _ROTATE_CALLS.get(key)
+    if cached is None:
+        dims = build()
+        if len(_ROTATE_CALLS) >= _MAX_ROTATE_CALLS:
+            _ROTATE_CALLS.clear()
+        cached = _ROTATE_CALLS[key] = ctypes.byref(dims)  # (keeps dims alive; never changed afterwards)
+    return cached
 
 
 def rotate(
@@ -941,19 +962,35 @@ def rotate(
     rows' dtype or fp32.  fp32 arithmetic, rounded once.  A position outside
     the table gives NaN rows.  ``out_query`` / ``out_key`` may be the inputs.
     """
-    device = _require_device(query, key, positions, cos_sin, query_weight, key_weight)
-    query, key, positions, rotation = _rotate_inputs(query, key, positions, cos_sin, query_weight, key_weight, eps,
-                                                     interleaved)
-    out_query = _rows_out(out_query, query, "out_query")
-    out_key = _rows_out(out_key, key, "out_key")
-    rows = _native.PaRotateRows(
-        query.data_ptr(), key.data_ptr(), None, query.stride(0), query.stride(1), key.stride(0), key.stride(1), 0, 0,
-        out_query.data_ptr(), out_query.stride(0), out_query.stride(1), out_key.data_ptr(), out_key.stride(0),
-        out_key.stride(1))
-    dims = _native.PaRowDims(int(query.shape[0]), int(query.shape[1]), int(key.shape[1]), int(query.shape[2]), 1, 0, 1,
-                             dtype_code(query.dtype), dtype_code(query.dtype))
-    with _current(device):
-        status = _native.load_library().pa_rotate(rows, rotation, dims, _stream(device))
+    if query.dim() == 3 and query.stride(2) != 1:
+        query = query.contiguous()
+    if key.dim() == 3 and key.stride(2) != 1:
+        key = key.contiguous()
+    positions = positions.contiguous()
+    eps, interleaved = float(eps), bool(interleaved)
+
+    def build():
+        _require_device(query, key, positions, cos_sin, query_weight, key_weight)
+        dims = _rotate_dims(query, key, positions, cos_sin, query_weight, key_weight, eps, interleaved)
+        for out, like, name in ((out_query, query, "query_out"), (out_key, key, "key_out")):
+            token, head = int(like.shape[1] * like.shape[2]), int(like.shape[2])
+            if out is not None:
+                _check_rows_out(out, like, name)
+                token, head = out.stride(0), out.stride(1)
+            setattr(dims, name + "_token_stride", token)
+            setattr(dims, name + "_head_stride", head)
+        return dims
+
+    dims = _kept((_kind(query), _kind(key), _kind(positions), _kind(cos_sin), _kind(query_weight), _kind(key_weight),
+                  eps, interleaved, _kind(out_query), _kind(out_key)), build)
+    if out_query is None:
+        out_query = query.new_empty(query.shape)
+    if out_key is None:
+        out_key = key.new_empty(key.shape)
+    with _current(query.device):
+        status = _native.load_library().pa_rotate(
+            dims, query.data_ptr(), key.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(), _ptr(query_weight),
+            _ptr(key_weight), out_query.data_ptr(), out_key.data_ptr(), _stream(query.device))
     _native.check(status, "pa_rotate")
     return out_query, out_key
 
@@ -985,35 +1022,50 @@ def rotate_and_cache(
     ``out`` may be ``query``.  A token whose position lies outside the table
     gets a NaN query row and no K row.
     """
-    device = _require_device(query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin, query_weight,
-                             key_weight)
-    if key_cache.dim() != 5 or value_cache.shape != key_cache.shape:
-        raise ValueError("caches must be 5-D (layers, blocks, block_size, heads, dim) and alike")
-    if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
-        raise ValueError("caches must be contiguous")
-    num_layers, total_blocks, block_size, num_kv_heads, head_dim = key_cache.shape
-    if key.shape != value.shape or key.dim() != 3 or tuple(key.shape[1:]) != (num_kv_heads, head_dim):
-        raise ValueError(f"Expected keys shape (T, {num_kv_heads}, {head_dim}), got {tuple(key.shape)}")
-    scales = _cache_scales(key_cache, value_cache, key_scales, value_scales)
-    if value.dtype != key.dtype or (scales is None and (key.dtype != key_cache.dtype or key.dtype != value_cache.dtype)):
-        raise ValueError("key/value dtype must match the cache dtype")
-    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != key.shape[0]:
-        raise ValueError("slot_mapping must be int64 with one entry per token")
-    query, key, positions, rotation = _rotate_inputs(query, key, positions, cos_sin, query_weight, key_weight, eps,
-                                                     interleaved)
-    value = value if value.stride(2) == 1 else value.contiguous()
-    slot_mapping = slot_mapping.contiguous()
-    out = _rows_out(out, query, "out")
-    rows = _native.PaRotateRows(
-        query.data_ptr(), key.data_ptr(), value.data_ptr(), query.stride(0), query.stride(1), key.stride(0),
-        key.stride(1), value.stride(0), value.stride(1), out.data_ptr(), out.stride(0), out.stride(1), None, 0, 0)
-    dims = _native.PaRowDims(int(query.shape[0]), int(query.shape[1]), num_kv_heads, head_dim, block_size, total_blocks,
-                             num_layers, dtype_code(query.dtype), cache_dtype_code(key_cache.dtype))
-    with _current(device):
+    if query.dim() == 3 and query.stride(2) != 1:
+        query = query.contiguous()
+    if key.dim() == 3 and key.stride(2) != 1:
+        key = key.contiguous()
+    if value.dim() == 3 and value.stride(2) != 1:
+        value = value.contiguous()
+    positions, slot_mapping = positions.contiguous(), slot_mapping.contiguous()
+    eps, interleaved = float(eps), bool(interleaved)
+
+    def build():
+        _require_device(query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin, query_weight,
+                        key_weight)
+        if key_cache.dim() != 5 or value_cache.shape != key_cache.shape:
+            raise ValueError("caches must be 5-D (layers, blocks, block_size, heads, dim) and alike")
+        if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+            raise ValueError("caches must be contiguous")
+        if key.shape != value.shape or key.dim() != 3 or key.shape[1:] != key_cache.shape[3:]:
+            raise ValueError(f"Expected keys shape (T, {key_cache.shape[3]}, {key_cache.shape[4]}), got "
+                             f"{tuple(key.shape)}")
+        scales = _cache_scales(key_cache, value_cache, key_scales, value_scales)
+        if value.dtype != key.dtype or (scales is None and not key.dtype == key_cache.dtype == value_cache.dtype):
+            raise ValueError("key/value dtype must match the cache dtype")
+        if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != key.shape[0]:
+            raise ValueError("slot_mapping must be int64 with one entry per token")
+        dims = _rotate_dims(query, key, positions, cos_sin, query_weight, key_weight, eps, interleaved)
+        dims.value_token_stride, dims.value_head_stride = value.stride(0), value.stride(1)
+        dims.query_out_token_stride, dims.query_out_head_stride = query.shape[1] * query.shape[2], query.shape[2]
+        if out is not None:
+            _check_rows_out(out, query, "out")
+            dims.query_out_token_stride, dims.query_out_head_stride = out.stride(0), out.stride(1)
+        dims.cache_dtype = cache_dtype_code(key_cache.dtype)
+        dims.num_layers, dims.total_blocks, dims.block_size = (int(n) for n in key_cache.shape[:3])
+        return dims
+
+    dims = _kept((_kind(query), _kind(key), _kind(value), _kind(key_cache), _kind(value_cache), _kind(slot_mapping),
+                  _kind(positions), _kind(cos_sin), _kind(query_weight), _kind(key_weight), eps, interleaved,
+                  _kind(key_scales), _kind(value_scales), _kind(out)), build)
+    if out is None:
+        out = query.new_empty(query.shape)
+    with _current(query.device):
         status = _native.load_library().pa_rotate_and_cache(
-            rows, rotation, dims, key_cache.data_ptr(), value_cache.data_ptr(),
-            None if scales is None else scales.key, None if scales is None else scales.value,
-            slot_mapping.data_ptr(), int(layer_idx), _stream(device))
+            dims, query.data_ptr(), key.data_ptr(), value.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(),
+            _ptr(query_weight), _ptr(key_weight), out.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+            _ptr(key_scales), _ptr(value_scales), slot_mapping.data_ptr(), int(layer_idx), _stream(query.device))
     _native.check(status, "pa_rotate_and_cache")
     return out
 
@@ -1435,6 +1487,46 @@ def _attention_step(query, key_cache, value_cache, layer_idx, step, scaling, out
     return rows_out
 
 
+def _attention_step8(query, key_cache, value_cache, layer_idx, step, scaling, out, new_key, new_value, key_scales,
+                     value_scales) -> torch.Tensor:
+    """:func:`attention` over an 8-bit cache as one library call, of a step with
+    work items; checks and shared arguments kept as :func:`_attention_step`
+    keeps them."""
+    if query.stride()[-1:] != (1,):
+        query = _query_view(query)
+    if new_key is not None:
+        new_key = new_key if new_key.stride()[-1:] == (1,) else new_key.contiguous()
+        new_value = new_value if new_value.stride()[-1:] == (1,) else new_value.contiguous()
+    key = (_kind(query), _kind(key_cache), _kind(value_cache), _kind(key_scales), _kind(value_scales),
+           _kind(new_key), _kind(new_value))
+    cached = step.__dict__.get("_layer_call8")
+    if cached is None or cached[0] != key:
+        q, dims, _ = _checked(query, key_cache, value_cache, step, key_scales, value_scales)
+        strides = None
+        if new_key is not None:
+            k, v = _new_rows(new_key, new_value, key_cache, step)
+            if k.dtype != q.dtype:
+                raise ValueError(f"new_key dtype {k.dtype} differs from the query dtype {q.dtype}")
+            strides = (k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+        # (the step's workspace of other head counts stays alive with the call)
+        cached = (key, ctypes.byref(_step_call(step, dims)), tuple(q.shape), strides, step._extra_ws)
+        step.__dict__["_layer_call8"] = cached
+    _, call_ref, shape, strides, _ = cached
+    if out is None:
+        rows_out = query.new_empty(shape)
+    else:
+        rows_out = _output_for(_query_view(query), key_cache, out)
+    rows = None
+    if strides is not None:
+        rows = ctypes.byref(_native.PaNewRows(new_key.data_ptr(), new_value.data_ptr(), *strides))
+    with _current(query.device):
+        status = _native.load_library().pa_attention_step_8bit(
+            call_ref, query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
+            value_scales.data_ptr(), int(layer_idx), rows, float(scaling), rows_out.data_ptr(), _stream(query.device))
+    _native.check(status, "pa_attention_step_8bit")
+    return rows_out
+
+
 def attention(
     query: torch.Tensor,
     key_cache: torch.Tensor,
@@ -1476,9 +1568,13 @@ def attention(
         raise ValueError("new_key and new_value are given together")
     need_prefill = step.num_prefill_items > 0
     need_decode = step.num_decode_items > 0
-    if new_key is not None and (need_prefill or need_decode) and key_cache.dtype != CODE_DTYPE:
-        if key_scales is not None or value_scales is not None:
-            raise ValueError(f"scales go with a cache of {CODE_DTYPE}, not {key_cache.dtype}")
+    if key_cache.dtype == CODE_DTYPE:
+        if (need_prefill or need_decode) and key_scales is not None and value_scales is not None:
+            return _attention_step8(query, key_cache, value_cache, layer_idx, step, scaling, out, new_key, new_value,
+                                    key_scales, value_scales)
+    elif key_scales is not None or value_scales is not None:
+        raise ValueError(f"scales go with a cache of {CODE_DTYPE}, not {key_cache.dtype}")
+    elif new_key is not None and (need_prefill or need_decode):
         return _attention_step(query, key_cache, value_cache, layer_idx, step, scaling, out, new_key, new_value,
                                fused_prefill_write)
     q, dims, scales = _checked(query, key_cache, value_cache, step, key_scales, value_scales)

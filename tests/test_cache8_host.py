@@ -63,16 +63,16 @@ def test_rope_table():
 
 
 def rotation_call(q=(3, 4, 64), k=(3, 2, 64), dtype=torch.bfloat16, kdtype=None, pos=None, table=None, **kw):
-    return ops._rotate_inputs(torch.zeros(q, dtype=dtype), torch.zeros(k, dtype=kdtype or dtype),
+    return ops._rotate_dims(torch.zeros(q, dtype=dtype), torch.zeros(k, dtype=kdtype or dtype),
                               torch.zeros(3, dtype=torch.int64) if pos is None else pos,
                               ops.rope_table(8, 64) if table is None else table, kw.get("qw"), kw.get("kw"), 1e-6, False)
 
 
 def test_rotation_arguments():
-    assert rotation_call()[3].rotary_dim == 64
+    assert rotation_call().rotary_dim == 64
     f32, bf16 = torch.ones(64), torch.ones(64, dtype=torch.bfloat16)
-    assert rotation_call(qw=f32, kw=f32)[3].weight_dtype == native.PA_DTYPE_F32
-    assert rotation_call(kw=bf16)[3].weight_dtype == native.PA_DTYPE_BF16
+    assert rotation_call(qw=f32, kw=f32).weight_dtype == native.PA_DTYPE_F32
+    assert rotation_call(kw=bf16).weight_dtype == native.PA_DTYPE_BF16
     bad = [dict(q=(3, 64)), dict(q=(2, 4, 64)), dict(k=(3, 2, 32)), dict(kdtype=torch.float32), dict(dtype=torch.float64),
            dict(pos=torch.zeros(3, dtype=torch.int32)), dict(pos=torch.zeros(4, dtype=torch.int64)),
            dict(table=ops.rope_table(8, 66)), dict(table=ops.rope_table(8, 64).double()),
@@ -86,13 +86,11 @@ def test_rotation_arguments():
 
 def test_outputs_of_rows():
     like = torch.zeros((3, 4, 64), dtype=torch.bfloat16)
-    assert ops._rows_out(None, like, "out").shape == like.shape
-    wide = torch.zeros((3, 8, 64), dtype=torch.bfloat16)[:, 2:6]
-    assert ops._rows_out(wide, like, "out") is wide
+    ops._check_rows_out(torch.zeros((3, 8, 64), dtype=torch.bfloat16)[:, 2:6], like, "out")
     for bad in (like.float(), like[:2], torch.zeros((1, 4, 64), dtype=torch.bfloat16).expand(3, 4, 64),
-                torch.zeros((3, 64, 4), dtype=torch.bfloat16).transpose(1, 2)):
+                torch.zeros((3, 64, 4), dtype=torch.bfloat16).transpose(1, 2), like.to("meta")):
         with pytest.raises(ValueError):
-            ops._rows_out(bad, like, "out")
+            ops._check_rows_out(bad, like, "out")
 
 
 def test_the_least_scale():
@@ -103,72 +101,71 @@ def test_the_least_scale():
 FAKE = 1 << 20  # never read: the call is refused first
 
 
-def row_dims(**kw):
+def dims_of(**kw):
     d = dict(num_tokens=3, num_query_heads=4, num_kv_heads=2, head_dim=64, block_size=16, total_blocks=4, num_layers=2,
-             dtype=native.PA_DTYPE_BF16, cache_dtype=native.PA_DTYPE_BF16)
+             dtype=native.PA_DTYPE_BF16, cache_dtype=native.PA_DTYPE_BF16, weight_dtype=native.PA_DTYPE_BF16,
+             num_positions=8, rotary_dim=64, eps=1e-6)
     d.update(kw)
-    return native.PaRowDims(*d.values())
+    return ctypes.byref(native.PaRotateDims(**d))
 
 
-def rotation(**kw):
-    d = dict(positions=FAKE, cos_sin=FAKE, num_positions=8, rotary_dim=64, interleaved=0, query_weight=None,
-             key_weight=None, weight_dtype=native.PA_DTYPE_BF16, eps=1e-6)
-    d.update(kw)
-    return native.PaRotation(*d.values())
+POINTERS = dict(query=FAKE, key=FAKE, value=FAKE, positions=FAKE, cos_sin=FAKE, query_weight=None, key_weight=None,
+                query_out=FAKE, key_cache=FAKE, value_cache=FAKE, key_scales=None, value_scales=None, slots=FAKE)
 
 
-def rows(**kw):
-    r = native.PaRotateRows(query=FAKE, key=FAKE, value=FAKE, query_out=FAKE, key_out=FAKE)
-    for name, value in kw.items():
-        setattr(r, name, value)
-    return r
+def rotate(dims, **kw):
+    p = {**POINTERS, **kw}
+    return native.load_library().pa_rotate(dims, p["query"], p["key"], p["positions"], p["cos_sin"], p["query_weight"],
+                                           p["key_weight"], p["query_out"], p.get("key_out", FAKE), None)
+
+
+def rotate_and_cache(dims, layer=0, **kw):
+    return native.load_library().pa_rotate_and_cache(dims, *{**POINTERS, **kw}.values(), layer, None)
 
 
 @needs_library
-@pytest.mark.parametrize("dims,rot,status", [
+@pytest.mark.parametrize("dims,pointers,status", [
     (dict(dtype=9), {}, native.PA_ERR_INVALID_ARGUMENT),
     (dict(dtype=native.PA_DTYPE_E4M3, cache_dtype=native.PA_DTYPE_E4M3), {}, native.PA_ERR_INVALID_ARGUMENT),
     (dict(num_tokens=-1), {}, native.PA_ERR_INVALID_ARGUMENT),
     (dict(num_query_heads=0), {}, native.PA_ERR_INVALID_ARGUMENT),
     (dict(num_kv_heads=0), {}, native.PA_ERR_INVALID_ARGUMENT),
-    (dict(head_dim=264), dict(rotary_dim=64), native.PA_ERR_UNSUPPORTED),
+    (dict(head_dim=264), {}, native.PA_ERR_UNSUPPORTED),
     (dict(num_tokens=1 << 30), {}, native.PA_ERR_UNSUPPORTED),
-    ({}, dict(rotary_dim=63), native.PA_ERR_INVALID_ARGUMENT),
-    ({}, dict(rotary_dim=66), native.PA_ERR_INVALID_ARGUMENT),
-    ({}, dict(rotary_dim=-2), native.PA_ERR_INVALID_ARGUMENT),
-    ({}, dict(num_positions=0), native.PA_ERR_INVALID_ARGUMENT),
+    (dict(rotary_dim=63), {}, native.PA_ERR_INVALID_ARGUMENT),
+    (dict(rotary_dim=66), {}, native.PA_ERR_INVALID_ARGUMENT),
+    (dict(rotary_dim=-2), {}, native.PA_ERR_INVALID_ARGUMENT),
+    (dict(num_positions=0), {}, native.PA_ERR_INVALID_ARGUMENT),
     ({}, dict(positions=None), native.PA_ERR_INVALID_ARGUMENT),
     ({}, dict(cos_sin=None), native.PA_ERR_INVALID_ARGUMENT),
-    ({}, dict(query_weight=FAKE, weight_dtype=native.PA_DTYPE_F16), native.PA_ERR_INVALID_ARGUMENT),
+    ({}, dict(query=None), native.PA_ERR_INVALID_ARGUMENT),
+    ({}, dict(key=None), native.PA_ERR_INVALID_ARGUMENT),
+    ({}, dict(query_out=None), native.PA_ERR_INVALID_ARGUMENT),
+    (dict(weight_dtype=native.PA_DTYPE_F16), dict(query_weight=FAKE), native.PA_ERR_INVALID_ARGUMENT),
+    (dict(num_tokens=0), {}, native.PA_OK),
 ])
-def test_rotations_the_library_refuses(dims, rot, status):
-    lib = native.load_library()
-    assert lib.pa_rotate(rows(), rotation(**rot), row_dims(**dims), None) == status
-    assert lib.pa_rotate_and_cache(rows(), rotation(**rot), row_dims(**dims), FAKE, FAKE, None, None, FAKE, 0,
-                                   None) == status
+def test_rotations_the_library_refuses(dims, pointers, status):
+    assert rotate(dims_of(**dims), **pointers) == status
+    assert rotate_and_cache(dims_of(**dims), **pointers) == status
 
 
 @needs_library
 def test_caches_the_library_refuses():
     lib = native.load_library()
     codes = dict(cache_dtype=native.PA_DTYPE_E4M3)
-
-    def call(dims, key_scales=None, value_scales=None, layer=0, cache=FAKE, slots=FAKE, **kw):
-        return lib.pa_rotate_and_cache(rows(**kw), rotation(), row_dims(**dims), cache, FAKE, key_scales, value_scales,
-                                       slots, layer, None)
-
     bad = native.PA_ERR_INVALID_ARGUMENT
-    assert call(codes) == bad
-    assert call(codes, FAKE, None) == bad
-    assert call({}, FAKE, FAKE) == bad
-    assert call(dict(cache_dtype=native.PA_DTYPE_F16)) == bad
-    assert call(dict(block_size=0)) == bad
-    assert call({}, layer=2) == bad and call({}, layer=-1) == bad
-    assert call({}, cache=None) == bad and call({}, slots=None) == bad
-    assert call({}, value=None) == bad and call({}, query_out=None) == bad
-    assert call(dict(block_size=257, **codes), FAKE, FAKE) == native.PA_ERR_UNSUPPORTED
-    assert call(dict(num_tokens=0)) == native.PA_OK  # nothing to do
-    assert b"scales" in (call(codes), lib.pa_last_error_message())[1]
+    assert rotate_and_cache(dims_of(**codes)) == bad
+    assert b"scales" in lib.pa_last_error_message()
+    assert rotate_and_cache(dims_of(**codes), key_scales=FAKE) == bad
+    assert rotate_and_cache(dims_of(), key_scales=FAKE, value_scales=FAKE) == bad
+    assert rotate_and_cache(dims_of(cache_dtype=native.PA_DTYPE_F16)) == bad
+    assert rotate_and_cache(dims_of(block_size=0)) == bad
+    assert rotate_and_cache(dims_of(), layer=2) == bad and rotate_and_cache(dims_of(), layer=-1) == bad
+    for name in ("key_cache", "value_cache", "slots", "value"):
+        assert rotate_and_cache(dims_of(), **{name: None}) == bad
+    assert rotate_and_cache(dims_of(block_size=257, **codes), key_scales=FAKE,
+                            value_scales=FAKE) == native.PA_ERR_UNSUPPORTED
+    assert rotate(None) == bad and rotate_and_cache(None) == bad and rotate(dims_of(), key_out=None) == bad
 
     def write(dtype=native.PA_DTYPE_BF16, key=FAKE, scales=FAKE, layer=0, bs=16, tokens=1, dim=64):
         return lib.pa_reshape_and_cache_8bit(key, FAKE, 64, 64, 64, 64, FAKE, FAKE, scales, scales, FAKE, tokens, 2,
@@ -202,3 +199,11 @@ def test_attention_the_library_refuses():
         ctypes.pointer(wrong)[0] = dims
         wrong.dtype = native.PA_DTYPE_E4M3
         assert call(d=wrong) == bad
+
+    def layer(call, scales=FAKE, rows=None):
+        return lib.pa_attention_step_8bit(call, FAKE, FAKE, FAKE, scales, scales, 0, rows, 1.0, FAKE, None)
+
+    one = native.PaStepCall(dims=dims, num_decode_items=1)
+    assert layer(None) == bad and layer(ctypes.byref(one), scales=None) == bad
+    assert layer(ctypes.byref(one), rows=ctypes.byref(native.PaNewRows())) == bad
+    assert layer(ctypes.byref(native.PaStepCall(dims=dims))) == native.PA_OK  # no work items
