@@ -110,15 +110,17 @@ class AttentionMetrics:
 
 
 def step_bytes(context_lens, num_query_tokens: int, num_query_heads: int, num_kv_heads: int, head_dim: int,
-               element_bytes: int, block_size: int) -> int:
+               element_bytes: int, block_size: int, row_bytes: int = 0) -> int:
     """Algorithmic HBM bytes of one layer's attention over a step: K and V of
     every context token once per KV head, the query and output rows, the
-    block-table entries and the context lengths."""
+    block-table entries and the context lengths.  ``row_bytes``: of a query
+    element over an 8-bit cache, whose blocks have two scales a KV head too
+    (0: the cache's element)."""
     ctx = [int(c) for c in context_lens]
-    kv = sum(ctx) * 2 * num_kv_heads * head_dim * element_bytes
-    qo = int(num_query_tokens) * num_query_heads * head_dim * 2 * element_bytes
-    tables = sum(-(-c // block_size) for c in ctx) * 4
-    return kv + qo + tables + 4 * len(ctx)
+    blocks = sum(-(-c // block_size) for c in ctx)
+    kv = sum(ctx) * 2 * num_kv_heads * head_dim * element_bytes + (blocks * 2 * num_kv_heads * 4 if row_bytes else 0)
+    qo = int(num_query_tokens) * num_query_heads * head_dim * 2 * (row_bytes or element_bytes)
+    return kv + qo + blocks * 4 + 4 * len(ctx)
 
 
 def cache_lines(manager=None, scheduler=None) -> List[str]:

@@ -130,7 +130,7 @@ class NativePagedBackend(AttentionBackend):
         if nbytes is None:
             nbytes = metrics.step_bytes(context.context_lens, context.num_query_tokens, int(query.shape[1]),
                                         store.num_heads, store.head_dim, store.key_cache.element_size(),
-                                        store.block_size)
+                                        store.block_size, query.element_size() if scales else 0)
             context._attention_bytes = nbytes
         recorder.end(start, nbytes, context.num_query_tokens, stream)
         return out.unsqueeze(0)

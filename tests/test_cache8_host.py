@@ -52,6 +52,13 @@ def test_a_cpu_store_of_codes_is_refused():
     assert pkg("memory.strategies").resolve_dtype("fp8") is CODE
 
 
+def test_bytes_of_a_step():
+    # 17 and 32 tokens in blocks of 16: two blocks each; K and V codes of two
+    # heads of 64, their scales, bf16 rows of 8 heads in and out, the table
+    got = pkg("metrics").step_bytes([17, 32], 2, 8, 2, 64, 1, 16, 2)
+    assert got == 49 * 2 * 2 * 64 + 4 * 2 * 2 * 4 + 2 * 8 * 64 * 2 * 2 + 4 * 4 + 2 * 4
+
+
 def test_rope_table():
     t = ops.rope_table(5, 8, theta=100.0)
     assert t.shape == (5, 8) and t.dtype == torch.float32

@@ -246,6 +246,14 @@ def test_decode_partitions(device, heads, kv_heads, dim, partition):
     attend(heads, kv_heads, dim, 16, starts, [1] * len(starts), torch.bfloat16, device, partition=partition)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [
+    (32, 16, 64, torch.bfloat16), (16, 16, 128, torch.float16), (32, 8, 128, torch.bfloat16)])
+def test_decode_of_many_sequences(device, heads, kv_heads, dim, dtype):
+    # launches of more work than the chip holds at once, some of it to merge
+    starts = [(7 * i) % 45 + (100 if i % 50 == 0 else 0) for i in range(540 * 8 // kv_heads)]
+    attend(heads, kv_heads, dim, 16, starts, [1] * len(starts), dtype, device, partition=64)
+
+
 @pytest.mark.parametrize("bs", [16, 4, 32])
 def test_missing_blocks_and_empty_rows(device, bs):
     # holes in the tables, a sequence whose only block is missing
@@ -351,6 +359,135 @@ def test_phases_streams_and_graphs(device):
         got = ops.attention(q, kc, vc, 0, step, 0.1, **args)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+def test_a_graph_of_two_layers_and_a_repacked_step(device):
+    # two captured graphs of one step, two layers each, that share its workspace
+    # and write their rows; the step moves on by a token between the replays
+    heads, kv, dim, bs, dtype = 8, 2, 64, 16, torch.bfloat16
+    starts, counts = [300, 40, 700], [1, 1, 1]
+    table = torch.arange(3 * 60, dtype=torch.int32, device=device).reshape(3, 60).flip(1).contiguous()
+    mine, want = (empty(2, 180, bs, kv, dim, device, garbage=True) for _ in range(2))
+    for c in (*mine[:2], *want[:2]):  # no NaN codes in the contexts
+        u = c.view(torch.uint8)
+        u[(u & 0x7F) == 0x7F] = 0x30
+    step = ops.pack_step(table, starts, counts, bs, num_kv_heads=kv, num_query_heads=heads, head_dim=dim, dtype=CODE,
+                         partition_size=128)
+    x = [torch.randn((3, heads + 2 * kv, dim), device=device).to(dtype) for _ in range(2)]
+    outs = [torch.empty((3, heads, dim), dtype=dtype, device=device) for _ in range(2)]
+
+    def layer(i, cache, step, out=None):
+        q, k, v = x[i].split([heads, kv, kv], dim=1)
+        return ops.attention(q, cache[0], cache[1], i, step, 0.125, out=out, new_key=k, new_value=v,
+                             key_scales=cache[2], value_scales=cache[3])
+
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    keep = [t.clone() for t in mine]
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph):
+            layer(i, mine, step, outs[i])
+    for t, k in zip(mine, keep):
+        assert torch.equal(t.view(torch.uint8), k.view(torch.uint8))  # (a capture runs nothing)
+    for move in range(4):
+        now = [s + move for s in starts]
+        if move:
+            step.repack(now)
+        fresh = ops.pack_step(table, now, counts, bs, num_kv_heads=kv, num_query_heads=heads, head_dim=dim, dtype=CODE,
+                              partition_size=128)
+        for t in x:
+            t.copy_(torch.randn_like(t.float()).to(dtype) * 2**move)
+        refs = [layer(i, want, fresh) for i in range(2)]
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i], refs[i]) and torch.isfinite(refs[i]).all()
+        for a, b in zip(mine, want):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,tokens", [(32, 8, 128, 1100), (9, 3, 64, 5000), (3, 1, 256, 3500)])
+def test_large_steps_are_their_parts(device, heads, kv_heads, dim, tokens):
+    # steps of more rows than the chip has lanes for, against calls of whole blocks
+    gen = torch.Generator(device=device).manual_seed(2)
+    x = torch.randn((tokens, heads + 2 * kv_heads, dim), generator=gen, device=device).to(torch.bfloat16)
+    q, k, v = x.split([heads, kv_heads, kv_heads], dim=1)
+    w = (1 + 0.1 * torch.randn(dim, generator=gen, device=device)).to(torch.bfloat16)
+    rope, pos = ops.rope_table(tokens, dim, device=device), torch.arange(tokens, device=device)
+    blocks = -(-tokens // 16) + 1
+    slots = torch.arange(tokens, device=device)
+    for codes in (False, True):
+        if codes:
+            mine, want = (empty(1, blocks, 16, kv_heads, dim, device) for _ in range(2))
+        else:
+            mine, want = ([torch.zeros((1, blocks, 16, kv_heads, dim), dtype=torch.bfloat16, device=device)
+                           for _ in range(2)] + [None, None] for _ in range(2))
+
+        def call(cache, lo, hi):
+            return ops.rotate_and_cache(q[lo:hi], k[lo:hi], v[lo:hi], cache[0], cache[1], slots[lo:hi], 0, pos[lo:hi],
+                                        rope, query_weight=w, key_scales=cache[2], value_scales=cache[3])
+
+        got = call(mine, 0, tokens)
+        parts = torch.cat([call(want, lo, min(lo + 160, tokens)) for lo in range(0, tokens, 160)])
+        assert torch.equal(got, parts)
+        for a, b in zip(mine, want):
+            assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_a_store_behind_the_layers_hook(device):
+    # a store of 8-bit codes as an engine runs it: prompts, a prompt in chunks,
+    # decodes and a swap, every layer's result against fp64 over what the store holds
+    heads, kv, dim, layers, dtype = 8, 2, 64, 2, torch.bfloat16
+    hook = pkg("model.paged_attention")
+    metrics = pkg("metrics")
+    request = pkg("engine.request").Request
+    store = pkg("memory.manager").PagedKVCacheManager(total_blocks=64, block_size=16, num_heads=kv, head_dim=dim,
+                                                      dtype=CODE, num_layers=layers, device=device, total_cpu_blocks=16)
+    store.num_query_heads = heads
+    gen = torch.Generator(device=device).manual_seed(5)
+
+    class Layer:
+        scaling = dim**-0.5
+
+    seqs = [request(i, list(range(n))) for i, n in enumerate((37, 120))]
+    for seq in seqs:
+        store.allocate_prefix_blocks(seq)
+    recorder = metrics.enable()
+    try:
+        for starts, counts in (([0, 0], [37, 64]), ([37, 64], [1, 56]), ([38, 120], [1, 1]), ([39, 121], [1, 1])):
+            for seq, start, count in zip(seqs, starts, counts):
+                while seq.block_table.get_tokens_count() < start + count:
+                    store.allocate_slot_for_next_token(seq)
+            context = hook.PagedStepContext(store, seqs, starts, counts)
+            t = sum(counts)
+            for i in range(layers):
+                x = 2 * torch.randn((1, heads + 2 * kv, t, dim), generator=gen, device=device).to(dtype)
+                q, k, v = x.split([heads, kv, kv], dim=1)
+                module = Layer()
+                module.paged_context, module.layer_idx = context, i
+                out = hook.paged_attention_forward(module, q, k, v)[0][0].cpu().double()
+                rows = [store.gather_layer_keys(i, context.gather_slots), store.gather_layer_values(i, context.gather_slots)]
+                new = torch.cat([torch.arange(c)[s:] + o for o, s, c in zip(
+                    (0, starts[0] + counts[0]), starts, [a + b for a, b in zip(starts, counts)])]).to(device)
+                # half a step of e4m3, or of its least numbers (values below 16 keep scales below 16 / 224)
+                for got, given in zip(rows, (k, v)):
+                    given = given[0].transpose(0, 1).float()
+                    off = (got[new].float() - given).abs()
+                    assert (off <= 2.0**-4 * given.abs() + 2.0**-10 * 16 / 224).all()
+                n = [a + b for a, b in zip(starts, counts)]
+                pool = [torch.zeros((2, 256, kv, dim), dtype=torch.float64) for _ in range(2)]
+                for p, r in zip(pool, rows):
+                    for j, part in enumerate(r.cpu().double().split(n)):
+                        p[j, :n[j]] = part
+                ref, size, _ = oracle.attention(q[0].transpose(0, 1).cpu(), *pool, [[0], [1]], starts, counts, dim**-0.5)
+                u = 2.0**-8
+                assert ((out - ref).abs() <= 1.01 * u * ref.abs() + (2 * u + 1.5e-5) * size).all()
+            store.swap_out(seqs[0])
+            store.swap_in(seqs[0])
+        torch.cuda.synchronize()
+        assert recorder.poll() > 0
+    finally:
+        metrics.disable()
 
 
 def test_blocks_are_copied_and_swapped_with_their_scales(device):
