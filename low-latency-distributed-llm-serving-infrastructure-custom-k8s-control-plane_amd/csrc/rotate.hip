@@ -17,8 +17,8 @@
 // that the launch and two dependent reads (position, then table).  bf16 rows,
 // cold caches: 8 tokens of 32/8 heads of 128 2.4 us; 2176 tokens with norms
 // (54.6 MB) 17.6 us, 3.1 TB/s; 4096 tokens 28.9 us, 3.5 TB/s.  The 8-bit write:
-// 256 decode tokens 6.0 us; 1400 tokens of 32/32 heads of 128, fp16 with norms
-// (58 MB) 28 us; 15000 tokens of 9/3 heads of 64 (75 MB) 27 us, 2.8 TB/s: there
+// 256 decode tokens 6.2 us; 1400 tokens of 32/32 heads of 128, fp16 with norms
+// (58 MB) 25.6 us; 15000 tokens of 9/3 heads of 64 (75 MB) 26.5 us, 2.8 TB/s: there
 // each chunk reads the rows that may belong to its last run, which the next one
 // reads again, and waits for slots, rows and scales one after the other.
 #include "cache8.hpp"
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs a) {
   rotate_rows<T, L, VEC, NR>(a, ln, tok, static_cast<int>(id - tok * units) * NR, heads);
 }
 
-// The 8-bit cache's write.  The first a.kv_groups workgroups take (chunk of C
+// The 8-bit cache's write.  The first a.kv_groups workgroups take (chunk of
 // tokens, KV head, tensor) each, the others rows of Q.
 //
 // A block's scale depends on all of its rows, so one workgroup has to see
@@ -336,14 +336,17 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs a) {
 // looks at up to block_size - 1 tokens past its end and leaves the first ones
 // to the chunk before where their run began there.  It takes the rows' largest
 // magnitudes (kept in LDS by an integer maximum of the floats' bits, which no
-// order changes), settles the scales, and writes the codes.  KEEP: the span is
-// at most two rows a group, which are loaded first of all, beside the slots,
-// and stay in registers; else the rows are read (and rotated) again.  A run
+// order changes), settles the scales, and writes the codes.  KEPT: the span is
+// at most this many rows a group, which are loaded first of all, beside the
+// slots, and stay in registers; 0: the rows are read (and rotated) again.  A run
 // that holds its block's first row starts the block afresh; the other rows of
 // any other block are re-coded if its scale grows.
-template <typename T, int L, bool VEC, bool KEEP, int NR>
+template <typename T, int L, bool VEC, int KEPT, int NR>
 __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs a) {
-  constexpr int C = kRotateThreads / L;  // tokens a chunk owns, rows at once
+  constexpr int C = kRotateThreads / L;                 // rows at once
+  constexpr int kOwn = KEPT > 0 ? (KEPT - 1) * C : C;   // tokens of a chunk
+  constexpr bool KEEP = KEPT > 0;
+  static_assert(kOwn <= kWave, "a lane for each of its runs");
   constexpr int kN = RowLane<T, L, VEC>::kN;
   const RowLane<T, L, VEC> ln(a, threadIdx.x % L);
   const int group = threadIdx.x / L;
@@ -355,25 +358,25 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
     rotate_rows<T, L, VEC, NR>(a, ln, tok, static_cast<int>(id - tok * units) * NR, a.num_query_heads);
     return;
   }
-  // Per run that begins in the chunk (at token C c + i): its block, whether it
+  // Per run that begins in the chunk (at token kOwn c + i): its block, whether it
   // holds the block's first row, its largest magnitude's bits, the scale the
   // block has (0 if it starts afresh); and one past the last run's last token.
-  __shared__ int64_t s_block[C];
-  __shared__ int s_fresh[C], s_end;
-  __shared__ uint32_t s_amax[C];
-  __shared__ float s_old[C];
+  __shared__ int64_t s_block[kOwn];
+  __shared__ int s_fresh[kOwn], s_end;
+  __shared__ uint32_t s_amax[kOwn];
+  __shared__ float s_old[kOwn];
   // Per token of the span: the run it belongs to (< 0: none of the chunk's),
   // and its row of the cache.
-  __shared__ int16_t s_run[C + kMaxCache8Block];
-  __shared__ int64_t s_slot[C + kMaxCache8Block];
+  __shared__ int16_t s_run[kOwn + kMaxCache8Block];
+  __shared__ int64_t s_slot[kOwn + kMaxCache8Block];
 
   const uint32_t units = 2 * a.num_kv_heads;
   const uint32_t chunk = quotient(blockIdx.x, units, a.kv_rcp);
   const int u = static_cast<int>(blockIdx.x - chunk * units);
   const bool is_v = u >= a.num_kv_heads;
   const int h = is_v ? u - a.num_kv_heads : u;
-  const int64_t t0 = static_cast<int64_t>(chunk) * C;
-  const int span = static_cast<int>(min<int64_t>(C + a.block_size - 1, a.num_tokens - t0));
+  const int64_t t0 = static_cast<int64_t>(chunk) * kOwn;
+  const int span = static_cast<int>(min<int64_t>(kOwn + a.block_size - 1, a.num_tokens - t0));
   const T* src = reinterpret_cast<const T*>(is_v ? a.value : a.key) + h * (is_v ? a.v_head_stride : a.k_head_stride);
   const int64_t tok_stride = is_v ? a.v_token_stride : a.k_token_stride;
   const void* w = is_v ? nullptr : a.key_weight;
@@ -405,7 +408,7 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
         if (fabsf(x[i]) < INFINITY) x[i] = fminf(fmaxf(x[i], -kMaxF16Row), kMaxF16Row);
     }
   };
-  constexpr int kKept = KEEP ? 2 : 1;
+  constexpr int kKept = KEEP ? KEPT : 1;
   float x[kKept][kN];
   Raw raw[kKept];
   float4 cs[kKept], sn[kKept];
@@ -413,13 +416,13 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
   bool ok[kKept];
   if constexpr (KEEP) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < kKept; ++k)
       load_row(min(group + k * C, span - 1), &raw[k], &pos[k], &ok[k], &cs[k], &sn[k]);
   }
 
   float* scales = (is_v ? a.value_scales : a.key_scales) + h;
-  float old = 0.f;  // lane i < C of the first wave: the scale of run i's block
-  if (threadIdx.x < C) {
+  float old = 0.f;  // lane i < kOwn of the first wave: the scale of run i's block
+  if (threadIdx.x < kOwn) {
     s_block[threadIdx.x] = -1;
     s_end = 0;
     s_fresh[threadIdx.x] = 0;
@@ -454,7 +457,7 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
       const uint64_t mask = __ballot(starts);
       const uint64_t upto = mask & (~uint64_t{0} >> (kWave - 1 - threadIdx.x));
       const int lead = upto != 0 ? base + 63 - __builtin_clzll(upto) : last;
-      const bool ours = lead >= 0 && lead < C && blk >= 0;
+      const bool ours = lead >= 0 && lead < kOwn && blk >= 0;
       if (j < span) {
         s_run[j] = static_cast<int16_t>(ours ? lead : -1);
         s_slot[j] = slot;
@@ -466,7 +469,7 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
       }
       if (mask != 0) last = base + 63 - __builtin_clzll(mask);
       // (run i begins at token i, so its lane holds its block)
-      if (base == 0 && threadIdx.x < C && ours && starts) old = scale_pow2(scales[blk * a.num_kv_heads]);
+      if (base == 0 && threadIdx.x < kOwn && ours && starts) old = scale_pow2(scales[blk * a.num_kv_heads]);
     }
   }
   __syncthreads();
@@ -484,7 +487,7 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
   };
   if constexpr (KEEP) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < kKept; ++k) {
       const int j = group + k * C;
       const int run = j < end ? s_run[j] : -1;
       ok[k] = run >= 0 && ok[k];
@@ -501,21 +504,21 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
       if (ok[0]) note(s_run[j], x[0]);
     }
   }
-  if (threadIdx.x < C) s_old[threadIdx.x] = s_fresh[threadIdx.x] ? 0.f : old;
+  if (threadIdx.x < kOwn) s_old[threadIdx.x] = s_fresh[threadIdx.x] ? 0.f : old;
   __syncthreads();
   auto new_scale = [&](int run) { return fmaxf(s_old[run], scale_for(__uint_as_float(s_amax[run]))); };
   // What the other rows of a run's block are re-coded by (1: not at all).
   auto recode = [&](int run) {
     return s_block[run] < 0 || s_fresh[run] ? 1.f : s_old[run] * inverse_pow2(new_scale(run));
   };
-  if (threadIdx.x < C && s_block[threadIdx.x] >= 0)
+  if (threadIdx.x < kOwn && s_block[threadIdx.x] >= 0)
     scales[s_block[threadIdx.x] * a.num_kv_heads] = new_scale(threadIdx.x);
   uint8_t* cache = reinterpret_cast<uint8_t*>(is_v ? a.value_cache : a.key_cache) + h * a.head_dim;
   const int64_t row_codes = static_cast<int64_t>(a.num_kv_heads) * a.head_dim;
   // Blocks whose scale grew: all of their rows; the run's own follow below.
   const int lane = threadIdx.x % kWave;
-  if (__any(lane < C && recode(min(lane, C - 1)) != 1.f)) {  // (alike in every wave)
-    for (int i = 0; i < C; ++i) {
+  if (__any(lane < kOwn && recode(min(lane, kOwn - 1)) != 1.f)) {  // (alike in every wave)
+    for (int i = 0; i < kOwn; ++i) {
       const float ratio = recode(i);
       if (ratio == 1.f) continue;
       uint8_t* rows = cache + s_block[i] * a.block_size * row_codes;
@@ -555,7 +558,7 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
   };
   if constexpr (KEEP) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < kKept; ++k)
       if (ok[k]) write(group + k * C, x[k]);
   } else {
     for (int j = group; j < end; j += C) {
@@ -566,6 +569,9 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
     }
   }
 }
+
+// Lanes the chip holds at a time: 2048 on each of 256 CUs.
+constexpr int64_t kResidentLanes = 256 * 2048;
 
 template <typename T, int L, bool VEC, int NR>
 static hipError_t launch_rotate_n(const RotateArgs& args, hipStream_t s) {
@@ -583,26 +589,36 @@ static hipError_t launch_rotate_n(const RotateArgs& args, hipStream_t s) {
     return hipGetLastError();
   }
   a.kv_rcp = 0xffffffffu / (2 * a.num_kv_heads);
-  a.kv_groups = static_cast<uint32_t>((a.num_tokens + kRows - 1) / kRows * (2 * a.num_kv_heads));
+  // Three rows a group, so that a chunk re-reads half as much of its
+  // neighbour's, once its rows of K and V alone would fill the chip (see
+  // kResidentLanes); a chunk of two has less to wait for.  Two against three:
+  // bf16, 32/8 heads of 128, 256 tokens 6.1 / 7.5 us, 1024 10.0 / 11.2, 2048
+  // 17.4 / 16.7; fp16, 32/32 of 128, 384 tokens 10.4 / 11.2, 512 13.4 / 12.8,
+  // 4096 69.1 / 61.8; 9/3 heads of 64, 8192 tokens 13.5 / 13.9, 16384 23.5 /
+  // 22.3; 8/2 heads of 256, 2048 tokens 10.0 / 10.8, 8192 31.7 / 29.1.
+  const bool keep = a.block_size <= kRows + 1;
+  const bool three = keep && static_cast<int64_t>(a.num_tokens) * 2 * a.num_kv_heads * L >= kResidentLanes;
+  const int own = three ? 2 * kRows : kRows;
+  a.kv_groups = static_cast<uint32_t>((a.num_tokens + own - 1) / own * (2 * a.num_kv_heads));
   a.log2_block = -1;
   for (int i = 0; i <= 8; ++i)
     if (1 << i == a.block_size) a.log2_block = i;
-  if (a.block_size <= kRows + 1)
-    hipLaunchKernelGGL((cache8_write_kernel<T, L, VEC, true, NR>), dim3(a.kv_groups + grid), dim3(kRotateThreads), 0, s, a);
+  if (three)
+    hipLaunchKernelGGL((cache8_write_kernel<T, L, VEC, 3, NR>), dim3(a.kv_groups + grid), dim3(kRotateThreads), 0, s, a);
+  else if (keep)
+    hipLaunchKernelGGL((cache8_write_kernel<T, L, VEC, 2, NR>), dim3(a.kv_groups + grid), dim3(kRotateThreads), 0, s, a);
   else
-    hipLaunchKernelGGL((cache8_write_kernel<T, L, VEC, false, NR>), dim3(a.kv_groups + grid), dim3(kRotateThreads), 0, s, a);
+    hipLaunchKernelGGL((cache8_write_kernel<T, L, VEC, 0, NR>), dim3(a.kv_groups + grid), dim3(kRotateThreads), 0, s, a);
   return hipGetLastError();
 }
 
 // Two heads to a group of lanes once one each would take more lanes than the
-// chip holds at a time (2048 on each of 256 CUs): from there on loads in
-// flight are what counts, and below it the depth of one row's work.  One
-// against two, bf16, 32/8 heads of 128 with norms: 256 tokens 4.6 / 4.9 us,
-// 512 6.7 / 6.7, 768 9.7 / 8.7, 4096 36.3 / 28.9; 9/3 heads of 64: 1024 tokens
-// 3.9 / 4.2 us, 4096 7.2 / 7.2; fp32, 8/8 heads of 64: 1024 5.6 / 6.2 us, 4096
-// 13.3 / 13.4.  Four: 18.2 us where two took 17.9 and one 21.3.
-constexpr int64_t kResidentLanes = 256 * 2048;
-
+// chip holds: from there on loads in flight are what counts, and below it the
+// depth of one row's work.  One against two, bf16, 32/8 heads of 128 with
+// norms: 256 tokens 4.6 / 4.9 us, 512 6.7 / 6.7, 768 9.7 / 8.7, 4096 36.3 /
+// 28.9; 9/3 heads of 64: 1024 tokens 3.9 / 4.2 us, 4096 7.2 / 7.2; fp32, 8/8
+// heads of 64: 1024 5.6 / 6.2 us, 4096 13.3 / 13.4.  Four: 18.2 us where two
+// took 17.9 and one 21.3.
 template <typename T, int L, bool VEC>
 static hipError_t launch_rotate_l(const RotateArgs& a, hipStream_t s) {
   if constexpr (VEC) {

@@ -406,21 +406,23 @@ def test_a_graph_of_two_layers_and_a_repacked_step(device):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
 
-@pytest.mark.parametrize("heads,kv_heads,dim,tokens", [(32, 8, 128, 1100), (9, 3, 64, 5000), (3, 1, 256, 3500)])
-def test_large_steps_are_their_parts(device, heads, kv_heads, dim, tokens):
+@pytest.mark.parametrize("heads,kv_heads,dim,bs,tokens", [
+    (32, 8, 128, 16, 1100), (9, 3, 64, 16, 5000), (3, 1, 256, 16, 3500), (8, 8, 128, 16, 2101), (9, 3, 64, 32, 11111),
+    (2, 2, 256, 8, 4203), (4, 2, 36, 4, 2100)])
+def test_large_steps_are_their_parts(device, heads, kv_heads, dim, bs, tokens):
     # steps of more rows than the chip has lanes for, against calls of whole blocks
     gen = torch.Generator(device=device).manual_seed(2)
     x = torch.randn((tokens, heads + 2 * kv_heads, dim), generator=gen, device=device).to(torch.bfloat16)
     q, k, v = x.split([heads, kv_heads, kv_heads], dim=1)
     w = (1 + 0.1 * torch.randn(dim, generator=gen, device=device)).to(torch.bfloat16)
     rope, pos = ops.rope_table(tokens, dim, device=device), torch.arange(tokens, device=device)
-    blocks = -(-tokens // 16) + 1
+    blocks = -(-tokens // bs) + 1
     slots = torch.arange(tokens, device=device)
     for codes in (False, True):
         if codes:
-            mine, want = (empty(1, blocks, 16, kv_heads, dim, device) for _ in range(2))
+            mine, want = (empty(1, blocks, bs, kv_heads, dim, device) for _ in range(2))
         else:
-            mine, want = ([torch.zeros((1, blocks, 16, kv_heads, dim), dtype=torch.bfloat16, device=device)
+            mine, want = ([torch.zeros((1, blocks, bs, kv_heads, dim), dtype=torch.bfloat16, device=device)
                            for _ in range(2)] + [None, None] for _ in range(2))
 
         def call(cache, lo, hi):
