@@ -919,12 +919,12 @@ def _check_rows_out(out: torch.Tensor, like: torch.Tensor, name: str) -> None:
 
 def _kind(t: Optional[torch.Tensor]):
     """What a call's checks depend on of one of its tensors."""
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
 # The checked dims of the last rotation calls, by everything the checks depend
 # on: a model's layers repeat the same call, whose checks took longer than its
-# launch (15 us a call, 10 with this).
+# launch (15 us a call, 9 with this).
 _ROTATE_CALLS: dict = {}
 _MAX_ROTATE_CALLS = 256
 
@@ -1056,9 +1056,16 @@ def rotate_and_cache(
         dims.num_layers, dims.total_blocks, dims.block_size = (int(n) for n in key_cache.shape[:3])
         return dims
 
-    dims = _kept((_kind(query), _kind(key), _kind(value), _kind(key_cache), _kind(value_cache), _kind(slot_mapping),
-                  _kind(positions), _kind(cos_sin), _kind(query_weight), _kind(key_weight), eps, interleaved,
-                  _kind(key_scales), _kind(value_scales), _kind(out)), build)
+    # (_kind written out: its calls would take 1 us)
+    dims = _kept((
+        query.shape, query.stride(), query.dtype, query.get_device(), key.shape, key.stride(), key.dtype,
+        key.get_device(), value.shape, value.stride(), value.dtype, value.get_device(), key_cache.shape,
+        key_cache.stride(), key_cache.dtype, key_cache.get_device(), value_cache.shape, value_cache.stride(),
+        value_cache.dtype, value_cache.get_device(), slot_mapping.shape, slot_mapping.dtype, slot_mapping.get_device(),
+        positions.shape, positions.dtype, positions.get_device(), cos_sin.shape, cos_sin.stride(), cos_sin.dtype,
+        cos_sin.get_device(), eps, interleaved, query_weight if query_weight is None else _kind(query_weight),
+        key_weight if key_weight is None else _kind(key_weight), key_scales if key_scales is None else _kind(key_scales),
+        value_scales if value_scales is None else _kind(value_scales), out if out is None else _kind(out)), build)
     if out is None:
         out = query.new_empty(query.shape)
     with _current(query.device):
