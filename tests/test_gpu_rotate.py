@@ -150,6 +150,27 @@ def test_rotate_and_cache_is_the_two_calls(device, heads, kv_heads, dim, rotary,
     assert torch.equal(mine[0], want[0]) and torch.equal(mine[1], want[1])
 
 
+@pytest.mark.parametrize("dim", [64, 36])
+def test_rows_that_do_not_turn(device, dim):
+    # the library's call without a table: norms alone
+    native = pkg("_native")
+    q, k, _ = rows(21, 4, 2, dim, torch.bfloat16)
+    w = weights(dim, torch.bfloat16)
+    outs = [torch.empty((21, n, dim), dtype=torch.bfloat16, device=device) for n in (4, 2)]
+    dims = native.PaRotateDims(
+        num_tokens=21, num_query_heads=4, num_kv_heads=2, head_dim=dim, dtype=native.PA_DTYPE_BF16,
+        weight_dtype=native.PA_DTYPE_BF16, eps=EPS, query_token_stride=q.stride(0), query_head_stride=dim,
+        key_token_stride=k.stride(0), key_head_stride=dim, query_out_token_stride=4 * dim, query_out_head_stride=dim,
+        key_out_token_stride=2 * dim, key_out_head_stride=dim)
+    status = native.load_library().pa_rotate(
+        dims, q.data_ptr(), k.data_ptr(), None, None, w[0].data_ptr(), w[1].data_ptr(), outs[0].data_ptr(),
+        outs[1].data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert status == native.PA_OK
+    still = torch.cat([torch.ones(1, dim // 2), torch.zeros(1, dim // 2)], 1)  # cosines, sines
+    for got, x, weight in zip(outs, (q, k), w):
+        check(got, x, weight, torch.zeros(21, dtype=torch.int64), still, False)
+
+
 def test_no_tokens(device):
     q, k, v = rows(0, 4, 2, 64, torch.bfloat16)
     table = ops.rope_table(4, 64, device=device)
