@@ -663,8 +663,9 @@ int pa_attention_step(const PaStepCall *call, const void *query, void *key_cache
  *    are re-coded with it (rounded to nearest even): their values stay but
  *    where they fall among the subnormal codes.
  *  - Rows are coded as the 16-bit cache would hold them, rounded to their type
- *    first; fp16 ones are limited to +-61440, the largest four-bit value below
- *    fp16's maximum.  Infinities and NaN become NaN and count for no scale.
+ *    first, and limited to the largest four-bit value below their type's
+ *    maximum: +-61440 in fp16, +-1.875 * 2^127 in bf16 and fp32.  Infinities
+ *    and NaN become NaN and count for no scale.
  *  - The tokens of one block follow each other in the call's slot_mapping (as
  *    pa_pack's scatter_slots have them), and no slot occurs twice.  (A mapping
  *    that breaks this reads and writes inside the caches, but leaves blocks

@@ -23,9 +23,11 @@ struct code8_t {
 // Least scale: 2^-64, so that a block of zeros has one and no product of a
 // code, a scale and a probability is lost among fp32's subnormals.
 constexpr int kMinScaleExp = -64;
-// Largest magnitude an fp16 row may hold: the largest four-bit value below
-// fp16's maximum (the next one, 65536, would read back as an infinity).
-constexpr float kMaxF16Row = 61440.f;
+// Largest magnitude a row may hold: the largest four-bit value below its type's
+// maximum (the next one, 2^16 in fp16 and 2^128 in bf16 and fp32, would read
+// back as an infinity).
+template <typename T>
+constexpr float kMaxRow8 = Elem<T>::kDtype == PA_DTYPE_F16 ? 61440.f : 0x1.ep127f;
 
 typedef __bf16 bf16x2c8 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2c8 __attribute__((ext_vector_type(2)));

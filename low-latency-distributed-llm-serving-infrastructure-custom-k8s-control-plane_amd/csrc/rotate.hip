@@ -404,8 +404,7 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       x[i] = rounded<T>(x[i]);
-      if constexpr (Elem<T>::kDtype == PA_DTYPE_F16)
-        if (fabsf(x[i]) < INFINITY) x[i] = fminf(fmaxf(x[i], -kMaxF16Row), kMaxF16Row);
+      if (fabsf(x[i]) < INFINITY) x[i] = fminf(fmaxf(x[i], -kMaxRow8<T>), kMaxRow8<T>);
     }
   };
   constexpr int kKept = KEEP ? KEPT : 1;

@@ -771,7 +771,8 @@ def reshape_and_cache(
     afresh, and one that writes later rows re-codes the block's others where
     its scale grows.  The tokens of a block follow each other in
     ``slot_mapping``, no slot occurs twice, and blocks have at most 256
-    tokens.  fp16 rows are limited to +-61440; infinities become NaN.
+    tokens.  Rows are limited to +-61440 (fp16) or
+    +-1.875 * 2^127; infinities become NaN.
     """
     device = _require_device(key, value, key_cache, value_cache, slot_mapping)
     if key_cache.dim() != 5 or value_cache.shape != key_cache.shape:
@@ -913,7 +914,12 @@ def _check_rows_out(out: torch.Tensor, like: torch.Tensor, name: str) -> None:
     head strides)."""
     if tuple(out.shape) != tuple(like.shape) or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} must have shape {tuple(like.shape)}, dtype {like.dtype} and be on {like.device}")
-    if out.stride(2) != 1 or any(out.shape[i] > 1 and out.stride(i) < out.shape[2] for i in (0, 1)):
+    span, own = int(out.shape[2]), out.stride(2) == 1
+    for stride, n in sorted((out.stride(i), int(out.shape[i])) for i in (0, 1)):
+        if n > 1:
+            own = own and stride >= span
+            span += (n - 1) * stride
+    if not own and out.numel() > 0:
         raise ValueError(f"{name} needs unit stride along D and rows of its own")
 
 

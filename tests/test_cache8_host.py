@@ -93,9 +93,11 @@ def test_rotation_arguments():
 
 def test_outputs_of_rows():
     like = torch.zeros((3, 4, 64), dtype=torch.bfloat16)
+    ops._check_rows_out(torch.zeros((4, 3, 64), dtype=torch.bfloat16).transpose(0, 1), like, "out")
     ops._check_rows_out(torch.zeros((3, 8, 64), dtype=torch.bfloat16)[:, 2:6], like, "out")
     for bad in (like.float(), like[:2], torch.zeros((1, 4, 64), dtype=torch.bfloat16).expand(3, 4, 64),
-                torch.zeros((3, 64, 4), dtype=torch.bfloat16).transpose(1, 2), like.to("meta")):
+                torch.zeros((3, 64, 4), dtype=torch.bfloat16).transpose(1, 2), like.to("meta"),
+                torch.zeros(1000, dtype=torch.bfloat16).as_strided((3, 4, 64), (64, 64, 1))):
         with pytest.raises(ValueError):
             ops._check_rows_out(bad, like, "out")
 

@@ -41,9 +41,8 @@ def same(mine, want, layer):
 def stored(x):
     """Rows as the write codes them, fp32 on the CPU."""
     y = x.float().cpu()
-    if x.dtype == torch.float16:
-        y = torch.where(torch.isfinite(y), y.clamp(-61440, 61440), y)
-    return y
+    most = 61440.0 if x.dtype == torch.float16 else 1.875 * 2.0**127
+    return torch.where(torch.isfinite(y), y.clamp(-most, most), y)
 
 
 def expect(mine, layer, k, v, slots):
@@ -105,6 +104,24 @@ def test_write_of_extremes(device):
     mine = empty(1, 1, 4, 1, 64, device)
     ops.reshape_and_cache(x, x, mine[0], mine[1], torch.zeros(1, dtype=torch.int64, device=device), 0, mine[2], mine[3])
     assert float(mine[0].float()[0, 0, 0, 0, 0] * mine[2][0, 0, 0]) == 61440.0
+
+
+@pytest.mark.parametrize("dtype,rows,count", [
+    (torch.bfloat16, 1, 1), (torch.float32, 1, 1), (torch.float16, 3, 1), (torch.float16, 3, 3)])
+def test_the_lowest_values_stay_finite(device, dtype, rows, count):
+    # V rows of a type's lowest value: a weighted mean of them, not an infinity
+    # (one row where a sum of two is past fp32)
+    mine = empty(1, 1, 16, 1, 64, device)
+    x = torch.full((rows, 1, 64), torch.finfo(dtype).min, dtype=dtype, device=device)
+    slots = torch.arange(rows, device=device)
+    ops.reshape_and_cache(torch.zeros_like(x), x, mine[0], mine[1], slots, 0, mine[2], mine[3])
+    table = torch.zeros((1, 1), dtype=torch.int32, device=device)
+    step = ops.pack_step(table, [rows - count], [count], 16, num_kv_heads=1, num_query_heads=4, head_dim=64, dtype=CODE)
+    out = ops.attention(torch.ones((count, 4, 64), dtype=dtype, device=device), mine[0], mine[1], 0, step, 0.1,
+                        key_scales=mine[2], value_scales=mine[3])
+    # equal weights of equal values: a weight's rounding and the result's, 2^-10 in fp16, on either side of the value
+    most = 61440.0 if dtype == torch.float16 else 1.875 * 2.0**127
+    assert ((out.double() / -most - 1).abs() <= 2.0**-9).all()
 
 
 def test_slots_outside_the_pool_are_skipped(device):
