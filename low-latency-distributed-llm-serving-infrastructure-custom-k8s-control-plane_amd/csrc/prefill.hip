@@ -74,8 +74,8 @@
 // comes one step earlier still.  All eight waves share the conversions (16 a
 // thread and step, against its 16 exponentials), which cost what the smaller
 // reads save and some more: bf16, four chunks of 512 at 4096, 32/8 heads of 128
-// (146 GFLOP), 179 us, 816 TFLOP/s (the 16-bit cache 164); 2048 at 6000, 285 us
-// (246).  fp16, 1000 ragged tokens, 16/4 heads of 80: 48 us, its longest unit's
+// (146 GFLOP), 177 us, 825 TFLOP/s (the 16-bit cache 164); 2048 at 6000, 272 us
+// (242).  fp16, 1000 ragged tokens, 16/4 heads of 80: 48 us, its longest unit's
 // chain of stages.
 //
 // Reference: the block-diagonal causal mask of app/model/paged_attention.py:
@@ -734,13 +734,10 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
         // Copies of this step: K of stage st+4, V of stage st+2 and (wave 0)
         // the id slot of stage st+8, each only if that stage exists.
         const bool cpk = st + 4 < nstages, cpv = st + 2 < nstages, cpi = st + kIdAhead < nstages;
+        [[maybe_unused]] constexpr int P = SLOT & 1;
         if constexpr (CODES) {
-          constexpr int P = SLOT & 1;
           if (st + 3 < nstages) write8(((SLOT + 3) & 3) * kRegion, kr8[P], ks8[P]);
-          if (st + 1 < nstages) write8(kVBase + ((SLOT + 1) & 3) * kRegion, vr8[P], vs8[P]);
           if (st + 5 < nstages) load8(st + 5, id8[(SLOT + 5) & 3], kbase, a.key_scales, kr8[P], ks8[P]);
-          if (st + 3 < nstages) load8(st + 3, id8[(SLOT + 3) & 3], vbase, a.value_scales, vr8[P], vs8[P]);
-          if (st + 6 < nstages) id8[(SLOT + 6) & 3] = load_id8(st + 6);
         }
         if (!CODES && wave < kCopyWaves && cpk)
           copy_step(st + 4, slot * kRegion, kbase, nkbase, nkstride, idk, ring_ids(st + 4));
@@ -818,6 +815,16 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
         if (!CODES && wave < kCopyWaves) {
           const int n = (cpk ? kDmaPerWave : 0) + (cpv ? kDmaPerWave : 0) + (wave == 0 && cpi ? 1 : 0);
           wait_vmcnt_at_most<2 * kDmaPerWave + 1>(n);
+        }
+        // (8-bit rows: V's conversions follow the products, K's go before them, which
+        // spreads both over the step; all of them ahead: four chunks of 512 at 4096,
+        // 32/8 heads of 128, 180 us, now 177; 2048 at 6000, 277 and 272; the chunks
+        // with 16/4 of 96, 96.3 and 91.5.)
+        if constexpr (CODES) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (st + 1 < nstages) write8(kVBase + ((SLOT + 1) & 3) * kRegion, vr8[P], vs8[P]);
+          if (st + 3 < nstages) load8(st + 3, id8[(SLOT + 3) & 3], vbase, a.value_scales, vr8[P], vs8[P]);
+          if (st + 6 < nstages) id8[(SLOT + 6) & 3] = load_id8(st + 6);
         }
         // (8-bit rows: this step's LDS writes)
         if constexpr (CODES) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
