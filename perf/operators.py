@@ -27,7 +27,6 @@ Lengths follow from the case alone (``lengths`` seeds them); values and the
 placement of blocks from the seed given to ``prepare``.
 """
 
-import functools
 import importlib
 import math
 
@@ -43,12 +42,6 @@ CODE = torch.float8_e4m3fn
 MAX_CODE = 448.0
 EPS = 1e-6
 LAYER = 1  # of the two layers each cache here has
-
-
-@functools.lru_cache(maxsize=None)
-def _framework():
-    # (imported once, as a program does: the name has no form for a statement)
-    return importlib.import_module(PACKAGE + ".paged_ops")
 
 
 def _case(name, op, dtype, heads, block=16, decodes=0, ctx=(0, 0), dist="uniform", prompts=0, new=(0, 0),
@@ -204,7 +197,7 @@ def prepare(case, seed):
     if case["op"] == "attend8":
         s["query"] = torch.randn((t, hq, d), generator=gen, device=dev).to(dtype)
         if own:
-            s["step"] = _framework().pack_step(
+            s["step"] = importlib.import_module(PACKAGE + ".paged_ops").pack_step(
                 s["table"], starts, counts, bs, num_kv_heads=hkv, num_query_heads=hq, head_dim=d, dtype=CODE)
         return s
     qkv = rows(t, hq + 2 * hkv, d).to(dtype)  # one projection's output, split as views
@@ -291,7 +284,7 @@ def run(state):
     s, c = state, state["case"]
     if not own:
         return _attend(s) if c["op"] == "attend8" else _append(s)
-    ops = _framework()
+    ops = importlib.import_module(PACKAGE + ".paged_ops")
     if c["op"] == "attend8":
         return ops.attention(s["query"], s["key_cache"], s["value_cache"], LAYER, s["step"], s["scaling"],
                              key_scales=s["key_scales"], value_scales=s["value_scales"])
