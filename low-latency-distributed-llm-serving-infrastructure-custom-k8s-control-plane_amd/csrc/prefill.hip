@@ -524,16 +524,20 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
         }
       };
       // ... and (bad_ids only) in a block outside the pool.  This one is applied
-      // at the start of the step that turns the tile into probabilities, outside
-      // the interleaved phases; the tile's maximum may then include such a
-      // position's (finite) score, which only moves the reference maximum.
+      // behind the interleaved phases, and the tile's maximum is then taken again:
+      // one that counted such a position's score would become the reference of
+      // rows whose own scores may all lie so far below it that their
+      // probabilities are zeros.
       auto mask_bad = [&](int t, f32x16& s) {
+        // (a lane a position: the ids of 16 of them in every lane cost 30 registers)
+        int p = t * kKvTile;
+        asm volatile("" : "+s"(p));  // (kept scalar, and the stage with it)
+        const int b = btg[min(p + (lane & 31), kv_last) >> log2_bs];
+        const uint32_t bad =
+            static_cast<uint32_t>(__ballot(static_cast<uint32_t>(b) >= static_cast<uint32_t>(a.total_blocks))) >> (4 * half);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int kv = t * kKvTile + 8 * (i >> 2) + 4 * half + (i & 3);
-          if (kv <= kv_lim && static_cast<uint32_t>(btg[kv >> log2_bs]) >= static_cast<uint32_t>(a.total_blocks))
-            s[i] = -INFINITY;
-        }
+        for (int i = 0; i < 16; ++i)
+          if ((bad >> (8 * (i >> 2) + (i & 3))) & 1u) s[i] = -INFINITY;
       };
 
       f32x16 acc[DB];
@@ -721,6 +725,7 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
       prefetch_ids(0);
       read_k(1, ka);
       mask_tile(kh, s0);
+      if (bad_ids) mask_bad(kh, s0);
       rescale(tile_max(s0));
 
       // One step: see the header comment.  s_cur holds the scores of this
@@ -742,7 +747,6 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
         if (!CODES && wave < kCopyWaves && cpk)
           copy_step(st + 4, slot * kRegion, kbase, nkbase, nkstride, idk, ring_ids(st + 4));
         const int idv_cur = idv;  // (the prefetch below replaces idv)
-        if (bad_ids) mask_bad(2 * st + kh, s_cur);
 
         // ---- A: S_next = K_next Q^T | P = exp2(S - m) | V^T reads
         // (fp16 over 8-bit rows: probabilities, of up to 2^8, times 2^6, in the
@@ -786,7 +790,7 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
         read_k((slot + 2) & (kKBufs - 1), ka);
         prefetch_ids(st + 1);
         if constexpr (MASKED) mask_tile(2 * (st + 1) + kh, sn);
-        const float tmax = tile_max(sn);
+        float tmax = tile_max(sn);
         l += rsum0 + rsum1;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -799,6 +803,10 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
           __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
           __builtin_amdgcn_sched_group_barrier(kSchedDsRead, (KS + 2) / (2 * DB), 0);
           __builtin_amdgcn_sched_group_barrier(kSchedValu, 2, 0);
+        }
+        if (MASKED && bad_ids) {
+          mask_bad(2 * (st + 1) + kh, sn);
+          tmax = tile_max(sn);
         }
         rescale(tmax);
         s_nxt = sn;

@@ -257,13 +257,18 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
     for (int i = 0; i < 16; ++i)
       if (8 * (i >> 2) + (i & 3) > lim) s[i] = -INFINITY;
   };
+  // (bad_ids only: behind the interleaved phases, and the tile's maximum, which
+  // counts no such position, is taken again)
   auto mask_bad = [&](int t, f32x16& s) {
+    // (a lane a position: the ids of 16 of them in every lane cost 30 registers)
+    int p = t * kTile;
+    asm volatile("" : "+s"(p));  // (kept scalar, and the stage with it)
+    const int b = btg[min(p + (lane & 31), kv_last) >> log2_bs];
+    const uint32_t bad =
+        static_cast<uint32_t>(__ballot(static_cast<uint32_t>(b) >= static_cast<uint32_t>(a.total_blocks))) >> (4 * half);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int kv = t * kTile + 8 * (i >> 2) + 4 * half + (i & 3);
-      if (kv <= kv_lim && static_cast<uint32_t>(btg[kv >> log2_bs]) >= static_cast<uint32_t>(a.total_blocks))
-        s[i] = -INFINITY;
-    }
+    for (int i = 0; i < 16; ++i)
+      if ((bad >> (8 * (i >> 2) + (i & 3))) & 1u) s[i] = -INFINITY;
   };
   auto max3 = [](float x, float y, float z) {
     float r;
@@ -332,6 +337,7 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
     for (int ks = 0; ks < kKS; ++ks) s0 = mfma32<T>(ka[ks], qreg[ks], s0);
     read_k(1, ka);
     mask_tile(0, s0);
+    if (bad_ids) mask_bad(0, s0);
     rescale(tile_max(s0));
   }
   stage_barrier();
@@ -342,7 +348,6 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
     constexpr bool MASKED = decltype(masked)::value;
     constexpr int SLOT = decltype(slot_c)::value;
     copy_step(st + 4, SLOT * kRegion, kbase, idk);
-    if (bad_ids) mask_bad(st, s_cur);
 
     // ---- A: S_next = K_next Q^T | P = exp2(S - m)
     const float msc = m * scale;
@@ -374,7 +379,7 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
       for (int kk = 0; kk < 2; ++kk) acc[db] = mfma32<T>(read_vt(SLOT, kk, db), pb[kk], acc[db]);
     read_k((SLOT + 2) & (kBufs - 1), ka);
     if constexpr (MASKED) mask_tile(st + 1, sn);
-    const float tmax = tile_max(sn);
+    float tmax = tile_max(sn);
     l += rsum0 + rsum1;
 #pragma unroll
     for (int ks = 0; ks < kKS; ++ks) {
@@ -387,6 +392,10 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
       __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
       __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
       __builtin_amdgcn_sched_group_barrier(kSchedValu, 1, 0);
+    }
+    if (MASKED && bad_ids) {
+      mask_bad(st + 1, sn);
+      tmax = tile_max(sn);
     }
     rescale(tmax);
     s_nxt = sn;

@@ -64,6 +64,7 @@ __device__ __forceinline__ const void* uniform_ptr(const void* p) {
   return reinterpret_cast<const void*>((static_cast<uint64_t>(hi) << 32) | lo);
 }
 __device__ __forceinline__ void dma4_s(uint32_t lds_base, uint32_t voff, const void* sbase) {
+  lds_base = __builtin_amdgcn_readfirstlane(lds_base);  // (in an SGPR, wherever the compiler keeps its terms)
   sbase = uniform_ptr(sbase);
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_base), "v"(voff), "s"(sbase)
                : "memory", "m0");
