@@ -385,8 +385,8 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
 
       // ---- copies ------------------------------------------------------------
       // Rows past the readable context re-read its last row, and an
-      // out-of-pool block id reads block 0 (finite values; their scores are
-      // masked).  No stage past the last is copied: a step's copies, and the
+      // out-of-pool block id reads block 0 (their scores are masked and
+      // their V rows cleared).  No stage past the last is copied: a step's copies, and the
       // count of them its wait allows in flight, depend on how many stages
       // remain.
       // Block ids of the first stages come from scalar loads of the table
@@ -528,16 +528,27 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
       // one that counted such a position's score would become the reference of
       // rows whose own scores may all lie so far below it that their
       // probabilities are zeros.
-      auto mask_bad = [&](int t, f32x16& s) {
-        // (a lane a position: the ids of 16 of them in every lane cost 30 registers)
+      auto missing = [&](int t) {  // (a lane a position; past the last one, as the copies, that one)
         int p = t * kKvTile;
         asm volatile("" : "+s"(p));  // (kept scalar, and the stage with it)
         const int b = btg[min(p + (lane & 31), kv_last) >> log2_bs];
-        const uint32_t bad =
-            static_cast<uint32_t>(__ballot(static_cast<uint32_t>(b) >= static_cast<uint32_t>(a.total_blocks))) >> (4 * half);
+        return static_cast<uint32_t>(b) >= static_cast<uint32_t>(a.total_blocks);
+      };
+      auto mask_bad = [&](int t, f32x16& s) {
+        const uint32_t bad = static_cast<uint32_t>(__ballot(missing(t))) >> (4 * half);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if ((bad >> (8 * (i >> 2) + (i & 3))) & 1u) s[i] = -INFINITY;
+      };
+      // Their V rows (block 0's, which may hold anything) become zeros, as a NaN
+      // or an infinity outlives a weight of zero.  Each wave clears the rows of
+      // the tile it reads itself (rows that several waves clear alike).
+      auto clear_bad = [&](int t, int slot) {
+        if (missing(t)) {
+          char* row = s_lds + kVBase + slot * kRegion + (kh * kKvTile + (lane & 31)) * ROW_BYTES + half * (ROW_BYTES / 2);
+#pragma unroll 1
+          for (int i = 0; i < ROW_BYTES / 32; ++i) st16(row + 16 * i, make_uint4(0, 0, 0, 0));
+        }
       };
 
       f32x16 acc[DB];
@@ -747,6 +758,7 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
         if (!CODES && wave < kCopyWaves && cpk)
           copy_step(st + 4, slot * kRegion, kbase, nkbase, nkstride, idk, ring_ids(st + 4));
         const int idv_cur = idv;  // (the prefetch below replaces idv)
+        if (!CODES && MASKED && bad_ids) clear_bad(2 * st + kh, slot);
 
         // ---- A: S_next = K_next Q^T | P = exp2(S - m) | V^T reads
         // (fp16 over 8-bit rows: probabilities, of up to 2^8, times 2^6, in the

@@ -259,16 +259,27 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
   };
   // (bad_ids only: behind the interleaved phases, and the tile's maximum, which
   // counts no such position, is taken again)
-  auto mask_bad = [&](int t, f32x16& s) {
-    // (a lane a position: the ids of 16 of them in every lane cost 30 registers)
+  auto missing = [&](int t) {  // (a lane a position; past the last one, as the copies, that one)
     int p = t * kTile;
     asm volatile("" : "+s"(p));  // (kept scalar, and the stage with it)
     const int b = btg[min(p + (lane & 31), kv_last) >> log2_bs];
-    const uint32_t bad =
-        static_cast<uint32_t>(__ballot(static_cast<uint32_t>(b) >= static_cast<uint32_t>(a.total_blocks))) >> (4 * half);
+    return static_cast<uint32_t>(b) >= static_cast<uint32_t>(a.total_blocks);
+  };
+  auto mask_bad = [&](int t, f32x16& s) {
+    const uint32_t bad = static_cast<uint32_t>(__ballot(missing(t))) >> (4 * half);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       if ((bad >> (8 * (i >> 2) + (i & 3))) & 1u) s[i] = -INFINITY;
+  };
+  // Their V rows (block 0's, which may hold anything) become zeros, as a NaN or
+  // an infinity outlives a weight of zero.  Every wave clears the tile's rows
+  // itself before it reads them.
+  auto clear_bad = [&](int t, int slot) {
+    if (missing(t)) {
+      char* row = s_lds + kVBase + slot * kRegion + (lane & 31) * kRowBytes + half * (kRowBytes / 2);
+#pragma unroll 1
+      for (int i = 0; i < kRowBytes / 32; ++i) st16(row + 16 * i, make_uint4(0, 0, 0, 0));
+    }
   };
   auto max3 = [](float x, float y, float z) {
     float r;
@@ -348,6 +359,7 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
     constexpr bool MASKED = decltype(masked)::value;
     constexpr int SLOT = decltype(slot_c)::value;
     copy_step(st + 4, SLOT * kRegion, kbase, idk);
+    if (MASKED && bad_ids) clear_bad(st, SLOT);
 
     // ---- A: S_next = K_next Q^T | P = exp2(S - m)
     const float msc = m * scale;

@@ -158,8 +158,8 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
       }
     };
     // Copies of stage x into buffer b.  Rows past the readable context
-    // re-read its last row and an out-of-pool block reads block 0 (finite
-    // values; their scores are masked).  APPEND: rows at or after the
+    // re-read its last row and an out-of-pool block reads block 0 (their
+    // scores are masked and their V rows cleared).  APPEND: rows at or after the
     // chunk's start come from the new rows -- one path per stage (all rows
     // before the chunk, all in it, or the stage that holds its start), as
     // per-lane address selects in every stage spilled registers in the
@@ -329,7 +329,15 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
           s[i] = fast_exp2(fmaf(s[i], scale, -msc));
           l += s[i];
         }
-        const char* vb = s_lds + b * kBufBytes + TBYTES;
+        char* vb = s_lds + b * kBufBytes + TBYTES;
+        // The V rows of out-of-pool blocks (block 0's, which may hold anything)
+        // become zeros, as a NaN or an infinity outlives a weight of zero.  Each
+        // wave clears the rows of its tile itself before it reads them.
+        if (bad_ids && static_cast<uint32_t>(s_sid[b][k_row]) >= static_cast<uint32_t>(a.total_blocks)) {
+#pragma unroll 1
+          for (int i = 0; i < ROWB / 32; ++i)
+            st16(vb + k_row * ROWB + h * (ROWB / 2) + 16 * i, make_uint4(0, 0, 0, 0));
+        }
         // V^T operand of MFMA j: V[token of score j][32 db + t], read one j ahead.
         auto read_v = [&](int j, float (&v)[DB]) {
           const int R = kh * kFmTile + 8 * (j >> 2) + 4 * h + (j & 3);

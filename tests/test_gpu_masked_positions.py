@@ -115,3 +115,42 @@ def test_scores_far_below_a_missing_blocks(device, heads, kv_heads, dim, bs, dty
 def test_far_below_a_block_of_the_other_sign(device, heads, kv_heads, dim, bs, dtype):
     # block 0 along -u: a score of +depth in a place that counts for nothing
     run(heads, kv_heads, dim, dtype, dtype, DEPTHS[dtype], -1.0, device, bs)
+
+
+@pytest.mark.parametrize("block0", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("heads,kv_heads,dim,bs,dtype", SHAPES)
+def test_block_0_of_no_sequence_holds_anything(device, heads, kv_heads, dim, bs, dtype, block0):
+    run(heads, kv_heads, dim, dtype, dtype, 2.0, block0, device, bs)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,bs,dtype", [(8, 2, 128, 16, torch.float16), (4, 4, 64, 16, torch.bfloat16),
+                                                         (6, 2, 80, 16, torch.bfloat16), (4, 2, 128, 4, torch.bfloat16),
+                                                         (4, 2, 64, 16, torch.float32)])
+@pytest.mark.parametrize("fused", [True, False])
+def test_new_rows_without_a_block_hold_anything(device, heads, kv_heads, dim, bs, dtype, fused):
+    # attention() writes the step's rows itself; those of missing blocks are NaN
+    # and go nowhere
+    q, held, pools, table = case(heads, kv_heads, dim, dtype, dtype, 2.0, float("nan"), bs)
+    blocks = held[0].shape[0]
+    rows = []
+    for pool in held[::2]:
+        flat = pool.reshape(-1, kv_heads, dim)
+        new = torch.full((sum(COUNTS), kv_heads, dim), float("nan"), dtype=dtype)
+        t = 0
+        for i, (s, c) in enumerate(zip(STARTS, COUNTS)):
+            for p in range(s, s + c):
+                b = int(table[i, p // bs])
+                if 0 <= b < blocks:
+                    new[t] = flat[b * bs + p % bs]
+                    flat[b * bs + p % bs] = 9.0  # (what the write replaces)
+                t += 1
+        rows.append(new)
+    kc, vc = (held[i][None].to(device) for i in (0, 2))
+    step = ops.pack_step(torch.from_numpy(table).to(device), STARTS, COUNTS, bs, num_kv_heads=kv_heads,
+                         num_query_heads=heads, head_dim=dim, dtype=dtype,
+                         prefill_tile=ops.prefill_tile_for(heads, kv_heads))
+    out = ops.attention(q.to(device), kc, vc, 0, step, dim**-0.5, new_key=rows[0].to(device),
+                        new_value=rows[1].to(device), fused_prefill_write=fused)
+    check(out, q, pools, table, dtype, 2.0)
+    for cache, pool in zip((kc, vc), pools):
+        assert torch.equal(cache[0, 1:].cpu().double(), pool[1:])
