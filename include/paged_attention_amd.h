@@ -759,8 +759,11 @@ typedef struct {
 
 /*
  * pa_decode_phases and pa_prefill over an 8-bit cache: dims.dtype is the
- * query's and the output's.  Same work lists, workspace (of dims), phases and
- * results for missing blocks and empty rows.
+ * query's and the output's, and what the cache's elements are read in: exactly
+ * so by bf16 and fp32 queries, and by fp16 ones where fp16 rows were written (of
+ * other rows a magnitude of 65520 or more is an infinity to them, and one below
+ * 2^-24 is rounded to a multiple of that).  Same work lists, workspace (of
+ * dims), phases and results for missing blocks and empty rows.
  */
 int pa_decode_8bit(int32_t phases, const void *query, const void *key_cache,
                    const void *value_cache, PaCacheScales scales,

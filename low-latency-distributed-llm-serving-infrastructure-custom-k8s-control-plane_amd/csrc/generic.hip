@@ -21,10 +21,17 @@
 
 namespace pa {
 
-template <typename C>
+// (A code's value as the matrix-core kernels read it: in the query's type.  That
+// is the value itself in bf16 and fp32; in fp16 an infinity from 65520 on.)
+template <typename T, typename C>
 __device__ __forceinline__ float cache_value(const C* p, float scale) {
-  if constexpr (sizeof(C) == 1) return code_to_f32<0>(p->bits) * scale;
-  else return load_scalar<C>(p);
+  if constexpr (sizeof(C) == 1) {
+    const float x = code_to_f32<0>(p->bits) * scale;
+    if constexpr (Elem<T>::kDtype == PA_DTYPE_F16) return half_lo<f16_t>(pack_half2<f16_t>(x, x));
+    return x;
+  } else {
+    return load_scalar<C>(p);
+  }
 }
 
 template <typename T, int EPL, bool kMasked, typename C = T>
@@ -115,8 +122,8 @@ __global__ __launch_bounds__(kWave) void generic_attention_kernel(GenericArgs a)
       for (int e = 0; e < EPL; ++e) {
         const int d = lane + e * kWave;
         const bool in = d < D;
-        part = fmaf(q[e], in ? cache_value<C>(krow + d, ks) : 0.f, part);
-        v[e] = in ? cache_value<C>(vrow + d, vs) : 0.f;
+        part = fmaf(q[e], in ? cache_value<T>(krow + d, ks) : 0.f, part);
+        v[e] = in ? cache_value<T>(vrow + d, vs) : 0.f;
       }
       const float score = wave_sum(part) * a.scale_log2e;
       const float m_new = fmaxf(m, score);

@@ -21,7 +21,9 @@ for the table).
 A cache of ``torch.float8_e4m3fn`` holds 8-bit codes, with fp32 scales
 [layers, blocks, H_kv] beside it (``key_scales`` / ``value_scales`` of (b), (c),
 (d) and :func:`attention`; see :func:`reshape_and_cache` for its rules).  Rows,
-query and output are then of any of the other types.
+query and output are then of any of the other types; attention reads an element
+in the query's type, so fp16 queries want a cache of values below 65520, such as
+fp16 rows leave (a larger one is an infinity to them).
 """
 
 from __future__ import annotations

@@ -303,6 +303,47 @@ def test_prefill_fp32_queries(device):
     attend(4, 2, 64, 16, [0, 33], [40, 20], torch.float32, device)
 
 
+@pytest.mark.parametrize("counts", [[1, 1], [20, 9]])
+@pytest.mark.parametrize("heads,kv_heads,dim,bs", [(4, 2, 128, 16), (2, 2, 64, 4), (6, 2, 80, 16), (4, 2, 64, 1),
+                                                   (2, 2, 40, 16), (2, 2, 256, 16)])
+def test_fp16_queries_over_values_past_fp16(device, heads, kv_heads, dim, bs, counts):
+    # bf16 rows with a value of 61440 and one of 65536: fp16 queries read the
+    # first as it is and the second as an infinity, whatever kernel runs
+    starts = [20 - counts[0], 21 - counts[1]]
+    blocks = 2 * -(-21 // bs)
+    gen = torch.Generator().manual_seed(dim)
+    k = 0.1 * torch.randn((41, kv_heads, dim), generator=gen)
+    v = torch.randn((41, kv_heads, dim), generator=gen)
+    v[3, 0, 5], v[2, 0, 3], v[22, 1, 7] = 61440.0, 65536.0, -65536.0
+    table = torch.arange(blocks, dtype=torch.int32).reshape(2, -1)
+    slots = torch.cat([torch.arange(20), torch.arange(21) + blocks // 2 * bs])
+    mine = empty(1, blocks, bs, kv_heads, dim, device)
+    ops.reshape_and_cache(k.to(torch.bfloat16).to(device), v.to(torch.bfloat16).to(device), mine[0], mine[1],
+                          slots.to(device), 0, mine[2], mine[3])
+    vals = [oracle.values(c[0].cpu(), s[0].cpu()) for c, s in ((mine[0], mine[2]), (mine[1], mine[3]))]
+    flat = vals[1].reshape(-1, kv_heads, dim)
+    assert flat[slots[3], 0, 5] == 61440 and flat[slots[2], 0, 3] == 65536 and flat[slots[22], 1, 7] == -65536
+    assert flat.abs()[slots].gt(60000).sum() == 3
+    flat[flat.abs() > 65000] = 0.0
+    q = torch.randn((sum(counts), heads, dim), generator=gen).to(torch.float16)
+    step = ops.pack_step(table.to(device), starts, counts, bs, num_kv_heads=kv_heads, num_query_heads=heads, head_dim=dim,
+                         dtype=CODE)
+    out = ops.attention(q.to(device), mine[0], mine[1], 0, step, dim**-0.5, key_scales=mine[2], value_scales=mine[3])
+    out = out.cpu().double()
+    ref, size, peak = oracle.attention(q, *vals, table.numpy(), starts, counts, dim**-0.5)
+    over = torch.zeros(out.shape, dtype=torch.bool)  # results that weigh an infinity
+    group = heads // kv_heads
+    over[:counts[0], :group, 3] = True
+    over[counts[0]:, group:, 7] = True
+    late = torch.cat([torch.arange(s, s + c) for s, c in zip(starts, counts)])
+    sees = (late >= torch.tensor([2] * counts[0] + [2] * counts[1]))[:, None, None]  # (both are their third tokens)
+    assert not torch.isfinite(out[over & sees]).any()
+    # the others: as in attend() above, with one term of a probability
+    u = 2.0**-11
+    bound = (1 + 2 * u) * u * ref.abs() + (2 * u + 1.5e-5) * size + 2.0**-24 + 2.0**-31 * peak
+    assert ((out - ref).abs() <= bound)[~over].all()
+
+
 # ---- together, as a server runs them ------------------------------------------
 
 
