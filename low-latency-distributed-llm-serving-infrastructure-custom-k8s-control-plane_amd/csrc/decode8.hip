@@ -2,8 +2,8 @@
 // fp16 queries, heads of 64 and 128, and of 80 and 96 on the LDS rows of 128.
 //
 // The split, the operand layouts, the softmax and the merge are those of
-// decode_mfma.hip: one workgroup per (sequence, context partition, KV head or
-// two adjacent ones), S^T = K Q^T and O^T = V^T P^T by v_mfma_f32_16x16x32 of
+// decode_mfma.hip: one workgroup per (sequence, context partition, KV head, or
+// two or four adjacent ones), S^T = K Q^T and O^T = V^T P^T by v_mfma_f32_16x16x32 of
 // the query's type, probabilities as two terms of it.  What differs:
 //  * Codes become 16-bit values in registers, between LDS and the product (K)
 //    or between the row pieces and the product (V), by v_cvt_scalef32_pk_*_fp8,
@@ -113,26 +113,18 @@ decode8_kernel(DecodeArgs a) {
   const int hkv = a.num_kv_heads;
   const uint32_t sub_groups = SHARED ? a.sub_groups : 1;
   const int G = SHARED ? a.group / a.sub_groups : a.group;
-  // Workgroup -> (item, KV head, sub-group), in gangs that share an XCD's L2
-  // (see decode_mfma.hip): sub-groups that read the same rows, and all of an
-  // item's heads where a workgroup's part of a row is less than two lines.
+  // Workgroup -> (item, KV head, sub-group): those of an item are a gang, which
+  // shares an XCD's L2 (see decode_mfma.hip), as a head's part of a row is one
+  // line of memory or less.
   const uint32_t units = static_cast<uint32_t>(hkv) / HEADS;
-  constexpr bool kGangUnits = kMemBytes % 256 != 0;
-  uint32_t g_id = blockIdx.x, member = 0;
-  if constexpr (kGangUnits || SHARED) {
-    const uint32_t gang = (kGangUnits ? units : 1) * sub_groups;
-    const uint32_t gangs = static_cast<uint32_t>(a.num_items) * (kGangUnits ? 1 : units);
-    const uint32_t run = quotient(blockIdx.x, kXcds * gang, a.run_rcp);
-    const uint32_t at_run = blockIdx.x - run * (kXcds * gang);
-    const uint32_t width = min(static_cast<uint32_t>(kXcds), gangs - run * kXcds);
-    member = width == kXcds ? at_run / kXcds : at_run / width;
-    g_id = run * kXcds + (at_run - member * width);
-  }
-  const int64_t item = kGangUnits ? g_id : quotient(g_id, units, a.unit_rcp);
-  const int unit = static_cast<int>(!kGangUnits ? g_id - static_cast<uint32_t>(item) * units
-                                    : SHARED    ? member / sub_groups
-                                                : member);
-  const int sg = !SHARED ? 0 : static_cast<int>(kGangUnits ? member - unit * sub_groups : member);
+  const uint32_t gang = units * sub_groups;
+  const uint32_t run = quotient(blockIdx.x, kXcds * gang, a.run_rcp);
+  const uint32_t at_run = blockIdx.x - run * (kXcds * gang);
+  const uint32_t width = min(static_cast<uint32_t>(kXcds), static_cast<uint32_t>(a.num_items) - run * kXcds);
+  const uint32_t member = width == kXcds ? at_run / kXcds : at_run / width;
+  const int64_t item = run * kXcds + (at_run - member * width);
+  const int unit = static_cast<int>(SHARED ? member / sub_groups : member);
+  const int sg = SHARED ? static_cast<int>(member - unit * sub_groups) : 0;
   const int kvh = unit * HEADS + wave / kHeadWaves;
   const int h0 = kvh * a.group + sg * G;  // first query head of the wave
   const int seq = a.items[2 * item];
@@ -528,10 +520,8 @@ struct Launch8 {
   hipError_t run() const {
     const uint32_t units = a.num_kv_heads / HEADS;
     const int64_t grid = num_items * units * a.sub_groups;
-    const uint32_t gang = (DM % 256 != 0 ? units : 1) * a.sub_groups;
     DecodeArgs b = a;
-    b.unit_rcp = 0xffffffffu / units;
-    b.run_rcp = 0xffffffffu / (kXcds * gang);
+    b.run_rcp = 0xffffffffu / (kXcds * units * a.sub_groups);
     if (a.log2_block_size < 4)
       hipLaunchKernelGGL((decode8_kernel<T, D, DM, SHARED, HEADS, true>), dim3(static_cast<uint32_t>(grid)),
                          dim3(kDecodeThreads), 0, stream, b);
@@ -559,8 +549,8 @@ hipError_t launch_decode8(const DecodeArgs& a, int dtype, int head_dim, int unit
   // wave each, so a row's pieces are read together and a CU touches fewer
   // pages.  Two heads -> four: 128 sequences of 128-8192 tokens, 32/8 heads of
   // 64, 132 -> 126 us; 256 of 2048, 32/8 of 128, at 1024, 206 -> 194 (512 of
-  // them 367 -> 348); 64 of 128-4096, 32/32, 201 -> 198.  With fewer workgroups
-  // a CU waits on its largest one: 16 of 256-1024, 32/8, 12.0 -> 13.9.
+  // them 367 -> 348).  With fewer workgroups a CU waits on its largest one: 16
+  // of 256-1024, 32/8, 12.0 -> 13.9.
   if (unit_heads == 2 && a.num_kv_heads % 4 == 0 &&
       num_items * (a.num_kv_heads / 4) >= 4 * static_cast<int64_t>(device_compute_units()))
     unit_heads = 4;
