@@ -569,8 +569,12 @@ __global__ __launch_bounds__(kRotateThreads) void cache8_write_kernel(RotateArgs
   }
 }
 
-// Lanes the chip holds at a time: 2048 on each of 256 CUs.
-constexpr int64_t kResidentLanes = 256 * 2048;
+// Lanes the device holds at a time: 2048 on each of its CUs (a whole chip's 256
+// where their count is unknown).
+static int64_t resident_lanes() {
+  const int cus = device_compute_units();
+  return 2048 * static_cast<int64_t>(cus > 0 ? cus : 256);
+}
 
 template <typename T, int L, bool VEC, int NR>
 static hipError_t launch_rotate_n(const RotateArgs& args, hipStream_t s) {
@@ -590,13 +594,13 @@ static hipError_t launch_rotate_n(const RotateArgs& args, hipStream_t s) {
   a.kv_rcp = 0xffffffffu / (2 * a.num_kv_heads);
   // Three rows a group, so that a chunk re-reads half as much of its
   // neighbour's, once its rows of K and V alone would fill the chip (see
-  // kResidentLanes); a chunk of two has less to wait for.  Two against three:
+  // resident_lanes); a chunk of two has less to wait for.  Two against three:
   // bf16, 32/8 heads of 128, 256 tokens 6.1 / 7.5 us, 1024 10.0 / 11.2, 2048
   // 17.4 / 16.7; fp16, 32/32 of 128, 384 tokens 10.4 / 11.2, 512 13.4 / 12.8,
   // 4096 69.1 / 61.8; 9/3 heads of 64, 8192 tokens 13.5 / 13.9, 16384 23.5 /
   // 22.3; 8/2 heads of 256, 2048 tokens 10.0 / 10.8, 8192 31.7 / 29.1.
   const bool keep = a.block_size <= kRows + 1;
-  const bool three = keep && static_cast<int64_t>(a.num_tokens) * 2 * a.num_kv_heads * L >= kResidentLanes;
+  const bool three = keep && static_cast<int64_t>(a.num_tokens) * 2 * a.num_kv_heads * L >= resident_lanes();
   const int own = three ? 2 * kRows : kRows;
   a.kv_groups = static_cast<uint32_t>((a.num_tokens + own - 1) / own * (2 * a.num_kv_heads));
   a.log2_block = -1;
@@ -622,7 +626,7 @@ template <typename T, int L, bool VEC>
 static hipError_t launch_rotate_l(const RotateArgs& a, hipStream_t s) {
   if constexpr (VEC) {
     const int64_t rows = static_cast<int64_t>(a.num_tokens) * (a.num_query_heads + 2 * a.num_kv_heads);
-    if (rows * L > kResidentLanes) return launch_rotate_n<T, L, VEC, 2>(a, s);
+    if (rows * L > resident_lanes()) return launch_rotate_n<T, L, VEC, 2>(a, s);
   }
   return launch_rotate_n<T, L, VEC, 1>(a, s);
 }
