@@ -559,6 +559,9 @@ hipError_t launch_decode8(const DecodeArgs& a, int dtype, int head_dim, int unit
   return hipErrorNotSupported;
 }
 
+// (What the partition is planned with.  The kernels of a head dim need the same
+// LDS whatever their heads and query type, and registers for the same waves, so
+// this holds for the four heads that launch_decode8 may take too.)
 hipError_t decode8_workgroups_per_cu(int head_dim, bool shared, int unit_heads, int* per_cu) {
   return visit8_dim<bf16_t>(head_dim, shared, unit_heads, Occupancy8{per_cu});
 }
