@@ -886,14 +886,18 @@ def _rotate_dims(query, key, positions, cos_sin, query_weight, key_weight, eps, 
         raise ValueError(f"query dtype {query.dtype} differs from key dtype {key.dtype}")
     code = dtype_code(query.dtype)
     tokens, dim = int(query.shape[0]), int(query.shape[2])
-    if positions.dtype != torch.int64 or positions.numel() != tokens:
-        raise ValueError("positions must be int64 with one entry per token")
-    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
-        raise ValueError("cos_sin must be a contiguous float32 (positions, rotary_dim) tensor (rope_table)")
-    rotary = int(cos_sin.shape[1])
-    if rotary % 2 or rotary > dim or rotary == 0 or cos_sin.shape[0] == 0:
-        raise ValueError(f"cos_sin must have an even rotary_dim of at most the head dim ({dim}) and a position, got "
-                         f"{tuple(cos_sin.shape)}")
+    if (positions is None) != (cos_sin is None):
+        raise ValueError("positions and cos_sin are given together (neither: no rotation)")
+    table_rows = rotary = 0
+    if cos_sin is not None:
+        if positions.dtype != torch.int64 or positions.numel() != tokens:
+            raise ValueError("positions must be int64 with one entry per token")
+        if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
+            raise ValueError("cos_sin must be a contiguous float32 (positions, rotary_dim) tensor (rope_table)")
+        table_rows, rotary = (int(n) for n in cos_sin.shape)
+        if rotary % 2 or rotary > dim or rotary == 0 or table_rows == 0:
+            raise ValueError(f"cos_sin must have an even rotary_dim of at most the head dim ({dim}) and a position, got "
+                             f"{tuple(cos_sin.shape)}")
     weight_dtype = None
     for w in (query_weight, key_weight):
         if w is None:
@@ -906,7 +910,7 @@ def _rotate_dims(query, key, positions, cos_sin, query_weight, key_weight, eps, 
     return _native.PaRotateDims(
         num_tokens=tokens, num_query_heads=int(query.shape[1]), num_kv_heads=int(key.shape[1]), head_dim=dim, dtype=code,
         weight_dtype=code if weight_dtype is None else dtype_code(weight_dtype), rotary_dim=rotary,
-        interleaved=int(interleaved), num_positions=int(cos_sin.shape[0]), eps=eps, cache_dtype=code,
+        interleaved=int(interleaved), num_positions=table_rows, eps=eps, cache_dtype=code,
         query_token_stride=query.stride(0), query_head_stride=query.stride(1), key_token_stride=key.stride(0),
         key_head_stride=key.stride(1))
 
@@ -950,8 +954,8 @@ def _kept(key, build):
 def rotate(
     query: torch.Tensor,
     key: torch.Tensor,
-    positions: torch.Tensor,
-    cos_sin: torch.Tensor,
+    positions: Optional[torch.Tensor],
+    cos_sin: Optional[torch.Tensor],
     *,
     query_weight: Optional[torch.Tensor] = None,
     key_weight: Optional[torch.Tensor] = None,
@@ -968,13 +972,15 @@ def rotate(
     [P, R] (:func:`rope_table`), R <= D elements of a head rotate.  Pairs are
     (i, i + R/2), or (2i, 2i + 1) with ``interleaved``.  Weights: [D], of the
     rows' dtype or fp32.  fp32 arithmetic, rounded once.  A position outside
-    the table gives NaN rows.  ``out_query`` / ``out_key`` may be the inputs.
+    the table gives NaN rows.  Without ``positions`` and ``cos_sin`` (None, None)
+    rows are normalised alone.  ``out_query`` may be ``query`` itself and
+    ``out_key`` ``key``; outputs and inputs overlap in no other way.
     """
     if query.dim() == 3 and query.stride(2) != 1:
         query = query.contiguous()
     if key.dim() == 3 and key.stride(2) != 1:
         key = key.contiguous()
-    positions = positions.contiguous()
+    positions = positions if positions is None else positions.contiguous()
     eps, interleaved = float(eps), bool(interleaved)
 
     def build():
@@ -997,7 +1003,7 @@ def rotate(
         out_key = key.new_empty(key.shape)
     with _current(query.device):
         status = _native.load_library().pa_rotate(
-            dims, query.data_ptr(), key.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(), _ptr(query_weight),
+            dims, query.data_ptr(), key.data_ptr(), _ptr(positions), _ptr(cos_sin), _ptr(query_weight),
             _ptr(key_weight), out_query.data_ptr(), out_key.data_ptr(), _stream(query.device))
     _native.check(status, "pa_rotate")
     return out_query, out_key
@@ -1011,8 +1017,8 @@ def rotate_and_cache(
     value_cache: torch.Tensor,
     slot_mapping: torch.Tensor,
     layer_idx: int,
-    positions: torch.Tensor,
-    cos_sin: torch.Tensor,
+    positions: Optional[torch.Tensor],
+    cos_sin: Optional[torch.Tensor],
     *,
     query_weight: Optional[torch.Tensor] = None,
     key_weight: Optional[torch.Tensor] = None,
@@ -1027,8 +1033,8 @@ def rotate_and_cache(
     bit the two calls (on rows that start at multiples of four elements);
     returns (or fills) the rotated query [T, H_q, D].
 
-    ``out`` may be ``query``.  A token whose position lies outside the table
-    gets a NaN query row and no K row.
+    ``out`` may be ``query`` itself.  A token whose position lies outside the
+    table gets a NaN query row and no K row.
     """
     if query.dim() == 3 and query.stride(2) != 1:
         query = query.contiguous()
@@ -1036,7 +1042,8 @@ def rotate_and_cache(
         key = key.contiguous()
     if value.dim() == 3 and value.stride(2) != 1:
         value = value.contiguous()
-    positions, slot_mapping = positions.contiguous(), slot_mapping.contiguous()
+    positions = positions if positions is None else positions.contiguous()
+    slot_mapping = slot_mapping.contiguous()
     eps, interleaved = float(eps), bool(interleaved)
 
     def build():
@@ -1070,15 +1077,16 @@ def rotate_and_cache(
         key.get_device(), value.shape, value.stride(), value.dtype, value.get_device(), key_cache.shape,
         key_cache.stride(), key_cache.dtype, key_cache.get_device(), value_cache.shape, value_cache.stride(),
         value_cache.dtype, value_cache.get_device(), slot_mapping.shape, slot_mapping.dtype, slot_mapping.get_device(),
-        positions.shape, positions.dtype, positions.get_device(), cos_sin.shape, cos_sin.stride(), cos_sin.dtype,
-        cos_sin.get_device(), eps, interleaved, query_weight if query_weight is None else _kind(query_weight),
+        positions if positions is None else (positions.shape, positions.dtype, positions.get_device()),
+        cos_sin if cos_sin is None else (cos_sin.shape, cos_sin.stride(), cos_sin.dtype, cos_sin.get_device()), eps,
+        interleaved, query_weight if query_weight is None else _kind(query_weight),
         key_weight if key_weight is None else _kind(key_weight), key_scales if key_scales is None else _kind(key_scales),
         value_scales if value_scales is None else _kind(value_scales), out if out is None else _kind(out)), build)
     if out is None:
         out = query.new_empty(query.shape)
     with _current(query.device):
         status = _native.load_library().pa_rotate_and_cache(
-            dims, query.data_ptr(), key.data_ptr(), value.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(),
+            dims, query.data_ptr(), key.data_ptr(), value.data_ptr(), _ptr(positions), _ptr(cos_sin),
             _ptr(query_weight), _ptr(key_weight), out.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
             _ptr(key_scales), _ptr(value_scales), slot_mapping.data_ptr(), int(layer_idx), _stream(query.device))
     _native.check(status, "pa_rotate_and_cache")

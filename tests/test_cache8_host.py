@@ -91,6 +91,15 @@ def test_rotation_arguments():
             rotation_call(**kw)
 
 
+def test_rows_without_a_rotation():
+    rows = [torch.zeros((3, n, 64), dtype=torch.bfloat16) for n in (4, 2)]
+    dims = ops._rotate_dims(*rows, None, None, None, torch.ones(64), 1e-6, False)
+    assert dims.rotary_dim == 0 and dims.num_positions == 0 and dims.weight_dtype == native.PA_DTYPE_F32
+    for pos, table in ((None, ops.rope_table(8, 64)), (torch.zeros(3, dtype=torch.int64), None)):
+        with pytest.raises(ValueError, match="together"):
+            ops._rotate_dims(*rows, pos, table, None, None, 1e-6, False)
+
+
 def test_outputs_of_rows():
     like = torch.zeros((3, 4, 64), dtype=torch.bfloat16)
     ops._check_rows_out(torch.zeros((4, 3, 64), dtype=torch.bfloat16).transpose(0, 1), like, "out")

@@ -171,6 +171,33 @@ def test_rows_that_do_not_turn(device, dim):
         check(got, x, weight, torch.zeros(21, dtype=torch.int64), still, False)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (3, 3, 64), (2, 1, 256), (2, 1, 36), (3, 1, 7)])
+def test_norms_alone(device, heads, kv_heads, dim, dtype):
+    # positions and a table of None: rows are normalised and stay where they are
+    q, k, v = rows(37, heads, kv_heads, dim, dtype)
+    w = weights(dim, dtype)
+    still = torch.cat([torch.ones(1, dim // 2), torch.zeros(1, dim // 2)], 1)  # cosines, sines
+    got = ops.rotate(q, k, None, None, query_weight=w[0], key_weight=w[1], eps=EPS)
+    for y, x, weight in zip(got, (q, k), w):
+        check(y, x, weight, torch.zeros(37, dtype=torch.int64), still, False)
+    same = ops.rotate(q, k, None, None)  # nothing to do: the rows
+    assert torch.equal(same[0], q) and torch.equal(same[1], k)
+    slots = torch.arange(37, device=device) + 3
+    for code in (dtype, oracle.CODE):
+        want, mine = ([t.to(code) for t in cache_of((2, 6, 8, kv_heads, dim), torch.float32, device)] for _ in range(2))
+        scales = [[torch.ones((2, 6, kv_heads), device=device) for _ in range(2)] for _ in range(2)]
+        if code is not oracle.CODE:
+            scales = [[None, None], [None, None]]
+        ops.reshape_and_cache(got[1], v, *want, slots, 1, *scales[0])
+        out = ops.rotate_and_cache(q, k, v, *mine, slots, 1, None, None, query_weight=w[0], key_weight=w[1], eps=EPS,
+                                   key_scales=scales[1][0], value_scales=scales[1][1])
+        assert torch.equal(out, got[0])
+        for a, b in zip(mine, want):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        assert code is not oracle.CODE or all(torch.equal(a, b) for a, b in zip(*scales))
+
+
 def test_no_tokens(device):
     q, k, v = rows(0, 4, 2, 64, torch.bfloat16)
     table = ops.rope_table(4, 64, device=device)
