@@ -87,7 +87,6 @@ decode8_kernel(DecodeArgs a) {
   constexpr int PE = D / 16;          // V codes of a lane's piece, blocks of the output
   constexpr int kRowBytes = D;        // an LDS row
   constexpr int kMemBytes = DM;       // a cache row
-  constexpr int kAccRow = D + 4;      // padded LDS row of one head's accumulators
   constexpr int kVLoads = 8;
   using VP = typename VCodes<D>::type;
 
@@ -100,8 +99,8 @@ decode8_kernel(DecodeArgs a) {
   __shared__ __align__(16) float s_sc[kDecodeWaves][2 * kTile8];
   // Per wave: the K rows of its tile, and after the last tile its
   // accumulators.
-  constexpr int kWaveBytes =
-      kMfmaHeads * kAccRow * 4 > kTile8 * kRowBytes ? kMfmaHeads * kAccRow * 4 : kTile8 * kRowBytes;
+  constexpr int kWaveBytes = kMfmaHeads * (D + 4) * 4;
+  static_assert(kWaveBytes >= kTile8 * kRowBytes, "a tile's K rows fit");
   __shared__ __align__(16) char s_wave[kDecodeWaves][kWaveBytes];
 
   const int tid = threadIdx.x;
@@ -111,22 +110,14 @@ decode8_kernel(DecodeArgs a) {
   const int c = lane >> 4;
   constexpr int kHeadWaves = kDecodeWaves / HEADS;  // waves per KV head
   const int hkv = a.num_kv_heads;
-  const uint32_t sub_groups = SHARED ? a.sub_groups : 1;
   const int G = SHARED ? a.group / a.sub_groups : a.group;
-  // Workgroup -> (item, KV head, sub-group): those of an item are a gang, which
-  // shares an XCD's L2 (see decode_mfma.hip), as a head's part of a row is one
-  // line of memory or less.
+  // Gangs of all of an item's workgroups: a head's part of a row is one line of
+  // memory or less.
   const uint32_t units = static_cast<uint32_t>(hkv) / HEADS;
-  const uint32_t gang = units * sub_groups;
-  const uint32_t run = quotient(blockIdx.x, kXcds * gang, a.run_rcp);
-  const uint32_t at_run = blockIdx.x - run * (kXcds * gang);
-  const uint32_t width = min(static_cast<uint32_t>(kXcds), static_cast<uint32_t>(a.num_items) - run * kXcds);
-  const uint32_t member = width == kXcds ? at_run / kXcds : at_run / width;
-  const int64_t item = run * kXcds + (at_run - member * width);
-  const int unit = static_cast<int>(SHARED ? member / sub_groups : member);
-  const int sg = SHARED ? static_cast<int>(member - unit * sub_groups) : 0;
-  const int kvh = unit * HEADS + wave / kHeadWaves;
-  const int h0 = kvh * a.group + sg * G;  // first query head of the wave
+  const DecodePlace place = decode_place<true, SHARED>(a, units);
+  const int64_t item = place.item;
+  const int kvh = place.unit * HEADS + wave / kHeadWaves;
+  const int h0 = kvh * a.group + place.sg * G;  // first query head of the wave
   const int seq = a.items[2 * item];
   const int part = a.items[2 * item + 1];
   const int64_t trow = a.rows != nullptr ? a.rows[seq] : seq;
@@ -438,57 +429,7 @@ decode8_kernel(DecodeArgs a) {
     }
   }
 
-  // ---- combine the waves -------------------------------------------------
-  l = sum_halves(sum_row_pairs(l));
-  float* acc_row = reinterpret_cast<float*>(s_k) + r * kAccRow + 4 * PE * c;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int b = 0; b < PE; b += 4)
-      *reinterpret_cast<float4*>(acc_row + PE * i + b) =
-          make_float4(acc[b][i], acc[b + 1][i], acc[b + 2][i], acc[b + 3][i]);
-  if (lane < kMfmaHeads) {
-    s_m[wave][lane] = m * scale;
-    s_l[wave][lane] = l;
-  }
-  __syncthreads();
-
-  const int hq = hkv * a.group;
-  const int nparts = ctx <= a.partition ? 1 : (ctx + a.partition - 1) / a.partition;
-  const int hu = unit * HEADS * a.group + sg * G;  // first query head of the workgroup
-  float* pacc = a.part_acc + (item * hq + hu) * DM;
-  T* out = reinterpret_cast<T*>(a.output) + (qtok * hq + hu) * DM;
-  for (int i = tid; i < HEADS * G * DM; i += kDecodeThreads) {
-    const int hg = i / DM;
-    const int kv = HEADS == 1 ? 0 : hg / G;
-    const int w0 = kv * kHeadWaves;  // the head's first wave
-    const int g = hg - kv * G;
-    const int e = g * kAccRow + (i - hg * DM);
-    float mx = s_m[w0][g];
-#pragma unroll
-    for (int w = 1; w < kHeadWaves; ++w) mx = fmaxf(mx, s_m[w0 + w][g]);
-    float o = 0.f, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kHeadWaves; ++w) {
-      const float f = fast_exp2(s_m[w0 + w][g] - mx);
-      o = fmaf(reinterpret_cast<const float*>(s_wave[w0 + w])[e], f, o);
-      sum = fmaf(s_l[w0 + w][g], f, sum);
-    }
-    if (nparts <= 1) {
-      store_scalar<T>(out + i, sum > 0.f ? o / sum : 0.f);
-    } else {
-      store_device(pacc + i, o);
-      if (i % DM == 0) {
-        float* pml = a.part_ml + (item * hq + hu + hg) * 2;
-        store_device(pml, mx);
-        store_device(pml + 1, sum);
-      }
-    }
-  }
-  if (nparts > 1 && n > 0 && a.merge_state != nullptr && seq >= 0 && seq < a.num_seqs)
-    merge_in_launch<T, DM, kMergeOutputs>(a, HEADS * G, part, item, ctx, nparts,
-                                          (static_cast<int64_t>(seq) * units + unit) * a.sub_groups + sg, hu, hq,
-                                          reinterpret_cast<T*>(a.output) + qtok * hq * DM);
+  combine_waves<T, D, DM, HEADS>(a, place, units, G, seq, part, ctx, n, qtok, m, l, acc, s_m, s_l, s_wave);
 }
 
 template <typename T, int D, int DM, typename Op>
