@@ -133,6 +133,30 @@ def test_slots_outside_the_pool_are_skipped(device):
     same(mine, want, 0)
 
 
+def test_positions_outside_the_table_leave_their_k_rows_out(device):
+    # beside a block's other rows: those are re-coded as the block grows, the
+    # skipped row's too; V rows are written all the same
+    bs, kv, dim = 8, 2, 64
+    gen = torch.Generator().manual_seed(8)
+    mine = empty(1, 4, bs, kv, dim, device, garbage=True)
+    slots = torch.tensor([3, 4, 5, 8, 9, 10, 31])
+    bad = torch.tensor([False, True, False, False, True, True, True])
+    x = 20 * torch.randn((7, 4, dim), generator=gen).to(torch.bfloat16)
+    q, k, v = x.to(device).split([2, 1, 1], dim=1)
+    k, v = k.expand(-1, kv, -1), v.expand(-1, kv, -1)
+    table = ops.rope_table(10, dim, device=device)
+    pos = torch.where(bad, torch.tensor(10), torch.arange(7)).to(device)
+    turned = ops.rotate(q, k.contiguous(), pos, table)[1]
+    want = []
+    for i, rows, at in ((0, turned, torch.where(bad, torch.tensor(-1), slots)), (1, v, slots)):
+        want += oracle.write(mine[i][0].cpu().clone(), mine[2 + i][0].cpu().clone(), stored(rows), at.tolist())
+    want[1][3], want[0][3] = mine[2][0, 3].cpu(), mine[0][0, 3].cpu()  # (nothing of it is written)
+    out = ops.rotate_and_cache(q, k, v, mine[0], mine[1], slots.to(device), 0, pos, table, key_scales=mine[2],
+                               value_scales=mine[3])
+    assert torch.equal(torch.isnan(out).all(-1).all(-1).cpu(), bad)
+    same(mine, want, 0)
+
+
 def test_token_by_token_keeps_the_values(device):
     # Appending one row at a time only ever re-codes by powers of two: the
     # values are those of the whole block at once, but for subnormal codes.
