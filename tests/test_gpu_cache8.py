@@ -368,6 +368,38 @@ def test_fp16_queries_over_values_past_fp16(device, heads, kv_heads, dim, bs, co
     assert ((out - ref).abs() <= bound)[~over].all()
 
 
+@pytest.mark.parametrize("dim,kv_heads,bs", [(128, 8, 16), (64, 8, 4), (40, 8, 16)])
+def test_caches_past_32_bit_offsets(device, dim, kv_heads, bs):
+    # a layer of more than 2^32 codes, its sequence in the last blocks: the same
+    # rows, codes and results as in a small cache
+    heads, need = 2 * kv_heads, 7
+    blocks = 2**32 // (bs * kv_heads * dim) + 100
+    small = [t.to(device) for t in empty(2, need, bs, kv_heads, dim, device)]
+    large = [torch.empty((2, blocks, bs, kv_heads, dim), dtype=torch.uint8, device=device).view(CODE) for _ in range(2)]
+    large += [torch.zeros((2, blocks, kv_heads), device=device) for _ in range(2)]
+    total = need * bs - 3
+    x = torch.randn((total, heads + 2 * kv_heads, dim), device=device).to(torch.bfloat16)
+    q, k, v = x.split([heads, kv_heads, kv_heads], dim=1)
+    rope = ops.rope_table(total, dim, device=device)
+    tables = [torch.arange(n - need, n, dtype=torch.int32, device=device).reshape(1, -1) for n in (need, blocks)]
+    for start, count in ((0, total - 1), (total - 1, 1)):
+        outs = []
+        for cache, table in zip((small, large), tables):
+            step = ops.pack_step(table, [start], [count], bs, num_kv_heads=kv_heads, num_query_heads=heads, head_dim=dim,
+                                 dtype=CODE)
+            part = slice(start, start + count)
+            rq = ops.rotate_and_cache(q[part], k[part], v[part], cache[0], cache[1], step.scatter_slots, 1,
+                                      step.position_ids, rope, key_scales=cache[2], value_scales=cache[3])
+            outs.append(ops.attention(rq, cache[0], cache[1], 1, step, dim**-0.5, key_scales=cache[2],
+                                      value_scales=cache[3]))
+        assert torch.equal(*outs) and torch.isfinite(outs[0]).all()
+    for a, b in zip(small[:2], large[:2]):
+        a, b = (t.view(torch.uint8)[1, -need:].reshape(need * bs, -1)[:total] for t in (a, b))
+        assert torch.equal(a, b)
+    for a, b in zip(small[2:], large[2:]):
+        assert torch.equal(a[1], b[1, -need:])
+
+
 # ---- together, as a server runs them ------------------------------------------
 
 
