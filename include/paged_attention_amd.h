@@ -656,8 +656,8 @@ int pa_attention_step(const PaStepCall *call, const void *query, void *key_cache
  *
  *  - A block's scale is the smallest power of two >= (largest finite magnitude
  *    of its rows) / 448, at least 2^-64, per KV head and tensor.
- *  - A call that writes a block's first row starts the block afresh: what it
- *    held counts for nothing.  So a block is filled from its first row on.
+ *  - A call whose slots name a block's first row starts the block afresh: what
+ *    it held counts for nothing.  So a block is filled from its first row on.
  *  - A call that writes other rows of a block keeps the larger of its scale
  *    and the one the new rows need.  If that is larger, the block's other rows
  *    are re-coded with it (rounded to nearest even): their values stay but
@@ -667,9 +667,10 @@ int pa_attention_step(const PaStepCall *call, const void *query, void *key_cache
  *    maximum: +-61440 in fp16, +-1.875 * 2^127 in bf16 and fp32.  Infinities
  *    and NaN become NaN and count for no scale.
  *  - The tokens of one block follow each other in the call's slot_mapping (as
- *    pa_pack's scatter_slots have them), and no slot occurs twice.  (A mapping
- *    that breaks this reads and writes inside the caches, but leaves blocks
- *    whose scale does not fit all of their codes.)
+ *    pa_pack's scatter_slots have them) with no other token between them, not
+ *    even one whose slot is skipped, and no slot occurs twice.  (A mapping that
+ *    breaks this reads and writes inside the caches, but leaves blocks whose
+ *    scale does not fit all of their codes.)
  *  - block_size is at most 256.
  *
  * pa_copy_blocks / pa_swap_blocks move codes and scales alike (a block of
@@ -716,7 +717,8 @@ typedef struct {
  * cos_sin float [num_positions, rotary_dim]: a position's cosines, then its
  * sines), the elements past R stay.  All of it in fp32, rounded once.  A token
  * whose position lies outside [0, num_positions) gets NaN rows.  query_out may
- * be query, and key_out key.  `dims` is read before the call returns.
+ * be query and key_out key, with their strides; outputs and inputs overlap in no
+ * other way.  `dims` is read before the call returns.
  */
 int pa_rotate(const PaRotateDims *dims, const void *query, const void *key,
               const int64_t *positions, const float *cos_sin,

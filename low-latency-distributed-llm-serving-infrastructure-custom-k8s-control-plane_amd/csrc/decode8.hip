@@ -17,12 +17,12 @@
 //    them.
 // What bounds it is HBM: half the bytes a token of the 16-bit cache, and 4 to 8
 // flops a byte of a group's heads, far below what the matrix units do.  bf16,
-// 256 sequences of 32-8192 tokens, 32/8 heads of 128 (778 MB): 142 us, 5.5 TB/s
-// (a pure read: 7.0); two of 60000-131000 (475 MB): 84 us, 5.7; fp16, 64 of
-// 128-4096, 32/32 heads (1.18 GB): 199 us, 5.9.  Between these and the read
+// 256 sequences of 32-8192 tokens, 32/8 heads of 128 (778 MB): 143 us, 5.4 TB/s
+// (a pure read: 7.0); two of 60000-131000 (475 MB): 83 us, 5.7; fp16, 64 of
+// 128-4096, 32/32 heads (1.18 GB): 198 us, 6.0.  Between these and the read
 // rate lie workgroups of unequal length on a CU's last round and the reads of
 // ids and scales ahead of a workgroup's first rows.  Eight sequences of 16-512
-// tokens, 8/8 heads of 64: 6.7 us, a chain of dependent reads.
+// tokens, 8/8 heads of 64: 6.9 us, a chain of dependent reads.
 #include <type_traits>
 
 #include "cache8.hpp"

@@ -57,7 +57,13 @@
 // runs of one kind in lock-step with the other wave of its SIMD.
 // The row sum is accumulated from the rounded probabilities the PV product
 // uses (v_dot2 against ones), per lane half, and the halves are added once
-// at the end.  Masking is applied only to tiles that cross the causal
+// at the end.  They enter that product as one 16-bit term: a weight is off by
+// half a step of the type at most, about what rounding the result costs (bf16,
+// four chunks of 512 at 4096: off by 0.0022 of the result where fp32
+// probabilities leave 0.0017, and 0.0016 is the result's rounding).  A second
+// term, as in the decode, whose products are free beside its reads, would make
+// 24 products of a tile's 16 (heads of 128), in a kernel that waits for little
+// else.  Masking is applied only to tiles that cross the causal
 // diagonal or the end of the context (or to every tile when some block id of
 // the sequence lies outside the pool: those positions are skipped, as in
 // decode), in a separate loop after the unmasked one, and the accumulator is
@@ -74,9 +80,12 @@
 // comes one step earlier still.  All eight waves share the conversions (16 a
 // thread and step, against its 16 exponentials), which cost what the smaller
 // reads save and some more: bf16, four chunks of 512 at 4096, 32/8 heads of 128
-// (146 GFLOP), 177 us, 825 TFLOP/s (the 16-bit cache 164); 2048 at 6000, 272 us
-// (242).  fp16, 1000 ragged tokens, 16/4 heads of 80: 48 us, its longest unit's
-// chain of stages.
+// (146 GFLOP), 170 us, 858 TFLOP/s (the 16-bit cache 152); 2048 at 6000, 262 us
+// (231): both repeated until the clocks have settled, which takes the chip tens
+// of launches (the first after a pause take 201 and 169 us, the fifteenth or
+// twentieth 233 and 203).
+// fp16, 1457 ragged tokens, 16/4 heads of 80: 44 us, its longest unit's chain of
+// 30 stages.
 //
 // Reference: the block-diagonal causal mask of app/model/paged_attention.py:
 // 92-118 applied by SDPA (paged_attention.py:170-178); query token j of a

@@ -15,12 +15,13 @@
 //
 // What bounds it is memory once a step has some ten thousand rows, and before
 // that the launch and two dependent reads (position, then table).  bf16 rows,
-// cold caches: 8 tokens of 32/8 heads of 128 2.4 us; 2176 tokens with norms
-// (54.6 MB) 17.6 us, 3.1 TB/s; 4096 tokens 28.9 us, 3.5 TB/s.  The 8-bit write:
-// 256 decode tokens 6.2 us; 1400 tokens of 32/32 heads of 128, fp16 with norms
-// (58 MB) 25.6 us; 15000 tokens of 9/3 heads of 64 (75 MB) 26.5 us, 2.8 TB/s: there
-// each chunk reads the rows that may belong to its last run, which the next one
-// reads again, and waits for slots, rows and scales one after the other.
+// cold caches: 8 tokens of 32/8 heads of 128 3.2 us; 2176 tokens with norms
+// (54.6 MB) 17.5 us, 3.1 TB/s; the rotation alone, 4096 tokens with norms (86 MB)
+// 25.8 us, 3.3 TB/s.  The 8-bit write: 256 decode tokens 6.8 us; 1406 tokens of
+// 32/32 heads of 128, fp16 with norms (58 MB) 25.2 us; 20183 tokens of 9/3 heads
+// of 64 (75 MB) 25.9 us, 2.9 TB/s: there each chunk reads the rows that may belong
+// to its last run, which the next one reads again, and waits for slots, rows and
+// scales one after the other.
 #include "cache8.hpp"
 #include "pa_common.hpp"
 #include "pa_launch.hpp"
@@ -598,7 +599,13 @@ static hipError_t launch_rotate_n(const RotateArgs& args, hipStream_t s) {
   // bf16, 32/8 heads of 128, 256 tokens 6.1 / 7.5 us, 1024 10.0 / 11.2, 2048
   // 17.4 / 16.7; fp16, 32/32 of 128, 384 tokens 10.4 / 11.2, 512 13.4 / 12.8,
   // 4096 69.1 / 61.8; 9/3 heads of 64, 8192 tokens 13.5 / 13.9, 16384 23.5 /
-  // 22.3; 8/2 heads of 256, 2048 tokens 10.0 / 10.8, 8192 31.7 / 29.1.
+  // 22.3; 8/2 heads of 256 in blocks of 8, 2048 tokens 10.0 / 10.8, 8192 31.7 /
+  // 29.1.  Blocks longer than a group's rows at once and one (33 tokens for heads
+  // of 64, 17 up to 128, 9 above) would need a span that does not fit the
+  // registers: their rows are loaded, normalised and turned twice.  bf16 32/8
+  // heads of 128, blocks of 16 and of 32: 256 tokens 7.2 / 7.4 us, 2048 17.5 /
+  // 21.9, 8192 53.5 / 73.6; 8/2 of 256, blocks of 8 and of 16: 6.6 / 6.6, 10.3 /
+  // 14.0, 29.2 / 39.1.
   const bool keep = a.block_size <= kRows + 1;
   const bool three = keep && static_cast<int64_t>(a.num_tokens) * 2 * a.num_kv_heads * L >= resident_lanes();
   const int own = three ? 2 * kRows : kRows;

@@ -769,11 +769,11 @@ def reshape_and_cache(
     An 8-bit cache (``torch.float8_e4m3fn``) takes rows of any type and its
     scales, fp32 [L, N, H_kv], which the call keeps: a block's scale is the
     smallest power of two that is at least its rows' largest magnitude / 448
-    (and 2^-64), a call that writes a block's first row starts the block
+    (and 2^-64), a call whose slots name a block's first row starts the block
     afresh, and one that writes later rows re-codes the block's others where
     its scale grows.  The tokens of a block follow each other in
-    ``slot_mapping``, no slot occurs twice, and blocks have at most 256
-    tokens.  Rows are limited to +-61440 (fp16) or
+    ``slot_mapping`` (with no skipped one between them), no slot occurs twice,
+    and blocks have at most 256 tokens.  Rows are limited to +-61440 (fp16) or
     +-1.875 * 2^127; infinities become NaN.
     """
     device = _require_device(key, value, key_cache, value_cache, slot_mapping)
