@@ -47,6 +47,11 @@ int elem_bytes(int dtype) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether the largest product is the largest score, by a factor that fp32 holds
+// in full: the fast kernels take a row's maximum, and mask, before they scale.
+// (The generic kernel scales first and takes any scaling.)
+bool ordered_scaling(float scaling) { return scaling >= 1e-30f; }
+
 int log2_exact(int v) {
   int r = 0;
   while ((1 << r) < v) ++r;
@@ -525,6 +530,7 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
   const int cache_eb = scales != nullptr ? 1 : eb;
   const int log2_bs = log2_exact(dims.block_size);
   const bool fast =
+      ordered_scaling(scaling) &&
       pa::decode_fast_path_supported(scales == nullptr ? dims.dtype : PA_DTYPE_E4M3, dims.head_dim, group,
                                      dims.block_size, dims.partition_size) &&
       (scales == nullptr || dims.dtype != PA_DTYPE_F32) &&
@@ -721,6 +727,7 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
   const int eb = elem_bytes(dims.dtype);
   const int cache_eb = scales != nullptr ? 1 : eb;
   const bool fast =
+      ordered_scaling(scaling) &&
       pa::prefill_fast_path_supported(dims.dtype, dims.head_dim, group, dims.block_size) &&
       (scales == nullptr || pa::prefill_codes_supported(dims.dtype, dims.head_dim)) &&
       prefill_tile == pa::prefill_tile_for(group) && dims.max_blocks_per_seq > 0 &&

@@ -154,3 +154,39 @@ def test_new_rows_without_a_block_hold_anything(device, heads, kv_heads, dim, bs
     check(out, q, pools, table, dtype, 2.0)
     for cache, pool in zip((kc, vc), pools):
         assert torch.equal(cache[0, 1:].cpu().double(), pool[1:])
+
+
+@pytest.mark.parametrize("scaling", [0.0, -0.1])
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype,cache_dtype", [
+    (8, 2, 128, torch.bfloat16, CODE), (4, 4, 64, torch.float16, CODE), (8, 2, 128, torch.bfloat16, torch.bfloat16),
+    (4, 4, 64, torch.float16, torch.float16), (6, 2, 80, torch.bfloat16, torch.bfloat16),
+    (2, 1, 256, torch.bfloat16, torch.bfloat16), (4, 2, 128, torch.float32, torch.float32),
+    (3, 1, 40, torch.float16, torch.float16)])
+@pytest.mark.parametrize("fused", [False, True])
+def test_scaling_of_zero_and_below(device, heads, kv_heads, dim, dtype, cache_dtype, scaling, fused):
+    # the softmax of -0.1 q.k, and (0) the mean of V, with missing blocks
+    q, held, pools, table = case(heads, kv_heads, dim, dtype, cache_dtype, 3.0, 0.0)
+    kc, ks, vc, vs = (None if t is None else t[None].to(device) for t in held)
+    step = ops.pack_step(torch.from_numpy(table).to(device), STARTS, COUNTS, 16, num_kv_heads=kv_heads,
+                         num_query_heads=heads, head_dim=dim, dtype=cache_dtype,
+                         prefill_tile=ops.prefill_tile_for(heads, kv_heads))
+    rows = {}
+    if fused:  # the rows that are there already, written again
+        if cache_dtype == CODE:
+            pytest.skip("8-bit rows are coded afresh")
+        at = [(int(table[i, p // 16]), p % 16) for i, (s, c) in enumerate(zip(STARTS, COUNTS)) for p in range(s, s + c)]
+        for name, pool in (("new_key", held[0]), ("new_value", held[2])):
+            rows[name] = torch.stack([pool[b, j] if 0 <= b < pool.shape[0] else torch.zeros_like(pool[0, 0])
+                                      for b, j in at]).to(device)
+        rows["fused_prefill_write"] = True
+    out = ops.attention(q.to(device), kc, vc, 0, step, scaling, key_scales=ks, value_scales=vs, **rows)
+    ref, size, peak = oracle.attention(q, *pools, table, STARTS, COUNTS, scaling)
+    out = out.cpu().double()
+    assert torch.isfinite(out).all()
+    # scores are below 3 * 1.5 * dim / 10 + 2 (see check)
+    u = oracle.ROW_EPS[dtype]
+    bound = (1 + 2 * u) * u * ref.abs() + (2 * u + 2 * (dim + 4) * 2.0**-24 * (dim / 2 + 2) + 1.5e-5) * size
+    if dtype == torch.float16:
+        bound = bound + 2.0**-24 + 2.0**-25 * peak
+    excess = ((out - ref).abs() - bound).max().item()
+    assert excess <= 0, f"{excess:.3e} over the bound"
