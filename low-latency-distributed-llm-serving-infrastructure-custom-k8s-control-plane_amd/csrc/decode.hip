@@ -793,7 +793,7 @@ __global__ __launch_bounds__(kDecodeThreads) PA_DECODE_OCCUPANCY(T, D, G) void d
       l = fmaf(s_l[w][g], f, l);
     }
     if (nparts <= 1) {
-      store_scalar<T>(out + i, l > 0.f ? o / l : 0.f);
+      store_scalar<T>(out + i, l != 0.f ? o / l : 0.f);
     } else {
       store_device(pacc + i, o);
       if (i % DM == 0) {

@@ -27,7 +27,8 @@ constexpr int kMfmaHeads = 16;
 // for the K elements (one after the other, eight heads of 128 took four).
 // Each element's arithmetic is the same whatever K, and both merge paths
 // (the merge kernel, K = 1, and the in-launch merge of the partition
-// kernel) run this, so they give the same bits.
+// kernel) run this, so they give the same bits.  (A sum of zero is a row that
+// attends nothing, whose result is zero; a NaN one, of a NaN score, stays.)
 constexpr int kMergeBatch = 8;
 constexpr int kMergeOutputs = 4;  // elements a thread of the in-launch merge merges at once
 
@@ -86,7 +87,7 @@ __device__ __forceinline__ void merge_partials(const float* ml, const float* acc
     mx = mn;
   }
 #pragma unroll
-  for (int k = 0; k < K; ++k) store_scalar<T>(out + k * estride, sum > 0.f ? o[k] / sum : 0.f);
+  for (int k = 0; k < K; ++k) store_scalar<T>(out + k * estride, sum != 0.f ? o[k] / sum : 0.f);
 }
 
 // The last of a sequence's partition workgroups (for this unit and

@@ -124,7 +124,7 @@ __device__ __forceinline__ void combine_waves(const DecodeArgs& a, const DecodeP
       sum = fmaf(s_l[w0 + w][g], f, sum);
     }
     if (nparts <= 1) {
-      store_scalar<T>(out + i, sum > 0.f ? o / sum : 0.f);
+      store_scalar<T>(out + i, sum != 0.f ? o / sum : 0.f);
     } else {
       store_device(pacc + i, o);
       if (i % DM == 0) {
