@@ -395,9 +395,9 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
       // ---- copies ------------------------------------------------------------
       // Rows past the readable context re-read its last row, and an
       // out-of-pool block id reads block 0 (their scores are masked and
-      // their V rows cleared).  No stage past the last is copied: a step's copies, and the
-      // count of them its wait allows in flight, depend on how many stages
-      // remain.
+      // the latter's V rows cleared).  No stage past the last is copied: a
+      // step's copies, and the count of them its wait allows in flight, depend
+      // on how many stages remain.
       // Block ids of the first stages come from scalar loads of the table
       // (constant address space: the table does not change during the launch).
       const_i32* btc = (const_i32*)(bt);

@@ -159,7 +159,7 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
     };
     // Copies of stage x into buffer b.  Rows past the readable context
     // re-read its last row and an out-of-pool block reads block 0 (their
-    // scores are masked and their V rows cleared).  APPEND: rows at or after the
+    // scores are masked and the latter's V rows cleared).  APPEND: rows at or after the
     // chunk's start come from the new rows -- one path per stage (all rows
     // before the chunk, all in it, or the stage that holds its start), as
     // per-lane address selects in every stage spilled registers in the
