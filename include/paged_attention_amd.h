@@ -793,6 +793,156 @@ int pa_attention_step_8bit(const PaStepCall *call, const void *query, void *key_
                            int32_t layer_idx, const PaNewRows *new_rows, float scaling,
                            void *output, void *stream);
 
+/* ---- (h) part of the context: windows with sinks, trees of drafted tokens -- */
+
+/* The query at position p sees the positions q <= p with p - q < window or
+ * q < sinks.  window 0: no window (sinks is then not read). */
+typedef struct {
+    int32_t window;
+    int32_t sinks;
+} PaWindow;
+
+/*
+ * No counterpart in the reference, whose mask is causal alone.  One layer of a
+ * packed step under a window (at least 1): pa_attention_step, or with scales
+ * (of an 8-bit cache; NULL otherwise) pa_attention_step_8bit, over what the
+ * window and the sinks leave; new_rows may be NULL.  Block-table entries of
+ * positions that no query of the step sees are not read, and neither are their
+ * rows.
+ *
+ * call->decode_items and merge_items describe partitions of call->dims.
+ * partition_size tokens of the SHORTER context that the decode walks: without
+ * the whole blocks between the last that holds a visible sink and the first of
+ * the window.  pa_window_context gives its length; a list made for longer
+ * contexts (their partitions in pa_pack's order) serves shorter ones as well.
+ * call->context_lens stays the sequences' own.
+ */
+int pa_attention_window(const PaStepCall *call, PaWindow window, const void *query,
+                        void *key_cache, void *value_cache, float *key_scales,
+                        float *value_scales, int32_t layer_idx,
+                        const PaNewRows *new_rows, float scaling, void *output,
+                        void *stream);
+
+/* Host code: the longest shorter context (see above) a sequence of up to
+ * `context` tokens has under the window. */
+int32_t pa_window_context(int32_t context, PaWindow window, int32_t block_size);
+
+/* Most nodes of one tree. */
+#define PA_MAX_TREE_NODES 1024
+
+/* What a step of trees shares: every sequence's new tokens are the nodes of a
+ * tree behind its context. */
+typedef struct {
+    int32_t num_seqs;
+    int32_t num_query_tokens;
+    int32_t num_query_heads;  /* (0: masks and positions alone, no lists) */
+    int32_t num_kv_heads;
+    int32_t head_dim;
+    int32_t dtype;            /* of the query */
+    int32_t block_size;
+    int32_t compute_units;    /* of the device (0: 256) */
+    int32_t split_stages;     /* > 0: use it; 0: choose */
+    PaWindow window;
+} PaTreeDims;
+
+typedef struct {
+    int64_t num_items;        /* sizes of pa_pack_tree's lists */
+    int64_t num_merge_items;
+    int64_t num_partial_rows; /* rows of partial results the attention keeps */
+    int32_t mask_words;
+    int32_t tile;             /* nodes per tile (0: no lists) */
+    int32_t split_stages;     /* stages of 64 positions per item */
+    int32_t bad_seq;          /* first sequence failing a check, or -1 */
+} PaTreePlan;
+
+/*
+ * Host code, no GPU call: sizes a step of trees from the HOST arrays of the
+ * sequences' starts and node counts (int64 [num_seqs], each count at most
+ * PA_MAX_TREE_NODES and, with a window, at most that) and chooses how the
+ * context is split over workgroups.  Shapes without a matrix-core kernel need
+ * no lists (tile 0).
+ */
+int pa_plan_tree(const int64_t *start_positions, const int64_t *node_counts,
+                 PaTreeDims dims, PaTreePlan *plan);
+
+/*
+ * No counterpart in the reference.  parents int32 [T]: each node's parent, an
+ * earlier node's index within its sequence, or -1 for a root (whose parent is
+ * the context's last token); anything else reads as -1.  Writes masks uint32
+ * [T, mask_words] (bit j % 32 of word j / 32: node j of the sequence is the
+ * node itself or an ancestor), positions int64 [T] (the start plus the node's
+ * depth) and, for a plan with a tile, the attention's work lists: items int32
+ * [num_items, 4], merge_items int32 [num_merge_items, 4] (16-byte aligned).
+ * Entries past a size in the plan are dropped, entries left over are marked.
+ */
+int pa_pack_tree(const int32_t *parents, const int32_t *context_lens,
+                 const int64_t *cu_seqlens, PaTreeDims dims, PaTreePlan plan,
+                 uint32_t *masks, int64_t *positions, int32_t *items,
+                 int32_t *merge_items, void *stream);
+
+typedef struct {
+    PaStepDims dims;
+    const int32_t *block_tables;
+    const int32_t *context_lens;
+    const int64_t *cu_seqlens;
+    const int64_t *scatter_slots;
+    const uint32_t *masks;
+    const int64_t *positions;
+    const int32_t *items;
+    const int32_t *merge_items;
+    void *workspace;          /* pa_tree_workspace_size(dims, num_partial_rows) */
+    size_t workspace_bytes;
+    PaTreePlan plan;
+    PaWindow window;          /* as the plan's */
+} PaTreeCall;
+
+/* Bytes of workspace pa_tree_attention needs (fp32 rows and their softmax
+ * statistics; no initial value).  Calls that share one must not overlap in
+ * time. */
+size_t pa_tree_workspace_size(PaStepDims dims, int64_t num_partial_rows);
+
+/*
+ * No counterpart in the reference.  One layer of a step of trees: with new_rows
+ * (may be NULL) pa_reshape_and_cache (_8bit) at call->scatter_slots -- node j of
+ * a sequence in the slot of position start + j -- then every node attends its
+ * sequence's context (under a window, what that leaves at the node's position),
+ * its ancestors and itself.  Scales: of an 8-bit cache, else NULL.  output
+ * [T, H_q, D] contiguous.
+ */
+int pa_tree_attention(const PaTreeCall *call, const void *query, void *key_cache,
+                      void *value_cache, float *key_scales, float *value_scales,
+                      int32_t layer_idx, const PaNewRows *new_rows, float scaling,
+                      void *output, void *stream);
+
+/*
+ * No counterpart in the reference.  From node 0 of each sequence on, the first
+ * child whose drafted token is the one predicted at its parent (drafted,
+ * predicted int64 [T]), until none is.  nodes int32 [T]: the path's nodes in
+ * the sequence's first rows, -1 behind; counts int32 [B]: their number;
+ * next_tokens int64 [B]: what the path's last node predicts (0 and -1 for a
+ * sequence without nodes).
+ */
+int pa_accept_tree(const int32_t *parents, const int64_t *cu_seqlens,
+                   const int64_t *drafted, const int64_t *predicted,
+                   int32_t num_seqs, int32_t num_query_tokens, int32_t *nodes,
+                   int32_t *counts, int64_t *next_tokens, void *stream);
+
+/*
+ * No counterpart in the reference.  In every layer and both caches the row of
+ * position start + nodes[first + j] moves to position start + j, j <
+ * counts[sequence]: a path's rows come to lie behind the context.  The kept
+ * nodes of a sequence ascend; at the first that does not, or is none of its
+ * nodes, the sequence's rows stay as they are from there on, as do rows to or
+ * from a missing block.  dims: sizes, dtype (of the cache's elements; with
+ * scales not read) and table rows of the step.  8-bit caches: a block that rows
+ * move into gets the largest scale among its own and those rows' blocks', and
+ * codes of smaller ones are re-coded with it.
+ */
+int pa_keep_rows(void *key_cache, void *value_cache, float *key_scales,
+                 float *value_scales, PaStepDims dims, const int32_t *block_tables,
+                 const int32_t *context_lens, const int64_t *cu_seqlens,
+                 const int32_t *nodes, const int32_t *counts, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,7 +15,7 @@ import threading
 from pathlib import Path
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libpaged_attention_amd.so"
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 PA_OK = 0
 PA_ERR_INVALID_ARGUMENT = 1
@@ -36,6 +36,8 @@ PA_DECODE_SCRATCH_BYTES = 64 << 20
 PA_DECODE_SCRATCH_STATE_BYTES = 1 << 20
 PA_STEP_PREFILL_WRITE = 1
 PA_STEP_NO_APPEND = 2
+
+PA_MAX_TREE_NODES = 1024
 
 PA_SWAP_OUT = 0
 PA_SWAP_IN = 1
@@ -69,6 +71,14 @@ EXPORTED_SYMBOLS = (
     "pa_decode_8bit",
     "pa_prefill_8bit",
     "pa_attention_step_8bit",
+    "pa_attention_window",
+    "pa_window_context",
+    "pa_plan_tree",
+    "pa_pack_tree",
+    "pa_tree_workspace_size",
+    "pa_tree_attention",
+    "pa_accept_tree",
+    "pa_keep_rows",
     "pa_map_host_memory",
     "pa_calibrate_mfma",
     "pa_calibrate_mfma_flops",
@@ -201,6 +211,58 @@ class PaStepCall(ctypes.Structure):
     ]
 
 
+class PaWindow(ctypes.Structure):
+    _fields_ = [
+        ("window", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+    ]
+
+
+class PaTreeDims(ctypes.Structure):
+    _fields_ = [
+        ("num_seqs", ctypes.c_int32),
+        ("num_query_tokens", ctypes.c_int32),
+        ("num_query_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("compute_units", ctypes.c_int32),
+        ("split_stages", ctypes.c_int32),
+        ("window", PaWindow),
+    ]
+
+
+class PaTreePlan(ctypes.Structure):
+    _fields_ = [
+        ("num_items", ctypes.c_int64),
+        ("num_merge_items", ctypes.c_int64),
+        ("num_partial_rows", ctypes.c_int64),
+        ("mask_words", ctypes.c_int32),
+        ("tile", ctypes.c_int32),
+        ("split_stages", ctypes.c_int32),
+        ("bad_seq", ctypes.c_int32),
+    ]
+
+
+class PaTreeCall(ctypes.Structure):
+    _fields_ = [
+        ("dims", PaStepDims),
+        ("block_tables", ctypes.c_void_p),
+        ("context_lens", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("scatter_slots", ctypes.c_void_p),
+        ("masks", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("items", ctypes.c_void_p),
+        ("merge_items", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("plan", PaTreePlan),
+        ("window", PaWindow),
+    ]
+
+
 class PaPlanParams(ctypes.Structure):
     _fields_ = [
         ("block_size", ctypes.c_int32),
@@ -315,6 +377,21 @@ _SIGNATURES = {
         ctypes.c_int,
         [_vp, _vp, _vp, PaCacheScales, _i32, PaStepDims, _vp, _vp, _vp, _vp, _i64, _i32, _f32, _vp, _vp],
     ),
+    "pa_attention_window": (
+        ctypes.c_int,
+        [ctypes.POINTER(PaStepCall), PaWindow, _vp, _vp, _vp, _vp, _vp, _i32, ctypes.POINTER(PaNewRows), _f32, _vp,
+         _vp],
+    ),
+    "pa_window_context": (_i32, [_i32, PaWindow, _i32]),
+    "pa_plan_tree": (ctypes.c_int, [_vp, _vp, PaTreeDims, ctypes.POINTER(PaTreePlan)]),
+    "pa_pack_tree": (ctypes.c_int, [_vp, _vp, _vp, PaTreeDims, PaTreePlan, _vp, _vp, _vp, _vp, _vp]),
+    "pa_tree_workspace_size": (_sz, [PaStepDims, _i64]),
+    "pa_tree_attention": (
+        ctypes.c_int,
+        [ctypes.POINTER(PaTreeCall), _vp, _vp, _vp, _vp, _vp, _i32, ctypes.POINTER(PaNewRows), _f32, _vp, _vp],
+    ),
+    "pa_accept_tree": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "pa_keep_rows": (ctypes.c_int, [_vp, _vp, _vp, _vp, PaStepDims, _vp, _vp, _vp, _vp, _vp, _vp]),
     "pa_map_host_memory": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_void_p)]),
     "pa_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "pa_last_error_message": (ctypes.c_char_p, []),

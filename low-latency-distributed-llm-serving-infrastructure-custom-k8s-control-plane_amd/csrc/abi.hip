@@ -149,7 +149,7 @@ int scratch_address(void** out, const char* who) {
 
 extern "C" {
 
-int pa_abi_version(void) { return 13; }
+int pa_abi_version(void) { return 14; }
 
 const char* pa_error_string(int code) {
   switch (code) {
@@ -502,7 +502,8 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
                   const int64_t* cu_seqlens, const int32_t* decode_items,
                   int64_t num_decode_items, const int32_t* merge_items, int64_t num_merge_items,
                   float scaling, void* output, void* workspace, size_t workspace_bytes,
-                  void* stream, const PaNewRows* new_rows = nullptr, const PaCacheScales* scales = nullptr) {
+                  void* stream, const PaNewRows* new_rows = nullptr, const PaCacheScales* scales = nullptr,
+                  PaWindow window = {0, 0}) {
   if (phases <= 0 || (phases & ~(PA_DECODE_PHASE_PARTITIONS | PA_DECODE_PHASE_MERGE)) != 0)
     return fail(PA_ERR_INVALID_ARGUMENT, "%s: phases must be a non-empty mask of "
                 "PA_DECODE_PHASE_PARTITIONS and PA_DECODE_PHASE_MERGE, got %d", who, phases);
@@ -530,7 +531,7 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
   const int cache_eb = scales != nullptr ? 1 : eb;
   const int log2_bs = log2_exact(dims.block_size);
   const bool fast =
-      ordered_scaling(scaling) &&
+      window.window == 0 && ordered_scaling(scaling) &&
       pa::decode_fast_path_supported(scales == nullptr ? dims.dtype : PA_DTYPE_E4M3, dims.head_dim, group,
                                      dims.block_size, dims.partition_size) &&
       (scales == nullptr || dims.dtype != PA_DTYPE_F32) &&
@@ -641,6 +642,8 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
   a.block_size = dims.block_size;
   a.total_blocks = dims.total_blocks;
   a.filter = 1;
+  a.window = window.window;
+  a.sinks = window.sinks;
   a.output = output;
   a.num_query_tokens = dims.num_query_tokens;
   a.num_query_heads = dims.num_query_heads;
@@ -707,7 +710,8 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
                  int32_t layer_idx, PaStepDims dims, const int32_t* block_tables,
                  const int32_t* context_lens, const int64_t* cu_seqlens, const int32_t* prefill_items,
                  int64_t num_prefill_items, int32_t prefill_tile, float scaling, void* output,
-                 void* stream, const PaNewRows* new_rows, const PaCacheScales* scales = nullptr) {
+                 void* stream, const PaNewRows* new_rows, const PaCacheScales* scales = nullptr,
+                 PaWindow window = {0, 0}) {
   int rc = check_step(dims, who);
   if (rc != PA_OK) return rc;
   if (layer_idx < 0 || layer_idx >= dims.num_layers)
@@ -727,7 +731,7 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
   const int eb = elem_bytes(dims.dtype);
   const int cache_eb = scales != nullptr ? 1 : eb;
   const bool fast =
-      ordered_scaling(scaling) &&
+      window.window == 0 && ordered_scaling(scaling) &&
       pa::prefill_fast_path_supported(dims.dtype, dims.head_dim, group, dims.block_size) &&
       (scales == nullptr || pa::prefill_codes_supported(dims.dtype, dims.head_dim)) &&
       prefill_tile == pa::prefill_tile_for(group) && dims.max_blocks_per_seq > 0 &&
@@ -803,6 +807,8 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
   a.block_size = dims.block_size;
   a.total_blocks = dims.total_blocks;
   a.filter = 2;
+  a.window = window.window;
+  a.sinks = window.sinks;
   a.output = output;
   a.num_query_tokens = dims.num_query_tokens;
   a.num_query_heads = dims.num_query_heads;
@@ -1115,6 +1121,246 @@ int pa_attention_step_8bit(const PaStepCall* call, const void* query, void* key_
                           c.num_decode_items, c.merge_items, c.num_merge_items, scaling, output, c.workspace,
                           c.workspace_bytes, stream);
   return PA_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+int check_window(const char* who, const PaWindow& w) {
+  if (w.window < 0 || (w.window > 0 && w.sinks < 0))
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: window and sinks must not be negative, got %d and %d", who, w.window,
+                w.sinks);
+  return PA_OK;
+}
+
+// The step's new rows into a cache of either kind, at their slots.
+int write_rows(const PaStepDims& d, const PaNewRows& rows, void* key_cache, void* value_cache, float* key_scales,
+               float* value_scales, const int64_t* slots, int32_t layer_idx, void* stream) {
+  if (key_scales != nullptr)
+    return pa_reshape_and_cache_8bit(rows.key, rows.value, rows.key_token_stride, rows.key_head_stride,
+                                     rows.value_token_stride, rows.value_head_stride, key_cache, value_cache,
+                                     key_scales, value_scales, slots, d.num_query_tokens, d.num_kv_heads, d.head_dim,
+                                     d.block_size, d.total_blocks, d.num_layers, layer_idx, d.dtype, stream);
+  return pa_reshape_and_cache(rows.key, rows.value, rows.key_token_stride, rows.key_head_stride,
+                              rows.value_token_stride, rows.value_head_stride, key_cache, value_cache, slots,
+                              d.num_query_tokens, d.num_kv_heads, d.head_dim, d.block_size, d.total_blocks,
+                              d.num_layers, layer_idx, d.dtype, stream);
+}
+
+int check_scales(const char* who, const float* key_scales, const float* value_scales) {
+  if ((key_scales == nullptr) != (value_scales == nullptr))
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: key_scales and value_scales are given together", who);
+  return PA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pa_attention_window(const PaStepCall* call, PaWindow window, const void* query, void* key_cache, void* value_cache,
+                        float* key_scales, float* value_scales, int32_t layer_idx, const PaNewRows* new_rows,
+                        float scaling, void* output, void* stream) {
+  const char* who = "pa_attention_window";
+  int rc = require(who, {{call, "call"}});
+  if (rc == PA_OK) rc = check_window(who, window);
+  if (rc == PA_OK) rc = check_scales(who, key_scales, value_scales);
+  if (rc != PA_OK) return rc;
+  if (window.window == 0) return fail(PA_ERR_INVALID_ARGUMENT, "%s: window must be positive", who);
+  const PaStepCall& c = *call;
+  const PaCacheScales scales{key_scales, value_scales};
+  const PaCacheScales* sp = key_scales != nullptr ? &scales : nullptr;
+  const int phases = PA_DECODE_PHASE_PARTITIONS | PA_DECODE_PHASE_MERGE;
+  if (new_rows != nullptr && sp == nullptr && c.num_prefill_items <= 0 && c.num_decode_items > 0) {
+    // (a step of single tokens: the decode launch writes their rows, if it can)
+    rc = decode_phases(who, false, phases, query, key_cache, value_cache, layer_idx, c.dims, c.block_tables,
+                       c.context_lens, c.cu_seqlens, c.decode_items, c.num_decode_items, c.merge_items,
+                       c.num_merge_items, scaling, output, c.workspace, c.workspace_bytes, stream, new_rows, nullptr,
+                       window);
+    if (rc != PA_ERR_UNSUPPORTED) return rc;
+  }
+  if (new_rows != nullptr) {
+    rc = write_rows(c.dims, *new_rows, key_cache, value_cache, key_scales, value_scales, c.scatter_slots, layer_idx,
+                    stream);
+    if (rc != PA_OK) return rc;
+  }
+  if (c.num_prefill_items > 0) {
+    rc = prefill_impl(who, query, key_cache, value_cache, layer_idx, c.dims, c.block_tables, c.context_lens,
+                      c.cu_seqlens, c.prefill_items, c.num_prefill_items, c.prefill_tile, scaling, output, stream,
+                      nullptr, sp, window);
+    if (rc != PA_OK) return rc;
+  }
+  if (c.num_decode_items > 0)
+    return decode_phases(who, false, phases, query, key_cache, value_cache, layer_idx, c.dims, c.block_tables,
+                         c.context_lens, c.cu_seqlens, c.decode_items, c.num_decode_items, c.merge_items,
+                         c.num_merge_items, scaling, output, c.workspace, c.workspace_bytes, stream, nullptr, sp,
+                         window);
+  return PA_OK;
+}
+
+int pa_pack_tree(const int32_t* parents, const int32_t* context_lens, const int64_t* cu_seqlens, PaTreeDims dims,
+                 PaTreePlan plan, uint32_t* masks, int64_t* positions, int32_t* items, int32_t* merge_items,
+                 void* stream) {
+  const char* who = "pa_pack_tree";
+  int rc = check_window(who, dims.window);
+  if (rc != PA_OK) return rc;
+  if (dims.num_seqs < 0 || dims.num_query_tokens < 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: negative batch size", who);
+  if (plan.mask_words <= 0 || plan.num_items < 0 || plan.num_merge_items < 0 || plan.num_partial_rows < 0 ||
+      (plan.tile > 0 && plan.split_stages <= 0))
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: not a plan of pa_plan_tree", who);
+  if (dims.num_seqs == 0 || dims.num_query_tokens == 0) return PA_OK;
+  rc = require(who, {{parents, "parents"}, {context_lens, "context_lens"}, {cu_seqlens, "cu_seqlens"},
+                     {masks, "masks"}, {positions, "positions"}});
+  if (rc != PA_OK) return rc;
+  if ((plan.num_items > 0 && items == nullptr) || (plan.num_merge_items > 0 && merge_items == nullptr) ||
+      !aligned16(items) || !aligned16(merge_items))
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: items and merge_items must be given for a plan that has them, 16-byte "
+                "aligned", who);
+  pa::PackTreeArgs a{};
+  a.parents = parents;
+  a.context_lens = context_lens;
+  a.cu_seqlens = cu_seqlens;
+  a.masks = masks;
+  a.positions = positions;
+  a.items = plan.tile > 0 ? reinterpret_cast<int4*>(items) : nullptr;
+  a.merge_items = reinterpret_cast<int4*>(merge_items);
+  a.max_items = plan.num_items;
+  a.max_merge_items = plan.num_merge_items;
+  a.max_partial_rows = plan.num_partial_rows;
+  a.num_seqs = dims.num_seqs;
+  a.num_query_tokens = dims.num_query_tokens;
+  a.mask_words = plan.mask_words;
+  a.tile = plan.tile;
+  a.split_stages = plan.split_stages;
+  a.window = dims.window.window;
+  a.sinks = dims.window.sinks;
+  return from_hip(pa::launch_pack_tree(a, static_cast<hipStream_t>(stream)), who);
+}
+
+size_t pa_tree_workspace_size(PaStepDims dims, int64_t num_partial_rows) {
+  const DecodeWorkspaceLayout w = decode_workspace_layout(dims, num_partial_rows);
+  return w.acc + w.ml;
+}
+
+int pa_tree_attention(const PaTreeCall* call, const void* query, void* key_cache, void* value_cache, float* key_scales,
+                      float* value_scales, int32_t layer_idx, const PaNewRows* new_rows, float scaling, void* output,
+                      void* stream) {
+  const char* who = "pa_tree_attention";
+  int rc = require(who, {{call, "call"}});
+  if (rc != PA_OK) return rc;
+  const PaTreeCall& c = *call;
+  const PaStepDims& d = c.dims;
+  rc = check_step(d, who);
+  if (rc == PA_OK) rc = check_window(who, c.window);
+  if (rc == PA_OK) rc = check_scales(who, key_scales, value_scales);
+  if (rc != PA_OK) return rc;
+  if (layer_idx < 0 || layer_idx >= d.num_layers)
+    return fail(PA_ERR_INVALID_ARGUMENT, "Layer index %d out of range (num_layers=%d)", layer_idx, d.num_layers);
+  if (c.plan.mask_words <= 0) return fail(PA_ERR_INVALID_ARGUMENT, "%s: not a plan of pa_plan_tree", who);
+  if (d.num_seqs == 0 || d.num_query_tokens == 0) return PA_OK;
+  rc = require(who, {{query, "query"}, {key_cache, "key_cache"}, {value_cache, "value_cache"}, {output, "output"},
+                     {c.block_tables, "block_tables"}, {c.context_lens, "context_lens"},
+                     {c.cu_seqlens, "cu_seqlens"}, {c.masks, "masks"}, {c.positions, "positions"}});
+  if (rc != PA_OK) return rc;
+  if (new_rows != nullptr) {
+    rc = write_rows(d, *new_rows, key_cache, value_cache, key_scales, value_scales, c.scatter_slots, layer_idx, stream);
+    if (rc != PA_OK) return rc;
+  }
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int eb = elem_bytes(d.dtype);
+  const int cache_eb = key_scales != nullptr ? 1 : eb;
+  if (!pa::generic_supported(d.dtype, d.head_dim))
+    return fail(PA_ERR_UNSUPPORTED, "%s: head_dim %d / dtype %d not supported", who, d.head_dim, d.dtype);
+  pa::GenericArgs a{};
+  a.query = query;
+  a.q_token_stride = d.q_token_stride;
+  a.q_head_stride = d.q_head_stride;
+  a.key_cache = layer_base(key_cache, d, layer_idx, cache_eb);
+  a.value_cache = layer_base(value_cache, d, layer_idx, cache_eb);
+  a.block_tables = c.block_tables;
+  a.rows = d.block_table_rows;
+  a.num_table_rows = d.num_table_rows > 0 ? d.num_table_rows : d.num_seqs;
+  a.context_lens = c.context_lens;
+  a.cu_seqlens = c.cu_seqlens;
+  a.num_seqs = d.num_seqs;
+  a.block_table_stride = d.max_blocks_per_seq;
+  a.block_size = d.block_size;
+  a.total_blocks = d.total_blocks;
+  a.output = output;
+  a.num_query_tokens = d.num_query_tokens;
+  a.num_query_heads = d.num_query_heads;
+  a.num_kv_heads = d.num_kv_heads;
+  a.head_dim = d.head_dim;
+  a.scale_log2e = scaling * pa::kLog2e;
+  if (key_scales != nullptr) {
+    a.key_scales = layer_scales(key_scales, d, layer_idx);
+    a.value_scales = layer_scales(value_scales, d, layer_idx);
+  }
+  a.window = c.window.window;
+  a.sinks = c.window.sinks;
+  a.masks = c.masks;
+  a.mask_words = c.plan.mask_words;
+  a.positions = c.positions;
+  return from_hip(pa::launch_generic(a, d.dtype, s), who);
+}
+
+int pa_accept_tree(const int32_t* parents, const int64_t* cu_seqlens, const int64_t* drafted, const int64_t* predicted,
+                   int32_t num_seqs, int32_t num_query_tokens, int32_t* nodes, int32_t* counts, int64_t* next_tokens,
+                   void* stream) {
+  const char* who = "pa_accept_tree";
+  if (num_seqs < 0 || num_query_tokens < 0) return fail(PA_ERR_INVALID_ARGUMENT, "%s: negative batch size", who);
+  if (num_seqs == 0) return PA_OK;
+  int rc = require(who, {{cu_seqlens, "cu_seqlens"}, {counts, "counts"}, {next_tokens, "next_tokens"}});
+  if (rc == PA_OK && num_query_tokens > 0)
+    rc = require(who, {{parents, "parents"}, {drafted, "drafted"}, {predicted, "predicted"}, {nodes, "nodes"}});
+  if (rc != PA_OK) return rc;
+  pa::AcceptTreeArgs a{parents, cu_seqlens, drafted, predicted, nodes, counts, next_tokens, num_seqs, num_query_tokens};
+  return from_hip(pa::launch_accept_tree(a, static_cast<hipStream_t>(stream)), who);
+}
+
+int pa_keep_rows(void* key_cache, void* value_cache, float* key_scales, float* value_scales, PaStepDims dims,
+                 const int32_t* block_tables, const int32_t* context_lens, const int64_t* cu_seqlens,
+                 const int32_t* nodes, const int32_t* counts, void* stream) {
+  const char* who = "pa_keep_rows";
+  int rc = check_scales(who, key_scales, value_scales);
+  if (rc != PA_OK) return rc;
+  const int eb = key_scales != nullptr ? 1 : elem_bytes(dims.dtype);
+  if (eb == 0) return fail(PA_ERR_INVALID_ARGUMENT, "%s: unknown dtype %d", who, dims.dtype);
+  if (dims.num_seqs < 0 || dims.num_query_tokens < 0 || dims.max_blocks_per_seq < 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: negative sizes", who);
+  if (dims.num_kv_heads <= 0 || dims.head_dim <= 0 || dims.block_size <= 0 || dims.total_blocks <= 0 ||
+      dims.num_layers <= 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: cache geometry must be positive", who);
+  if (dims.num_layers > 32767 || dims.num_kv_heads > 65535 || (key_scales != nullptr && dims.head_dim > 256))
+    return fail(PA_ERR_UNSUPPORTED, "%s: more layers or heads, or wider 8-bit heads, than a launch takes", who);
+  if (dims.num_seqs == 0 || dims.num_query_tokens == 0) return PA_OK;
+  rc = require(who, {{key_cache, "key_cache"}, {value_cache, "value_cache"}, {block_tables, "block_tables"},
+                     {context_lens, "context_lens"}, {cu_seqlens, "cu_seqlens"}, {nodes, "nodes"},
+                     {counts, "counts"}});
+  if (rc != PA_OK) return rc;
+  pa::KeepRowsArgs a{};
+  a.key_cache = key_cache;
+  a.value_cache = value_cache;
+  a.key_scales = key_scales;
+  a.value_scales = value_scales;
+  a.nodes = nodes;
+  a.counts = counts;
+  a.block_tables = block_tables;
+  a.rows = dims.block_table_rows;
+  a.context_lens = context_lens;
+  a.cu_seqlens = cu_seqlens;
+  a.num_table_rows = dims.num_table_rows > 0 ? dims.num_table_rows : dims.num_seqs;
+  a.block_table_stride = dims.max_blocks_per_seq;
+  a.num_seqs = dims.num_seqs;
+  a.num_query_tokens = dims.num_query_tokens;
+  a.num_layers = dims.num_layers;
+  a.total_blocks = dims.total_blocks;
+  a.block_size = dims.block_size;
+  a.num_kv_heads = dims.num_kv_heads;
+  a.head_dim = dims.head_dim;
+  a.row_bytes = static_cast<int64_t>(dims.num_kv_heads) * dims.head_dim * eb;
+  return from_hip(pa::launch_keep_rows(a, static_cast<hipStream_t>(stream)), who);
 }
 
 }  // extern "C"

@@ -27,7 +27,7 @@ LIBRARY_PATH = PACKAGE_DIR / LIBRARY_NAME
 OFFLOAD_ARCH = "gfx950"
 
 SOURCES = ["abi.hip", "plan.cpp", "pack.hip", "cache_write.hip", "rotate.hip", "decode.hip", "decode_mfma.hip", "decode8.hip", "generic.hip", "prefill.hip",
-           "prefill256.hip", "prefill_f32.hip", "copy_blocks.hip", "calibrate.hip"]
+           "prefill256.hip", "prefill_f32.hip", "tree.hip", "copy_blocks.hip", "calibrate.hip"]
 
 HIP_FLAGS = [
     "-O3",

@@ -15,9 +15,12 @@
 // the lanes splitting the head dimension.
 // C: the caches' elements, T or the 8-bit cache's codes (block tables only);
 // a lane then resolves its token's two scales with its slot.
+// SPAN (block tables only): a window with sinks, whose hidden chunks are left
+// out, or a tree, whose nodes see one another by their masks' bits.
 #include "cache8.hpp"
 #include "pa_common.hpp"
 #include "pa_launch.hpp"
+#include "span.hpp"
 
 namespace pa {
 
@@ -34,7 +37,9 @@ __device__ __forceinline__ float cache_value(const C* p, float scale) {
   }
 }
 
-template <typename T, int EPL, bool kMasked, typename C = T>
+enum { kSpanAll = 0, kSpanWindow = 1, kSpanTree = 2 };
+
+template <typename T, int EPL, bool kMasked, typename C = T, int SPAN = kSpanAll>
 __global__ __launch_bounds__(kWave) void generic_attention_kernel(GenericArgs a) {
   const int lane = threadIdx.x;
   const int hq = a.num_query_heads;
@@ -49,6 +54,8 @@ __global__ __launch_bounds__(kWave) void generic_attention_kernel(GenericArgs a)
   int seq = 0;
   int64_t trow = 0;
   int n_ctx;
+  [[maybe_unused]] int left = 0;   // first position of the query's window
+  [[maybe_unused]] int start = 0;  // of the tree's nodes
   if constexpr (kMasked) {
     n_ctx = a.num_context_tokens;
   } else {
@@ -66,6 +73,12 @@ __global__ __launch_bounds__(kWave) void generic_attention_kernel(GenericArgs a)
     const int64_t pos = a.context_lens[seq] - count + (t - first);
     n_ctx = static_cast<int>(pos + 1);
     if (n_ctx < 0) n_ctx = 0;
+    if constexpr (SPAN == kSpanWindow) left = window_start(static_cast<int>(pos), a.window);
+    if constexpr (SPAN == kSpanTree) {
+      // (a node's position is its depth's; its place among the rows is n_ctx - 1)
+      start = static_cast<int>(a.context_lens[seq] - count);
+      left = min(window_start(static_cast<int>(a.positions[t]), a.window), start);
+    }
   }
 
   const T* qrow = reinterpret_cast<const T*>(a.query) + t * a.q_token_stride + h * a.q_head_stride;
@@ -84,10 +97,19 @@ __global__ __launch_bounds__(kWave) void generic_attention_kernel(GenericArgs a)
   for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
 
   for (int c0 = 0; c0 < n_ctx; c0 += kWave) {
+    if constexpr (SPAN != kSpanAll)
+      if (c0 >= a.sinks) c0 = max(c0, left & -kWave);
     const int c = c0 + lane;
     int64_t slot = -1;
     float kscale = 1.f, vscale = 1.f;
-    if (c < n_ctx) {
+    bool seen = c < n_ctx;
+    if constexpr (SPAN != kSpanAll) seen = seen && (c >= left || c < a.sinks);
+    if constexpr (SPAN == kSpanTree) {
+      const int j = c - start;
+      if (c < n_ctx && j >= 0)
+        seen = (j >> 5) < a.mask_words && (a.masks[static_cast<int64_t>(t) * a.mask_words + (j >> 5)] >> (j & 31) & 1u) != 0;
+    }
+    if (seen) {
       if constexpr (kMasked) {
         if (a.mask[static_cast<int64_t>(t) * n_ctx + c] != 0) {
           slot = a.gather_slots[c];
@@ -342,18 +364,27 @@ bool generic_supported(int dtype, int head_dim) {
   return head_dim >= 1 && head_dim <= 256;
 }
 
-template <typename T, bool kMasked, typename C = T>
-static hipError_t launch_generic_t(const GenericArgs& a, hipStream_t s) {
+template <typename T, bool kMasked, typename C, int SPAN>
+static hipError_t launch_generic_s(const GenericArgs& a, hipStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.num_query_tokens) * a.num_query_heads;
   if (rows <= 0) return hipSuccess;
   const dim3 grid(static_cast<uint32_t>(rows));
   if (a.head_dim <= 64)
-    hipLaunchKernelGGL((generic_attention_kernel<T, 1, kMasked, C>), grid, dim3(kWave), 0, s, a);
+    hipLaunchKernelGGL((generic_attention_kernel<T, 1, kMasked, C, SPAN>), grid, dim3(kWave), 0, s, a);
   else if (a.head_dim <= 128)
-    hipLaunchKernelGGL((generic_attention_kernel<T, 2, kMasked, C>), grid, dim3(kWave), 0, s, a);
+    hipLaunchKernelGGL((generic_attention_kernel<T, 2, kMasked, C, SPAN>), grid, dim3(kWave), 0, s, a);
   else
-    hipLaunchKernelGGL((generic_attention_kernel<T, 4, kMasked, C>), grid, dim3(kWave), 0, s, a);
+    hipLaunchKernelGGL((generic_attention_kernel<T, 4, kMasked, C, SPAN>), grid, dim3(kWave), 0, s, a);
   return hipGetLastError();
+}
+
+template <typename T, bool kMasked, typename C = T>
+static hipError_t launch_generic_t(const GenericArgs& a, hipStream_t s) {
+  if constexpr (!kMasked) {
+    if (a.masks != nullptr) return launch_generic_s<T, kMasked, C, kSpanTree>(a, s);
+    if (a.window > 0) return launch_generic_s<T, kMasked, C, kSpanWindow>(a, s);
+  }
+  return launch_generic_s<T, kMasked, C, kSpanAll>(a, s);
 }
 
 // Most workgroups that get 16 waves each (segments of 8192 slots) instead of

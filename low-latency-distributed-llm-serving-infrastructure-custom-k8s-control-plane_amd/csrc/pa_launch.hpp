@@ -100,6 +100,14 @@ struct GenericArgs {
   // 8-bit caches (else null): base of the layer, [blocks, H_kv]
   const float* key_scales;
   const float* value_scales;
+  // Block-table source: a window (0: the whole context) with sinks, and of
+  // trees (else null) the nodes' masks (bit j of a row: node j of its sequence is
+  // seen) and positions.
+  int32_t window;
+  int32_t sinks;
+  const uint32_t* masks;  // [T, mask_words]
+  const int64_t* positions;
+  int32_t mask_words;
 };
 
 // Packing of one step (pack.hip): a one-workgroup scan and a per-sequence
@@ -264,6 +272,80 @@ struct PrefillArgs {
   const float* key_scales;
   const float* value_scales;
 };
+
+// A step's trees of drafted tokens (tree.hip): masks and positions of the nodes
+// from their parents, and the attention's work lists.
+struct PackTreeArgs {
+  const int32_t* parents;       // [T]
+  const int32_t* context_lens;
+  const int64_t* cu_seqlens;
+  uint32_t* masks;              // [T, mask_words]
+  int64_t* positions;           // [T]
+  int4* items;                  // (sequence, tile, split, first partial row or -1), or null
+  int4* merge_items;            // (sequence, tile, splits, first partial row)
+  int64_t max_items;
+  int64_t max_merge_items;
+  int64_t max_partial_rows;
+  int32_t num_seqs;
+  int32_t num_query_tokens;
+  int32_t mask_words;
+  int32_t tile;                 // nodes per tile
+  int32_t split_stages;         // stages per item
+  int32_t window;
+  int32_t sinks;
+};
+hipError_t launch_pack_tree(const PackTreeArgs& a, hipStream_t stream);
+
+struct AcceptTreeArgs {
+  const int32_t* parents;
+  const int64_t* cu_seqlens;
+  const int64_t* drafted;
+  const int64_t* predicted;
+  int32_t* nodes;         // [T]
+  int32_t* counts;        // [B]
+  int64_t* next_tokens;   // [B]
+  int32_t num_seqs;
+  int32_t num_query_tokens;
+};
+hipError_t launch_accept_tree(const AcceptTreeArgs& a, hipStream_t stream);
+
+struct KeepRowsArgs {
+  void* key_cache;
+  void* value_cache;
+  float* key_scales;    // 8-bit caches (else null), [layers, blocks, H_kv]
+  float* value_scales;
+  const int32_t* nodes;
+  const int32_t* counts;
+  const int32_t* block_tables;
+  const int32_t* rows;
+  const int32_t* context_lens;
+  const int64_t* cu_seqlens;
+  int32_t num_table_rows;
+  int32_t block_table_stride;
+  int32_t num_seqs;
+  int32_t num_query_tokens;
+  int32_t num_layers;
+  int32_t total_blocks;
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int64_t row_bytes;    // H_kv * D * element bytes
+};
+hipError_t launch_keep_rows(const KeepRowsArgs& a, hipStream_t stream);
+
+// The partials of tiles that were split, joined into output rows.
+struct MergeTreeArgs {
+  const int4* merge_items;
+  int64_t num_merge;
+  const int64_t* cu_seqlens;
+  const float* part_acc;  // [partial rows, H_q, D]
+  const float* part_ml;   // [partial rows, H_q, 2]
+  void* output;
+  int32_t num_query_heads;
+  int32_t num_query_tokens;
+  int32_t tile;
+};
+hipError_t launch_merge_tree(const MergeTreeArgs& a, int dtype, int head_dim, hipStream_t stream);
 
 bool decode_fast_path_supported(int dtype, int head_dim, int group, int block_size,
                                 int partition);

@@ -9,6 +9,7 @@
 #include "decode_shape.hpp"
 #include "pa_error.hpp"
 #include "paged_attention_amd.h"
+#include "span.hpp"
 
 namespace {
 
@@ -239,3 +240,132 @@ int pa_plan_step_for(const int64_t* starts, const int64_t* counts, const int64_t
 }
 
 }  // extern "C"
+
+// ---- windows and trees ------------------------------------------------------
+
+extern "C" int32_t pa_window_context(int32_t context, PaWindow window, int32_t block_size) {
+  if (window.window <= 0 || block_size <= 0 || context <= 0) return context;
+  // The sinks' whole blocks, and the window from anywhere in its first block.
+  const int64_t sinks = ceil_div(window.sinks > 0 ? window.sinks : 0, block_size) * block_size;
+  const int64_t most = sinks + window.window + block_size - 1;
+  return most < context ? static_cast<int32_t>(most) : context;
+}
+
+namespace {
+
+// A step of trees as pa_pack_tree lists it, for one size of an item.
+struct TreeSizes {
+  int64_t items = 0, merges = 0, rows = 0;
+};
+struct Trees {
+  const int64_t* starts;
+  const int64_t* counts;
+  const PaTreeDims& d;
+  int tile;
+  TreeSizes sizes(int64_t split) const {
+    TreeSizes z;
+    each([&](int64_t n, int64_t stages) {
+      const int64_t splits = ceil_div(stages, split);
+      z.items += splits;
+      if (splits > 1) {
+        z.merges += 1;
+        z.rows += splits * n;
+      }
+    });
+    return z;
+  }
+  template <typename F>
+  void each(const F& f) const {
+    for (int32_t i = 0; i < d.num_seqs; ++i)
+      for (int64_t t0 = 0; t0 < counts[i]; t0 += tile) {
+        const int64_t n = counts[i] - t0 < tile ? counts[i] - t0 : tile;
+        f(n, static_cast<int64_t>(pa::tree_span(static_cast<int>(starts[i]), static_cast<int>(t0 + n), d.window.window,
+                                                d.window.sinks, pa::kTreeStage).count));
+      }
+  }
+};
+
+// Stages per item: one workgroup a CU takes items in turn, each of which costs
+// its stages and kItemStages more (its prologue and end); tiles in several items
+// are joined by a launch of its own.  The smallest modelled time wins, the
+// larger item of two alike.
+constexpr double kItemStages = 4.0;
+constexpr double kMergeStages = 6.0;
+int32_t choose_split(const Trees& t, const PaTreeDims& d) {
+  const int64_t per_item = d.num_kv_heads * static_cast<int64_t>(pa::decode_sub_groups(d.num_query_heads / d.num_kv_heads));
+  const int64_t cus = d.compute_units > 0 ? d.compute_units : 256;
+  int64_t longest = 1;
+  t.each([&](int64_t, int64_t stages) { longest = stages > longest ? stages : longest; });
+  double best = 0;
+  int32_t pick = 0;
+  for (int64_t split = longest;; split = split * 3 / 4 < split ? split * 3 / 4 : split - 1) {
+    if (split < 1) break;
+    double total = 0;
+    int64_t items = 0;
+    bool merged = false;
+    t.each([&](int64_t, int64_t stages) {
+      const int64_t n = ceil_div(stages, split);
+      items += n;
+      merged |= n > 1;
+      total += stages + kItemStages * n;
+    });
+    const double rounds = static_cast<double>(ceil_div(items * per_item, cus));
+    const double even = total * per_item / cus;
+    const double longest_item = (longest < split ? longest : split) + kItemStages;
+    // (items of one size in whole rounds; of many sizes the snake evens them out)
+    double time = even > longest_item ? even : longest_item;
+    const double whole = rounds * longest_item;
+    time = 0.5 * time + 0.5 * (whole < time ? time : whole);
+    if (merged) time += kMergeStages;
+    if (pick == 0 || time < best) {
+      best = time;
+      pick = static_cast<int32_t>(split);
+    }
+    if (items * per_item > 8 * cus) break;
+  }
+  return pick > 0 ? pick : 1;
+}
+
+}  // namespace
+
+extern "C" int pa_plan_tree(const int64_t* start_positions, const int64_t* node_counts, PaTreeDims dims,
+                            PaTreePlan* plan) {
+  if (plan == nullptr || dims.num_seqs < 0 ||
+      (dims.num_seqs > 0 && (start_positions == nullptr || node_counts == nullptr)))
+    return pa::set_error(PA_ERR_INVALID_ARGUMENT, "pa_plan_tree: missing arrays or a negative batch size");
+  memset(plan, 0, sizeof(*plan));
+  plan->bad_seq = -1;
+  if (dims.block_size <= 0 || dims.window.window < 0 || dims.window.sinks < 0 || dims.split_stages < 0)
+    return pa::set_error(PA_ERR_INVALID_ARGUMENT, "pa_plan_tree: block_size must be positive, window, sinks and "
+                         "split_stages not negative");
+  if (dims.num_query_heads < 0 || dims.num_kv_heads < 0 ||
+      (dims.num_query_heads > 0 && (dims.num_kv_heads == 0 || dims.num_query_heads % dims.num_kv_heads != 0)))
+    return pa::set_error(PA_ERR_INVALID_ARGUMENT, "pa_plan_tree: num_query_heads must be a multiple of num_kv_heads");
+  int64_t most = 0;
+  for (int32_t i = 0; i < dims.num_seqs; ++i) {
+    const int64_t s = start_positions[i], n = node_counts[i];
+    if (s < 0 || n < 0 || n > PA_MAX_TREE_NODES || s + n > 0x7fffffffLL ||
+        (dims.window.window > 0 && n > dims.window.window)) {
+      plan->bad_seq = i;
+      return pa::set_error(PA_ERR_INVALID_ARGUMENT,
+                           "pa_plan_tree: sequence %d: a tree of %lld nodes at %lld (at most %d nodes, and no more "
+                           "than the window)", i, static_cast<long long>(n), static_cast<long long>(s),
+                           PA_MAX_TREE_NODES);
+    }
+    most = n > most ? n : most;
+  }
+  plan->mask_words = static_cast<int32_t>(ceil_div(most > 0 ? most : 1, 32));
+  if (dims.num_query_heads == 0) return PA_OK;
+  const int group = dims.num_query_heads / dims.num_kv_heads;
+  if (!pa::tree_fast_path_supported(dims.dtype, dims.head_dim, group, dims.block_size)) return PA_OK;
+  plan->tile = pa_prefill_tile(dims.num_query_heads, dims.num_kv_heads);
+  const Trees trees{start_positions, node_counts, dims, plan->tile};
+  plan->split_stages = dims.split_stages > 0 ? dims.split_stages : choose_split(trees, dims);
+  const TreeSizes z = trees.sizes(plan->split_stages);
+  if (z.items > 0x7fffffff || z.rows > 0x7fffffff)
+    return pa::set_error(PA_ERR_UNSUPPORTED, "pa_plan_tree: too many work items");
+  plan->num_items = z.items;
+  plan->num_merge_items = z.merges;
+  plan->num_partial_rows = z.rows;
+  return PA_OK;
+}

@@ -98,6 +98,7 @@
 #include "pa_common.hpp"
 #include "pa_launch.hpp"
 #include "prefill_common.hpp"
+#include "span.hpp"
 
 namespace pa {
 
@@ -1043,6 +1044,8 @@ bool prefill_fast_path_supported(int dtype, int head_dim, int group, int block_s
   if (block_size <= 0 || (block_size & (block_size - 1)) != 0) return false;
   return true;
 }
+
+bool tree_fast_path_supported(int, int, int, int) { return false; }
 
 bool prefill_append_supported(int dtype, int head_dim) {
   // Every fast-path kernel but the one for heads of 256.

@@ -1,0 +1,79 @@
+// What part of the context a query sees under a window with sinks, and how the
+// tuned kernels leave the rest out: the query at position p sees the positions
+// q <= p with p - q < window or q < sinks.  Used by the kernels and, for the
+// work lists, by the host (no HIP types).
+#pragma once
+
+#include <stdint.h>
+
+#ifdef __HIPCC__
+#define PA_HOST_DEVICE __host__ __device__ inline
+#else
+#define PA_HOST_DEVICE inline
+#endif
+
+namespace pa {
+
+// Most nodes of one tree (pa_pack_tree keeps a sequence's parents in LDS).
+constexpr int kMaxTreeNodes = 1024;
+
+PA_HOST_DEVICE int span_min(int a, int b) { return a < b ? a : b; }
+PA_HOST_DEVICE int span_max(int a, int b) { return a > b ? a : b; }
+
+// First position of the window of the query at position p (window >= 1; 0: no
+// window).
+PA_HOST_DEVICE int window_start(int p, int window) { return window > 0 ? span_max(p - window + 1, 0) : 0; }
+
+// A single query at the end of a context of ctx positions, in whole blocks of
+// 2^log2_bs tokens.  The blocks between the last one that holds sinks and the
+// first one of the window are left out: the kernel walks a context of `ctx`
+// positions without them, whose block column c is column c of the sequence's
+// table, or c + skip from column `sinks` on.  Of that shorter context the
+// positions [hole, hole_end), in the two blocks beside the cut, are not seen.
+struct DecodeSpan {
+  int ctx;
+  int sinks, skip;
+  int hole, hole_end;
+};
+PA_HOST_DEVICE DecodeSpan decode_span(int ctx, int window, int sinks, int log2_bs) {
+  const int lo = window_start(ctx - 1, window);
+  const int s = span_min(sinks, lo);
+  DecodeSpan d;
+  d.sinks = (s >> log2_bs) + ((s & ((1 << log2_bs) - 1)) != 0 ? 1 : 0);
+  d.skip = span_max((lo >> log2_bs) - d.sinks, 0);
+  d.ctx = ctx - (d.skip << log2_bs);
+  d.hole = s;
+  d.hole_end = lo - (d.skip << log2_bs);
+  return d;
+}
+
+// The queries of a tile, the first window of which starts at lo and the last
+// of which sees positions below `end`, in stages of `stage` positions: those of
+// the sinks first, then from the window's first stage on, `gap` stages left out
+// between them.
+struct StageSpan {
+  int sinks, gap;
+  int count;
+};
+PA_HOST_DEVICE StageSpan stage_span(int lo, int end, int sinks, int stage) {
+  StageSpan t;
+  const int s = span_min(sinks, lo);
+  t.sinks = s / stage + (s % stage != 0 ? 1 : 0);
+  t.gap = span_max(lo / stage - t.sinks, 0);
+  t.count = span_max((end > 0 ? (end - 1) / stage + 1 : 0) - t.gap, 0);
+  return t;
+}
+
+// The stages of a tree's tile, whose last query is node `nodes` - 1 of its
+// sequence (the root, at position `start`, sees the first window of them all).
+PA_HOST_DEVICE StageSpan tree_span(int start, int nodes, int window, int sinks, int stage) {
+  return stage_span(window_start(start, window), start + nodes, sinks, stage);
+}
+
+// Whether the matrix-core kernel of trees (prefill.hip, prefill_f32.hip) serves
+// the shape: its tiles of prefill_tile_for() nodes walk stages of kTreeStage
+// positions.
+constexpr int kTreeStage = 64;
+bool tree_fast_path_supported(int dtype, int head_dim, int group, int block_size);
+
+}  // namespace pa

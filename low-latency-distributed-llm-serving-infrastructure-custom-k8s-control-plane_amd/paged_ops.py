@@ -18,6 +18,12 @@ projections' rows: :func:`rotate_and_cache` normalises and rotates Q and K and
 does (b) in the same launch (:func:`rotate` without a cache, :func:`rope_table`
 for the table).
 
+Layers that see a part of their context take :func:`attention` with ``window`` and
+``sinks``.  Steps that verify trees of drafted tokens: :func:`pack_tree` (masks and
+positions from the nodes' parents), :func:`tree_attention` in every layer,
+:func:`accept_tree` (the path of the tokens that the model itself chose) and
+:func:`keep_rows` (that path's K and V rows moved behind the context).
+
 A cache of ``torch.float8_e4m3fn`` holds 8-bit codes, with fp32 scales
 [layers, blocks, H_kv] beside it (``key_scales`` / ``value_scales`` of (b), (c),
 (d) and :func:`attention`; see :func:`reshape_and_cache` for its rules).  Rows,
@@ -31,7 +37,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
-from typing import Optional, Sequence, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -268,6 +274,10 @@ class PackedStep:
         self._extra_ws = None
         self._generation = 0  # the pool's pack count when this step was packed
         self._merge_state_bytes = 0  # merge records at the end of the decode workspace
+        self._heads = None  # (H_kv, H_q, D, cache dtype) the step was packed for, as far as given
+        self._windows = {}  # decode work lists of layers with a window (see _window_step)
+        self._packs = 0  # repacks so far
+        self._partition_given = False
 
     # -- addresses and views ---------------------------------------------------
     def ptr(self, name: str) -> int:
@@ -340,6 +350,15 @@ class PackedStep:
             raise ValueError("repack needs a step of the same sizes; pack a new step instead")
         if self.table_width and plan.max_blocks > self.table_width:
             raise ValueError("repack: a context grew past the step's block table")
+        windows = [(sub, _window_starts(starts, counts, self.block_size, key[0], key[1]))
+                   for key, sub in self._windows.items() if sub is not self]
+        for sub, shorter in windows:
+            p = _plan(shorter, counts, self.block_size, self.prefill_tile, sub.partition_size, 1, 1, 1, 1, 1)
+            if (p.num_decode_items, p.num_merge_items) != (sub.num_decode_items, sub.num_merge_items):
+                raise ValueError("repack needs a step of the same sizes under its windows too; pack a new step instead")
+        self._packs += 1
+        for sub, shorter in windows:
+            sub.repack(shorter, counts)
         self._inputs = (starts, counts, self._inputs[2])
         self.__dict__.pop("_layer_call", None)  # (its default for the prefill write)
         self.num_context_tokens = int(plan.num_context_tokens)
@@ -354,6 +373,9 @@ class PackedStep:
         of the layers and change the step with :meth:`repack` between
         replays."""
         _run_pack(self)
+        for sub in self._windows.values():
+            if sub is not self:
+                _run_pack(sub)
 
     @property
     def table_width(self) -> int:
@@ -666,8 +688,8 @@ def pack_step(
     ``start_positions`` / ``new_token_counts``: the host lists of the step.
     ``allocated_tokens``: per sequence, the tokens it has slots for; a step
     reaching past them is a ValueError (as the reference's slot mapping).
-    ``partition_size``: decode split-K partition in tokens; by default the
-    planner picks it from the step and the head counts (and, when
+    ``partition_size``: decode split-K partition in tokens (under windows too);
+    by default the planner picks it from the step and the head counts (and, when
     ``head_dim`` and the cache ``dtype`` are given, from how many KV heads
     one decode workgroup reads and the kernel's occupancy).
     ``prefill_tile``: query tokens per prefill work item; by default the
@@ -740,6 +762,8 @@ def pack_step(
     step = PackedStep(buffer, layout, plan, block_size, prefill_tile, block_tables, table_rows, pooled,
                       head_shape, (starts, counts, rows_arr))
     step._merge_state_bytes = state_bytes  # cleared by every pa_pack of the step
+    step._partition_given = partition_size is not None
+    step._heads = (int(num_kv_heads), hq, None if head_dim is None else int(head_dim), dtype)
     upd = None if not n_upd else np.ascontiguousarray(updates, dtype=np.int32)
     gather = _run_pack(step, with_gather=with_gather, updates=upd, fresh=True)
     if with_gather:
@@ -1563,6 +1587,9 @@ def attention(
     fused_prefill_write: Optional[bool] = None,
     key_scales: Optional[torch.Tensor] = None,
     value_scales: Optional[torch.Tensor] = None,
+    *,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> torch.Tensor:
     """Attention of a whole flattened step (decode + prefill sequences) -> [T, H_q, D].
 
@@ -1586,9 +1613,21 @@ def attention(
     ``key_scales`` / ``value_scales``: of an 8-bit cache, whose rows the
     cache-write kernel writes ahead of the attention (a block's scale has to
     be settled before anything reads the block).
+
+    ``window`` (at least 1) and ``sinks``: the query at position p sees the
+    positions q <= p with p - q < window or q < sinks.  What no query of the step
+    sees is not read, and its table entries may be -1.  The first call of a step
+    with a window packs the decode's work lists for it, which later layers and
+    :meth:`PackedStep.rerun` reuse: make one before a graph is captured.  New rows
+    are written ahead of the attention on a step with prompts.
     """
     if (new_key is None) != (new_value is None):
         raise ValueError("new_key and new_value are given together")
+    if window is not None:
+        return _attention_window(query, key_cache, value_cache, layer_idx, step, scaling, out, new_key, new_value,
+                                 key_scales, value_scales, window, sinks)
+    if sinks:
+        raise ValueError("sinks go with a window")
     need_prefill = step.num_prefill_items > 0
     need_decode = step.num_decode_items > 0
     if key_cache.dtype == CODE_DTYPE:
@@ -1614,6 +1653,432 @@ def attention(
     if step.num_query_tokens > 0 and step.num_decode_items == 0 and step.num_prefill_items == 0:
         out.zero_()
     return out
+
+
+# ---------------------------------------------------------------------------
+# part of the context: windows
+
+
+def _window_of(window, sinks) -> Tuple[int, int]:
+    """(window, sinks) as the library takes them; ValueError for what is none."""
+    if int(window) != window or window < 1:
+        raise ValueError(f"window must be a positive number of tokens, got {window}")
+    if int(sinks) != sinks or sinks < 0:
+        raise ValueError(f"sinks must be a number of tokens, got {sinks}")
+    return min(int(window), _INT32_MAX), min(int(sinks), _INT32_MAX)
+
+
+def _window_starts(starts: np.ndarray, counts: np.ndarray, block_size: int, window: int, sinks: int) -> np.ndarray:
+    """Starts that give each single-token sequence the longest shorter context it
+    can have under the window (pa_window_context)."""
+    most = -(-sinks // block_size) * block_size + window + block_size - 1
+    return np.where(counts == 1, np.minimum(starts, most - 1), starts)
+
+
+def _window_step(step: PackedStep, window: int, sinks: int, num_kv_heads: int, num_query_heads: int, head_dim: int,
+                 cache_dtype: torch.dtype) -> PackedStep:
+    """A step whose decode work lists are those of ``step`` under a window: of
+    the shorter contexts that its decode walks, at their longest, so that the
+    lists stay while contexts grow.  ``step`` itself where no context is shorter
+    (its lists serve shorter contexts as well)."""
+    key = (window, sinks, num_kv_heads, num_query_heads, head_dim, cache_dtype)
+    sub = step._windows.get(key)
+    if sub is not None:
+        return sub
+    starts, counts, rows = step._inputs
+    shorter = _window_starts(starts, counts, step.block_size, window, sinks)
+    if step.num_decode_items == 0 or bool((shorter == starts).all()):
+        sub = step
+    else:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first attention of a step under a window packs its work lists, which a graph "
+                               "cannot capture: make one such call before")
+        device = step.buffer.device
+        per_item = decode_workgroups_per_item(cache_dtype, head_dim, num_kv_heads, num_query_heads)
+        per_cu = _occupancy_on(device, cache_dtype, head_dim, num_kv_heads, num_query_heads)
+        given = step.partition_size if step._partition_given else 0
+        partition = int(_plan(shorter, counts, step.block_size, step.prefill_tile, given, num_kv_heads, num_query_heads,
+                              per_item, per_cu, _compute_units(device), None,
+                              cache_dtype_code(cache_dtype) if per_cu else -1, head_dim).partition_size)
+        longest = int((shorter + 1)[counts == 1].max())
+        if longest > partition and not given:
+            # (as many partitions of one size: the windows' length is no power of two)
+            partition = (-(-longest // -(-longest // partition)) + 31) // 32 * 32
+        sub = pack_step(step._source_table, shorter, counts, step.block_size, prefill_tile=step.prefill_tile,
+                        partition_size=partition, num_kv_heads=num_kv_heads,
+                        num_query_heads=num_query_heads, head_dim=head_dim, dtype=cache_dtype, rows=rows)
+    step._windows[key] = sub
+    return sub
+
+
+def _attention_window(query, key_cache, value_cache, layer_idx, step, scaling, out, new_key, new_value, key_scales,
+                      value_scales, window, sinks) -> torch.Tensor:
+    """:func:`attention` under a window as one library call; checks and shared
+    arguments kept as :func:`_attention_step` keeps them."""
+    if query.stride()[-1:] != (1,):
+        query = _query_view(query)
+    if new_key is not None:
+        new_key = new_key if new_key.stride()[-1:] == (1,) else new_key.contiguous()
+        new_value = new_value if new_value.stride()[-1:] == (1,) else new_value.contiguous()
+    key = (window, sinks, _kind(query), _kind(key_cache), _kind(value_cache), _kind(key_scales), _kind(value_scales),
+           _kind(new_key), _kind(new_value))
+    calls = step.__dict__.setdefault("_window_calls", {})
+    cached = calls.get(key)
+    if cached is None:
+        limits = _window_of(window, sinks)
+        q, dims, _ = _checked(query, key_cache, value_cache, step, key_scales, value_scales)
+        strides = None
+        if new_key is not None:
+            k, v = _new_rows(new_key, new_value, key_cache, step)
+            if k.dtype != q.dtype:
+                raise ValueError(f"new_key dtype {k.dtype} differs from the query dtype {q.dtype}")
+            strides = (k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+        call = _step_call(step, dims)
+        sub = step
+        if step.num_decode_items > 0:
+            sub = _window_step(step, *limits, int(dims.num_kv_heads), int(dims.num_query_heads), int(dims.head_dim),
+                               key_cache.dtype)
+        if sub is not step:
+            lists = _step_call(sub, dims)
+            for name in ("decode_items", "num_decode_items", "merge_items", "num_merge_items", "workspace",
+                         "workspace_bytes"):
+                setattr(call, name, getattr(lists, name))
+            call.dims.partition_size = sub.partition_size
+        # (the steps' workspaces of other head counts stay alive with the call)
+        cached = (ctypes.byref(call), _native.PaWindow(*limits), tuple(q.shape), strides, step._extra_ws, sub._extra_ws)
+        if len(calls) >= 64:
+            calls.clear()
+        calls[key] = cached
+    call_ref, limits, shape, strides, _, _ = cached
+    if out is None:
+        rows_out = query.new_empty(shape)
+    else:
+        rows_out = _output_for(_query_view(query), key_cache, out)
+    if step.num_decode_items == 0 and step.num_prefill_items == 0:
+        return rows_out.zero_()
+    rows = None
+    if strides is not None:
+        rows = ctypes.byref(_native.PaNewRows(new_key.data_ptr(), new_value.data_ptr(), *strides))
+    with _current(query.device):
+        status = _native.load_library().pa_attention_window(
+            call_ref, limits, query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), _ptr(key_scales),
+            _ptr(value_scales), int(layer_idx), rows, float(scaling), rows_out.data_ptr(), _stream(query.device))
+    _native.check(status, "pa_attention_window")
+    return rows_out
+
+
+# ---------------------------------------------------------------------------
+# trees of drafted tokens
+
+
+class TreeStep:
+    """The trees of a step (what pa_pack_tree writes), in one device allocation.
+
+    ``masks`` int32 [T, words]: bit j % 32 of word j // 32 of a node's row is set
+    where node j of its sequence is the node itself or one of its ancestors.
+    ``position_ids`` int64 [T]: the sequence's start plus the node's depth.  The
+    attention's work lists and the workspace of its partial results are kept
+    beside them; calls that share a tree must not overlap in time.
+    """
+
+    def __init__(self, step: PackedStep, parents: torch.Tensor, dims, plan, head_shape, window, sinks, buffer,
+                 layout) -> None:
+        self.step = step
+        self.parents = parents
+        self.window = window
+        self.sinks = sinks
+        self._dims, self._plan, self._heads = dims, plan, head_shape
+        self._buffer, self._layout = buffer, layout
+        self._packs = -1
+
+    def _view(self, name: str) -> torch.Tensor:
+        off, dtype, shape = self._layout.fields[name]
+        count = int(np.prod(shape))
+        return self._buffer[off : off + count * _ELEM[dtype]].view(dtype).view(shape)
+
+    @property
+    def masks(self) -> torch.Tensor:
+        return self._view("masks")
+
+    @property
+    def position_ids(self) -> torch.Tensor:
+        return self._view("positions")
+
+    def ptr(self, name: str) -> int:
+        return self._buffer.data_ptr() + self._layout.fields[name][0]
+
+    def rerun(self) -> None:
+        """Rerun the packing kernel on the parents and the step's lengths as they
+        are on the device now: nothing is read from the host or allocated, so it
+        can be captured in a graph (behind :meth:`PackedStep.rerun`)."""
+        step, device = self.step, self._buffer.device
+        with _current(device):
+            status = _native.load_library().pa_pack_tree(
+                self.parents.data_ptr(), step.ptr("context_lens"), step.ptr("cu_seqlens"), self._dims, self._plan,
+                self.ptr("masks"), self.ptr("positions"), self.ptr("items"), self.ptr("merge_items"),
+                _stream(device))
+        _native.check(status, "pa_pack_tree")
+
+    def repack(self, parents=None) -> None:
+        """Pack the trees anew after :meth:`PackedStep.repack`, or with other
+        ``parents``, every output at its address.  ValueError where the step now
+        needs longer work lists than this tree has: pack a new one."""
+        plan = _plan_tree(self.step, self._dims, self._plan.split_stages)
+        had = self._plan
+        if plan.num_items > had.num_items or plan.num_merge_items > had.num_merge_items or \
+                plan.num_partial_rows > had.num_partial_rows or plan.mask_words > had.mask_words:
+            raise ValueError("repack: the step's trees need longer work lists; pack a new tree instead")
+        if parents is not None:
+            self.parents.copy_(_parents(self.step, parents))
+        self.rerun()
+        self._packs = self.step._packs
+
+
+def _parents(step: PackedStep, parents) -> torch.Tensor:
+    """int32 [T] parents on the step's device."""
+    t = parents if isinstance(parents, torch.Tensor) else torch.as_tensor(np.asarray(parents, dtype=np.int64))
+    if t.dtype.is_floating_point or t.dtype == torch.bool or t.numel() != step.num_query_tokens:
+        raise ValueError(f"parents must be one integer per new token ({step.num_query_tokens}), got {tuple(t.shape)} "
+                         f"of {t.dtype}")
+    if t.is_cuda and t.device != step.buffer.device:
+        raise RuntimeError(f"tensors on different devices: {step.buffer.device} and {t.device}")
+    if t.dtype != torch.int32:
+        t = t.clamp(-1, _INT32_MAX).to(torch.int32)  # (no larger value is a parent)
+    if not t.is_cuda:
+        t = t.to(step.buffer.device)
+    return t.reshape(-1).contiguous()
+
+
+def _plan_tree(step: PackedStep, dims, split_stages: int):
+    plan = _native.PaTreePlan()
+    planned = _native.PaTreeDims.from_buffer_copy(dims)
+    planned.split_stages = split_stages
+    starts, counts, _ = step._inputs
+    lib = _native.load_library()
+    status = lib.pa_plan_tree(starts.ctypes.data, counts.ctypes.data, planned, ctypes.byref(plan))
+    if status != _native.PA_OK:
+        if plan.bad_seq >= 0:
+            raise ValueError(lib.pa_last_error_message().decode(errors="replace"))
+        _native.check(status, "pa_plan_tree")
+    return plan
+
+
+def pack_tree(
+    step: PackedStep,
+    parents,
+    *,
+    num_kv_heads: Optional[int] = None,
+    num_query_heads: Optional[int] = None,
+    head_dim: Optional[int] = None,
+    dtype: Optional[torch.dtype] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
+) -> TreeStep:
+    """Masks, positions and attention work lists of a step whose sequences' new
+    tokens are trees of drafted tokens.
+
+    ``parents``: one integer per new token, an int32 device tensor (kept and read
+    by every later run) or anything that becomes one: the index, within its
+    sequence, of an earlier node, or -1 for a root; anything else counts as -1.
+    Up to 1024 nodes a tree.  The head counts, head dim and query ``dtype`` the
+    attention will have are by default those the step was packed for (a step of
+    no known ``head_dim`` gets no work lists: give them here).  ``window`` /
+    ``sinks``: of the layers that attend through this tree (at least the largest
+    tree's nodes, which always see their ancestors); layers of another window take
+    a tree of their own.
+    """
+    heads = step._heads or (8, 32, None, None)
+    hkv = int(num_kv_heads or heads[0])
+    hq = int(num_query_heads or (heads[1] if num_kv_heads is None else 4 * hkv))
+    dim = int(head_dim or heads[2] or 0)
+    dtype = dtype or heads[3] or torch.float32
+    if dtype == CODE_DTYPE:
+        dtype = torch.bfloat16  # (the lists are those of any query)
+    limits = (0, 0)
+    if window is not None:
+        limits = _window_of(window, sinks)
+    elif sinks:
+        raise ValueError("sinks go with a window")
+    device = step.buffer.device
+    dims = _native.PaTreeDims(
+        num_seqs=step.num_seqs, num_query_tokens=step.num_query_tokens, num_query_heads=hq if dim else 0,
+        num_kv_heads=hkv if dim else 0, head_dim=dim, dtype=dtype_code(dtype), block_size=step.block_size,
+        compute_units=_compute_units(device), window=_native.PaWindow(*limits))
+    plan = _plan_tree(step, dims, 0)
+    parents = _parents(step, parents)
+    layout = _Layout()
+    layout.add("masks", torch.int32, (step.num_query_tokens, int(plan.mask_words)))
+    layout.add("positions", torch.int64, (step.num_query_tokens,))
+    layout.add("items", torch.int32, (int(plan.num_items), 4))
+    layout.add("merge_items", torch.int32, (int(plan.num_merge_items), 4))
+    layout.add("workspace", torch.uint8, (decode_workspace_bytes(int(plan.num_partial_rows), hq, dim),))
+    buffer = torch.empty(layout.nbytes, dtype=torch.uint8, device=device)
+    tree = TreeStep(step, parents, dims, plan, (hkv, hq, dim) if dim else None, *limits, buffer, layout)
+    tree.rerun()
+    tree._packs = step._packs
+    return tree
+
+
+def _check_tree(step: PackedStep, tree: TreeStep) -> None:
+    if tree.step is not step:
+        raise ValueError("the tree was packed for another step")
+    if tree._packs != step._packs:
+        raise RuntimeError("the step was repacked: repack its tree (TreeStep.repack) as well")
+
+
+def tree_attention(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    layer_idx: int,
+    step: PackedStep,
+    tree: TreeStep,
+    scaling: float,
+    out: Optional[torch.Tensor] = None,
+    new_key: Optional[torch.Tensor] = None,
+    new_value: Optional[torch.Tensor] = None,
+    key_scales: Optional[torch.Tensor] = None,
+    value_scales: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of a step of trees -> [T, H_q, D]: every node sees its sequence's
+    context (the ``start`` positions before its tree; under the tree's window, of
+    these what the window and the sinks leave at the node's position), its
+    ancestors and itself.
+
+    Node j of a sequence has its K and V rows at position start + j, where the
+    step's scatter slots put them: already, or with ``new_key`` / ``new_value``
+    ([T, H_kv, D]), which are written first.  Queries, caches and scales as
+    :func:`attention` takes them.
+    """
+    if (new_key is None) != (new_value is None):
+        raise ValueError("new_key and new_value are given together")
+    _check_tree(step, tree)
+    if query.stride()[-1:] != (1,):
+        query = _query_view(query)
+    if new_key is not None:
+        new_key = new_key if new_key.stride()[-1:] == (1,) else new_key.contiguous()
+        new_value = new_value if new_value.stride()[-1:] == (1,) else new_value.contiguous()
+    key = (_kind(query), _kind(key_cache), _kind(value_cache), _kind(key_scales), _kind(value_scales),
+           _kind(new_key), _kind(new_value))
+    cached = tree.__dict__.get("_layer_call")
+    if cached is None or cached[0] != key:
+        q, dims, _ = _checked(query, key_cache, value_cache, step, key_scales, value_scales)
+        heads = (int(dims.num_kv_heads), int(dims.num_query_heads), int(dims.head_dim))
+        if tree._heads is None:
+            raise ValueError("the tree has no attention work lists: give pack_tree the head counts and head_dim")
+        if heads != tree._heads:
+            raise ValueError(f"the tree was packed for (H_kv, H_q, D) {tree._heads}, not {heads}")
+        strides = None
+        if new_key is not None:
+            k, v = _new_rows(new_key, new_value, key_cache, step)
+            if k.dtype != q.dtype:
+                raise ValueError(f"new_key dtype {k.dtype} differs from the query dtype {q.dtype}")
+            strides = (k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+        call = _native.PaTreeCall(
+            dims=dims, block_tables=step.ptr("block_tables"), context_lens=step.ptr("context_lens"),
+            cu_seqlens=step.ptr("cu_seqlens"), scatter_slots=step.ptr("scatter_slots"), masks=tree.ptr("masks"),
+            positions=tree.ptr("positions"), items=tree.ptr("items"), merge_items=tree.ptr("merge_items"),
+            workspace=tree.ptr("workspace"), workspace_bytes=tree._layout.fields["workspace"][2][0], plan=tree._plan,
+            window=_native.PaWindow(tree.window, tree.sinks))
+        cached = (key, ctypes.byref(call), tuple(q.shape), strides)
+        tree.__dict__["_layer_call"] = cached
+    _, call_ref, shape, strides = cached
+    if out is None:
+        rows_out = query.new_empty(shape)
+    else:
+        rows_out = _output_for(_query_view(query), key_cache, out)
+    rows = None
+    if strides is not None:
+        rows = ctypes.byref(_native.PaNewRows(new_key.data_ptr(), new_value.data_ptr(), *strides))
+    with _current(query.device):
+        status = _native.load_library().pa_tree_attention(
+            call_ref, query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), _ptr(key_scales),
+            _ptr(value_scales), int(layer_idx), rows, float(scaling), rows_out.data_ptr(), _stream(query.device))
+    _native.check(status, "pa_tree_attention")
+    return rows_out
+
+
+class AcceptedPath(NamedTuple):
+    """What :func:`accept_tree` found: ``nodes`` int32 [T], the path's nodes in
+    each sequence's first rows and -1 behind them; ``counts`` int32 [B], their
+    number; ``next_tokens`` int64 [B], what each path's last node predicts."""
+
+    nodes: torch.Tensor
+    counts: torch.Tensor
+    next_tokens: torch.Tensor
+
+
+def accept_tree(step: PackedStep, tree: TreeStep, drafted: torch.Tensor, predicted: torch.Tensor) -> AcceptedPath:
+    """The path of each tree whose tokens the model itself would have chosen: from
+    node 0 (the sequence's last known token) on, the first child whose ``drafted``
+    token is the one ``predicted`` at its parent, until there is none.  Both int64
+    [T]: the nodes' own tokens, and the model's choice after each.  All on the
+    device: nothing is read back."""
+    _check_tree(step, tree)
+    device = _require_device(drafted, predicted, step.buffer)
+    for name, t in (("drafted", drafted), ("predicted", predicted)):
+        if t.dtype != torch.int64 or t.numel() != step.num_query_tokens:
+            raise ValueError(f"{name} must be int64 with one entry per new token ({step.num_query_tokens}), got "
+                             f"{tuple(t.shape)} of {t.dtype}")
+    drafted, predicted = drafted.contiguous(), predicted.contiguous()
+    t, b = step.num_query_tokens, step.num_seqs
+    path = AcceptedPath(torch.empty(t, dtype=torch.int32, device=device),
+                        torch.empty(b, dtype=torch.int32, device=device),
+                        torch.empty(b, dtype=torch.int64, device=device))
+    with _current(device):
+        status = _native.load_library().pa_accept_tree(
+            tree.parents.data_ptr(), step.ptr("cu_seqlens"), drafted.data_ptr(), predicted.data_ptr(), b, t,
+            path.nodes.data_ptr(), path.counts.data_ptr(), path.next_tokens.data_ptr(), _stream(device))
+    _native.check(status, "pa_accept_tree")
+    return path
+
+
+def keep_rows(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    step: PackedStep,
+    nodes: torch.Tensor,
+    counts: torch.Tensor,
+    key_scales: Optional[torch.Tensor] = None,
+    value_scales: Optional[torch.Tensor] = None,
+) -> None:
+    """Moves kept nodes' K and V rows behind their sequence's context, in every
+    layer: the row of position start + node of the j-th kept node goes to position
+    start + j.
+
+    ``nodes`` int32 [T] (a sequence's kept nodes in its first rows, ascending) and
+    ``counts`` int32 [B] (:func:`accept_tree`).  From the first entry that does not
+    ascend, or is none of the sequence's nodes, its rows stay as they are.  In an
+    8-bit cache a block that rows move into takes the largest scale among its own
+    and those of the blocks they come from.
+    """
+    device = _require_device(key_cache, value_cache, step.buffer, nodes, counts)
+    if key_cache.dim() != 5 or value_cache.shape != key_cache.shape:
+        raise ValueError("caches must be 5-D (layers, blocks, block_size, heads, dim) and alike")
+    if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+        raise ValueError("caches must be contiguous")
+    if key_cache.dtype != value_cache.dtype:
+        raise ValueError("key and value cache must have the same dtype")
+    if int(key_cache.shape[2]) != step.block_size:
+        raise ValueError(f"the step was packed for blocks of {step.block_size}, the cache has {key_cache.shape[2]}")
+    for name, t, n in (("nodes", nodes, step.num_query_tokens), ("counts", counts, step.num_seqs)):
+        if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor of {n}, got {tuple(t.shape)} of {t.dtype}")
+    if step.num_query_tokens > 0 and step.max_new_tokens > _native.PA_MAX_TREE_NODES:
+        raise ValueError(f"a sequence has {step.max_new_tokens} new tokens, a tree at most {_native.PA_MAX_TREE_NODES}")
+    scales = _cache_scales(key_cache, value_cache, key_scales, value_scales)
+    num_layers, total_blocks, block_size, num_kv_heads, head_dim = (int(n) for n in key_cache.shape)
+    dims = _native.PaStepDims(
+        num_seqs=step.num_seqs, num_query_tokens=step.num_query_tokens, num_query_heads=num_kv_heads,
+        num_kv_heads=num_kv_heads, head_dim=head_dim, block_size=block_size, total_blocks=total_blocks,
+        num_layers=num_layers, max_blocks_per_seq=step.table_width, dtype=cache_dtype_code(key_cache.dtype),
+        num_table_rows=step._source_rows, block_table_rows=step.ptr("rows") if step._pooled else None)
+    with _current(device):
+        status = _native.load_library().pa_keep_rows(
+            key_cache.data_ptr(), value_cache.data_ptr(), scales.key if scales else None,
+            scales.value if scales else None, dims, step.ptr("block_tables"), step.ptr("context_lens"),
+            step.ptr("cu_seqlens"), nodes.data_ptr(), counts.data_ptr(), _stream(device))
+    _native.check(status, "pa_keep_rows")
 
 
 def paged_attention_flat(
