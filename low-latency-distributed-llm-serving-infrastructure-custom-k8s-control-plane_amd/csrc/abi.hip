@@ -530,8 +530,15 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
   const int eb = elem_bytes(dims.dtype);
   const int cache_eb = scales != nullptr ? 1 : eb;
   const int log2_bs = log2_exact(dims.block_size);
+  // Under a window the partition launch always merges itself (its list may hold
+  // partitions that a sequence does not have), so its records' fields (items
+  // below 2^24, partitions of a sequence below 2^16) have to take the step.
+  const bool records_fit =
+      num_decode_items < 65535 ||
+      (window.window > 0 && num_decode_items < (1 << 24) - 1 && dims.partition_size > 0 &&
+       static_cast<int64_t>(dims.max_blocks_per_seq) * dims.block_size / dims.partition_size < 65535);
   const bool fast =
-      window.window == 0 && ordered_scaling(scaling) &&
+      ordered_scaling(scaling) && (window.window == 0 || records_fit) &&
       pa::decode_fast_path_supported(scales == nullptr ? dims.dtype : PA_DTYPE_E4M3, dims.head_dim, group,
                                      dims.block_size, dims.partition_size) &&
       (scales == nullptr || dims.dtype != PA_DTYPE_F32) &&
@@ -603,7 +610,9 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
     a.group = group;
     a.sub_groups = pa::decode_workgroups_per_head(dims.dtype, dims.head_dim, group);
     // A record's fields hold counts and items below 65535.
-    a.merge_state = num_decode_items < 65535 ? merge_state : nullptr;
+    a.merge_state = records_fit ? merge_state : nullptr;
+    a.window = window.window;
+    a.sinks = window.sinks;
     a.num_seqs = dims.num_seqs;
     if (scales != nullptr) {
       a.key_scales = layer_scales(scales->key, dims, layer_idx);

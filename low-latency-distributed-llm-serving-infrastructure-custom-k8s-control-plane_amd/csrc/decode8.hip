@@ -28,6 +28,7 @@
 #include "cache8.hpp"
 #include "decode_common.hpp"
 #include "decode_mfma_common.hpp"
+#include "span.hpp"
 
 namespace pa {
 
@@ -76,8 +77,8 @@ __device__ __forceinline__ void read_codes(const uint32_t (&at)[KP], u32x4m (&k)
         : "memory");
 }
 
-// SMALL: blocks of fewer than 16 tokens.
-template <typename T, int D, int DM, bool SHARED, int HEADS, bool SMALL>
+// SMALL: blocks of fewer than 16 tokens.  WINDOW: as in decode_mfma.hip.
+template <typename T, int D, int DM, bool SHARED, int HEADS, bool SMALL, bool WINDOW>
 __global__ __launch_bounds__(kDecodeThreads) __attribute__((amdgpu_waves_per_eu(4))) void
 decode8_kernel(DecodeArgs a) {
   static_assert(sizeof(T) == 2, "16-bit queries");
@@ -127,11 +128,19 @@ decode8_kernel(DecodeArgs a) {
   const int p0 = part * a.partition;
   const int log2_bs = a.log2_block_size;
   const int bs_mask = (1 << log2_bs) - 1;
+  [[maybe_unused]] DecodeSpan span{};  // (its context is the one of this launch)
+  if constexpr (WINDOW) {
+    asm volatile("" : "+s"(ctx), "+s"(qtok));
+    span = decode_span(ctx, a.window, a.sinks, log2_bs);
+    ctx = span.ctx;
+    if (part > 0 && p0 >= ctx) return;  // (a list made for a longer one)
+  }
   const int first_blk = p0 >> log2_bs;
   const int nblk = SMALL ? 0 : ((p0 + a.partition - 1) >> log2_bs) - first_blk + 1;  // ids kept in LDS
   // (an id outside the pool becomes -1)
   auto table_entry = [&](int i) {
-    const int col = first_blk + i;
+    int col = first_blk + i;
+    if constexpr (WINDOW) col += col >= span.sinks ? span.skip : 0;
     const int b = row_ok && col < a.block_table_stride ? a.block_tables[trow * a.block_table_stride + col] : -1;
     return b >= a.total_blocks ? -1 : b;
   };
@@ -140,6 +149,10 @@ decode8_kernel(DecodeArgs a) {
   asm volatile("" : "+s"(ctx), "+s"(qtok));
   const int n = max(0, min(a.partition, ctx - p0));
   const int ntiles = (n + kTile8 - 1) / kTile8;
+  // Whether tokens [t, t + count) of the partition meet the hole of the span.
+  [[maybe_unused]] auto in_hole = [&](int t, int count) {
+    return WINDOW && p0 + t < span.hole_end && p0 + t + count > span.hole;
+  };
   const int64_t row_bytes = static_cast<int64_t>(hkv) * kMemBytes;
   const char* kbase = reinterpret_cast<const char*>(a.key_cache) + kvh * kMemBytes;
   const char* vbase = reinterpret_cast<const char*>(a.value_cache) + kvh * kMemBytes;
@@ -180,7 +193,7 @@ decode8_kernel(DecodeArgs a) {
   };
   auto live_tokens = [&](int tile) {
     const int t = tile * kTile8 + lane % kTile8;
-    return static_cast<uint32_t>(__ballot(t < n && block_of(min(t, n - 1)) >= 0));
+    return static_cast<uint32_t>(__ballot(t < n && !in_hole(t, 1) && block_of(min(t, n - 1)) >= 0));
   };
 
   VP vt[kVLoads];  // V of a tile: tokens 4c .. 4c+3 of each group
@@ -339,7 +352,8 @@ decode8_kernel(DecodeArgs a) {
         const bool on = (mine >> (16 * g + i)) & 1u;
         s[g][i] = on ? s[g][i] : -INFINITY;
         if (!on) vt[4 * g + i] = VP{};
-        if (i % 2 == 0) vs[g][i / 2] = on ? vs[g][i / 2] : 1.f;
+        // (a pair's scale is set aside with both of its tokens)
+        if (i % 2 == 0) vs[g][i / 2] = ((mine >> (16 * g + i)) & 3u) != 0 ? vs[g][i / 2] : 1.f;
       }
   };
   auto attend = [&]() {
@@ -412,7 +426,7 @@ decode8_kernel(DecodeArgs a) {
       for (; tile + kHeadWaves < ntiles; tile += kHeadWaves) {
         const int b = locate(tile + kHeadWaves);
         scores();
-        if (hole) mask(live_tokens(tile));
+        if (hole || in_hole(tile * kTile8, kTile8)) mask(live_tokens(tile));
 #pragma unroll
         for (int i = 0; i < kVLoads; ++i) asm volatile("" : "+v"(vt[i]));
         __builtin_amdgcn_sched_barrier(0);
@@ -424,7 +438,7 @@ decode8_kernel(DecodeArgs a) {
         __builtin_amdgcn_sched_barrier(0);
       }
       scores();
-      if (hole || n - tile * kTile8 < kTile8) mask(live_tokens(tile));
+      if (hole || n - tile * kTile8 < kTile8 || in_hole(tile * kTile8, kTile8)) mask(live_tokens(tile));
       attend();
     }
   }
@@ -459,15 +473,19 @@ struct Launch8 {
   hipStream_t stream;
   template <typename T, int D, int DM, bool SHARED, int HEADS>
   hipError_t run() const {
+    return a.window > 0 ? launch<T, D, DM, SHARED, HEADS, true>() : launch<T, D, DM, SHARED, HEADS, false>();
+  }
+  template <typename T, int D, int DM, bool SHARED, int HEADS, bool WINDOW>
+  hipError_t launch() const {
     const uint32_t units = a.num_kv_heads / HEADS;
     const int64_t grid = num_items * units * a.sub_groups;
     DecodeArgs b = a;
     b.run_rcp = 0xffffffffu / (kXcds * units * a.sub_groups);
     if (a.log2_block_size < 4)
-      hipLaunchKernelGGL((decode8_kernel<T, D, DM, SHARED, HEADS, true>), dim3(static_cast<uint32_t>(grid)),
+      hipLaunchKernelGGL((decode8_kernel<T, D, DM, SHARED, HEADS, true, WINDOW>), dim3(static_cast<uint32_t>(grid)),
                          dim3(kDecodeThreads), 0, stream, b);
     else
-      hipLaunchKernelGGL((decode8_kernel<T, D, DM, SHARED, HEADS, false>), dim3(static_cast<uint32_t>(grid)),
+      hipLaunchKernelGGL((decode8_kernel<T, D, DM, SHARED, HEADS, false, WINDOW>), dim3(static_cast<uint32_t>(grid)),
                          dim3(kDecodeThreads), 0, stream, b);
     return hipGetLastError();
   }
@@ -477,7 +495,7 @@ struct Occupancy8 {
   int* per_cu;
   template <typename T, int D, int DM, bool SHARED, int HEADS>
   hipError_t run() const {
-    return hipOccupancyMaxActiveBlocksPerMultiprocessor(per_cu, decode8_kernel<T, D, DM, SHARED, HEADS, false>,
+    return hipOccupancyMaxActiveBlocksPerMultiprocessor(per_cu, decode8_kernel<T, D, DM, SHARED, HEADS, false, false>,
                                                         kDecodeThreads, 0);
   }
 };

@@ -67,6 +67,7 @@
 
 #include "decode_common.hpp"
 #include "decode_mfma_common.hpp"
+#include "span.hpp"
 
 namespace pa {
 
@@ -124,7 +125,10 @@ __device__ __forceinline__ void read_k(const uint32_t (&at)[KJ], u32x4m (&k)[2][
         : "memory");
 }
 
-template <typename T, int D, int DM, bool SHARED, int HEADS>
+// WINDOW: the context without the blocks that a window and its sinks leave out
+// (decode_span()); tiles that meet the hole beside the cut are masked, the others
+// run as without one.
+template <typename T, int D, int DM, bool SHARED, int HEADS, bool WINDOW>
 __global__ __launch_bounds__(kDecodeThreads) __attribute__((amdgpu_waves_per_eu(3))) void
 decode_mfma_kernel(DecodeArgs a) {
   static_assert(sizeof(T) == 2, "16-bit caches");
@@ -172,13 +176,21 @@ decode_mfma_kernel(DecodeArgs a) {
   const int p0 = part * a.partition;
   const int log2_bs = a.log2_block_size;
   const int bs_mask = (1 << log2_bs) - 1;
+  [[maybe_unused]] DecodeSpan span{};  // (its context is the one of this launch)
+  if constexpr (WINDOW) {
+    asm volatile("" : "+s"(ctx), "+s"(qtok));
+    span = decode_span(ctx, a.window, a.sinks, log2_bs);
+    ctx = span.ctx;
+    if (part > 0 && p0 >= ctx) return;  // (a list made for a longer one)
+  }
   // Block ids of the partition -> LDS (invalid ids become -1).  The whole
   // span is read, whatever the context length, so that the reads do not wait
   // for it.
   const int first_blk = p0 >> log2_bs;
   const int nblk = ((p0 + a.partition - 1) >> log2_bs) - first_blk + 1;
   auto table_entry = [&](int i) {
-    const int col = first_blk + i;
+    int col = first_blk + i;
+    if constexpr (WINDOW) col += col >= span.sinks ? span.skip : 0;
     return row_ok && col < a.block_table_stride ? a.block_tables[trow * a.block_table_stride + col] : -1;
   };
   auto valid_block = [&](int b) { return b < 0 || b >= a.total_blocks ? -1 : b; };
@@ -186,6 +198,10 @@ decode_mfma_kernel(DecodeArgs a) {
   // (both scalar loads issued before either is waited for: one round trip)
   asm volatile("" : "+s"(ctx), "+s"(qtok));
   const int n = max(0, min(a.partition, ctx - p0));
+  // Whether tokens [t, t + count) of the partition meet the hole of the span.
+  [[maybe_unused]] auto in_hole = [&](int t, int count) {
+    return WINDOW && p0 + t < span.hole_end && p0 + t + count > span.hole;
+  };
   const int64_t row_bytes = static_cast<int64_t>(hkv) * kMemBytes;
   const char* kbase = reinterpret_cast<const char*>(a.key_cache) + kvh * kMemBytes;
   const char* vbase = reinterpret_cast<const char*>(a.value_cache) + kvh * kMemBytes;
@@ -357,7 +373,7 @@ decode_mfma_kernel(DecodeArgs a) {
   auto mask = [&](int tile) {
     const int t = tile * kMfmaTile + (lane & (kMfmaTile - 1));
     const uint32_t live =
-        static_cast<uint32_t>(__ballot(t < n && s_blk[((p0 + min(t, n - 1)) >> log2_bs) - first_blk] >= 0));
+        static_cast<uint32_t>(__ballot(t < n && !in_hole(t, 1) && s_blk[((p0 + min(t, n - 1)) >> log2_bs) - first_blk] >= 0));
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -437,6 +453,7 @@ decode_mfma_kernel(DecodeArgs a) {
         scores(VInFlight());
 #pragma unroll
         for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(vt[i]));
+        if (in_hole(tile * kMfmaTile, kMfmaTile)) mask(tile);
         write_new_rows(tile + kHeadWaves);
         __builtin_amdgcn_sched_barrier(0);
         load_k();
@@ -491,13 +508,17 @@ struct MfmaLaunch {
   hipStream_t stream;
   template <typename T, int D, int DM, bool SHARED, int HEADS>
   hipError_t run() const {
+    return a.window > 0 ? launch<T, D, DM, SHARED, HEADS, true>() : launch<T, D, DM, SHARED, HEADS, false>();
+  }
+  template <typename T, int D, int DM, bool SHARED, int HEADS, bool WINDOW>
+  hipError_t launch() const {
     const uint32_t units = a.num_kv_heads / HEADS;
     const int64_t grid = num_items * units * a.sub_groups;
     const uint32_t gang = (DM * 2 % 256 != 0 ? units : 1) * a.sub_groups;
     DecodeArgs b = a;
     b.unit_rcp = 0xffffffffu / units;
     b.run_rcp = 0xffffffffu / (kXcds * gang);
-    hipLaunchKernelGGL((decode_mfma_kernel<T, D, DM, SHARED, HEADS>), dim3(static_cast<uint32_t>(grid)),
+    hipLaunchKernelGGL((decode_mfma_kernel<T, D, DM, SHARED, HEADS, WINDOW>), dim3(static_cast<uint32_t>(grid)),
                        dim3(kDecodeThreads), 0, stream, b);
     return hipGetLastError();
   }
@@ -507,7 +528,7 @@ struct MfmaOccupancy {
   int* per_cu;
   template <typename T, int D, int DM, bool SHARED, int HEADS>
   hipError_t run() const {
-    return hipOccupancyMaxActiveBlocksPerMultiprocessor(per_cu, decode_mfma_kernel<T, D, DM, SHARED, HEADS>,
+    return hipOccupancyMaxActiveBlocksPerMultiprocessor(per_cu, decode_mfma_kernel<T, D, DM, SHARED, HEADS, false>,
                                                         kDecodeThreads, 0);
   }
 };

@@ -63,6 +63,10 @@ struct DecodeArgs {
   // 8-bit caches (else null): base of the layer, [blocks, H_kv].
   const float* key_scales;
   const float* value_scales;
+  // A window (0: the whole context) with sinks: the items are partitions of the
+  // shorter contexts of decode_span(), and merge_state is not null.
+  int32_t window;
+  int32_t sinks;
 };
 
 // Generic one-wave-per-(query token, head) attention: any head_dim <= 256,
