@@ -11,6 +11,7 @@
 #include "pa_common.hpp"
 #include "pa_error.hpp"
 #include "pa_launch.hpp"
+#include "span.hpp"
 
 namespace {
 
@@ -740,7 +741,8 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
   const int eb = elem_bytes(dims.dtype);
   const int cache_eb = scales != nullptr ? 1 : eb;
   const bool fast =
-      window.window == 0 && ordered_scaling(scaling) &&
+      ordered_scaling(scaling) &&
+      (window.window == 0 || pa::prefill_window_supported(dims.dtype, dims.head_dim)) &&
       pa::prefill_fast_path_supported(dims.dtype, dims.head_dim, group, dims.block_size) &&
       (scales == nullptr || pa::prefill_codes_supported(dims.dtype, dims.head_dim)) &&
       prefill_tile == pa::prefill_tile_for(group) && dims.max_blocks_per_seq > 0 &&
@@ -795,6 +797,8 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
       a.key_scales = layer_scales(scales->key, dims, layer_idx);
       a.value_scales = layer_scales(scales->value, dims, layer_idx);
     }
+    a.window = window.window;
+    a.sinks = window.sinks;
     return from_hip(pa::launch_prefill(a, dims.dtype, dims.head_dim, group, num_prefill_items, s), who);
   }
   if (!pa::generic_supported(dims.dtype, dims.head_dim))
@@ -1279,6 +1283,72 @@ int pa_tree_attention(const PaTreeCall* call, const void* query, void* key_cache
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int eb = elem_bytes(d.dtype);
   const int cache_eb = key_scales != nullptr ? 1 : eb;
+  const int group = d.num_query_heads / d.num_kv_heads;
+  const bool fast =
+      c.plan.tile > 0 && c.plan.split_stages > 0 && c.plan.tile == pa::prefill_tile_for(group) &&
+      ordered_scaling(scaling) && pa::tree_fast_path_supported(d.dtype, d.head_dim, group, d.block_size) &&
+      (key_scales == nullptr || pa::prefill_codes_supported(d.dtype, d.head_dim)) && d.max_blocks_per_seq > 0 &&
+      static_cast<int64_t>(d.block_size) * d.num_kv_heads * d.head_dim * cache_eb <= 0xffffffffLL &&
+      aligned16(query) && aligned16(key_cache) && aligned16(value_cache) && aligned16(output) &&
+      (d.q_token_stride * eb) % 16 == 0 && (d.q_head_stride * eb) % 16 == 0;
+  if (fast) {
+    rc = require(who, {{c.items, "items"}});
+    if (rc != PA_OK) return rc;
+    if (c.plan.num_merge_items > 0 && c.merge_items == nullptr)
+      return fail(PA_ERR_INVALID_ARGUMENT, "%s: merge_items is required by this plan", who);
+    if (!aligned16(c.items) || !aligned16(c.merge_items))
+      return fail(PA_ERR_INVALID_ARGUMENT, "%s: items and merge_items must be 16-byte aligned", who);
+    const DecodeWorkspaceLayout wl = decode_workspace_layout(d, c.plan.num_partial_rows);
+    if (c.plan.num_partial_rows > 0 &&
+        (c.workspace == nullptr || !aligned16(c.workspace) || c.workspace_bytes < wl.acc + wl.ml))
+      return fail(PA_ERR_WORKSPACE, "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", who,
+                  wl.acc + wl.ml, c.workspace_bytes);
+    pa::PrefillArgs a{};
+    a.query = query;
+    a.q_token_stride = d.q_token_stride;
+    a.q_head_stride = d.q_head_stride;
+    a.key_cache = layer_base(key_cache, d, layer_idx, cache_eb);
+    a.value_cache = layer_base(value_cache, d, layer_idx, cache_eb);
+    a.block_tables = c.block_tables;
+    a.rows = d.block_table_rows;
+    a.num_table_rows = d.num_table_rows > 0 ? d.num_table_rows : d.num_seqs;
+    a.context_lens = c.context_lens;
+    a.cu_seqlens = c.cu_seqlens;
+    a.items = c.items;
+    a.output = output;
+    a.block_table_stride = d.max_blocks_per_seq;
+    a.num_kv_heads = d.num_kv_heads;
+    a.total_blocks = d.total_blocks;
+    a.log2_block_size = log2_exact(d.block_size);
+    a.scale_log2e = scaling * pa::kLog2e;
+    a.group = group;
+    a.sub_groups = pa::decode_sub_groups(group);
+    if (key_scales != nullptr) {
+      a.key_scales = layer_scales(key_scales, d, layer_idx);
+      a.value_scales = layer_scales(value_scales, d, layer_idx);
+    }
+    a.window = c.window.window;
+    a.sinks = c.window.sinks;
+    a.masks = c.masks;
+    a.mask_words = c.plan.mask_words;
+    a.positions = c.positions;
+    a.part_acc = reinterpret_cast<float*>(c.workspace);
+    a.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(c.workspace) + wl.acc);
+    a.split_stages = c.plan.split_stages;
+    rc = from_hip(pa::launch_prefill(a, d.dtype, d.head_dim, group, c.plan.num_items, s), who);
+    if (rc != PA_OK) return rc;
+    pa::MergeTreeArgs m{};
+    m.merge_items = reinterpret_cast<const int4*>(c.merge_items);
+    m.num_merge = c.plan.num_merge_items;
+    m.cu_seqlens = c.cu_seqlens;
+    m.part_acc = a.part_acc;
+    m.part_ml = a.part_ml;
+    m.output = output;
+    m.num_query_heads = d.num_query_heads;
+    m.num_query_tokens = d.num_query_tokens;
+    m.tile = c.plan.tile;
+    return from_hip(pa::launch_merge_tree(m, d.dtype, d.head_dim, s), who);
+  }
   if (!pa::generic_supported(d.dtype, d.head_dim))
     return fail(PA_ERR_UNSUPPORTED, "%s: head_dim %d / dtype %d not supported", who, d.head_dim, d.dtype);
   pa::GenericArgs a{};

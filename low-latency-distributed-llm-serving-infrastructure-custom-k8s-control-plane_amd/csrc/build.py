@@ -26,7 +26,7 @@ LIBRARY_NAME = "libpaged_attention_amd.so"
 LIBRARY_PATH = PACKAGE_DIR / LIBRARY_NAME
 OFFLOAD_ARCH = "gfx950"
 
-SOURCES = ["prefill.hip", "decode.hip", "decode_window.hip", "abi.hip", "plan.cpp", "pack.hip", "cache_write.hip", "rotate.hip", "decode_mfma.hip",
+SOURCES = ["prefill.hip", "prefill_window.hip", "prefill_tree.hip", "decode.hip", "decode_window.hip", "abi.hip", "plan.cpp", "pack.hip", "cache_write.hip", "rotate.hip", "decode_mfma.hip",
            "decode8.hip", "generic.hip",
            "prefill256.hip", "prefill_f32.hip", "tree.hip", "copy_blocks.hip", "calibrate.hip"]
 
@@ -49,7 +49,8 @@ HIP_FLAGS = [
 # accumulators in architectural VGPRs (no AGPR copies around the softmax
 # rescale); the one for heads of 256 (one wave per SIMD) leaves them to the
 # AGPRs.
-EXTRA_FLAGS = {"prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+EXTRA_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+               for name in ("prefill.hip", "prefill_window.hip", "prefill_tree.hip")}
 
 
 def _hipcc() -> str:

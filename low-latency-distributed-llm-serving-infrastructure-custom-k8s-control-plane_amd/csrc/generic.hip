@@ -37,8 +37,6 @@ __device__ __forceinline__ float cache_value(const C* p, float scale) {
   }
 }
 
-enum { kSpanAll = 0, kSpanWindow = 1, kSpanTree = 2 };
-
 template <typename T, int EPL, bool kMasked, typename C = T, int SPAN = kSpanAll>
 __global__ __launch_bounds__(kWave) void generic_attention_kernel(GenericArgs a) {
   const int lane = threadIdx.x;

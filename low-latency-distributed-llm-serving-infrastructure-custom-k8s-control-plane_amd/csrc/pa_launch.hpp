@@ -275,6 +275,18 @@ struct PrefillArgs {
   // 8-bit caches (else null): base of the layer, [blocks, H_kv].
   const float* key_scales;
   const float* value_scales;
+  // A window (0: the whole context) with sinks.
+  int32_t window;
+  int32_t sinks;
+  // Trees (else null): their nodes' masks and positions.  `items` are then
+  // pa_pack_tree's, and several of one tile leave their results in part_acc
+  // [rows, H_q, D] and part_ml [rows, H_q, 2].
+  const uint32_t* masks;
+  const int64_t* positions;
+  float* part_acc;
+  float* part_ml;
+  int32_t mask_words;
+  int32_t split_stages;
 };
 
 // A step's trees of drafted tokens (tree.hip): masks and positions of the nodes
@@ -386,12 +398,19 @@ bool prefill_fast_path_supported(int dtype, int head_dim, int group, int block_s
 bool prefill_append_supported(int dtype, int head_dim);
 // Whether the fast path of this shape also reads an 8-bit cache.
 bool prefill_codes_supported(int dtype, int head_dim);
+// Whether the fast path of this shape also takes a window.
+bool prefill_window_supported(int dtype, int head_dim);
 // Compute units of the current device (cached per device; 0 if unknown): the
 // width of the persistent prefill launches.
 int device_compute_units();
 int prefill_tile_for(int group);
 hipError_t launch_prefill(const PrefillArgs& a, int dtype, int head_dim, int group,
                           int64_t num_items, hipStream_t stream);
+// prefill_window.hip, prefill_tree.hip: 16-bit heads of 64 to 128.
+hipError_t launch_prefill_window(const PrefillArgs& a, int dtype, int head_dim, int group, int64_t num_items,
+                                 hipStream_t stream);
+hipError_t launch_prefill_tree(const PrefillArgs& a, int dtype, int head_dim, int group, int64_t num_items,
+                               hipStream_t stream);
 hipError_t launch_prefill256(const PrefillArgs& a, int dtype, int group, int64_t num_items, hipStream_t stream);
 // fp32 caches: the fp32 MFMA kernel of prefill_f32.hip (same units and rows).
 hipError_t launch_prefill_f32(const PrefillArgs& a, int head_dim, int group, int64_t num_items,

@@ -1,0 +1,11 @@
+// The matrix-core prefill's instances for windows with sinks.
+#include "prefill_span.hpp"
+
+namespace pa {
+
+hipError_t launch_prefill_window(const PrefillArgs& a, int dtype, int head_dim, int group, int64_t num_items,
+                                 hipStream_t stream) {
+  return launch_prefill_span<kSpanWindow>(a, dtype, head_dim, group, num_items, stream);
+}
+
+}  // namespace pa

@@ -14,6 +14,10 @@
 
 namespace pa {
 
+// What a kernel instance's queries see: the whole context, a window with sinks of
+// it, or a tree of drafted tokens behind it (or behind a window of it).
+enum { kSpanAll = 0, kSpanWindow = 1, kSpanTree = 2 };
+
 // Most nodes of one tree (pa_pack_tree keeps a sequence's parents in LDS).
 constexpr int kMaxTreeNodes = 1024;
 
