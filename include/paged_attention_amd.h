@@ -838,7 +838,7 @@ typedef struct {
     int32_t num_query_heads;  /* (0: masks and positions alone, no lists) */
     int32_t num_kv_heads;
     int32_t head_dim;
-    int32_t dtype;            /* of the query */
+    int32_t dtype;            /* of the cache (PA_DTYPE_E4M3: 8-bit codes) */
     int32_t block_size;
     int32_t compute_units;    /* of the device (0: 256) */
     int32_t split_stages;     /* > 0: use it; 0: choose */
@@ -872,13 +872,15 @@ int pa_plan_tree(const int64_t *start_positions, const int64_t *node_counts,
  * [T, mask_words] (bit j % 32 of word j / 32: node j of the sequence is the
  * node itself or an ancestor), positions int64 [T] (the start plus the node's
  * depth) and, for a plan with a tile, the attention's work lists: items int32
- * [num_items, 4], merge_items int32 [num_merge_items, 4] (16-byte aligned).
+ * [num_items, 8], merge_items int32 [num_merge_items, 4] (16-byte aligned).
+ * block_table_rows: as in PaStepDims of the attention.
  * Entries past a size in the plan are dropped, entries left over are marked.
  */
 int pa_pack_tree(const int32_t *parents, const int32_t *context_lens,
-                 const int64_t *cu_seqlens, PaTreeDims dims, PaTreePlan plan,
-                 uint32_t *masks, int64_t *positions, int32_t *items,
-                 int32_t *merge_items, void *stream);
+                 const int64_t *cu_seqlens, const int32_t *block_table_rows,
+                 PaTreeDims dims, PaTreePlan plan, uint32_t *masks,
+                 int64_t *positions, int32_t *items, int32_t *merge_items,
+                 void *stream);
 
 typedef struct {
     PaStepDims dims;

@@ -384,7 +384,7 @@ _SIGNATURES = {
     ),
     "pa_window_context": (_i32, [_i32, PaWindow, _i32]),
     "pa_plan_tree": (ctypes.c_int, [_vp, _vp, PaTreeDims, ctypes.POINTER(PaTreePlan)]),
-    "pa_pack_tree": (ctypes.c_int, [_vp, _vp, _vp, PaTreeDims, PaTreePlan, _vp, _vp, _vp, _vp, _vp]),
+    "pa_pack_tree": (ctypes.c_int, [_vp, _vp, _vp, _vp, PaTreeDims, PaTreePlan, _vp, _vp, _vp, _vp, _vp]),
     "pa_tree_workspace_size": (_sz, [PaStepDims, _i64]),
     "pa_tree_attention": (
         ctypes.c_int,

@@ -1211,8 +1211,8 @@ int pa_attention_window(const PaStepCall* call, PaWindow window, const void* que
   return PA_OK;
 }
 
-int pa_pack_tree(const int32_t* parents, const int32_t* context_lens, const int64_t* cu_seqlens, PaTreeDims dims,
-                 PaTreePlan plan, uint32_t* masks, int64_t* positions, int32_t* items, int32_t* merge_items,
+int pa_pack_tree(const int32_t* parents, const int32_t* context_lens, const int64_t* cu_seqlens,
+                 const int32_t* block_table_rows, PaTreeDims dims, PaTreePlan plan, uint32_t* masks, int64_t* positions, int32_t* items, int32_t* merge_items,
                  void* stream) {
   const char* who = "pa_pack_tree";
   int rc = check_window(who, dims.window);
@@ -1234,6 +1234,7 @@ int pa_pack_tree(const int32_t* parents, const int32_t* context_lens, const int6
   a.parents = parents;
   a.context_lens = context_lens;
   a.cu_seqlens = cu_seqlens;
+  a.rows = block_table_rows;
   a.masks = masks;
   a.positions = positions;
   a.items = plan.tile > 0 ? reinterpret_cast<int4*>(items) : nullptr;
@@ -1285,7 +1286,8 @@ int pa_tree_attention(const PaTreeCall* call, const void* query, void* key_cache
   const int cache_eb = key_scales != nullptr ? 1 : eb;
   const int group = d.num_query_heads / d.num_kv_heads;
   const bool fast =
-      c.plan.tile > 0 && c.plan.split_stages > 0 && c.plan.tile == pa::prefill_tile_for(group) &&
+      c.plan.tile > 0 && c.plan.split_stages > 0 && c.plan.split_stages <= pa::tree_max_stages(d.block_size) &&
+      c.plan.tile == pa::tree_tile_for(key_scales != nullptr ? PA_DTYPE_E4M3 : d.dtype, d.head_dim, group) &&
       ordered_scaling(scaling) && pa::tree_fast_path_supported(d.dtype, d.head_dim, group, d.block_size) &&
       (key_scales == nullptr || pa::prefill_codes_supported(d.dtype, d.head_dim)) && d.max_blocks_per_seq > 0 &&
       static_cast<int64_t>(d.block_size) * d.num_kv_heads * d.head_dim * cache_eb <= 0xffffffffLL &&

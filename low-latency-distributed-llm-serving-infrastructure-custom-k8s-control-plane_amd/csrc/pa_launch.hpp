@@ -297,7 +297,8 @@ struct PackTreeArgs {
   const int64_t* cu_seqlens;
   uint32_t* masks;              // [T, mask_words]
   int64_t* positions;           // [T]
-  int4* items;                  // (sequence, tile, split, first partial row or -1), or null
+  const int32_t* rows;          // row of the block table per sequence, or null (row = seq)
+  int4* items;                  // kTreeItemInts each, or null
   int4* merge_items;            // (sequence, tile, splits, first partial row)
   int64_t max_items;
   int64_t max_merge_items;
@@ -406,7 +407,11 @@ int device_compute_units();
 int prefill_tile_for(int group);
 hipError_t launch_prefill(const PrefillArgs& a, int dtype, int head_dim, int group,
                           int64_t num_items, hipStream_t stream);
-// prefill_window.hip, prefill_tree.hip: 16-bit heads of 64 to 128.
+// prefill_window.hip, prefill_tree.hip (over 8-bit caches): 16-bit heads of 64 to
+// 128; tree_attention.hip: trees over 16-bit caches, heads of 64 to 256.
+hipError_t launch_tree_attention256(const PrefillArgs& a, int dtype, int group, int64_t num_items, hipStream_t stream);
+hipError_t launch_tree_attention(const PrefillArgs& a, int dtype, int head_dim, int group, int64_t num_items,
+                                 hipStream_t stream);
 hipError_t launch_prefill_window(const PrefillArgs& a, int dtype, int head_dim, int group, int64_t num_items,
                                  hipStream_t stream);
 hipError_t launch_prefill_tree(const PrefillArgs& a, int dtype, int head_dim, int group, int64_t num_items,

@@ -265,7 +265,7 @@ struct Trees {
   TreeSizes sizes(int64_t split) const {
     TreeSizes z;
     each([&](int64_t n, int64_t stages) {
-      const int64_t splits = ceil_div(stages, split);
+      const int64_t splits = pa::tree_split(static_cast<int>(stages), static_cast<int>(split)).runs;
       z.items += splits;
       if (splits > 1) {
         z.merges += 1;
@@ -273,6 +273,11 @@ struct Trees {
       }
     });
     return z;
+  }
+  // Stages of a sequence's last tile, which sees all that the others see.
+  int64_t longest_of(int32_t i) const {
+    return counts[i] > 0 ? pa::tree_span(static_cast<int>(starts[i]), static_cast<int>(counts[i]), d.window.window,
+                                         d.window.sinks, pa::kTreeStage).count : 0;
   }
   template <typename F>
   void each(const F& f) const {
@@ -285,45 +290,61 @@ struct Trees {
   }
 };
 
-// Stages per item: one workgroup a CU takes items in turn, each of which costs
-// its stages and kItemStages more (its prologue and end); tiles in several items
-// are joined by a launch of its own.  The smallest modelled time wins, the
-// larger item of two alike.
-constexpr double kItemStages = 4.0;
-constexpr double kMergeStages = 6.0;
+// Stages per item, by the modelled time of the candidates.  Measured on 32/8 heads
+// of 128 with 47 to 2026 stages of 64 tokens a KV head (a unit is an item's KV head):
+//  * a unit costs 8.4 us beside its stages, a stage at least 1.85 us of its
+//    workgroup, and the caches' rows, read once for all tiles of a sequence, come
+//    at 5.5 TB/s (3.06 us a stage of every resident workgroup);
+//  * units that do not all fit the chip at once share its workgroups, and the last
+//    ones leave part of it idle;
+//  * tiles in several runs are joined by a launch of its own.
+// Within 10 % of 28 measured times of four steps (1 to 47 stages an item), and the
+// pick within 6 % of the fastest.
+struct TreeCost {
+  double unit, stage, bytes;  // us
+  int slots;                  // workgroups resident on a CU
+};
+TreeCost tree_cost(int dtype, int head_dim) {
+  const double row = head_dim * (dtype == PA_DTYPE_E4M3 ? 1 : 2) / 256.0;
+  if (dtype == PA_DTYPE_E4M3) return {10.0, 1.1, 1.53 * row, 1};  // (prefill.hip's kernel: a CU each)
+  if (head_dim == 256) return {8.4, 2.6, 1.53 * row, 1};
+  return head_dim == 64 ? TreeCost{8.4, 1.2, 4.6 * row, 3} : TreeCost{8.4, 1.85, 3.06 * row, 2};
+}
 int32_t choose_split(const Trees& t, const PaTreeDims& d) {
-  const int64_t per_item = d.num_kv_heads * static_cast<int64_t>(pa::decode_sub_groups(d.num_query_heads / d.num_kv_heads));
-  const int64_t cus = d.compute_units > 0 ? d.compute_units : 256;
-  int64_t longest = 1;
-  t.each([&](int64_t, int64_t stages) { longest = stages > longest ? stages : longest; });
+  const int64_t heads = d.num_kv_heads * static_cast<int64_t>(pa::decode_sub_groups(d.num_query_heads / d.num_kv_heads));
+  const TreeCost c = tree_cost(d.dtype, d.head_dim);
+  const int64_t slots = static_cast<int64_t>(c.slots) * (d.compute_units > 0 ? d.compute_units : 256);
+  int64_t longest = 1, all = 0, unique = 0;
+  for (int32_t i = 0; i < d.num_seqs; ++i) unique += t.longest_of(i);
+  t.each([&](int64_t, int64_t stages) {
+    longest = stages > longest ? stages : longest;
+    all += stages;
+  });
   double best = 0;
   int32_t pick = 0;
-  for (int64_t split = longest;; split = split * 3 / 4 < split ? split * 3 / 4 : split - 1) {
-    if (split < 1) break;
-    double total = 0;
-    int64_t items = 0;
-    bool merged = false;
+  for (int64_t split = longest; split >= 1; split = split * 4 / 5 < split - 1 ? split * 4 / 5 : split - 1) {
+    int64_t items = 0, run = 0, runs = 0;
     t.each([&](int64_t, int64_t stages) {
-      const int64_t n = ceil_div(stages, split);
-      items += n;
-      merged |= n > 1;
-      total += stages + kItemStages * n;
+      const pa::TreeSplit cut = pa::tree_split(static_cast<int>(stages), static_cast<int>(split));
+      items += cut.runs;
+      run = cut.stages > run ? cut.stages : run;
+      runs = cut.runs > runs ? cut.runs : runs;
     });
-    const double rounds = static_cast<double>(ceil_div(items * per_item, cus));
-    const double even = total * per_item / cus;
-    const double longest_item = (longest < split ? longest : split) + kItemStages;
-    // (items of one size in whole rounds; of many sizes the snake evens them out)
-    double time = even > longest_item ? even : longest_item;
-    const double whole = rounds * longest_item;
-    time = 0.5 * time + 0.5 * (whole < time ? time : whole);
-    if (merged) time += kMergeStages;
+    const double units = static_cast<double>(items * heads);
+    double chain = run * c.stage;
+    double bytes = unique * heads * c.bytes / slots + 0.2 * run * c.bytes;
+    if (units > slots) {
+      chain = (units * c.unit + all * heads * c.stage) / slots + 0.5 * chain;
+      bytes += units * c.unit / slots;
+    }
+    const double time = c.unit + (chain > bytes ? chain : bytes) + (runs > 1 ? 2.0 + 0.25 * runs : 0.0);
     if (pick == 0 || time < best) {
       best = time;
       pick = static_cast<int32_t>(split);
     }
-    if (items * per_item > 8 * cus) break;
+    if (units > 8.0 * slots) break;
   }
-  return pick > 0 ? pick : 1;
+  return pick;
 }
 
 }  // namespace
@@ -358,9 +379,11 @@ extern "C" int pa_plan_tree(const int64_t* start_positions, const int64_t* node_
   if (dims.num_query_heads == 0) return PA_OK;
   const int group = dims.num_query_heads / dims.num_kv_heads;
   if (!pa::tree_fast_path_supported(dims.dtype, dims.head_dim, group, dims.block_size)) return PA_OK;
-  plan->tile = pa_prefill_tile(dims.num_query_heads, dims.num_kv_heads);
+  plan->tile = pa::tree_tile_for(dims.dtype, dims.head_dim, group);
   const Trees trees{start_positions, node_counts, dims, plan->tile};
   plan->split_stages = dims.split_stages > 0 ? dims.split_stages : choose_split(trees, dims);
+  const int32_t most_stages = pa::tree_max_stages(dims.block_size);
+  plan->split_stages = plan->split_stages < most_stages ? plan->split_stages : most_stages;
   const TreeSizes z = trees.sizes(plan->split_stages);
   if (z.items > 0x7fffffff || z.rows > 0x7fffffff)
     return pa::set_error(PA_ERR_UNSUPPORTED, "pa_plan_tree: too many work items");

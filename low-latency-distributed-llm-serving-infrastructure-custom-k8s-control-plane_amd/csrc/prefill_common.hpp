@@ -75,6 +75,13 @@ __device__ __forceinline__ void dma16_s(uint32_t lds_base, uint32_t voff, const 
                "s"(sbase)
                : "memory", "m0");
 }
+// The same with the streaming hint, for rows that no other workgroup reads.
+__device__ __forceinline__ void dma16_s_nt(uint32_t lds_base, uint32_t voff, const void* sbase) {
+  sbase = uniform_ptr(sbase);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds_base), "v"(voff),
+               "s"(sbase)
+               : "memory", "m0");
+}
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");

@@ -44,7 +44,7 @@ constexpr int kIdAhead = 8;      // stages between an id slot's copy and the sta
 template <typename T, int D, int DM, bool LANE_IDS, bool APPEND, bool CODES = false, int SPAN = kSpanAll>
 __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a) {
   constexpr bool TREE = SPAN == kSpanTree;
-  constexpr int kItemInts = TREE ? 4 : 2;
+  constexpr int kItemInts = TREE ? kTreeItemInts : 2;
   static_assert(SPAN == kSpanAll || !APPEND, "their rows are written before");
   static_assert(Elem<T>::kBytes == 2, "16-bit rows (bf16 or fp16)");
   static_assert(!CODES || (!LANE_IDS && !APPEND), "8-bit copies take any block size; their rows are written before");
@@ -294,8 +294,9 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
       span = stage_span(seen_lo, kv_end, a.sinks, kStage);
       nstages = span.count;
       if constexpr (TREE) {
-        stage0 = split * a.split_stages;
-        nstages = min(nstages - stage0, a.split_stages);
+        const TreeSplit cut = tree_split(nstages, a.split_stages);
+        stage0 = split * cut.stages;
+        nstages = min(nstages - stage0, cut.stages);
         if (seq < 0 || nstages <= 0) ntok = 0;
       }
     }

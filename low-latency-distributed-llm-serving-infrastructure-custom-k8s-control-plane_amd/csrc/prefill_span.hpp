@@ -20,6 +20,8 @@ static hipError_t launch_prefill_span_d(const PrefillArgs& args, int group, int6
   const dim3 grid(static_cast<uint32_t>(cus > 0 ? std::min<int64_t>(a.num_units, cus) : a.num_units));
   if (a.key_scales != nullptr)
     hipLaunchKernelGGL((prefill_kernel<T, D, DM, false, false, true, SPAN>), grid, dim3(kPrefillThreads), 0, s, a);
+  else if constexpr (SPAN == kSpanTree)
+    return hipErrorNotSupported;  // (tree_attention.hip)
   else if ((1 << a.log2_block_size) >= kCopyRows)
     hipLaunchKernelGGL((prefill_kernel<T, D, DM, false, false, false, SPAN>), grid, dim3(kPrefillThreads), 0, s, a);
   else

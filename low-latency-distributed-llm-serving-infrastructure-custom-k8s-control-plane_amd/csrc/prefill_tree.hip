@@ -1,4 +1,4 @@
-// The matrix-core prefill's instances for trees of drafted tokens.
+// The matrix-core prefill's instances for trees of drafted tokens over 8-bit caches.
 #include "prefill_span.hpp"
 
 namespace pa {

@@ -74,10 +74,35 @@ PA_HOST_DEVICE StageSpan tree_span(int start, int nodes, int window, int sinks, 
   return stage_span(window_start(start, window), start + nodes, sinks, stage);
 }
 
-// Whether the matrix-core kernel of trees (prefill.hip, prefill_f32.hip) serves
-// the shape: its tiles of prefill_tile_for() nodes walk stages of kTreeStage
-// positions.
+// Whether the matrix-core kernels of trees (tree_attention.hip, and prefill.hip
+// over 8-bit caches) serve the shape: (dtype: the cache's; 8-bit codes
+// under 16-bit queries); its tiles walk stages of kTreeStage positions.
 constexpr int kTreeStage = 64;
+// Query rows of a tile over 16-bit caches, heads of up to 128; nodes of a tile of
+// any shape (dtype: the cache's).
+constexpr int kTreeRows = 64;
+int tree_tile_for(int dtype, int head_dim, int group);
+// A tile's stages in runs of at most `most`, as even as whole stages allow.
+struct TreeSplit {
+  int runs, stages;
+};
+PA_HOST_DEVICE TreeSplit tree_split(int count, int most) {
+  TreeSplit t;
+  t.runs = count > 0 ? (count - 1) / most + 1 : 0;
+  t.stages = t.runs > 0 ? (count - 1) / t.runs + 1 : 1;
+  return t;
+}
+// An item of a tree's work list: sequence (-1: an entry that is not needed), tile,
+// run of stages, first row of its partial results or -1; first token, nodes,
+// context before the tree and table row of the sequence.
+constexpr int kTreeItemInts = 8;
+// Block ids that the kernel keeps of a run, and the most stages whose columns (and
+// the two more at each end of the sinks' and the window's) they cover.
+constexpr int kTreeIds = 3584;
+PA_HOST_DEVICE int tree_max_stages(int block_size) {
+  const long long n = static_cast<long long>(kTreeIds - 8) * block_size / kTreeStage;
+  return n < (1 << 24) ? static_cast<int>(n) : 1 << 24;
+}
 bool tree_fast_path_supported(int dtype, int head_dim, int group, int block_size);
 
 }  // namespace pa

@@ -16,7 +16,6 @@
 #include <algorithm>
 
 #include "cache8.hpp"
-#include "decode_common.hpp"
 #include "pa_common.hpp"
 #include "pa_launch.hpp"
 #include "span.hpp"
@@ -53,7 +52,7 @@ __device__ __forceinline__ TreeWork tree_work(const PackTreeArgs& a, int start, 
   for (int t0 = 0; t0 < count; t0 += a.tile) {
     const int n = min(a.tile, count - t0);
     const int stages = tree_span(start, t0 + n, a.window, a.sinks, kTreeStage).count;
-    const int splits = (stages + a.split_stages - 1) / a.split_stages;
+    const int splits = tree_split(stages, a.split_stages).runs;
     w.items += splits;
     if (splits > 1) {
       w.merges += 1;
@@ -131,12 +130,16 @@ __global__ __launch_bounds__(kTreeThreads) void pack_tree_kernel(PackTreeArgs a)
   for (int t0 = 0; t0 < s.count; t0 += a.tile) {
     const int n = min(a.tile, s.count - t0);
     const int stages = tree_span(start, t0 + n, a.window, a.sinks, kTreeStage).count;
-    const int splits = (stages + a.split_stages - 1) / a.split_stages;
+    const int splits = tree_split(stages, a.split_stages).runs;
     // (a tile whose partials would not fit is left out: the host sizes them)
     const bool fits = splits == 1 || static_cast<int64_t>(rows) + static_cast<int64_t>(splits) * n <= a.max_partial_rows;
     for (int k = tid; k < splits; k += kTreeThreads)
       if (items + k < a.max_items)
-        a.items[items + k] = make_int4(fits ? seq : -1, t0 / a.tile, k, splits > 1 ? rows + k * n : -1);
+      {
+        int4* item = a.items + 2 * static_cast<int64_t>(items + k);
+        item[0] = make_int4(fits ? seq : -1, t0 / a.tile, k, splits > 1 ? rows + k * n : -1);
+        item[1] = make_int4(static_cast<int>(s.first), s.count, start, a.rows != nullptr ? a.rows[seq] : seq);
+      }
     if (splits > 1) {
       if (tid == 0 && merges < a.max_merge_items)
         a.merge_items[merges] = make_int4(fits ? seq : -1, t0 / a.tile, splits, rows);
@@ -146,35 +149,69 @@ __global__ __launch_bounds__(kTreeThreads) void pack_tree_kernel(PackTreeArgs a)
     items += splits;
   }
   if (seq == a.num_seqs - 1) {
-    for (int64_t i = items + tid; i < a.max_items; i += kTreeThreads) a.items[i] = make_int4(-1, 0, 0, -1);
+    for (int64_t i = items + tid; i < a.max_items; i += kTreeThreads) a.items[2 * i] = make_int4(-1, 0, 0, -1);
     for (int64_t i = merges + tid; i < a.max_merge_items; i += kTreeThreads) a.merge_items[i] = make_int4(-1, 0, 0, 0);
   }
 }
 
-// A workgroup a node of a split tile: four elements of one head a thread, by
-// the arithmetic of the decode's merge.
+// A thread four elements of one head of a node of a split tile, kMergeRuns
+// partials a round trip with a running maximum (the stored maxima are in the exp2
+// domain); slots past the last partial read it again and get no weight.  The
+// partials are in L2 or beside it: what counts is the number of round trips, so
+// the loads of a batch go out together and a node's heads spread over workgroups
+// (26 nodes of 32 heads of 128 in 24 runs: one workgroup a node, eight partials a
+// trip 13.2 us).
+constexpr int kMergeRuns = 16;
 template <typename T, int D>
 __global__ __launch_bounds__(kTreeThreads) void merge_tree_kernel(MergeTreeArgs a) {
   const int64_t m = blockIdx.x / a.tile;
   const int tok = static_cast<int>(blockIdx.x - m * a.tile);
   const int4 item = a.merge_items[m];
-  if (item.x < 0) return;
+  const int r = blockIdx.y * kTreeThreads + threadIdx.x;
+  const int hq = a.num_query_heads;
+  if (item.x < 0 || r >= hq * (D / 4)) return;
   const int64_t first = a.cu_seqlens[item.x];
   const int64_t count = min<int64_t>(a.cu_seqlens[item.x + 1], a.num_query_tokens) - first;
   const int64_t t0 = static_cast<int64_t>(item.y) * a.tile;
   const int n = static_cast<int>(min<int64_t>(a.tile, count - t0));
   if (tok >= n) return;
-  const int hq = a.num_query_heads;
-  constexpr int RUN = D / kMergeOutputs;
-  const int64_t row = static_cast<int64_t>(item.w) + tok;
-  T* out = reinterpret_cast<T*>(a.output) + (first + t0 + tok) * hq * D;
-  for (int r = threadIdx.x; r < hq * RUN; r += kTreeThreads) {
-    const int h = r / RUN;
-    const int e = h * D + (r - h * RUN);
-    merge_partials<T, kMergeOutputs>(a.part_ml + (row * hq + h) * 2, a.part_acc + row * hq * D + e, RUN,
-                                     2 * static_cast<int64_t>(hq) * n, static_cast<int64_t>(hq) * D * n, 0, item.z, -1,
-                                     item.z, out + e);
+  const int h = r / (D / 4);
+  const int64_t row = (static_cast<int64_t>(item.w) + tok) * hq + h;  // of the first run, n * hq rows apart
+  const int64_t step = static_cast<int64_t>(hq) * n;
+  const float4* acc = reinterpret_cast<const float4*>(a.part_acc) + row * (D / 4) + (r - h * (D / 4));
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row;
+  float mx = kScoreFloor, sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p = 0; p < item.z; p += kMergeRuns) {
+    float2 s[kMergeRuns];
+    float4 x[kMergeRuns];
+#pragma unroll
+    for (int u = 0; u < kMergeRuns; ++u) {
+      const int64_t at = min(p + u, item.z - 1) * step;
+      s[u] = ml[at];
+      x[u] = acc[at * (D / 4)];
+    }
+    float mn = mx;
+#pragma unroll
+    for (int u = 0; u < kMergeRuns; ++u) mn = fmaxf(mn, s[u].x);
+    const float keep = fast_exp2(mx - mn);
+    sum *= keep;
+    o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll
+    for (int u = 0; u < kMergeRuns; ++u) {
+      const float w = p + u < item.z ? fast_exp2(s[u].x - mn) : 0.f;
+      if (p + u < item.z) {
+        sum = fmaf(s[u].y, w, sum);
+        o = make_float4(fmaf(x[u].x, w, o.x), fmaf(x[u].y, w, o.y), fmaf(x[u].z, w, o.z), fmaf(x[u].w, w, o.w));
+      }
+    }
+    mx = mn;
   }
+  // (a sum of zero is a row that attends nothing, whose result is zero; a NaN stays)
+  T* out = reinterpret_cast<T*>(a.output) + (first + t0 + tok) * hq * D + static_cast<int64_t>(r) * 4;
+  const float e[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) store_scalar<T>(out + i, sum != 0.f ? e[i] / sum : 0.f);
 }
 
 // One wave a sequence: at each node the lanes look for its first child (they
@@ -371,6 +408,7 @@ hipError_t launch_merge_t(const MergeTreeArgs& a, int head_dim, dim3 grid, hipSt
     case 64: hipLaunchKernelGGL((merge_tree_kernel<T, 64>), grid, dim3(kTreeThreads), 0, s, a); break;
     case 80: hipLaunchKernelGGL((merge_tree_kernel<T, 80>), grid, dim3(kTreeThreads), 0, s, a); break;
     case 96: hipLaunchKernelGGL((merge_tree_kernel<T, 96>), grid, dim3(kTreeThreads), 0, s, a); break;
+    case 256: hipLaunchKernelGGL((merge_tree_kernel<T, 256>), grid, dim3(kTreeThreads), 0, s, a); break;
     case 128: hipLaunchKernelGGL((merge_tree_kernel<T, 128>), grid, dim3(kTreeThreads), 0, s, a); break;
     default: return hipErrorNotSupported;
   }
@@ -411,7 +449,8 @@ hipError_t launch_keep_rows(const KeepRowsArgs& a, hipStream_t stream) {
 
 hipError_t launch_merge_tree(const MergeTreeArgs& a, int dtype, int head_dim, hipStream_t stream) {
   if (a.num_merge <= 0) return hipSuccess;
-  const dim3 grid(static_cast<uint32_t>(a.num_merge * a.tile));
+  const int threads = a.num_query_heads * (head_dim / 4);
+  const dim3 grid(static_cast<uint32_t>(a.num_merge * a.tile), (threads + kTreeThreads - 1) / kTreeThreads);
   if (dtype == PA_DTYPE_F32) return launch_merge_t<float>(a, head_dim, grid, stream);
   if (dtype == PA_DTYPE_BF16) return launch_merge_t<bf16_t>(a, head_dim, grid, stream);
   if (dtype == PA_DTYPE_F16) return launch_merge_t<f16_t>(a, head_dim, grid, stream);

@@ -1814,9 +1814,9 @@ class TreeStep:
         step, device = self.step, self._buffer.device
         with _current(device):
             status = _native.load_library().pa_pack_tree(
-                self.parents.data_ptr(), step.ptr("context_lens"), step.ptr("cu_seqlens"), self._dims, self._plan,
-                self.ptr("masks"), self.ptr("positions"), self.ptr("items"), self.ptr("merge_items"),
-                _stream(device))
+                self.parents.data_ptr(), step.ptr("context_lens"), step.ptr("cu_seqlens"),
+                step.ptr("rows") if step._pooled else None, self._dims, self._plan, self.ptr("masks"),
+                self.ptr("positions"), self.ptr("items"), self.ptr("merge_items"), _stream(device))
         _native.check(status, "pa_pack_tree")
 
     def repack(self, parents=None) -> None:
@@ -1880,7 +1880,7 @@ def pack_tree(
     ``parents``: one integer per new token, an int32 device tensor (kept and read
     by every later run) or anything that becomes one: the index, within its
     sequence, of an earlier node, or -1 for a root; anything else counts as -1.
-    Up to 1024 nodes a tree.  The head counts, head dim and query ``dtype`` the
+    Up to 1024 nodes a tree.  The head counts, head dim and cache ``dtype`` the
     attention will have are by default those the step was packed for (a step of
     no known ``head_dim`` gets no work lists: give them here).  ``window`` /
     ``sinks``: of the layers that attend through this tree (at least the largest
@@ -1892,8 +1892,6 @@ def pack_tree(
     hq = int(num_query_heads or (heads[1] if num_kv_heads is None else 4 * hkv))
     dim = int(head_dim or heads[2] or 0)
     dtype = dtype or heads[3] or torch.float32
-    if dtype == CODE_DTYPE:
-        dtype = torch.bfloat16  # (the lists are those of any query)
     limits = (0, 0)
     if window is not None:
         limits = _window_of(window, sinks)
@@ -1902,14 +1900,14 @@ def pack_tree(
     device = step.buffer.device
     dims = _native.PaTreeDims(
         num_seqs=step.num_seqs, num_query_tokens=step.num_query_tokens, num_query_heads=hq if dim else 0,
-        num_kv_heads=hkv if dim else 0, head_dim=dim, dtype=dtype_code(dtype), block_size=step.block_size,
+        num_kv_heads=hkv if dim else 0, head_dim=dim, dtype=cache_dtype_code(dtype), block_size=step.block_size,
         compute_units=_compute_units(device), window=_native.PaWindow(*limits))
     plan = _plan_tree(step, dims, 0)
     parents = _parents(step, parents)
     layout = _Layout()
     layout.add("masks", torch.int32, (step.num_query_tokens, int(plan.mask_words)))
     layout.add("positions", torch.int64, (step.num_query_tokens,))
-    layout.add("items", torch.int32, (int(plan.num_items), 4))
+    layout.add("items", torch.int32, (int(plan.num_items), 8))
     layout.add("merge_items", torch.int32, (int(plan.num_merge_items), 4))
     layout.add("workspace", torch.uint8, (decode_workspace_bytes(int(plan.num_partial_rows), hq, dim),))
     buffer = torch.empty(layout.nbytes, dtype=torch.uint8, device=device)
