@@ -742,7 +742,6 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
   const int cache_eb = scales != nullptr ? 1 : eb;
   const bool fast =
       ordered_scaling(scaling) &&
-      (window.window == 0 || pa::prefill_window_supported(dims.dtype, dims.head_dim)) &&
       pa::prefill_fast_path_supported(dims.dtype, dims.head_dim, group, dims.block_size) &&
       (scales == nullptr || pa::prefill_codes_supported(dims.dtype, dims.head_dim)) &&
       prefill_tile == pa::prefill_tile_for(group) && dims.max_blocks_per_seq > 0 &&

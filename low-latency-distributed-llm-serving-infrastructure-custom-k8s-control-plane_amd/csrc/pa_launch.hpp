@@ -399,8 +399,6 @@ bool prefill_fast_path_supported(int dtype, int head_dim, int group, int block_s
 bool prefill_append_supported(int dtype, int head_dim);
 // Whether the fast path of this shape also reads an 8-bit cache.
 bool prefill_codes_supported(int dtype, int head_dim);
-// Whether the fast path of this shape also takes a window.
-bool prefill_window_supported(int dtype, int head_dim);
 // Compute units of the current device (cached per device; 0 if unknown): the
 // width of the persistent prefill launches.
 int device_compute_units();

@@ -305,9 +305,10 @@ struct TreeCost {
   int slots;                  // workgroups resident on a CU
 };
 TreeCost tree_cost(int dtype, int head_dim) {
-  const double row = head_dim * (dtype == PA_DTYPE_E4M3 ? 1 : 2) / 256.0;
+  const double row = head_dim * (dtype == PA_DTYPE_E4M3 ? 1 : dtype == PA_DTYPE_F32 ? 4 : 2) / 256.0;
+  if (dtype == PA_DTYPE_F32) return {8.4, 4.4 * row, 1.53 * row, 1};  // (prefill_f32.hip's)
   if (dtype == PA_DTYPE_E4M3) return {10.0, 1.1, 1.53 * row, 1};  // (prefill.hip's kernel: a CU each)
-  if (head_dim == 256) return {8.4, 2.6, 1.53 * row, 1};
+  if (head_dim == 256) return {8.4, 2.9, 1.53 * row, 1};
   return head_dim == 64 ? TreeCost{8.4, 1.2, 4.6 * row, 3} : TreeCost{8.4, 1.85, 3.06 * row, 2};
 }
 int32_t choose_split(const Trees& t, const PaTreeDims& d) {

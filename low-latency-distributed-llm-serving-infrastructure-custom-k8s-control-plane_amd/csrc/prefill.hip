@@ -110,15 +110,9 @@ bool prefill_fast_path_supported(int dtype, int head_dim, int group, int block_s
   return true;
 }
 
-bool prefill_window_supported(int dtype, int head_dim) {
-  return (dtype == PA_DTYPE_BF16 || dtype == PA_DTYPE_F16) &&
-         (head_dim == 64 || head_dim == 80 || head_dim == 96 || head_dim == 128);
-}
-
 bool tree_fast_path_supported(int dtype, int head_dim, int group, int block_size) {
   if (dtype == PA_DTYPE_E4M3) return head_dim <= 128 && prefill_fast_path_supported(PA_DTYPE_BF16, head_dim, group, block_size);
-  return (dtype == PA_DTYPE_BF16 || dtype == PA_DTYPE_F16) &&
-         prefill_fast_path_supported(dtype, head_dim, group, block_size);
+  return prefill_fast_path_supported(dtype, head_dim, group, block_size);
 }
 
 bool prefill_append_supported(int dtype, int head_dim) {
@@ -191,13 +185,13 @@ static hipError_t launch_prefill_t(const PrefillArgs& a, int group, int64_t num_
 hipError_t launch_prefill(const PrefillArgs& a, int dtype, int head_dim, int group,
                           int64_t num_items, hipStream_t stream) {
   if (num_items <= 0) return hipSuccess;
+  if (dtype == PA_DTYPE_F32) return launch_prefill_f32(a, head_dim, group, num_items, stream);
   if (a.masks != nullptr)
     return a.key_scales != nullptr ? launch_prefill_tree(a, dtype, head_dim, group, num_items, stream)
                                    : launch_tree_attention(a, dtype, head_dim, group, num_items, stream);
-  if (a.window > 0) return launch_prefill_window(a, dtype, head_dim, group, num_items, stream);
-  if (dtype == PA_DTYPE_F32) return launch_prefill_f32(a, head_dim, group, num_items, stream);
   if (head_dim == 256)
     return a.new_key != nullptr ? hipErrorNotSupported : launch_prefill256(a, dtype, group, num_items, stream);
+  if (a.window > 0) return launch_prefill_window(a, dtype, head_dim, group, num_items, stream);
   if (dtype == PA_DTYPE_BF16) {
     if (head_dim == 128) return launch_prefill_t<bf16_t, 128, 128>(a, group, num_items, stream);
     if (head_dim == 96) return launch_prefill_t<bf16_t, 128, 96>(a, group, num_items, stream);

@@ -29,6 +29,7 @@
 #include "pa_common.hpp"
 #include "pa_launch.hpp"
 #include "prefill_common.hpp"
+#include "span.hpp"
 
 namespace pa {
 
@@ -54,7 +55,8 @@ constexpr int kIdSlotBytes = 256;
 constexpr int kIdAhead = 8;
 constexpr int kLdsBytes = kIdBase + kIdSlots * kIdSlotBytes;
 
-template <typename T, bool LANE_IDS>
+// WINDOW: a window with sinks, as in prefill_kernel.hpp.
+template <typename T, bool LANE_IDS, bool WINDOW>
 __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
   static_assert(Elem<T>::kBytes == 2, "16-bit caches (bf16 or fp16)");
   __shared__ __attribute__((aligned(16))) char s_lds[kLdsBytes];
@@ -114,11 +116,30 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
   const int kv_read = static_cast<int>(
       min(static_cast<int64_t>(kv_end), static_cast<int64_t>(bt_stride) << log2_bs));
   const int kv_last = kv_read - 1;
-  const int nstages = (kv_end + kTile - 1) / kTile;
+  int nstages = (kv_end + kTile - 1) / kTile;
+  // WINDOW: the context without what no query of the tile sees, [seen_lo, ...) and
+  // [0, seen_sinks), in whole stages.
+  [[maybe_unused]] StageSpan span{0, 0, 0};
+  [[maybe_unused]] int seen_lo = 0, seen_sinks = 0;
+  if constexpr (WINDOW) {
+    seen_lo = window_start(start + tok0, a.window);
+    seen_sinks = min(a.sinks, seen_lo);
+    span = stage_span(seen_lo, kv_end, a.sinks, kTile);
+    nstages = span.count;
+  }
+  auto stage_at = [&](int x) { return (!WINDOW || x < span.sinks ? x : x + span.gap) * kTile; };
   const float scale = a.scale_log2e;
   const int last_col = bt_stride - 1;
-  const int ncols = (kv_read + bs_mask) >> log2_bs;
-  int scan0 = tid < ncols ? btg[tid] : 0;
+  // (WINDOW: the columns of seen positions, of the sinks first.)
+  int ncols = (kv_read + bs_mask) >> log2_bs;
+  [[maybe_unused]] int nsink = 0, seen_col = 0;
+  if constexpr (WINDOW) {
+    nsink = (min(seen_sinks, kv_read) + bs_mask) >> log2_bs;
+    seen_col = seen_lo >> log2_bs;
+    ncols = nsink + max(0, ncols - seen_col);
+  }
+  auto scan_col = [&](int c) { return !WINDOW || c < nsink ? c : seen_col + (c - nsink); };
+  int scan0 = tid < ncols ? btg[scan_col(tid)] : 0;
   bool bad_ids = false;
 
   // ---- copies (wave cw copies rows [8 cw, 8 cw + 8) of a stage) ----------------
@@ -139,7 +160,7 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
     return static_cast<uint32_t>(b) < static_cast<uint32_t>(a.total_blocks) ? static_cast<uint32_t>(b) : 0u;
   };
   const_i32* btc = (const_i32*)(bt);
-  auto col0 = [&](int x) { return min((x * kTile) >> log2_bs, last_col); };
+  auto col0 = [&](int x) { return min(stage_at(x) >> log2_bs, last_col); };
   auto dma_ids = [&](int x) {
     const int c0 = col0(x);
     dma4_s(lds0 + kIdBase + (x & (kIdSlots - 1)) * kIdSlotBytes,
@@ -155,7 +176,7 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
   };
   const int id_last = btc[min(kv_last >> log2_bs, last_col)];
   auto copy_each = [&](int x, uint32_t region, const char* base, auto get_id) {
-    const int p0 = x * kTile + cw * kCopyRows;
+    const int p0 = stage_at(x) + cw * kCopyRows;
     const uint32_t dst0 = lds0 + region + cw * kCopyRows * kRowBytes;
     if constexpr (!LANE_IDS) {
 #pragma unroll
@@ -178,7 +199,7 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
 #pragma unroll
       for (int j = 0; j < kDmaPerWave; ++j) {
         pos[j] = min(p0 + j * kRowsPerDma + delta, kv_last);
-        b[j] = pos[j] >= x * kTile ? ring_id(x, pos[j]) : id_last;
+        b[j] = pos[j] >= stage_at(x) ? ring_id(x, pos[j]) : id_last;
       }
 #pragma unroll
       for (int j = 0; j < kDmaPerWave; ++j)
@@ -189,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
   };
 
   auto copy_step = [&](int x, uint32_t region, const char* base, int id_fast) {
-    const int p0 = x * kTile + cw * kCopyRows;
+    const int p0 = stage_at(x) + cw * kCopyRows;
     if (!LANE_IDS && one_block && p0 + kCopyRows - 1 <= kv_last) {
       const uint32_t bb = valid_block(__builtin_amdgcn_readfirstlane(id_fast));
       const char* src = base + (static_cast<uint64_t>(bb) * block_bytes +
@@ -209,7 +230,7 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
   for (int x = 0; x < 4; ++x)
 #pragma unroll
     for (int j = 0; j < kDmaPerWave; ++j)
-      first_ids[x][j] = btc[min(x * kTile + cw * kCopyRows + j * kRowsPerDma, kv_last) >> log2_bs];
+      first_ids[x][j] = btc[min(stage_at(x) + cw * kCopyRows + j * kRowsPerDma, kv_last) >> log2_bs];
   auto copy_prologue = [&](int x, uint32_t region, const char* base) {
     copy_each(x, region, base, [&](int j, int) { return first_ids[x][j]; });
   };
@@ -251,7 +272,20 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
   };
 
   const int kv_lim = min(qpos, kv_last);
+  [[maybe_unused]] const int row_lo = WINDOW ? window_start(qpos, a.window) : 0;
   auto mask_tile = [&](int t, f32x16& s) {
+    if constexpr (WINDOW) {
+      const int at = stage_at(t) + 4 * half;
+      // (what is computed for a stage past the last counts for nothing)
+      const int lim = t < nstages ? kv_lim - at : -1;
+      const int low = row_lo - at, sink = a.sinks - at;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int o = 8 * (i >> 2) + (i & 3);
+        s[i] = (o > lim) | ((o < low) & (o >= sink)) ? -INFINITY : s[i];
+      }
+      return;
+    }
     const int lim = kv_lim - (t * kTile + 4 * half);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -260,7 +294,7 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
   // (bad_ids only: behind the interleaved phases, and the tile's maximum, which
   // counts no such position, is taken again)
   auto missing = [&](int t) {  // (a lane a position; past the last one, as the copies, that one)
-    int p = t * kTile;
+    int p = stage_at(t);
     asm volatile("" : "+s"(p));  // (kept scalar, and the stage with it)
     const int b = btg[min(p + (lane & 31), kv_last) >> log2_bs];
     return static_cast<uint32_t>(b) >= static_cast<uint32_t>(a.total_blocks);
@@ -274,8 +308,19 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
   // Their V rows (block 0's, which may hold anything) become zeros, as a NaN or
   // an infinity outlives a weight of zero.  Every wave clears the tile's rows
   // itself before it reads them.
+  // (WINDOW: so do the rows between the sinks and the first window; a stage that
+  // has some is in a masked step.)
+  [[maybe_unused]] auto has_hole = [&](int t) {
+    return WINDOW && stage_at(t) < seen_lo && stage_at(t) + kTile > seen_sinks;
+  };
   auto clear_bad = [&](int t, int slot) {
-    if (missing(t)) {
+    bool gone = false;
+    if constexpr (WINDOW) {
+      const int p = stage_at(t) + (lane & 31);
+      gone = p >= seen_sinks && p < seen_lo;
+    }
+    if (bad_ids) gone = gone || missing(t);
+    if (gone) {
       char* row = s_lds + kVBase + slot * kRegion + (lane & 31) * kRowBytes + half * (kRowBytes / 2);
 #pragma unroll 1
       for (int i = 0; i < kRowBytes / 32; ++i) st16(row + 16 * i, make_uint4(0, 0, 0, 0));
@@ -332,7 +377,7 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
   asm volatile("" : "+v"(scan0));
   int bad_local = static_cast<uint32_t>(scan0) >= static_cast<uint32_t>(a.total_blocks) ? 1 : 0;
   for (int c = tid + kThreads; c < ncols; c += kThreads)
-    bad_local |= static_cast<uint32_t>(btg[c]) >= static_cast<uint32_t>(a.total_blocks) ? 1 : 0;
+    bad_local |= static_cast<uint32_t>(btg[scan_col(c)]) >= static_cast<uint32_t>(a.total_blocks) ? 1 : 0;
   bad_ids = __syncthreads_or(bad_local) != 0;
   const int first_masked = bad_ids ? 0 : min(start + tok0 + 1, kv_read) / kTile;
   copy_prologue(3, 3 * kRegion, kbase);
@@ -359,7 +404,7 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
     constexpr bool MASKED = decltype(masked)::value;
     constexpr int SLOT = decltype(slot_c)::value;
     copy_step(st + 4, SLOT * kRegion, kbase, idk);
-    if (MASKED && bad_ids) clear_bad(st, SLOT);
+    if (MASKED && (bad_ids || has_hole(st))) clear_bad(st, SLOT);
 
     // ---- A: S_next = K_next Q^T | P = exp2(S - m)
     const float msc = m * scale;
@@ -426,8 +471,20 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
   using S1 = std::integral_constant<int, 1>;
   using S2 = std::integral_constant<int, 2>;
   using S3 = std::integral_constant<int, 3>;
-  const int n_main = min(max(first_masked - 1, 0), nstages);
+  int n_main = min(max(first_masked - 1, 0), nstages);
   int st = 0;
+  if constexpr (WINDOW) {
+    // Whole stages that every row sees: from the last row's window on, to the first
+    // row's limit.
+    const int from = (window_start(start + tok0 + ntok - 1, a.window) + kTile - 1) / kTile - span.gap;
+    n_main = bad_ids ? 0 : min(max(first_masked - span.gap - 1, 0), nstages - 1);
+    for (; st < from && st + 3 < nstages; st += 4) {
+      step(st, s0, s1, M{}, S0{});
+      step(st + 1, s1, s0, M{}, S1{});
+      step(st + 2, s0, s1, M{}, S2{});
+      step(st + 3, s1, s0, M{}, S3{});
+    }
+  }
   for (; st + 3 < n_main; st += 4) {
     step(st, s0, s1, U{}, S0{});
     step(st + 1, s1, s0, U{}, S1{});
@@ -463,13 +520,13 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
     }
 }
 
-template <typename T>
+template <typename T, bool WINDOW>
 hipError_t launch_t(const PrefillArgs& a, int64_t num_items, hipStream_t s) {
   const dim3 grid(static_cast<uint32_t>(num_items * a.num_kv_heads * a.sub_groups));
   if ((1 << a.log2_block_size) >= kRowsPerDma)
-    hipLaunchKernelGGL((prefill256_kernel<T, false>), grid, dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((prefill256_kernel<T, false, WINDOW>), grid, dim3(kThreads), 0, s, a);
   else
-    hipLaunchKernelGGL((prefill256_kernel<T, true>), grid, dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((prefill256_kernel<T, true, WINDOW>), grid, dim3(kThreads), 0, s, a);
   return hipGetLastError();
 }
 
@@ -478,8 +535,10 @@ hipError_t launch_t(const PrefillArgs& a, int64_t num_items, hipStream_t s) {
 hipError_t launch_prefill256(const PrefillArgs& a, int dtype, int group, int64_t num_items, hipStream_t stream) {
   const int g = group / a.sub_groups;
   if (g < 1 || g > 8) return hipErrorNotSupported;
-  if (dtype == PA_DTYPE_BF16) return launch_t<bf16_t>(a, num_items, stream);
-  if (dtype == PA_DTYPE_F16) return launch_t<f16_t>(a, num_items, stream);
+  if (dtype == PA_DTYPE_BF16)
+    return a.window > 0 ? launch_t<bf16_t, true>(a, num_items, stream) : launch_t<bf16_t, false>(a, num_items, stream);
+  if (dtype == PA_DTYPE_F16)
+    return a.window > 0 ? launch_t<f16_t, true>(a, num_items, stream) : launch_t<f16_t, false>(a, num_items, stream);
   return hipErrorNotSupported;
 }
 

@@ -12,6 +12,7 @@
 #include "pa_common.hpp"
 #include "pa_launch.hpp"
 #include "prefill_common.hpp"
+#include "span.hpp"
 
 namespace pa {
 
@@ -54,8 +55,11 @@ __device__ __forceinline__ f32x16 mfma_f32(float a, float b, f32x16 c) {
 // stores its own tile's rows from the stage buffers into the cache while
 // each stage is in LDS (their block ids staged in LDS once per unit), so no
 // unit reads a row another one writes.
-template <int D, bool APPEND>
+// SPAN: a window with sinks, or trees of drafted tokens, as in prefill_kernel.hpp.
+template <int D, bool APPEND, int SPAN>
 __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArgs a) {
+  constexpr bool TREE = SPAN == kSpanTree;
+  static_assert(SPAN == kSpanAll || !APPEND, "their rows are written before");
   constexpr int ROWB = D * 4;                  // bytes of a K or V row
   constexpr int CH = D / 4;                    // 16-byte chunks of a row
   constexpr int DB = D / 32;                   // 32-wide d blocks of the output
@@ -110,16 +114,19 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
     const int unit = (U - 1 - rank) - item * units;
     const int kvh = unit / a.sub_groups;
     const int h0 = kvh * a.group + (unit - kvh * a.sub_groups) * G;  // first query head
-    const int seq = a.items[2 * item];
-    const int qt = a.items[2 * item + 1];
-    const int64_t first = a.cu_seqlens[seq];
-    const int count = static_cast<int>(a.cu_seqlens[seq + 1] - first);
-    const int ctx = a.context_lens[seq];
-    const int start = ctx - count;
+    const int32_t* rec = a.items + static_cast<int64_t>(item) * (TREE ? kTreeItemInts : 2);
+    const int seq = rec[0];
+    const int qt = rec[1];
+    if (TREE && seq < 0) continue;  // (an entry that the list does not need; the whole workgroup)
+    const int64_t first = TREE ? rec[4] : a.cu_seqlens[seq];
+    const int count = TREE ? rec[5] : static_cast<int>(a.cu_seqlens[seq + 1] - first);
+    const int start = TREE ? rec[6] : a.context_lens[seq] - count;
+    const int ctx = start + count;
     const int tok0 = qt * MTOK;
     const int ntok = min(MTOK, count - tok0);
     if (ntok <= 0) continue;  // (the whole workgroup)
-    const int64_t trow = a.rows != nullptr ? a.rows[seq] : seq;
+    const int64_t trow = TREE ? rec[7] : a.rows != nullptr ? a.rows[seq] : seq;
+    [[maybe_unused]] const int part_row = TREE ? rec[3] : -1;
     const bool row_ok = trow >= 0 && trow < a.num_table_rows;
     const int32_t* bt = a.block_tables + (row_ok ? trow * a.block_table_stride : 0);
     const int bt_stride = row_ok ? a.block_table_stride : 1;
@@ -143,17 +150,53 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
     const int kv_read = static_cast<int>(
         min(static_cast<int64_t>(kv_end), static_cast<int64_t>(bt_stride) << log2_bs));
     const int kv_last = kv_read - 1;
-    const int nstages = (kv_end + kFmStage - 1) / kFmStage;
+    int nstages = (kv_end + kFmStage - 1) / kFmStage;
+    // SPAN: the context without what no query of the tile sees, [seen_lo, ...) and
+    // [0, seen_sinks), in whole stages; TREE: a run of them.
+    [[maybe_unused]] StageSpan span{0, 0, 0};
+    [[maybe_unused]] int seen_lo = 0, seen_sinks = 0, stage0 = 0;
+    if constexpr (SPAN != kSpanAll) {
+      static_assert(kFmStage == kTreeStage, "the stages of the work lists");
+      seen_lo = TREE ? min(window_start(start, a.window), start) : window_start(start + tok0, a.window);
+      seen_sinks = min(a.sinks, seen_lo);
+      span = stage_span(seen_lo, kv_end, a.sinks, kFmStage);
+      nstages = span.count;
+      if constexpr (TREE) {
+        const TreeSplit cut = tree_split(nstages, a.split_stages);
+        stage0 = rec[2] * cut.stages;
+        nstages = min(nstages - stage0, cut.stages);
+        if (nstages <= 0) continue;
+      }
+    }
+    auto stage_at = [&](int x) {
+      if constexpr (SPAN == kSpanAll) return x * kFmStage;
+      const int at = x + stage0;
+      return (at < span.sinks ? at : at + span.gap) * kFmStage;
+    };
+    auto hidden = [&](int p) { return SPAN != kSpanAll && p >= seen_sinks && p < seen_lo; };
     const bool live = tok < ntok && g < G;
     const int qpos = start + tok0 + tok;  // causal limit (inclusive)
     const int lim = min(qpos, kv_last);
+    // SPAN: where the row's window starts (and the tile's last one); TREE: its mask.
+    [[maybe_unused]] int row_lo = 0, last_lo = 0;
+    [[maybe_unused]] const uint32_t* row_mask = nullptr;
+    if constexpr (SPAN == kSpanWindow) {
+      row_lo = window_start(qpos, a.window);
+      last_lo = window_start(start + tok0 + ntok - 1, a.window);
+    }
+    if constexpr (TREE) {
+      const int64_t node = first + tok0 + (live ? tok : 0);
+      if (a.window > 0) row_lo = min(window_start(static_cast<int>(a.positions[node]), a.window), start);
+      last_lo = min(window_start(start + count - 1, a.window), start);
+      row_mask = a.masks + node * a.mask_words;
+    }
 
     // Block ids of the rows this lane copies in stage x; -1 without a row.
     int ids[kCopies];
     auto load_ids = [&](int x) {
 #pragma unroll
       for (int c = 0; c < kCopies; ++c) {
-        const int p = min(x * kFmStage + kWaves * 0 + 8 * wave + c * RPC + crow, kv_last);
+        const int p = min(stage_at(x) + 8 * wave + c * RPC + crow, kv_last);
         ids[c] = row_ok ? bt[p >> log2_bs] : -1;
       }
     };
@@ -173,7 +216,7 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
 #pragma unroll
       for (int c = 0; c < kCopies; ++c) {
         const int R = 8 * wave + c * RPC + cr;
-        const int pc = min(x * kFmStage + R, kv_last);
+        const int pc = min(stage_at(x) + R, kv_last);
         const int piece = (cp ^ chunk_swizzle<CH>(R)) * 16;
         const uint32_t dst = lds0 + b * kBufBytes + (8 * wave + c * RPC) * ROWB;
         src_of(c, pc, piece, dst);
@@ -229,9 +272,17 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
     // every tile.
     bool bad_ids;
     {
-      const int ncols = (kv_read + bs_mask) >> log2_bs;
+      // (SPAN: of the seen positions of the unit's stages.)
+      int first_col = 0, ncols = (kv_read + bs_mask) >> log2_bs;
       bool bad = !row_ok;
-      for (int col = lane; col < ncols && row_ok; col += kWave)
+      if constexpr (SPAN != kSpanAll) {
+        const int s0 = stage0 * kFmStage, s1 = min(min(seen_sinks, s0 + nstages * kFmStage), kv_read);
+        for (int col = (s0 >> log2_bs) + lane; col < (s1 + bs_mask) >> log2_bs && row_ok; col += kWave)
+          bad |= static_cast<uint32_t>(bt[col]) >= static_cast<uint32_t>(a.total_blocks);
+        first_col = max(seen_lo, stage_at(0)) >> log2_bs;
+        ncols = (min(kv_read, stage_at(nstages - 1) + kFmStage) + bs_mask) >> log2_bs;
+      }
+      for (int col = first_col + lane; col < ncols && row_ok; col += kWave)
         bad |= static_cast<uint32_t>(bt[col]) >= static_cast<uint32_t>(a.total_blocks);
       bad_ids = __builtin_amdgcn_ballot_w64(bad) != 0;
     }
@@ -255,7 +306,7 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
         issue(st + 1, b ^ 1);
         if (st + 2 < nstages) load_ids(st + 2);
       }
-      const int p0 = st * kFmStage + kh * kFmTile;  // the tile's first position
+      const int p0 = stage_at(st) + kh * kFmTile;  // the tile's first position
       if (p0 <= kv_last) {  // (wave-uniform: a tile past the context adds nothing)
         const char* kb = s_lds + b * kBufBytes + k_off;
         f32x16 s;
@@ -291,18 +342,32 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
         // here: gated as `p > lim || (bad_ids && ...)`, this ROCm's hipcc
         // emitted the -INF write on the `p > lim` path only, and positions in
         // out-of-pool blocks kept their scores.
-        if (bad_ids || p0 + kFmTile - 1 > min(start + tok0, kv_last)) {
+        bool edge = bad_ids || p0 + kFmTile - 1 > min(start + tok0, kv_last);
+        if constexpr (SPAN != kSpanAll) edge |= p0 < last_lo;
+        if constexpr (TREE) edge |= p0 + kFmTile > start;
+        if (edge) {
           // (every id read first, then one select per score)
           const int32_t* sid = s_sid[b] + kh * kFmTile + 4 * h;
           int4 idq[4];
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) idq[q4] = *reinterpret_cast<const int4*>(sid + 8 * q4);
+          [[maybe_unused]] uint32_t bits = ~0u;  // TREE: of the lane's positions, from p0 + 4 h on
+          if constexpr (TREE) {
+            if (p0 + kFmTile > start) {
+              const int n = p0 + 4 * h - start;
+              auto word = [&](int w) { return w < 0 ? ~0u : w < a.mask_words ? row_mask[w] : 0u; };
+              bits = static_cast<uint32_t>(
+                  ((static_cast<uint64_t>(word((n >> 5) + 1)) << 32) | word(n >> 5)) >> (n & 31));
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int tt = 8 * (i >> 2) + 4 * h + (i & 3);
             const int4 q = idq[i >> 2];
             const int id = (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
-            const bool off = (p0 + tt > lim) | (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.total_blocks));
+            bool off = (p0 + tt > lim) | (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.total_blocks));
+            if constexpr (SPAN != kSpanAll) off |= (p0 + tt < row_lo) & (p0 + tt >= a.sinks);
+            if constexpr (TREE) off |= ((bits >> (8 * (i >> 2) + (i & 3))) & 1u) == 0;
             s[i] = off ? -INFINITY : s[i];
           }
         }
@@ -333,7 +398,9 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
         // The V rows of out-of-pool blocks (block 0's, which may hold anything)
         // become zeros, as a NaN or an infinity outlives a weight of zero.  Each
         // wave clears the rows of its tile itself before it reads them.
-        if (bad_ids && static_cast<uint32_t>(s_sid[b][k_row]) >= static_cast<uint32_t>(a.total_blocks)) {
+        // (SPAN: so do those that no row of the unit sees.)
+        if ((bad_ids && static_cast<uint32_t>(s_sid[b][k_row]) >= static_cast<uint32_t>(a.total_blocks)) ||
+            hidden(p0 + t)) {
 #pragma unroll 1
           for (int i = 0; i < ROWB / 32; ++i)
             st16(vb + k_row * ROWB + h * (ROWB / 2) + 16 * i, make_uint4(0, 0, 0, 0));
@@ -407,6 +474,9 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
         const float a1 = fast_exp2((m - mm) * scale);
         const float a2 = fast_exp2((ml.x - mm) * scale);
         const float lt = l * a1 + ml.y * a2;
+        [[maybe_unused]] const int64_t prow = (static_cast<int64_t>(part_row) + tok) * hq + h0 + g;
+        if (TREE && part_row >= 0 && live && h == 0)
+          *reinterpret_cast<float2*>(a.part_ml + prow * 2) = make_float2(mm * scale, lt);
         const float inv = lt > 0.f ? 1.f / lt : 0.f;
         float* orow = reinterpret_cast<float*>(a.output) +
                       ((first + tok0 + tok) * hq + h0 + g) * static_cast<int64_t>(D) + 4 * h;
@@ -415,6 +485,13 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {
             const float4 o2 = *reinterpret_cast<const float4*>(region + db * 16 + 4 * q4);
+            if (TREE && part_row >= 0) {  // one of a tile's runs: the sums as they are, for merge_tree_kernel
+              if (live)
+                *reinterpret_cast<float4*>(a.part_acc + prow * D + db * 32 + 8 * q4 + 4 * h) =
+                    make_float4(acc[db][4 * q4] * a1 + o2.x * a2, acc[db][4 * q4 + 1] * a1 + o2.y * a2,
+                                acc[db][4 * q4 + 2] * a1 + o2.z * a2, acc[db][4 * q4 + 3] * a1 + o2.w * a2);
+              continue;
+            }
             const float4 o = make_float4((acc[db][4 * q4] * a1 + o2.x * a2) * inv,
                                          (acc[db][4 * q4 + 1] * a1 + o2.y * a2) * inv,
                                          (acc[db][4 * q4 + 2] * a1 + o2.z * a2) * inv,
@@ -429,7 +506,7 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
   }
 }
 
-template <int D, bool APPEND>
+template <int D, bool APPEND, int SPAN = kSpanAll>
 static hipError_t launch_prefill_f32_mfma(const PrefillArgs& args, int group, int64_t num_items,
                                           hipStream_t s) {
   const int g = group / args.sub_groups;
@@ -442,7 +519,7 @@ static hipError_t launch_prefill_f32_mfma(const PrefillArgs& args, int group, in
   // over its share of the units; fewer units than CUs run one each.
   const int cus = device_compute_units();
   const int64_t wgs = cus > 0 ? std::min<int64_t>(a.num_units, cus) : a.num_units;
-  hipLaunchKernelGGL((prefill_f32_mfma_kernel<D, APPEND>), dim3(static_cast<uint32_t>(wgs)), dim3(kFmThreads), 0, s,
+  hipLaunchKernelGGL((prefill_f32_mfma_kernel<D, APPEND, SPAN>), dim3(static_cast<uint32_t>(wgs)), dim3(kFmThreads), 0, s,
                      a);
   return hipGetLastError();
 }
@@ -451,6 +528,14 @@ hipError_t launch_prefill_f32(const PrefillArgs& a, int head_dim, int group, int
                               hipStream_t stream) {
   if (num_items <= 0) return hipSuccess;
   const bool append = a.new_key != nullptr;
+  if (a.masks != nullptr || a.window > 0) {
+    if (append || (head_dim != 64 && head_dim != 128)) return hipErrorNotSupported;
+    if (a.masks != nullptr)
+      return head_dim == 128 ? launch_prefill_f32_mfma<128, false, kSpanTree>(a, group, num_items, stream)
+                             : launch_prefill_f32_mfma<64, false, kSpanTree>(a, group, num_items, stream);
+    return head_dim == 128 ? launch_prefill_f32_mfma<128, false, kSpanWindow>(a, group, num_items, stream)
+                           : launch_prefill_f32_mfma<64, false, kSpanWindow>(a, group, num_items, stream);
+  }
   if (head_dim == 128)
     return append ? launch_prefill_f32_mfma<128, true>(a, group, num_items, stream)
                   : launch_prefill_f32_mfma<128, false>(a, group, num_items, stream);

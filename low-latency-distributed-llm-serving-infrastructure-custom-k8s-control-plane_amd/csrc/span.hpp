@@ -74,8 +74,8 @@ PA_HOST_DEVICE StageSpan tree_span(int start, int nodes, int window, int sinks, 
   return stage_span(window_start(start, window), start + nodes, sinks, stage);
 }
 
-// Whether the matrix-core kernels of trees (tree_attention.hip, and prefill.hip
-// over 8-bit caches) serve the shape: (dtype: the cache's; 8-bit codes
+// Whether the matrix-core kernels of trees (tree_attention.hip; over 8-bit and fp32
+// caches prefill.hip and prefill_f32.hip) serve the shape: (dtype: the cache's; 8-bit codes
 // under 16-bit queries); its tiles walk stages of kTreeStage positions.
 constexpr int kTreeStage = 64;
 // Query rows of a tile over 16-bit caches, heads of up to 128; nodes of a tile of

@@ -391,7 +391,7 @@ hipError_t launch_t(const PrefillArgs& a, int head_dim, dim3 grid, hipStream_t s
 
 int tree_tile_for(int dtype, int head_dim, int group) {
   const int g = group / decode_sub_groups(group);
-  return (dtype == PA_DTYPE_E4M3 || head_dim == 256 ? prefill_tile_for(group) : kTreeRows / g);
+  return dtype == PA_DTYPE_E4M3 || dtype == PA_DTYPE_F32 || head_dim == 256 ? prefill_tile_for(group) : kTreeRows / g;
 }
 
 hipError_t launch_tree_attention(const PrefillArgs& a, int dtype, int head_dim, int group, int64_t num_items,
