@@ -1772,40 +1772,32 @@ def _attention_window(query, key_cache, value_cache, layer_idx, step, scaling, o
 
 
 class TreeStep:
-    """The trees of a step (what pa_pack_tree writes), in one device allocation.
+    """The trees of a step (what pa_pack_tree writes).
 
     ``masks`` int32 [T, words]: bit j % 32 of word j // 32 of a node's row is set
     where node j of its sequence is the node itself or one of its ancestors.
     ``position_ids`` int64 [T]: the sequence's start plus the node's depth.  The
-    attention's work lists and the workspace of its partial results are kept
-    beside them; calls that share a tree must not overlap in time.
+    masks, the attention's work lists and the workspace of its partial results are kept
+    in one buffer; calls that share a tree must not overlap in time.
     """
 
-    def __init__(self, step: PackedStep, parents: torch.Tensor, dims, plan, head_shape, window, sinks, buffer,
-                 layout) -> None:
+    def __init__(self, step: PackedStep, parents: torch.Tensor, dims, plan, heads, limits, position_ids, buffer,
+                 offsets, workspace_bytes) -> None:
         self.step = step
         self.parents = parents
-        self.window = window
-        self.sinks = sinks
-        self._dims, self._plan, self._heads = dims, plan, head_shape
-        self._buffer, self._layout = buffer, layout
+        self.position_ids = position_ids
+        self.window, self.sinks = limits
+        self._dims, self._plan, self._heads = dims, plan, heads
+        self._buffer = buffer
+        base = buffer.data_ptr()
+        self._masks, self._items, self._merge_items, self._workspace = (base + at for at in offsets)
+        self._workspace_bytes = workspace_bytes
         self._packs = -1
-
-    def _view(self, name: str) -> torch.Tensor:
-        off, dtype, shape = self._layout.fields[name]
-        count = int(np.prod(shape))
-        return self._buffer[off : off + count * _ELEM[dtype]].view(dtype).view(shape)
 
     @property
     def masks(self) -> torch.Tensor:
-        return self._view("masks")
-
-    @property
-    def position_ids(self) -> torch.Tensor:
-        return self._view("positions")
-
-    def ptr(self, name: str) -> int:
-        return self._buffer.data_ptr() + self._layout.fields[name][0]
+        shape = (self.step.num_query_tokens, int(self._plan.mask_words))
+        return self._buffer[: 4 * shape[0] * shape[1]].view(torch.int32).view(shape)
 
     def rerun(self) -> None:
         """Rerun the packing kernel on the parents and the step's lengths as they
@@ -1815,8 +1807,8 @@ class TreeStep:
         with _current(device):
             status = _native.load_library().pa_pack_tree(
                 self.parents.data_ptr(), step.ptr("context_lens"), step.ptr("cu_seqlens"),
-                step.ptr("rows") if step._pooled else None, self._dims, self._plan, self.ptr("masks"),
-                self.ptr("positions"), self.ptr("items"), self.ptr("merge_items"), _stream(device))
+                step.ptr("rows") if step._pooled else None, self._dims, self._plan, self._masks,
+                self.position_ids.data_ptr(), self._items, self._merge_items, _stream(device))
         _native.check(status, "pa_pack_tree")
 
     def repack(self, parents=None) -> None:
@@ -1837,25 +1829,25 @@ class TreeStep:
 def _parents(step: PackedStep, parents) -> torch.Tensor:
     """int32 [T] parents on the step's device."""
     t = parents if isinstance(parents, torch.Tensor) else torch.as_tensor(np.asarray(parents, dtype=np.int64))
+    device = step.buffer.device
+    if t.dtype == torch.int32 and t.device == device and t.numel() == step.num_query_tokens and t.is_contiguous():
+        return t
     if t.dtype.is_floating_point or t.dtype == torch.bool or t.numel() != step.num_query_tokens:
         raise ValueError(f"parents must be one integer per new token ({step.num_query_tokens}), got {tuple(t.shape)} "
                          f"of {t.dtype}")
-    if t.is_cuda and t.device != step.buffer.device:
-        raise RuntimeError(f"tensors on different devices: {step.buffer.device} and {t.device}")
+    if t.is_cuda and t.device != device:
+        raise RuntimeError(f"tensors on different devices: {device} and {t.device}")
     if t.dtype != torch.int32:
         t = t.clamp(-1, _INT32_MAX).to(torch.int32)  # (no larger value is a parent)
-    if not t.is_cuda:
-        t = t.to(step.buffer.device)
-    return t.reshape(-1).contiguous()
+    return t.to(device).reshape(-1).contiguous()
 
 
 def _plan_tree(step: PackedStep, dims, split_stages: int):
     plan = _native.PaTreePlan()
-    planned = _native.PaTreeDims.from_buffer_copy(dims)
-    planned.split_stages = split_stages
+    dims.split_stages = split_stages
     starts, counts, _ = step._inputs
     lib = _native.load_library()
-    status = lib.pa_plan_tree(starts.ctypes.data, counts.ctypes.data, planned, ctypes.byref(plan))
+    status = lib.pa_plan_tree(starts.ctypes.data, counts.ctypes.data, dims, ctypes.byref(plan))
     if status != _native.PA_OK:
         if plan.bad_seq >= 0:
             raise ValueError(lib.pa_last_error_message().decode(errors="replace"))
@@ -1898,20 +1890,21 @@ def pack_tree(
     elif sinks:
         raise ValueError("sinks go with a window")
     device = step.buffer.device
-    dims = _native.PaTreeDims(
-        num_seqs=step.num_seqs, num_query_tokens=step.num_query_tokens, num_query_heads=hq if dim else 0,
-        num_kv_heads=hkv if dim else 0, head_dim=dim, dtype=cache_dtype_code(dtype), block_size=step.block_size,
-        compute_units=_compute_units(device), window=_native.PaWindow(*limits))
+    tokens = step.num_query_tokens
+    dims = _native.PaTreeDims(  # (in the order of its fields)
+        step.num_seqs, tokens, hq if dim else 0, hkv if dim else 0, dim, cache_dtype_code(dtype), step.block_size,
+        _compute_units(device), 0, _native.PaWindow(*limits))
     plan = _plan_tree(step, dims, 0)
     parents = _parents(step, parents)
-    layout = _Layout()
-    layout.add("masks", torch.int32, (step.num_query_tokens, int(plan.mask_words)))
-    layout.add("positions", torch.int64, (step.num_query_tokens,))
-    layout.add("items", torch.int32, (int(plan.num_items), 8))
-    layout.add("merge_items", torch.int32, (int(plan.num_merge_items), 4))
-    layout.add("workspace", torch.uint8, (decode_workspace_bytes(int(plan.num_partial_rows), hq, dim),))
-    buffer = torch.empty(layout.nbytes, dtype=torch.uint8, device=device)
-    tree = TreeStep(step, parents, dims, plan, (hkv, hq, dim) if dim else None, *limits, buffer, layout)
+    # masks | items | merge items | workspace
+    items = _align(4 * tokens * plan.mask_words)
+    merge_items = items + _align(32 * plan.num_items)
+    workspace = merge_items + _align(16 * plan.num_merge_items)
+    workspace_bytes = decode_workspace_bytes(plan.num_partial_rows, hq, dim)
+    buffer = torch.empty(workspace + workspace_bytes, dtype=torch.uint8, device=device)
+    position_ids = torch.empty(tokens, dtype=torch.int64, device=device)
+    tree = TreeStep(step, parents, dims, plan, (hkv, hq, dim) if dim else None, limits, position_ids, buffer,
+                    (0, items, merge_items, workspace), workspace_bytes)
     tree.rerun()
     tree._packs = step._packs
     return tree
@@ -1974,9 +1967,9 @@ def tree_attention(
             strides = (k.stride(0), k.stride(1), v.stride(0), v.stride(1))
         call = _native.PaTreeCall(
             dims=dims, block_tables=step.ptr("block_tables"), context_lens=step.ptr("context_lens"),
-            cu_seqlens=step.ptr("cu_seqlens"), scatter_slots=step.ptr("scatter_slots"), masks=tree.ptr("masks"),
-            positions=tree.ptr("positions"), items=tree.ptr("items"), merge_items=tree.ptr("merge_items"),
-            workspace=tree.ptr("workspace"), workspace_bytes=tree._layout.fields["workspace"][2][0], plan=tree._plan,
+            cu_seqlens=step.ptr("cu_seqlens"), scatter_slots=step.ptr("scatter_slots"), masks=tree._masks,
+            positions=tree.position_ids.data_ptr(), items=tree._items, merge_items=tree._merge_items,
+            workspace=tree._workspace, workspace_bytes=tree._workspace_bytes, plan=tree._plan,
             window=_native.PaWindow(tree.window, tree.sinks))
         cached = (key, ctypes.byref(call), tuple(q.shape), strides)
         tree.__dict__["_layer_call"] = cached
@@ -2013,22 +2006,24 @@ def accept_tree(step: PackedStep, tree: TreeStep, drafted: torch.Tensor, predict
     [T]: the nodes' own tokens, and the model's choice after each.  All on the
     device: nothing is read back."""
     _check_tree(step, tree)
-    device = _require_device(drafted, predicted, step.buffer)
-    for name, t in (("drafted", drafted), ("predicted", predicted)):
-        if t.dtype != torch.int64 or t.numel() != step.num_query_tokens:
-            raise ValueError(f"{name} must be int64 with one entry per new token ({step.num_query_tokens}), got "
-                             f"{tuple(t.shape)} of {t.dtype}")
-    drafted, predicted = drafted.contiguous(), predicted.contiguous()
+    device = step.buffer.device
     t, b = step.num_query_tokens, step.num_seqs
-    path = AcceptedPath(torch.empty(t, dtype=torch.int32, device=device),
-                        torch.empty(b, dtype=torch.int32, device=device),
-                        torch.empty(b, dtype=torch.int64, device=device))
+    for name, x in (("drafted", drafted), ("predicted", predicted)):
+        if x.dtype != torch.int64 or x.numel() != t:
+            raise ValueError(f"{name} must be int64 with one entry per new token ({t}), got {tuple(x.shape)} of "
+                             f"{x.dtype}")
+        if x.device != device:
+            _require_device(x, step.buffer)
+    drafted, predicted = drafted.contiguous(), predicted.contiguous()
+    nodes = torch.empty(t, dtype=torch.int32, device=device)
+    counts = torch.empty(b, dtype=torch.int32, device=device)
+    next_tokens = torch.empty(b, dtype=torch.int64, device=device)
     with _current(device):
         status = _native.load_library().pa_accept_tree(
             tree.parents.data_ptr(), step.ptr("cu_seqlens"), drafted.data_ptr(), predicted.data_ptr(), b, t,
-            path.nodes.data_ptr(), path.counts.data_ptr(), path.next_tokens.data_ptr(), _stream(device))
+            nodes.data_ptr(), counts.data_ptr(), next_tokens.data_ptr(), _stream(device))
     _native.check(status, "pa_accept_tree")
-    return path
+    return AcceptedPath(nodes, counts, next_tokens)
 
 
 def keep_rows(
@@ -2050,32 +2045,37 @@ def keep_rows(
     8-bit cache a block that rows move into takes the largest scale among its own
     and those of the blocks they come from.
     """
-    device = _require_device(key_cache, value_cache, step.buffer, nodes, counts)
-    if key_cache.dim() != 5 or value_cache.shape != key_cache.shape:
-        raise ValueError("caches must be 5-D (layers, blocks, block_size, heads, dim) and alike")
-    if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
-        raise ValueError("caches must be contiguous")
-    if key_cache.dtype != value_cache.dtype:
-        raise ValueError("key and value cache must have the same dtype")
-    if int(key_cache.shape[2]) != step.block_size:
-        raise ValueError(f"the step was packed for blocks of {step.block_size}, the cache has {key_cache.shape[2]}")
-    for name, t, n in (("nodes", nodes, step.num_query_tokens), ("counts", counts, step.num_seqs)):
-        if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 tensor of {n}, got {tuple(t.shape)} of {t.dtype}")
-    if step.num_query_tokens > 0 and step.max_new_tokens > _native.PA_MAX_TREE_NODES:
+    key = (_kind(key_cache), _kind(value_cache), _kind(key_scales), _kind(value_scales), _kind(nodes), _kind(counts))
+    cached = step.__dict__.get("_keep_call")
+    if cached is None or cached[0] != key:
+        _require_device(key_cache, value_cache, step.buffer, nodes, counts)
+        if key_cache.dim() != 5 or value_cache.shape != key_cache.shape:
+            raise ValueError("caches must be 5-D (layers, blocks, block_size, heads, dim) and alike")
+        if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+            raise ValueError("caches must be contiguous")
+        if key_cache.dtype != value_cache.dtype:
+            raise ValueError("key and value cache must have the same dtype")
+        if int(key_cache.shape[2]) != step.block_size:
+            raise ValueError(f"the step was packed for blocks of {step.block_size}, the cache has {key_cache.shape[2]}")
+        for name, t, n in (("nodes", nodes, step.num_query_tokens), ("counts", counts, step.num_seqs)):
+            if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous int32 tensor of {n}, got {tuple(t.shape)} of {t.dtype}")
+        _cache_scales(key_cache, value_cache, key_scales, value_scales)
+        num_layers, total_blocks, block_size, num_kv_heads, head_dim = (int(n) for n in key_cache.shape)
+        dims = _native.PaStepDims(
+            num_seqs=step.num_seqs, num_query_tokens=step.num_query_tokens, num_query_heads=num_kv_heads,
+            num_kv_heads=num_kv_heads, head_dim=head_dim, block_size=block_size, total_blocks=total_blocks,
+            num_layers=num_layers, max_blocks_per_seq=step.table_width, dtype=cache_dtype_code(key_cache.dtype),
+            num_table_rows=step._source_rows, block_table_rows=step.ptr("rows") if step._pooled else None)
+        cached = step.__dict__["_keep_call"] = (key, dims)
+    if step.max_new_tokens > _native.PA_MAX_TREE_NODES:
         raise ValueError(f"a sequence has {step.max_new_tokens} new tokens, a tree at most {_native.PA_MAX_TREE_NODES}")
-    scales = _cache_scales(key_cache, value_cache, key_scales, value_scales)
-    num_layers, total_blocks, block_size, num_kv_heads, head_dim = (int(n) for n in key_cache.shape)
-    dims = _native.PaStepDims(
-        num_seqs=step.num_seqs, num_query_tokens=step.num_query_tokens, num_query_heads=num_kv_heads,
-        num_kv_heads=num_kv_heads, head_dim=head_dim, block_size=block_size, total_blocks=total_blocks,
-        num_layers=num_layers, max_blocks_per_seq=step.table_width, dtype=cache_dtype_code(key_cache.dtype),
-        num_table_rows=step._source_rows, block_table_rows=step.ptr("rows") if step._pooled else None)
+    device = key_cache.device
     with _current(device):
         status = _native.load_library().pa_keep_rows(
-            key_cache.data_ptr(), value_cache.data_ptr(), scales.key if scales else None,
-            scales.value if scales else None, dims, step.ptr("block_tables"), step.ptr("context_lens"),
-            step.ptr("cu_seqlens"), nodes.data_ptr(), counts.data_ptr(), _stream(device))
+            key_cache.data_ptr(), value_cache.data_ptr(), _ptr(key_scales), _ptr(value_scales), cached[1],
+            step.ptr("block_tables"), step.ptr("context_lens"), step.ptr("cu_seqlens"), nodes.data_ptr(),
+            counts.data_ptr(), _stream(device))
     _native.check(status, "pa_keep_rows")
 
 
