@@ -236,6 +236,18 @@ class BlockTablePool:
             if not self._rebuild:
                 self._pending += (row, col, block)
 
+    def truncate(self, row: int, blocks: int) -> None:
+        """Forget a row's blocks from column ``blocks`` on."""
+        with self._lock:
+            n = int(self.blocks[row])
+            if n <= blocks:
+                return
+            if not self._rebuild:
+                for col in range(blocks, n):
+                    self._pending += (row, col, -1)
+            self.host[row, blocks:n] = -1
+            self.blocks[row] = blocks
+
     def take_updates(self):
         """(rebuild, updates): whether the device copy must be rebuilt from
         ``host``, else the int32 [n, 3] triples to apply; clears the queue.
@@ -307,6 +319,19 @@ class SequenceBlockTable:
         self._tokens += n
         if self._pool is not None:
             self._pool.tokens[self.row] = self._tokens
+
+    def truncate(self, n: int) -> None:
+        """Keep the first ``n`` tokens; blocks past them return to the allocator."""
+        if not 0 <= n <= self._tokens:
+            raise ValueError(f"cannot keep {n} of {self._tokens} tokens")
+        keep = -(-n // self._block_size)
+        for block in self._blocks[keep:]:
+            self._allocator.free_block(block)
+        del self._blocks[keep:]
+        self._tokens = n
+        if self._pool is not None and self.row >= 0:
+            self._pool.truncate(self.row, keep)
+            self._pool.tokens[self.row] = n
 
     def append_block(self, block_id: int) -> None:
         self._allocator._validate(block_id)

@@ -339,6 +339,25 @@ class PagedKVCacheManager:
              self.gather_layer_values(layer, slots).permute(1, 0, 2).unsqueeze(0))
             for layer in range(self.num_layers))
 
+    # -- trees of drafted tokens --------------------------------------------------------
+    def keep_accepted(self, context, path) -> List[int]:
+        """End a step of trees (a ``PagedStepContext`` with parents): the K and V
+        rows of each sequence's accepted ``path`` (``paged_ops.accept_tree``) move
+        behind its context, in every layer, and its table keeps the context and
+        those tokens only.  Returns how many tokens each sequence keeps of its tree
+        (the one copy to the host of such a step)."""
+        if not self.on_gpu:
+            raise RuntimeError("keep_accepted needs a store in device memory")
+        step = context.packed
+        if step is None:
+            return []
+        paged_ops.keep_rows(self.key_cache, self.value_cache, step, path.nodes, path.counts, self.key_scales,
+                            self.value_scales)
+        kept = path.counts.tolist()
+        for seq, start, n in zip(context.sequences, context.start_positions, kept):
+            seq.block_table.truncate(start + n)
+        return kept
+
     # -- swap to the host pool -------------------------------------------------------
     def host_pool(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """The pinned host swap space (allocated on first use): K and V of

@@ -58,9 +58,10 @@ class AttentionBackend(ABC):
         ...
 
 
-def dense_sdpa(query, store, layer_idx, context, scaling, dropout) -> torch.Tensor:
+def dense_sdpa(query, store, layer_idx, context, scaling, dropout, window=None) -> torch.Tensor:
     """Gather the step's whole context of one layer into dense [1, H_kv, C, D]
-    K/V and run torch SDPA under the block-diagonal causal mask; returns
+    K/V and run torch SDPA under the context's mask (block-diagonal and causal, or
+    of its window or trees); returns
     [1, T, H_q, D] (the computation of attention_backends.py:55-78 and of the
     inline path paged_attention.py:165-180)."""
     slots = context.gather_slots
@@ -68,7 +69,8 @@ def dense_sdpa(query, store, layer_idx, context, scaling, dropout) -> torch.Tens
     v = store.gather_layer_values(layer_idx, slots).transpose(0, 1).unsqueeze(0)
     out = F.scaled_dot_product_attention(
         query, k, v,
-        attn_mask=context.attention_mask(query.device),
+        attn_mask=context.attention_mask(query.device) if window is None else context.attention_mask(query.device,
+                                                                                                    window),
         dropout_p=dropout,
         scale=scaling,
         enable_gqa=query.shape[1] != k.shape[1],
@@ -85,8 +87,8 @@ class TorchSdpBackend(AttentionBackend):
     def supports(self, context: "PagedStepContext", num_query_tokens: int) -> bool:
         return True
 
-    def attend(self, query, store, layer_idx, context, scaling, dropout):
-        return dense_sdpa(query, store, layer_idx, context, scaling, dropout)
+    def attend(self, query, store, layer_idx, context, scaling, dropout, window=None):
+        return dense_sdpa(query, store, layer_idx, context, scaling, dropout, window)
 
 
 class NativePagedBackend(AttentionBackend):
@@ -101,11 +103,11 @@ class NativePagedBackend(AttentionBackend):
             and context.store.on_gpu
         )
 
-    def attend(self, query, store, layer_idx, context, scaling, dropout, new_key=None, new_value=None):
+    def attend(self, query, store, layer_idx, context, scaling, dropout, new_key=None, new_value=None, window=None):
         """``new_key`` / ``new_value`` ([T, H_kv, D] on the store's device, its
         dtype): the layer's new rows, written into the cache first
         (:func:`paged_ops.attention`); without them the caller has written
-        them."""
+        them.  ``window``: of this layer, with the context's sinks."""
         if context.packed is None:
             if not native_kernel_available():
                 raise RuntimeError(
@@ -119,21 +121,36 @@ class NativePagedBackend(AttentionBackend):
             scales = {"key_scales": store.key_scales, "value_scales": store.value_scales}
         recorder = metrics.current()
         if recorder is None:
-            out = paged_ops.attention(query, store.key_cache, store.value_cache, layer_idx, step, scaling,
-                                      new_key=new_key, new_value=new_value, **scales)
-            return out.unsqueeze(0)
+            return self._launch(query, store, layer_idx, context, step, scaling, new_key, new_value, window,
+                                scales).unsqueeze(0)
         stream = torch.cuda.current_stream(query.device)
         start = recorder.begin(stream)
-        out = paged_ops.attention(query, store.key_cache, store.value_cache, layer_idx, step, scaling,
-                                  new_key=new_key, new_value=new_value, **scales)
-        nbytes = getattr(context, "_attention_bytes", None)
+        out = self._launch(query, store, layer_idx, context, step, scaling, new_key, new_value, window, scales)
+        known = context.__dict__.setdefault("_attention_bytes", {})
+        nbytes = known.get(window)
         if nbytes is None:
-            nbytes = metrics.step_bytes(context.context_lens, context.num_query_tokens, int(query.shape[1]),
-                                        store.num_heads, store.head_dim, store.key_cache.element_size(),
-                                        store.block_size, query.element_size() if scales else 0)
-            context._attention_bytes = nbytes
+            lens = context.context_lens
+            if window is not None:  # what the window of the first new token and the sinks leave
+                lens = [min(c, window + n - 1 + context.sinks) for c, n in zip(lens, context.new_token_counts)]
+            nbytes = known[window] = metrics.step_bytes(
+                lens, context.num_query_tokens, int(query.shape[1]), store.num_heads, store.head_dim,
+                store.key_cache.element_size(), store.block_size, query.element_size() if scales else 0)
         recorder.end(start, nbytes, context.num_query_tokens, stream)
         return out.unsqueeze(0)
+
+    @staticmethod
+    def _launch(query, store, layer_idx, context, step, scaling, new_key, new_value, window, scales):
+        # (a window that no context of the step reaches past is none, but in a
+        # captured launch, which may serve longer contexts)
+        if window is not None and step.max_context <= window and not torch.cuda.is_current_stream_capturing():
+            window = None
+        if getattr(context, "parents", None) is not None:
+            tree = context.tree_for(int(query.shape[1]), window)
+            return paged_ops.tree_attention(query, store.key_cache, store.value_cache, layer_idx, step, tree, scaling,
+                                            new_key=new_key, new_value=new_value, **scales)
+        limits = {} if window is None else {"window": window, "sinks": context.sinks}
+        return paged_ops.attention(query, store.key_cache, store.value_cache, layer_idx, step, scaling,
+                                   new_key=new_key, new_value=new_value, **scales, **limits)
 
 
 _BACKENDS = {

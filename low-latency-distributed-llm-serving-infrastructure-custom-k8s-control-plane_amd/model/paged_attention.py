@@ -58,6 +58,24 @@ def _offsets(counts: np.ndarray) -> torch.Tensor:
     return torch.from_numpy(out)
 
 
+def _depths(parents: List[int]) -> np.ndarray:
+    """int64 [n] depth of each node; a parent that is no earlier node is none."""
+    depth = np.zeros(len(parents), dtype=np.int64)
+    for i, p in enumerate(parents):
+        if 0 <= p < i:
+            depth[i] = depth[p] + 1
+    return depth
+
+
+def _ancestors(parents: List[int]) -> np.ndarray:
+    """bool [n, n]: node j is node i or one of its ancestors."""
+    over = np.eye(len(parents), dtype=bool)
+    for i, p in enumerate(parents):
+        if 0 <= p < i:
+            over[i] |= over[p]
+    return over
+
+
 class PagedStepContext:
     """Slot bookkeeping and attention layout of one engine step
     (paged_attention.py:37-118).
@@ -68,10 +86,19 @@ class PagedStepContext:
     device), num_query_tokens, num_context_tokens.  ``packed`` is the GPU
     description of the step (None on a CPU store).  The host-side lists and
     offsets are built on first use: a GPU step needs none of them.
+
+    ``window`` / ``sinks``: every layer's queries see at most the last ``window``
+    positions and the first ``sinks`` ones (a layer that passes a
+    ``sliding_window`` of its own sees the smaller of the two, and those sinks).
+    ``parents``: one list per sequence, for a step whose new tokens are trees of
+    drafted ones (the index of each node's parent in its sequence's list, -1 for
+    a root); a node's position is then its depth's, and it sees its sequence's
+    context, its ancestors and itself.
     """
 
     def __init__(self, store, sequences: List, start_positions: List[int], new_token_counts: List[int],
-                 prefill_tile: Optional[int] = None) -> None:
+                 prefill_tile: Optional[int] = None, *, window: Optional[int] = None, sinks: int = 0,
+                 parents: Optional[List[List[int]]] = None) -> None:
         if not (len(sequences) == len(start_positions) == len(new_token_counts)):
             raise ValueError(
                 f"sequences ({len(sequences)}), start_positions ({len(start_positions)}) "
@@ -81,7 +108,18 @@ class PagedStepContext:
         self.sequences = sequences if isinstance(sequences, list) else list(sequences)
         self.packed: Optional[paged_ops.PackedStep] = None
         self._gather_slots: Optional[torch.Tensor] = None
-        self._mask: Optional[torch.Tensor] = None
+        self._masks: dict = {}
+        if window is not None and window < 1:
+            raise ValueError(f"window must be a positive number of tokens, got {window}")
+        if sinks < 0:
+            raise ValueError(f"sinks must be a number of tokens, got {sinks}")
+        if parents is not None and [len(p) for p in parents] != [int(c) for c in new_token_counts]:
+            raise ValueError("parents must have one list per sequence with one entry per new token")
+        self.window = window
+        self.sinks = int(sinks)
+        self.parents = parents
+        self._trees: dict = {}
+        self._parents_on: Optional[torch.Tensor] = None  # the parents on the store's device
         self._rows, self._starts, self._counts = store.step_rows(self.sequences, start_positions, new_token_counts)
         if store.on_gpu:
             if self.sequences:
@@ -134,6 +172,27 @@ class PagedStepContext:
                                                partition_size=self.packed.partition_size)
         return self.packed
 
+    def window_of(self, sliding_window: Optional[int]) -> Optional[int]:
+        """The window of a layer that passes ``sliding_window`` (None: none)."""
+        if sliding_window is None or self.window is None:
+            return self.window if sliding_window is None else int(sliding_window)
+        return min(int(sliding_window), self.window)
+
+    def tree_for(self, num_query_heads: int, window: Optional[int] = None) -> paged_ops.TreeStep:
+        """The step's packed trees for layers of ``num_query_heads`` under ``window``."""
+        step = self.packed_for(num_query_heads)
+        tree = self._trees.get((num_query_heads, window))
+        if tree is None or tree.step is not step:
+            if self._parents_on is None:
+                flat = torch.tensor([p for parents in self.parents for p in parents], dtype=torch.int32)
+                self._parents_on = flat.pin_memory().to(step.buffer.device, non_blocking=True)
+            tree = paged_ops.pack_tree(step, self._parents_on, num_kv_heads=self.store.num_heads,
+                                       num_query_heads=num_query_heads, head_dim=self.store.head_dim,
+                                       dtype=self.store.dtype, window=window,
+                                       sinks=self.sinks if window is not None else 0)
+            self._trees[(num_query_heads, window)] = tree
+        return tree
+
     @property
     def gather_slots(self) -> torch.Tensor:
         """int64 [C]: slots of every context token, sequence by sequence."""
@@ -155,33 +214,49 @@ class PagedStepContext:
     def position_ids(self, device: torch.device) -> torch.Tensor:
         """[1, T] positions, restarting at every sequence boundary."""
         if self.packed is not None and torch.device(device) == self.packed.buffer.device:
+            if self.parents is not None:
+                return self.tree_for(int(self.store.num_query_heads or self.store.num_heads)).position_ids.unsqueeze(0)
             return self.packed.position_ids.unsqueeze(0)
         counts = np.asarray(self.new_token_counts, dtype=np.int64)
         total = int(counts.sum()) if counts.size else 0
         owner = np.repeat(np.arange(counts.size), counts)
         first = self.cu_seqlens.numpy()[:-1]
-        pos = np.arange(total, dtype=np.int64) - first[owner] + np.asarray(self.start_positions, np.int64)[owner]
+        inside = np.arange(total, dtype=np.int64) - first[owner]
+        if self.parents is not None and total:
+            inside = np.concatenate([_depths(p) for p in self.parents])
+        pos = inside + np.asarray(self.start_positions, np.int64)[owner]
         return torch.from_numpy(pos).to(device).unsqueeze(0)
 
-    def attention_mask(self, device: torch.device) -> torch.Tensor:
+    def attention_mask(self, device: torch.device, window: Optional[int] = None) -> torch.Tensor:
         """Block-diagonal causal mask, bool (1, 1, T, C), True = attended:
         query token i of sequence s (position start_s + i) sees context
         position j of the same sequence when j <= start_s + i.
 
+        Under a window it sees those with position - j < window or j < sinks, and
+        the nodes of a tree see, of the new tokens, their ancestors and themselves.
+
         Only the SDPA path materialises it; the HIP kernels evaluate the same
         rule from cu_seqlens and context_lens."""
         device = torch.device(device)
-        if self._mask is not None and self._mask.device == device:
-            return self._mask
+        mask = self._masks.get((device, window))
+        if mask is not None:
+            return mask
         q_seq = torch.repeat_interleave(torch.arange(len(self.new_token_counts)),
                                         torch.tensor(self.new_token_counts, dtype=torch.long))
         c_seq = torch.repeat_interleave(torch.arange(len(self.context_lens)),
                                         torch.tensor(self.context_lens, dtype=torch.long))
         q_pos = self.position_ids(torch.device("cpu"))[0]
         c_pos = torch.arange(self.num_context_tokens) - self.cu_context_offsets[c_seq]
-        mask = (q_seq[:, None] == c_seq[None, :]) & (c_pos[None, :] <= q_pos[:, None])
-        self._mask = mask[None, None].to(device)
-        return self._mask
+        own = q_seq[:, None] == c_seq[None, :]
+        mask = own & (c_pos[None, :] <= q_pos[:, None])
+        if window is not None:
+            mask &= (q_pos[:, None] - c_pos[None, :] < window) | (c_pos[None, :] < self.sinks)
+        if self.parents is not None:
+            first, end = self.cu_seqlens.tolist(), self.cu_context_offsets.tolist()
+            for i, parents in enumerate(self.parents):
+                mask[first[i]:first[i + 1], end[i + 1] - len(parents):end[i + 1]] = torch.from_numpy(_ancestors(parents))
+        mask = self._masks[(device, window)] = mask[None, None].to(device)
+        return mask
 
 
 def _default_backend(store):
@@ -210,13 +285,19 @@ def paged_attention_forward(
     """Per-layer hook (paged_attention.py:138-180): write the layer's new K/V
     into the paged blocks, then attend through the installed backend.  A CPU
     store falls back to SDPA for shapes the backend refuses, or runs the
-    inline SDPA path with none installed; a GPU store runs the HIP kernels."""
+    inline SDPA path with none installed; a GPU store runs the HIP kernels.
+
+    ``sliding_window``, which transformers hands over for layers that have one,
+    limits the layer to that window (the context's ``window`` limits every layer,
+    and its ``sinks`` stay visible in both)."""
     context: PagedStepContext = module.paged_context
     store = context.store
     layer_idx = module.layer_idx
     # [1, H_kv, T, D] projections -> [T, H_kv, D] views (no copy)
     new_key, new_value = key[0].transpose(0, 1), value[0].transpose(0, 1)
     scale = module.scaling if scaling is None else scaling
+    window = context.window_of(kwargs.get("sliding_window"))
+    limits = {} if window is None else {"window": window}
     backend = _BACKEND if _BACKEND is not None else _default_backend(store)
     if store.on_gpu:
         from .attention_backends import NativePagedBackend
@@ -231,15 +312,15 @@ def paged_attention_forward(
         # step of single-token sequences) before it attends.
         new_key, new_value = store.checked_layer_kv(layer_idx, new_key, new_value, context.num_query_tokens)
         return backend.attend(query, store, layer_idx, context, scale, dropout, new_key=new_key,
-                              new_value=new_value), None
+                              new_value=new_value, **limits), None
     store.scatter_layer_kv(layer_idx, new_key, new_value, context.scatter_slots)
     if backend is not None:
         if not backend.supports(context, query.shape[2]):
             backend = _get_fallback_backend()
-        return backend.attend(query, store, layer_idx, context, scale, dropout), None
+        return backend.attend(query, store, layer_idx, context, scale, dropout, **limits), None
     from .attention_backends import dense_sdpa
 
-    return dense_sdpa(query, store, layer_idx, context, scale, dropout), None
+    return dense_sdpa(query, store, layer_idx, context, scale, dropout, **limits), None
 
 
 def _decoder(model) -> torch.nn.Module:
