@@ -112,17 +112,33 @@ tree_attention_kernel(PrefillArgs a) {
   // Whether no other workgroup reads the rows, nor part of their 128-byte lines.
   const bool alone = a.sub_groups == 1 && run.count <= kRows / G && MEM_ROW % 128 == 0;
   auto piece_in = [&](int j) { return !MASKD || chunk_off[j] < MEM_ROW; };
+  // Where a tile's rows lie: offsets of its two halves from the tensors' bases when
+  // each is within a block and all its rows are the context's; else row by row.
+  struct Place {
+    uint64_t at[2];
+    int p0;
+    bool whole;
+  };
+  auto place_of = [&](int t) {
+    Place w;
+    w.p0 = run.tile_at(t);
+    w.whole = log2_bs >= 4 && w.p0 + kTreeKvTile - 1 <= run.kv_last;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int p = w.p0 + 16 * s;
+      const uint32_t b = max(__builtin_amdgcn_readfirstlane(id_at(t, p)), 0);
+      w.at[s] = static_cast<uint64_t>(b) * block_bytes + static_cast<uint32_t>(p & bs_mask) * row_bytes;
+    }
+    return w;
+  };
   // Rows past the readable context repeat its last one, and a missing block reads
   // block 0 (their scores are masked, the latter's V rows cleared).
-  auto copy = [&](int t, uint32_t region, const char* base) {
-    const int p0 = run.tile_at(t);
+  auto copy = [&](int t, const Place& w, uint32_t region, const char* base) {
     const uint32_t dst0 = lds0 + region;
-    if (log2_bs >= 4 && p0 + kTreeKvTile - 1 <= run.kv_last) {
+    if (w.whole) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const int p = p0 + 16 * s;
-        const uint32_t b = max(__builtin_amdgcn_readfirstlane(id_at(t, p)), 0);
-        const char* src = base + (static_cast<uint64_t>(b) * block_bytes + static_cast<uint32_t>(p & bs_mask) * row_bytes);
+        const char* src = base + w.at[s];
         if (alone) {
 #pragma unroll
           for (int j = 0; j < kHalfCopies; ++j)
@@ -138,7 +154,7 @@ tree_attention_kernel(PrefillArgs a) {
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int j = 0; j < kHalfCopies; ++j) {
-          const int pos = min(p0 + 16 * s + j * kRowsPerDma + delta, run.kv_last);
+          const int pos = min(w.p0 + 16 * s + j * kRowsPerDma + delta, run.kv_last);
           const uint32_t b = max(id_at(t, pos), 0);
           if (piece_in(j))
             dma16(dst0 + (s * kHalfCopies + j) * (kWave * 16),
@@ -163,6 +179,12 @@ tree_attention_kernel(PrefillArgs a) {
       const int col = 16 * ((lane >> 4) & 1) + 4 * (li & 3) + 32 * db;
       v_off[db][hi] = kVBase + r * ROW_BYTES + (((col >> 3) ^ chunk_swizzle<CHUNKS>(r)) * 16) + (col & 7) * 2;
     }
+
+  // The accumulators leave the matrix registers within a rescale alone (left to
+  // itself, the compiler copies all of them at each tile, for the case of one).
+  auto in_matrix_registers = [](f32x16& x) {
+    if constexpr (D > 64) asm("" : "+a"(x));
+  };
 
   // The unit with its live blocks of rows, NB of two.
   auto attend = [&](auto blocks) {
@@ -195,8 +217,10 @@ tree_attention_kernel(PrefillArgs a) {
       // Row pieces past the head are never copied: zero them before any copy lands.
       for (int i = tid; i < kWaves * kWaveBytes / 16; i += kThreads) st16(s_lds + 16 * i, make_uint4(0, 0, 0, 0));
     }
-    // (also waits for the query and the masks, which no copy then follows)
     const bool bad_ids = __syncthreads_or(bad ? 1 : 0) != 0;
+    // The query and the masks arrive before the copies go out: a wait for them in the
+    // loop would be one for the copies behind them (the compiler sees this wait).
+    __builtin_amdgcn_s_waitcnt(kWaitLoads);
 
     f32x16 acc[NB][DB];
     float m[NB], l[NB];  // l: this lane's half of the row sum
@@ -213,16 +237,18 @@ tree_attention_kernel(PrefillArgs a) {
     const int n = (run.ntiles - wave + kWaves - 1) / kWaves;  // tiles of this wave
     const int from = run.from(a.window), to = run.to();
     if (n > 0) {
-      copy(wave, 0, kbase);
-      copy(wave, kVBase, vbase);
+      const Place w = place_of(wave);
+      copy(wave, w, 0, kbase);
+      copy(wave, w, kVBase, vbase);
     }
     if (n > 1) {
-      copy(wave + kWaves, kRegion, kbase);
-      copy(wave + kWaves, kVBase + kRegion, vbase);
+      const Place w = place_of(wave + kWaves);
+      copy(wave + kWaves, w, kRegion, kbase);
+      copy(wave + kWaves, w, kVBase + kRegion, vbase);
     }
-    for (int i = 0; i < n; ++i) {
+    auto step = [&](int i, auto which) {  // (tile i of the wave, in slot i & 1)
+      constexpr int slot = decltype(which)::value * kRegion;
       const int t = wave + i * kWaves;
-      const int slot = (i & 1) * kRegion;
       const int next = i + 1 < n ? 1 : 0, after = i + 2 < n ? 1 : 0;
       const bool edge = bad_ids || t < from || t >= to;
       // K of this tile (V of it and both of the next may be in flight).
@@ -230,6 +256,7 @@ tree_attention_kernel(PrefillArgs a) {
       uint4 ka[KS];
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) ka[ks] = *reinterpret_cast<const uint4*>(ring + slot + k_off[ks]);
+      const Place w = place_of(t + 2 * kWaves);  // (past the run: some place in it, not used)
       f32x16 s[NB];
 #pragma unroll
       for (int b = 0; b < NB; ++b)
@@ -240,7 +267,7 @@ tree_attention_kernel(PrefillArgs a) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) s[b] = mfma32<T>(ka[ks], qreg[b][ks], s[b]);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the slot has been read)
-      if (after) copy(t + 2 * kWaves, slot, kbase);
+      if (after) copy(t + 2 * kWaves, w, slot, kbase);
       uint4 pb[NB][2];
       if (edge) {
         uint32_t gone = 0;
@@ -257,6 +284,27 @@ tree_attention_kernel(PrefillArgs a) {
           }
         }
       }
+      // V of this tile (both of the next and K of the one after may be in flight).
+      wait_vmcnt_at_most<3 * kCopies>(kCopies * (2 * next + after));
+      if (edge && (bad_ids || run.has_hole(t))) {
+        const int p = run.tile_at(t) + (lane & 31);
+        if (run.hidden(p) || (bad_ids && id_at(t, min(p, run.kv_last)) < 0)) {
+          char* r = ring + kVBase + slot + (lane & 31) * ROW_BYTES + half * (ROW_BYTES / 2);
+#pragma unroll 1
+          for (int j = 0; j < ROW_BYTES / 32; ++j) st16(r + 16 * j, make_uint4(0, 0, 0, 0));
+        }
+      }
+      // (its operands are read while the softmax runs)
+      uint4 va[DB][2];
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          const char* base = ring + slot + kk * 16 * ROW_BYTES;
+          const uint2 lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(base + v_off[db][0]));
+          const uint2 hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(base + v_off[db][1]));
+          va[db][kk] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         // The reference maximum moves only when a tile's maximum exceeds it by more
@@ -268,9 +316,12 @@ tree_attention_kernel(PrefillArgs a) {
           const float alpha = fast_exp2((m[b] - m_new) * scale);
           l[b] *= alpha;
 #pragma unroll
-          for (int db = 0; db < DB; ++db)
+          for (int db = 0; db < DB; ++db) {
+            in_matrix_registers(acc[b][db]);
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[b][db][j] *= alpha;
+            in_matrix_registers(acc[b][db]);
+          }
           m[b] = m_new;
         }
         const float msc = m[b] * scale;
@@ -290,29 +341,18 @@ tree_attention_kernel(PrefillArgs a) {
         }
         l[b] += sum0 + sum1;
       }
-      // V of this tile (both of the next and K of the one after may be in flight).
-      wait_vmcnt_at_most<3 * kCopies>(kCopies * (2 * next + after));
-      if (edge && (bad_ids || run.has_hole(t))) {
-        const int p = run.tile_at(t) + (lane & 31);
-        if (run.hidden(p) || (bad_ids && id_at(t, min(p, run.kv_last)) < 0)) {
-          char* r = ring + kVBase + slot + (lane & 31) * ROW_BYTES + half * (ROW_BYTES / 2);
-#pragma unroll 1
-          for (int j = 0; j < ROW_BYTES / 32; ++j) st16(r + 16 * j, make_uint4(0, 0, 0, 0));
-        }
-      }
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          const char* base = ring + slot + kk * 16 * ROW_BYTES;
-          const uint2 lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(base + v_off[db][0]));
-          const uint2 hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(base + v_off[db][1]));
-          const uint4 va = make_uint4(lo.x, lo.y, hi.x, hi.y);
-#pragma unroll
-          for (int b = 0; b < NB; ++b) acc[b][db] = mfma32<T>(va, pb[b][kk], acc[b][db]);
-        }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (after) copy(t + 2 * kWaves, kVBase + slot, vbase);
+      if (after) copy(t + 2 * kWaves, w, kVBase + slot, vbase);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int b = 0; b < NB; ++b) acc[b][db] = mfma32<T>(va[db][kk], pb[b][kk], acc[b][db]);
+    };
+    for (int i = 0; i < n; i += 2) {
+      step(i, std::integral_constant<int, 0>());
+      if (i + 1 < n) step(i + 1, std::integral_constant<int, 1>());
     }
 
     // ---- the four waves of each row joined ---------------------------------------
