@@ -110,6 +110,20 @@ __device__ __forceinline__ int chunk_swizzle(int r) {
   else return 4 * ((r >> 1) & 1) + ((r >> 2) & 3);
 }
 
+// The lowest n bits (none for n <= 0, all from 32 on).
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n > 0 ? (1u << n) - 1u : 0u; }
+
+// Scores of a lane's positions that it does not see, by the bits of those that it
+// does: score i is at position 8 (i / 4) + i % 4 from the lane's first (two
+// instructions a score; comparisons with each limit took up to nine).
+__device__ __forceinline__ void hide(f32x16& s, uint32_t seen) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t on = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(seen), 8 * (i >> 2) + (i & 3), 1));
+    s[i] = __uint_as_float((on & __float_as_uint(s[i])) | (~on & 0xff800000u));
+  }
+}
+
 constexpr float kLazyRescale = 8.f;  // log2 headroom before a row maximum moves
 
 }  // namespace pa

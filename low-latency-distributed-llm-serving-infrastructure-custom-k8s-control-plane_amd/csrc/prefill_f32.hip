@@ -41,8 +41,8 @@ namespace pa {
 // in flight (128 KB for heads of 128), one barrier per stage.  Per 32x32
 // tile a wave runs 2 D / 2 MFMAs (64 + 64 for heads of 128) against about 80
 // vector instructions of softmax, so the matrix cores set the pace.
-constexpr int kFmThreads = 512;  // 4 row groups x 2 context halves
 constexpr int kFmRows = 128;     // query rows per unit
+constexpr int kFmGroups = kFmRows / 32;  // row groups of 32
 constexpr int kFmTile = 32;      // context tokens per wave per stage
 constexpr int kFmStage = 2 * kFmTile;
 
@@ -56,8 +56,16 @@ __device__ __forceinline__ f32x16 mfma_f32(float a, float b, f32x16 c) {
 // each stage is in LDS (their block ids staged in LDS once per unit), so no
 // unit reads a row another one writes.
 // SPAN: a window with sinks, or trees of drafted tokens, as in prefill_kernel.hpp.
-template <int D, bool APPEND, int SPAN>
-__global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArgs a) {
+// RG: row groups that a workgroup takes of a unit's four, with two waves (context
+// halves) each.  Where units are few, two workgroups of two groups take one: a
+// workgroup's two waves a SIMD share its matrix core, so each stage takes half the
+// time (7 tiles of 128 rows of 8 heads of 64, up to 300 new tokens under a window of
+// 500: @RG4@ us with four groups, @RG2@ with two).
+template <int D, bool APPEND, int SPAN, int RG = kFmGroups>
+__global__ __launch_bounds__(2 * RG * kWave) void prefill_f32_mfma_kernel(PrefillArgs a) {
+  constexpr int kFmThreads = 2 * RG * kWave;
+  constexpr int kParts = kFmGroups / RG;  // workgroups of a unit
+  static_assert(SPAN != kSpanAll || kParts == 1, "a unit's rows are written by one workgroup");
   constexpr bool TREE = SPAN == kSpanTree;
   static_assert(SPAN == kSpanAll || !APPEND, "their rows are written before");
   constexpr int ROWB = D * 4;                  // bytes of a K or V row
@@ -65,12 +73,13 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
   constexpr int DB = D / 32;                   // 32-wide d blocks of the output
   constexpr int RPC = kWave / CH;              // rows one copy covers
   constexpr int kWaves = kFmThreads / kWave;
-  constexpr int kCopies = kFmStage / RPC / kWaves;  // copies per wave per tensor and stage
+  constexpr int kWaveRows = kFmStage / kWaves;  // rows of a stage that a wave copies
+  constexpr int kCopies = kWaveRows / RPC;      // copies per wave per tensor and stage
   constexpr int TBYTES = kFmStage * ROWB;     // one tensor's rows of a stage
   constexpr int kBufBytes = 2 * TBYTES;        // K, then V
   constexpr int kMerge = DB * 16 + 4;          // floats a lane hands over (acc, m, l, padding)
   static_assert(kCopies >= 1 && kCopies * RPC * kWaves == kFmStage, "stage / copy geometry");
-  static_assert(4 * kWave * kMerge * 4 <= 2 * kBufBytes, "the merge fits the stage buffers");
+  static_assert(RG * kWave * kMerge * 4 <= 2 * kBufBytes, "the merge fits the stage buffers");
 
   __shared__ __attribute__((aligned(16))) char s_lds[2 * kBufBytes];
   // Block id of every row of each stage buffer (-1 without a table row),
@@ -83,11 +92,12 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
   const int tid = threadIdx.x;
   const int lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int rg = wave & 3;
-  const int kh = wave >> 2;
+  const int rg = wave % RG;
+  const int kh = wave / RG;
   const int t = lane & 31;
   const int h = lane >> 5;
-  const int row = rg * 32 + t;  // this lane's query row of a unit
+  const int part = static_cast<int>(blockIdx.x) % kParts;
+  const int row = (part * RG + rg) * 32 + t;  // this lane's query row of a unit
   const int g = row / MTOK;
   const int tok = row - g * MTOK;
   const int hkv = a.num_kv_heads;
@@ -98,15 +108,15 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(s_lds));
   const float scale = a.scale_log2e;
   const int hq = hkv * a.group;
-  // Copies: wave w fills rows [8 w, 8 w + 8) of K and of V of a stage, RPC
+  // Copies: wave w fills kWaveRows rows from w kWaveRows on of K and of V of a stage, RPC
   // rows per copy; lane i lands at chunk position i % CH of row i / CH and
   // fetches the chunk the swizzle puts there.
   const int crow = lane / CH;
   const int cpos = lane % CH;
 
   const int U = static_cast<int>(a.num_units);
-  const int W = static_cast<int>(gridDim.x);
-  const int wg = static_cast<int>(blockIdx.x);
+  const int W = static_cast<int>(gridDim.x) / kParts;
+  const int wg = static_cast<int>(blockIdx.x) / kParts;
   for (int r = 0;; ++r) {
     const int rank = (r & 1) ? (r + 1) * W - 1 - wg : r * W + wg;
     if (rank >= U) break;
@@ -124,7 +134,14 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
     const int ctx = start + count;
     const int tok0 = qt * MTOK;
     const int ntok = min(MTOK, count - tok0);
-    if (ntok <= 0) continue;  // (the whole workgroup)
+    // The tokens of the tile that the workgroup's rows hold: all, or, where its part is
+    // of one head, from `from` on.
+    int from = 0, to = ntok;
+    if (kParts > 1 && RG * 32 <= MTOK) {
+      from = part * RG * 32 % MTOK;
+      to = min(ntok, from + RG * 32);
+    }
+    if (to <= from) continue;  // (the whole workgroup)
     const int64_t trow = TREE ? rec[7] : a.rows != nullptr ? a.rows[seq] : seq;
     [[maybe_unused]] const int part_row = TREE ? rec[3] : -1;
     const bool row_ok = trow >= 0 && trow < a.num_table_rows;
@@ -145,7 +162,7 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
       nv0 = reinterpret_cast<const char*>(a.new_value) + kvh * a.new_value_head_stride * 4 +
             (first - start) * static_cast<int64_t>(nvstride);
     }
-    const int kv_end = min(ctx, start + tok0 + ntok);  // exclusive
+    const int kv_end = min(ctx, start + tok0 + to);  // exclusive
     // Positions that have a block-table column (the rest are never read).
     const int kv_read = static_cast<int>(
         min(static_cast<int64_t>(kv_end), static_cast<int64_t>(bt_stride) << log2_bs));
@@ -157,7 +174,7 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
     [[maybe_unused]] int seen_lo = 0, seen_sinks = 0, stage0 = 0;
     if constexpr (SPAN != kSpanAll) {
       static_assert(kFmStage == kTreeStage, "the stages of the work lists");
-      seen_lo = TREE ? min(window_start(start, a.window), start) : window_start(start + tok0, a.window);
+      seen_lo = TREE ? min(window_start(start, a.window), start) : window_start(start + tok0 + from, a.window);
       seen_sinks = min(a.sinks, seen_lo);
       span = stage_span(seen_lo, kv_end, a.sinks, kFmStage);
       nstages = span.count;
@@ -196,7 +213,7 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
     auto load_ids = [&](int x) {
 #pragma unroll
       for (int c = 0; c < kCopies; ++c) {
-        const int p = min(stage_at(x) + 8 * wave + c * RPC + crow, kv_last);
+        const int p = min(stage_at(x) + kWaveRows * wave + c * RPC + crow, kv_last);
         ids[c] = row_ok ? bt[p >> log2_bs] : -1;
       }
     };
@@ -215,10 +232,10 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
       asm volatile("" : "+v"(cr), "+v"(cp));
 #pragma unroll
       for (int c = 0; c < kCopies; ++c) {
-        const int R = 8 * wave + c * RPC + cr;
+        const int R = kWaveRows * wave + c * RPC + cr;
         const int pc = min(stage_at(x) + R, kv_last);
         const int piece = (cp ^ chunk_swizzle<CH>(R)) * 16;
-        const uint32_t dst = lds0 + b * kBufBytes + (8 * wave + c * RPC) * ROWB;
+        const uint32_t dst = lds0 + b * kBufBytes + (kWaveRows * wave + c * RPC) * ROWB;
         src_of(c, pc, piece, dst);
         if (cp == 0) s_sid[b][R] = ids[c];
       }
@@ -342,7 +359,7 @@ __global__ __launch_bounds__(kFmThreads) void prefill_f32_mfma_kernel(PrefillArg
         // here: gated as `p > lim || (bad_ids && ...)`, this ROCm's hipcc
         // emitted the -INF write on the `p > lim` path only, and positions in
         // out-of-pool blocks kept their scores.
-        bool edge = bad_ids || p0 + kFmTile - 1 > min(start + tok0, kv_last);
+        bool edge = bad_ids || p0 + kFmTile - 1 > min(start + tok0 + from, kv_last);
         if constexpr (SPAN != kSpanAll) edge |= p0 < last_lo;
         if constexpr (TREE) edge |= p0 + kFmTile > start;
         if (edge) {
@@ -515,12 +532,20 @@ static hipError_t launch_prefill_f32_mfma(const PrefillArgs& args, int group, in
   a.num_units = num_items * a.num_kv_heads * a.sub_groups;
   // Unit ranks are 32-bit and a workgroup's ranks reach about twice the count.
   if (a.num_units > (int64_t{1} << 30)) return hipErrorInvalidValue;
+  const int cus = device_compute_units();
+  if constexpr (SPAN == kSpanWindow) {
+    if (2 * a.num_units <= cus) {  // two workgroups a unit, all at once
+      constexpr int RG = kFmGroups / 2;
+      hipLaunchKernelGGL((prefill_f32_mfma_kernel<D, APPEND, SPAN, RG>), dim3(static_cast<uint32_t>(2 * a.num_units)),
+                         dim3(2 * RG * kWave), 0, s, a);
+      return hipGetLastError();
+    }
+  }
   // One workgroup per CU (the stage buffers hold one per CU), each looping
   // over its share of the units; fewer units than CUs run one each.
-  const int cus = device_compute_units();
   const int64_t wgs = cus > 0 ? std::min<int64_t>(a.num_units, cus) : a.num_units;
-  hipLaunchKernelGGL((prefill_f32_mfma_kernel<D, APPEND, SPAN>), dim3(static_cast<uint32_t>(wgs)), dim3(kFmThreads), 0, s,
-                     a);
+  hipLaunchKernelGGL((prefill_f32_mfma_kernel<D, APPEND, SPAN>), dim3(static_cast<uint32_t>(wgs)),
+                     dim3(2 * kFmGroups * kWave), 0, s, a);
   return hipGetLastError();
 }
 

@@ -529,12 +529,7 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
                   ((static_cast<uint64_t>(word((node >> 5) + 1)) << 32) | word(node >> 5)) >> (node & 31));
             }
           }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int o = 8 * (i >> 2) + (i & 3);
-            const bool off = (o > lim) | ((o < low) & (o >= sink)) | (TREE && ((bits >> o) & 1u) == 0);
-            s[i] = off ? -INFINITY : s[i];
-          }
+          hide(s, bits & below(lim + 1) & (~below(low) | below(sink)));
           return;
         }
         const int lim = kv_lim - (t * kKvTile + 4 * half);

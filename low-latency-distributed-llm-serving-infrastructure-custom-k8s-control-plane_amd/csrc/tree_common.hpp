@@ -97,9 +97,6 @@ struct TreeRun {
 // s_waitcnt's immediate for vmcnt(0) alone.
 constexpr int kWaitLoads = 0x0F70;
 
-// The lowest n bits (none for n <= 0, all from 32 on).
-__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n > 0 ? (1u << n) - 1u : 0u; }
-
 // A query row's masks.  The first 64 bits of its node's word stay in registers.
 struct TreeRow {
   const uint32_t* words;
@@ -133,13 +130,7 @@ struct TreeRow {
       };
       bits = static_cast<uint32_t>(((static_cast<uint64_t>(word((n >> 5) + 1)) << 32) | word(n >> 5)) >> (n & 31));
     }
-    // Bit o: position at + o is seen.
-    bits &= below(last + 1) & (~below(low) | below(sink));
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t off = ~static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(bits), 8 * (i >> 2) + (i & 3), 1));
-      s[i] = __uint_as_float((off & 0xff800000u) | (~off & __float_as_uint(s[i])));
-    }
+    hide(s, bits & below(last + 1) & (~below(low) | below(sink)));
   }
 };
 

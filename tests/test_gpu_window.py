@@ -56,6 +56,15 @@ def test_window_steps_of_one_kind(device, kind, heads, kv_heads, dim, dtype):
     case.check(out)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 8, 64), (6, 2, 64), (16, 16, 128), (32, 8, 128)])
+def test_window_of_few_and_many_fp32_tiles(device, heads, kv_heads, dim):
+    """Tiles that two workgroups take, and as many as the chip's workgroups or more."""
+    for starts, counts in [([0, 40, 300], [70, 129, 64]), ([40 + i for i in range(18)], [130 + i for i in range(18)])]:
+        case = Case(starts, counts, heads, kv_heads, dim, FP32, window=90, sinks=5, seed=dim)
+        out, _ = run(case, device)
+        case.check(out)
+
+
 @pytest.mark.parametrize("heads,kv_heads,dim,dtype,cache_dtype", [
     (8, 2, 128, BF16, BF16), (8, 8, 64, FP16, FP16), (6, 2, 80, BF16, BF16), (4, 2, 256, BF16, BF16),
     (4, 2, 64, FP32, FP32), (8, 2, 128, BF16, CODE), (3, 1, 40, FP16, FP16)])
