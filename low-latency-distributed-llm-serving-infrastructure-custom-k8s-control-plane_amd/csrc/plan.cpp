@@ -6,6 +6,9 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <memory>
+#include <new>
+
 #include "decode_shape.hpp"
 #include "pa_error.hpp"
 #include "paged_attention_amd.h"
@@ -292,14 +295,16 @@ struct Trees {
 
 // Stages per item, by the modelled time of the candidates.  Measured on 32/8 heads
 // of 128 with 47 to 2026 stages of 64 tokens a KV head (a unit is an item's KV head):
-//  * a unit costs 8.4 us beside its stages, a stage at least 1.85 us of its
-//    workgroup, and the caches' rows, read once for all tiles of a sequence, come
-//    at 5.5 TB/s (3.06 us a stage of every resident workgroup);
+//  * a unit costs 8.4 us beside its stages, a stage 1.5 us of its workgroup, and the
+//    caches' rows, read once for all tiles of a sequence, come at 5.5 TB/s (3.06 us a
+//    stage of every resident workgroup);
 //  * units that do not all fit the chip at once share its workgroups, and the last
 //    ones leave part of it idle;
 //  * tiles in several runs are joined by a launch of its own.
-// Within 10 % of 28 measured times of four steps (1 to 47 stages an item), and the
-// pick within 6 % of the fastest.
+// Of 15 splits of nine steps each (four of 32/8 and 32/32 heads of 128; 16-bit heads of
+// 64 and 256; 8-bit and fp32 caches) the pick was the fastest or within 2 % of it in
+// six, within 9 % in the others; one run a tile took up to 11 times as long, one stage
+// a run up to four times.
 struct TreeCost {
   double unit, stage, bytes;  // us
   int slots;                  // workgroups resident on a CU
@@ -307,30 +312,38 @@ struct TreeCost {
 TreeCost tree_cost(int dtype, int head_dim) {
   const double row = head_dim * (dtype == PA_DTYPE_E4M3 ? 1 : dtype == PA_DTYPE_F32 ? 4 : 2) / 256.0;
   if (dtype == PA_DTYPE_F32) return {8.4, 4.4 * row, 1.53 * row, 1};  // (prefill_f32.hip's)
-  if (dtype == PA_DTYPE_E4M3) return {10.0, 1.1, 1.53 * row, 1};  // (prefill.hip's kernel: a CU each)
+  if (dtype == PA_DTYPE_E4M3) return {10.0, 1.2, 1.53 * row, 1};  // (prefill.hip's kernel: a CU each)
   if (head_dim == 256) return {8.4, 2.9, 1.53 * row, 1};
-  return head_dim == 64 ? TreeCost{8.4, 1.2, 4.6 * row, 3} : TreeCost{8.4, 1.85, 3.06 * row, 2};
+  return head_dim == 64 ? TreeCost{8.4, 1.0, 4.6 * row, 3} : TreeCost{8.4, 1.5, 3.06 * row, 2};
 }
 int32_t choose_split(const Trees& t, const PaTreeDims& d) {
   const int64_t heads = d.num_kv_heads * static_cast<int64_t>(pa::decode_sub_groups(d.num_query_heads / d.num_kv_heads));
   const TreeCost c = tree_cost(d.dtype, d.head_dim);
   const int64_t slots = static_cast<int64_t>(c.slots) * (d.compute_units > 0 ? d.compute_units : 256);
   int64_t longest = 1, all = 0, unique = 0;
-  for (int32_t i = 0; i < d.num_seqs; ++i) unique += t.longest_of(i);
+  int64_t num_tiles = 0;
+  for (int32_t i = 0; i < d.num_seqs; ++i) {
+    unique += t.longest_of(i);
+    num_tiles += ceil_div(t.counts[i], t.tile);
+  }
+  std::unique_ptr<int[]> tiles(new (std::nothrow) int[num_tiles > 0 ? num_tiles : 1]);
+  if (!tiles) return 1 << 24;  // (every tile one run)
+  int64_t at = 0;
   t.each([&](int64_t, int64_t stages) {
     longest = stages > longest ? stages : longest;
     all += stages;
+    tiles[at++] = static_cast<int>(stages);
   });
   double best = 0;
-  int32_t pick = 0;
-  for (int64_t split = longest; split >= 1; split = split * 4 / 5 < split - 1 ? split * 4 / 5 : split - 1) {
+  int64_t pick = 0;
+  auto consider = [&](int64_t split) {  // (false: smaller ones only make more units of too many)
     int64_t items = 0, run = 0, runs = 0;
-    t.each([&](int64_t, int64_t stages) {
-      const pa::TreeSplit cut = pa::tree_split(static_cast<int>(stages), static_cast<int>(split));
+    for (int64_t i = 0; i < num_tiles; ++i) {
+      const pa::TreeSplit cut = pa::tree_split(tiles[i], static_cast<int>(split));
       items += cut.runs;
       run = cut.stages > run ? cut.stages : run;
       runs = cut.runs > runs ? cut.runs : runs;
-    });
+    }
     const double units = static_cast<double>(items * heads);
     double chain = run * c.stage;
     double bytes = unique * heads * c.bytes / slots + 0.2 * run * c.bytes;
@@ -341,11 +354,17 @@ int32_t choose_split(const Trees& t, const PaTreeDims& d) {
     const double time = c.unit + (chain > bytes ? chain : bytes) + (runs > 1 ? 2.0 + 0.25 * runs : 0.0);
     if (pick == 0 || time < best) {
       best = time;
-      pick = static_cast<int32_t>(split);
+      pick = split;
     }
-    if (units > 8.0 * slots) break;
-  }
-  return pick;
+    return units <= 8.0 * slots;
+  };
+  // In steps of a fifth, then around the best of those in finer ones.
+  for (int64_t split = longest; split >= 1; split = split * 4 / 5 < split - 1 ? split * 4 / 5 : split - 1)
+    if (!consider(split)) break;
+  const int64_t around = pick, step = around / 24 + 1;
+  for (int64_t split = around + 5 * step; split > 0 && split >= around - 5 * step; split -= step)
+    if (split <= longest && split != around) consider(split);
+  return static_cast<int32_t>(pick);
 }
 
 }  // namespace
