@@ -14,6 +14,7 @@
 // node as its parent, or is a root; a parent that is no earlier node of the
 // sequence reads as a root, so every walk up ends.
 #include <algorithm>
+#include <type_traits>
 
 #include "cache8.hpp"
 #include "pa_common.hpp"
@@ -43,9 +44,10 @@ __device__ __forceinline__ int parent_of(const int32_t* parents, int64_t first, 
   return p >= 0 && p < node ? p : -1;
 }
 
-// Items, merge items and partial rows of a sequence's tiles.
+// Items, merge items and partial rows of a sequence's tiles (64-bit: contexts of the
+// device's arrays may be longer than those the lists were sized for).
 struct TreeWork {
-  int items, merges, rows;
+  int64_t items, merges, rows;
 };
 __device__ __forceinline__ TreeWork tree_work(const PackTreeArgs& a, int start, int count) {
   TreeWork w{0, 0, 0};
@@ -56,7 +58,7 @@ __device__ __forceinline__ TreeWork tree_work(const PackTreeArgs& a, int start, 
     w.items += splits;
     if (splits > 1) {
       w.merges += 1;
-      w.rows += splits * n;
+      w.rows += static_cast<int64_t>(splits) * n;
     }
   }
   return w;
@@ -69,13 +71,13 @@ __device__ __forceinline__ TreeWork tree_work(const PackTreeArgs& a, int start, 
 // behind the lists' ends, so that a launch sized for more work skips them.
 __global__ __launch_bounds__(kTreeThreads) void pack_tree_kernel(PackTreeArgs a) {
   __shared__ int s_parent[kMaxTreeNodes];
-  __shared__ int s_sum[kTreeThreads / kWave][3];
+  __shared__ int64_t s_sum[kTreeThreads / kWave][3];
   const int tid = threadIdx.x;
   const int seq = blockIdx.x;
   const TreeSeq s = tree_seq(a.cu_seqlens, seq, a.num_query_tokens);
   const int start = a.context_lens[seq] - s.count;
   for (int i = tid; i < s.count; i += kTreeThreads) s_parent[i] = parent_of(a.parents, s.first, i);
-  int items = 0, merges = 0, rows = 0;
+  int64_t items = 0, merges = 0, rows = 0;
   if (a.items != nullptr) {
     for (int j = tid; j < seq; j += kTreeThreads) {
       const TreeSeq o = tree_seq(a.cu_seqlens, j, a.num_query_tokens);
@@ -86,9 +88,9 @@ __global__ __launch_bounds__(kTreeThreads) void pack_tree_kernel(PackTreeArgs a)
     }
 #pragma unroll
     for (int o = kWave / 2; o >= 1; o >>= 1) {
-      items += __shfl_xor(items, o, kWave);
-      merges += __shfl_xor(merges, o, kWave);
-      rows += __shfl_xor(rows, o, kWave);
+      items += __shfl_xor(static_cast<long long>(items), o, kWave);
+      merges += __shfl_xor(static_cast<long long>(merges), o, kWave);
+      rows += __shfl_xor(static_cast<long long>(rows), o, kWave);
     }
     if (tid % kWave == 0) {
       s_sum[tid / kWave][0] = items;
@@ -132,19 +134,18 @@ __global__ __launch_bounds__(kTreeThreads) void pack_tree_kernel(PackTreeArgs a)
     const int stages = tree_span(start, t0 + n, a.window, a.sinks, kTreeStage).count;
     const int splits = tree_split(stages, a.split_stages).runs;
     // (a tile whose partials would not fit is left out: the host sizes them)
-    const bool fits = splits == 1 || static_cast<int64_t>(rows) + static_cast<int64_t>(splits) * n <= a.max_partial_rows;
+    const bool fits = splits == 1 || rows + static_cast<int64_t>(splits) * n <= a.max_partial_rows;
     for (int k = tid; k < splits; k += kTreeThreads)
-      if (items + k < a.max_items)
-      {
-        int4* item = a.items + 2 * static_cast<int64_t>(items + k);
-        item[0] = make_int4(fits ? seq : -1, t0 / a.tile, k, splits > 1 ? rows + k * n : -1);
+      if (items + k < a.max_items) {
+        int4* item = a.items + 2 * (items + k);
+        item[0] = make_int4(fits ? seq : -1, t0 / a.tile, k, splits > 1 && fits ? static_cast<int>(rows) + k * n : -1);
         item[1] = make_int4(static_cast<int>(s.first), s.count, start, a.rows != nullptr ? a.rows[seq] : seq);
       }
     if (splits > 1) {
       if (tid == 0 && merges < a.max_merge_items)
-        a.merge_items[merges] = make_int4(fits ? seq : -1, t0 / a.tile, splits, rows);
+        a.merge_items[merges] = make_int4(fits ? seq : -1, t0 / a.tile, splits, fits ? static_cast<int>(rows) : 0);
       merges += 1;
-      rows += splits * n;
+      rows += static_cast<int64_t>(splits) * n;
     }
     items += splits;
   }
@@ -162,6 +163,7 @@ __global__ __launch_bounds__(kTreeThreads) void pack_tree_kernel(PackTreeArgs a)
 // (26 nodes of 32 heads of 128 in 24 runs: one workgroup a node, eight partials a
 // trip 13.2 us).
 constexpr int kMergeRuns = 16;
+constexpr int kFewRuns = 4;
 template <typename T, int D>
 __global__ __launch_bounds__(kTreeThreads) void merge_tree_kernel(MergeTreeArgs a) {
   const int64_t m = blockIdx.x / a.tile;
@@ -182,36 +184,43 @@ __global__ __launch_bounds__(kTreeThreads) void merge_tree_kernel(MergeTreeArgs 
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row;
   float mx = kScoreFloor, sum = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p = 0; p < item.z; p += kMergeRuns) {
-    float2 s[kMergeRuns];
-    float4 x[kMergeRuns];
+  auto join = [&](auto runs) {
+    constexpr int R = decltype(runs)::value;
+    for (int p = 0; p < item.z; p += R) {
+      float2 s[R];
+      float4 x[R];
 #pragma unroll
-    for (int u = 0; u < kMergeRuns; ++u) {
-      const int64_t at = min(p + u, item.z - 1) * step;
-      s[u] = ml[at];
-      x[u] = acc[at * (D / 4)];
-    }
-    float mn = mx;
-#pragma unroll
-    for (int u = 0; u < kMergeRuns; ++u) mn = fmaxf(mn, s[u].x);
-    const float keep = fast_exp2(mx - mn);
-    sum *= keep;
-    o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
-#pragma unroll
-    for (int u = 0; u < kMergeRuns; ++u) {
-      const float w = p + u < item.z ? fast_exp2(s[u].x - mn) : 0.f;
-      if (p + u < item.z) {
-        sum = fmaf(s[u].y, w, sum);
-        o = make_float4(fmaf(x[u].x, w, o.x), fmaf(x[u].y, w, o.y), fmaf(x[u].z, w, o.z), fmaf(x[u].w, w, o.w));
+      for (int u = 0; u < R; ++u) {
+        const int64_t at = min(p + u, item.z - 1) * step;
+        s[u] = ml[at];
+        x[u] = acc[at * (D / 4)];
       }
+      float mn = mx;
+#pragma unroll
+      for (int u = 0; u < R; ++u) mn = fmaxf(mn, s[u].x);
+      const float keep = fast_exp2(mx - mn);
+      sum *= keep;
+      o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll
+      for (int u = 0; u < R; ++u) {
+        const float w = p + u < item.z ? fast_exp2(s[u].x - mn) : 0.f;
+        if (p + u < item.z) {
+          sum = fmaf(s[u].y, w, sum);
+          o = make_float4(fmaf(x[u].x, w, o.x), fmaf(x[u].y, w, o.y), fmaf(x[u].z, w, o.z), fmaf(x[u].w, w, o.w));
+        }
+      }
+      mx = mn;
     }
-    mx = mn;
-  }
+  };
+  if (item.z <= kFewRuns) join(std::integral_constant<int, kFewRuns>());
+  else join(std::integral_constant<int, kMergeRuns>());
   // (a sum of zero is a row that attends nothing, whose result is zero; a NaN stays)
   T* out = reinterpret_cast<T*>(a.output) + (first + t0 + tok) * hq * D + static_cast<int64_t>(r) * 4;
-  const float e[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) store_scalar<T>(out + i, sum != 0.f ? e[i] / sum : 0.f);
+  o = sum != 0.f ? make_float4(o.x / sum, o.y / sum, o.z / sum, o.w / sum) : make_float4(0.f, 0.f, 0.f, 0.f);
+  if constexpr (sizeof(T) == 4)
+    *reinterpret_cast<float4*>(out) = o;
+  else
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack_half2<T>(o.x, o.y), pack_half2<T>(o.z, o.w));
 }
 
 // One wave a sequence: at each node the lanes look for its first child (they
