@@ -1959,6 +1959,9 @@ def tree_attention(
             raise ValueError("the tree has no attention work lists: give pack_tree the head counts and head_dim")
         if heads != tree._heads:
             raise ValueError(f"the tree was packed for (H_kv, H_q, D) {tree._heads}, not {heads}")
+        if int(tree._dims.dtype) != cache_dtype_code(key_cache.dtype):
+            # (its lists are another kernel's, and the generic one takes 100 times as long)
+            raise ValueError(f"the tree was packed for another dtype than the cache's: give pack_tree {key_cache.dtype}")
         strides = None
         if new_key is not None:
             k, v = _new_rows(new_key, new_value, key_cache, step)

@@ -365,6 +365,8 @@ def test_refusals(device):
         ops.tree_attention(q, k, v, 1, other, tree, 1.0)
     with pytest.raises(ValueError, match="was packed for"):
         ops.tree_attention(q[:, :4], k, v, 1, step, tree, 1.0)
+    with pytest.raises(ValueError, match="another dtype than the cache's"):
+        ops.tree_attention(q, k, v, 1, step, ops.pack_tree(step, parents, dtype=FP16), 1.0)
     with pytest.raises(RuntimeError, match="Layer index"):
         ops.tree_attention(q, k, v, 2, step, tree, 1.0)
     with pytest.raises(ValueError, match="together"):
