@@ -180,12 +180,6 @@ tree_attention_kernel(PrefillArgs a) {
       v_off[db][hi] = kVBase + r * ROW_BYTES + (((col >> 3) ^ chunk_swizzle<CHUNKS>(r)) * 16) + (col & 7) * 2;
     }
 
-  // The accumulators leave the matrix registers within a rescale alone (left to
-  // itself, the compiler copies all of them at each tile, for the case of one).
-  auto in_matrix_registers = [](f32x16& x) {
-    if constexpr (D > 64) asm("" : "+a"(x));
-  };
-
   // The unit with its live blocks of rows, NB of two.
   auto attend = [&](auto blocks) {
     constexpr int NB = decltype(blocks)::value;
@@ -317,10 +311,10 @@ tree_attention_kernel(PrefillArgs a) {
           l[b] *= alpha;
 #pragma unroll
           for (int db = 0; db < DB; ++db) {
-            in_matrix_registers(acc[b][db]);
+            if constexpr (D > 64) in_matrix_registers(acc[b][db]);
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[b][db][j] *= alpha;
-            in_matrix_registers(acc[b][db]);
+            if constexpr (D > 64) in_matrix_registers(acc[b][db]);
           }
           m[b] = m_new;
         }

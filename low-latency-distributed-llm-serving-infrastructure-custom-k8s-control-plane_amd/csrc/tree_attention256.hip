@@ -106,6 +106,7 @@ __global__ __launch_bounds__(kThreads) void tree_attention256_kernel(PrefillArgs
     for (int i = tid + kThreads; i < run.ncols; i += kThreads) stage(i, entry(i));
   }
   const bool bad_ids = __syncthreads_or(bad ? 1 : 0) != 0;
+  __builtin_amdgcn_s_waitcnt(kWaitLoads);  // (the query and the masks, as in tree_attention.hip)
 
   // ---- copies: wave w copies rows [8 w, 8 w + 8) of a step ---------------------
   const int delta = lane / CHUNKS;
@@ -208,9 +209,12 @@ __global__ __launch_bounds__(kThreads) void tree_attention256_kernel(PrefillArgs
       const float alpha = fast_exp2((m - m_new) * scale);
       l *= alpha;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+      for (int db = 0; db < DB; ++db) {
+        in_matrix_registers(acc[db]);
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
+        in_matrix_registers(acc[db]);
+      }
       m = m_new;
     }
   };
