@@ -26,9 +26,10 @@ LIBRARY_NAME = "libpaged_attention_amd.so"
 LIBRARY_PATH = PACKAGE_DIR / LIBRARY_NAME
 OFFLOAD_ARCH = "gfx950"
 
-SOURCES = ["prefill.hip", "prefill_window.hip", "prefill_tree.hip", "decode.hip", "decode_window.hip", "abi.hip", "plan.cpp", "pack.hip", "cache_write.hip", "rotate.hip", "decode_mfma.hip",
-           "decode8.hip", "generic.hip",
-           "prefill256.hip", "prefill_f32.hip", "tree.hip", "tree_attention.hip", "tree_attention256.hip", "copy_blocks.hip", "calibrate.hip"]
+SOURCES = ["prefill.hip", "prefill_window.hip", "prefill_tree.hip", "decode.hip", "decode_window.hip", "abi.hip",
+           "plan.cpp", "pack.hip", "cache_write.hip", "rotate.hip", "decode_mfma.hip", "decode8.hip", "generic.hip",
+           "prefill256.hip", "prefill_f32.hip", "tree.hip", "tree_attention.hip", "tree_attention256.hip",
+           "copy_blocks.hip", "calibrate.hip"]
 
 HIP_FLAGS = [
     "-O3",

@@ -1,7 +1,7 @@
 // Paged-attention decode for gfx950 on the vector units: one workgroup per
 // (sequence, context partition of up to 4096 tokens, KV head), split-K merge
 // after.  fp32 caches and 16-bit heads of 256 run here; 16-bit heads of 64 to
-// 128 run on the matrix cores (decode_mfma.hip).
+// 128 run on the matrix cores (decode_mfma.hip).  The kernel itself: decode_kernel.hpp.
 //
 // The workgroup (4 waves) serves the G = H_q / H_kv query heads that share
 // one KV head, so every K/V row of the partition is read from HBM once

@@ -77,7 +77,8 @@ __device__ __forceinline__ void read_codes(const uint32_t (&at)[KP], u32x4m (&k)
         : "memory");
 }
 
-// SMALL: blocks of fewer than 16 tokens.  WINDOW: as in decode_mfma.hip.
+// SMALL: blocks of fewer than 16 tokens.  WINDOW: as in decode_mfma.hip (64 sequences of
+// 128-8192 tokens, 32/32 heads of 128, window 2048, 16 sinks: 174 us, 5.8 TB/s).
 template <typename T, int D, int DM, bool SHARED, int HEADS, bool SMALL, bool WINDOW>
 __global__ __launch_bounds__(kDecodeThreads) __attribute__((amdgpu_waves_per_eu(4))) void
 decode8_kernel(DecodeArgs a) {

@@ -1,4 +1,5 @@
-// Causal chunked prefill over the paged cache with gfx950 MFMA tiles.
+// Causal chunked prefill over the paged cache with gfx950 MFMA tiles (the kernel
+// itself: prefill_kernel.hpp).
 //
 // A unit of work is (sequence, query tile, KV head).  The tile holds 128
 // query rows = (128 / G) query tokens x the G query heads that share the KV
@@ -98,7 +99,7 @@
 namespace pa {
 
 bool prefill_fast_path_supported(int dtype, int head_dim, int group, int block_size) {
-  // bf16 / fp16: the MFMA kernel below (heads of 80 and 96 on rows of 128)
+  // bf16 / fp16: prefill_kernel.hpp's (heads of 80 and 96 on rows of 128)
   // and prefill256_kernel for heads of 256; fp32: prefill_f32_mfma_kernel
   // (v_mfma_f32_32x32x2_f32), heads of 64 and 128.
   if (dtype != PA_DTYPE_BF16 && dtype != PA_DTYPE_F16 && dtype != PA_DTYPE_F32) return false;
@@ -123,7 +124,7 @@ bool prefill_append_supported(int dtype, int head_dim) {
 }
 
 bool prefill_codes_supported(int dtype, int head_dim) {
-  // The kernel of this file.
+  // prefill_kernel.hpp's.
   return (dtype == PA_DTYPE_BF16 || dtype == PA_DTYPE_F16) && head_dim <= 128;
 }
 

@@ -55,7 +55,8 @@ constexpr int kIdSlotBytes = 256;
 constexpr int kIdAhead = 8;
 constexpr int kLdsBytes = kIdBase + kIdSlots * kIdSlotBytes;
 
-// WINDOW: a window with sinks, as in prefill_kernel.hpp.
+// WINDOW: a window with sinks, as in prefill_kernel.hpp (4 prompts of 2048 tokens at 0
+// to 12288, 16/4 heads, window 2048, 4 sinks: 397 us, 607 TFLOP/s).
 template <typename T, bool LANE_IDS, bool WINDOW>
 __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
   static_assert(Elem<T>::kBytes == 2, "16-bit caches (bf16 or fp16)");
@@ -279,11 +280,7 @@ __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
       // (what is computed for a stage past the last counts for nothing)
       const int lim = t < nstages ? kv_lim - at : -1;
       const int low = row_lo - at, sink = a.sinks - at;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int o = 8 * (i >> 2) + (i & 3);
-        s[i] = (o > lim) | ((o < low) & (o >= sink)) ? -INFINITY : s[i];
-      }
+      hide(s, below(lim + 1) & (~below(low) | below(sink)));
       return;
     }
     const int lim = kv_lim - (t * kTile + 4 * half);

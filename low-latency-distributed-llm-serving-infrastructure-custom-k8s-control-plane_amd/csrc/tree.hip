@@ -1,5 +1,6 @@
-// Trees of drafted tokens: what surrounds their attention (prefill.hip and
-// prefill_f32.hip, generic.hip) in a verification step.
+// Trees of drafted tokens: what surrounds their attention (tree_attention.hip,
+// tree_attention256.hip, prefill_tree.hip, prefill_f32.hip, generic.hip) in a
+// verification step.
 //
 //  pack_tree_kernel    the nodes' masks and positions from their parents, and
 //                      the attention's work lists;
@@ -68,7 +69,8 @@ __device__ __forceinline__ TreeWork tree_work(const PackTreeArgs& a, int start, 
 // indices fall, so its mask's words come out from the last to the first.  For
 // the work lists every workgroup adds up what the sequences before its own
 // need (a step of 64 sequences: a read each); the last one marks the entries
-// behind the lists' ends, so that a launch sized for more work skips them.
+// behind the lists' ends, so that a launch sized for more work skips them.  One tree of
+// 26 nodes 3.4 us, 48 of 16-64 nodes 6.6.
 __global__ __launch_bounds__(kTreeThreads) void pack_tree_kernel(PackTreeArgs a) {
   __shared__ int s_parent[kMaxTreeNodes];
   __shared__ int64_t s_sum[kTreeThreads / kWave][3];
@@ -160,8 +162,9 @@ __global__ __launch_bounds__(kTreeThreads) void pack_tree_kernel(PackTreeArgs a)
 // domain); slots past the last partial read it again and get no weight.  The
 // partials are in L2 or beside it: what counts is the number of round trips, so
 // the loads of a batch go out together and a node's heads spread over workgroups
-// (26 nodes of 32 heads of 128 in 24 runs: one workgroup a node, eight partials a
-// trip 13.2 us).
+// (26 nodes of 32 heads of 128 in 16 runs: 3.9 us; one workgroup a node, eight partials
+// a trip: 13.2).  Up to four runs go in a batch of four (8 trees of 64 nodes, 32 heads
+// of 128, two runs each: 5.4 us; sixteen slots, most of them the last run again: 9.2).
 constexpr int kMergeRuns = 16;
 constexpr int kFewRuns = 4;
 template <typename T, int D>
@@ -224,7 +227,8 @@ __global__ __launch_bounds__(kTreeThreads) void merge_tree_kernel(MergeTreeArgs 
 }
 
 // One wave a sequence: at each node the lanes look for its first child (they
-// come behind it) that drafted the token predicted there.
+// come behind it) that drafted the token predicted there: two round trips a node of
+// the path.  One tree of 26 nodes 2.6 us, 48 of 16-64 nodes 5.2.
 __global__ __launch_bounds__(kWave) void accept_tree_kernel(AcceptTreeArgs a) {
   __shared__ int s_parent[kMaxTreeNodes];
   const int lane = threadIdx.x;
@@ -288,7 +292,9 @@ __device__ __forceinline__ bool kept_ok(const KeepRowsArgs& a, const KeptSeq& k,
 // A workgroup a (sequence, layer, tensor), a thread the same 16 (or fewer)
 // bytes of every row: rows move down in order (the kept nodes ascend, so no row
 // is written before it has been read), and no thread waits for another but for
-// the slots of the next 64 rows.
+// the slots of the next 64 rows.  48 trees of 16-64 nodes, 32 layers, 8 heads of 128: 12
+// us (20 MB, 1.6 TB/s: the counts, the nodes, the table and the rows are read one after
+// the other); one tree 4.6.
 template <typename V>
 __global__ __launch_bounds__(kTreeThreads) void keep_rows_kernel(KeepRowsArgs a) {
   constexpr int kBatch = 8;
@@ -344,7 +350,8 @@ __global__ __launch_bounds__(kTreeThreads) void keep_rows_kernel(KeepRowsArgs a)
 // that is larger, its rows are re-coded with it, and so is each row that moves
 // in from a block of a smaller one (to nearest even; values but those among the
 // subnormal codes stay).  A block that rows come from later still has its own
-// codes and scale then.
+// codes and scale then.  The same 48 trees: 39 us, the rows of a block one after
+// another.
 __global__ __launch_bounds__(kWave) void keep_rows8_kernel(KeepRowsArgs a) {
   constexpr int kCodes = 4;  // codes of a row a lane holds, kWave apart
   const int lane = threadIdx.x;

@@ -5,20 +5,27 @@
 // stages of one tile of a sequence's nodes, and its record holds all that a unit
 // has to know of its sequence.  The tile has 64 query rows, node after node, the
 // query heads of the KV head (or sub-group) side by side: two blocks of 32, of which
-// a small tree fills one.  Wave w takes tiles w, w + 4, ... of 32 context tokens of
+// a small tree fills one.  Wave w takes tiles w, w + 2, ... of 32 context tokens of
 // the run for all rows, with flash-style online softmax in fp32, and keeps its own K
-// and V in its own part of LDS, two tiles deep: no wave waits for another until the
-// four are joined at the end.
+// and V in its own part of LDS, two tiles deep: no wave waits for another until they
+// are joined at the end.
 //   S^T[kv][row] = sum_d K[kv][d] Q[row][d]
 //   O^T[d][row] += sum_kv V^T[d][kv] P^T[kv][row]     (v_mfma_f32_32x32x16)
 // with the layouts, the swizzled LDS rows, the direct global -> LDS copies, the
-// transpose read of V and the lazy rescale of prefill.hip.  An operand of K or V
+// transpose read of V and the lazy rescale of prefill_kernel.hpp.  An operand of K or V
 // read from LDS serves both blocks of rows, whose products and softmax do not
 // depend on each other.
 //
-// What bounds it is the cache's bytes, read once for a tile's rows, and for short
-// runs the chain of round trips at a unit's start (record; block ids, query and
-// masks; K and V).
+// What bounds it is the cache's bytes, read once for a tile's rows (32 trees of 9-17
+// nodes after 100-8000 tokens, 32/8 heads of 128: 108 us and 9 for the join, 5.0 TB/s;
+// 8 of 64 nodes after 1000-4000, 32/32 heads: 67 and 5.5, 5.1 TB/s); for trees whose
+// tiles share a short context the one wave a SIMD, whose products and softmax follow
+// each other (2 of 40-60 nodes under a window of 8192: 35 and 5.5 us, 310 TFLOP/s); for
+// short runs the chain of round trips at a unit's start (record; block ids, query and
+// masks; K and V: one of 26 nodes after 3000, 16 and 4 us).  The causal prefill's tiles,
+// shared by eight waves, took 145, 95, and 28 us where this now takes 118, 73 and 19.6.
+// V's operands read behind the softmax, and the accumulators copied out of the matrix
+// registers at each tile: 133, 91 and 21 us.
 //
 // Masks: a node sees the context before the tree (under a window, from where its
 // own position's window starts, and the sinks) and of the tree what its mask's
@@ -349,7 +356,7 @@ tree_attention_kernel(PrefillArgs a) {
       if (i + 1 < n) step(i + 1, std::integral_constant<int, 1>());
     }
 
-    // ---- the four waves of each row joined ---------------------------------------
+    // ---- the waves of each row joined ---------------------------------------------
     // Each wave leaves its accumulators in its own rings, in 16-byte pieces (piece c
     // of lane i at (c * 64 + i) * 16), and finishes NB DB of the pieces for all.
 #pragma unroll

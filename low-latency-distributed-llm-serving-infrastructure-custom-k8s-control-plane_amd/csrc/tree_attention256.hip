@@ -9,6 +9,10 @@
 // a live row only copy.)  The rings have four slots each of K and V, filled three
 // steps ahead: K of step st+5 goes out in step st, when K of st+1 is in registers
 // already, and V of st+3.  Items, masks and partial results as there.
+//
+// 16 trees of 9-17 nodes after 100-6000 tokens, 16/4 heads: 58 us, 3.5 TB/s (a unit's
+// start, its steps' chain between barriers, and the join); 66 us while the compiler
+// moved the accumulators at each step and waited for the query in the loop.
 #include <type_traits>
 
 #include "tree_common.hpp"
