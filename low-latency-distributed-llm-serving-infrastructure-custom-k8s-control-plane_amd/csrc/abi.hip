@@ -1211,8 +1211,8 @@ int pa_attention_window(const PaStepCall* call, PaWindow window, const void* que
 }
 
 int pa_pack_tree(const int32_t* parents, const int32_t* context_lens, const int64_t* cu_seqlens,
-                 const int32_t* block_table_rows, PaTreeDims dims, PaTreePlan plan, uint32_t* masks, int64_t* positions, int32_t* items, int32_t* merge_items,
-                 void* stream) {
+                 const int32_t* block_table_rows, PaTreeDims dims, PaTreePlan plan, uint32_t* masks,
+                 int64_t* positions, int32_t* items, int32_t* merge_items, void* stream) {
   const char* who = "pa_pack_tree";
   int rc = check_window(who, dims.window);
   if (rc != PA_OK) return rc;
@@ -1276,10 +1276,12 @@ int pa_tree_attention(const PaTreeCall* call, const void* query, void* key_cache
                      {c.block_tables, "block_tables"}, {c.context_lens, "context_lens"},
                      {c.cu_seqlens, "cu_seqlens"}, {c.masks, "masks"}, {c.positions, "positions"}});
   if (rc != PA_OK) return rc;
-  if (new_rows != nullptr) {
-    rc = write_rows(d, *new_rows, key_cache, value_cache, key_scales, value_scales, c.scatter_slots, layer_idx, stream);
-    if (rc != PA_OK) return rc;
-  }
+  // (behind every check, so that a refused call writes nothing)
+  auto write_new = [&] {
+    return new_rows == nullptr ? PA_OK
+                               : write_rows(d, *new_rows, key_cache, value_cache, key_scales, value_scales,
+                                            c.scatter_slots, layer_idx, stream);
+  };
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int eb = elem_bytes(d.dtype);
   const int cache_eb = key_scales != nullptr ? 1 : eb;
@@ -1336,6 +1338,8 @@ int pa_tree_attention(const PaTreeCall* call, const void* query, void* key_cache
     a.part_acc = reinterpret_cast<float*>(c.workspace);
     a.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(c.workspace) + wl.acc);
     a.split_stages = c.plan.split_stages;
+    rc = write_new();
+    if (rc != PA_OK) return rc;
     rc = from_hip(pa::launch_prefill(a, d.dtype, d.head_dim, group, c.plan.num_items, s), who);
     if (rc != PA_OK) return rc;
     pa::MergeTreeArgs m{};
@@ -1382,6 +1386,8 @@ int pa_tree_attention(const PaTreeCall* call, const void* query, void* key_cache
   a.masks = c.masks;
   a.mask_words = c.plan.mask_words;
   a.positions = c.positions;
+  rc = write_new();
+  if (rc != PA_OK) return rc;
   return from_hip(pa::launch_generic(a, d.dtype, s), who);
 }
 

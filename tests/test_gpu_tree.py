@@ -348,6 +348,20 @@ def test_a_step_together(device):
         assert captured.nodes.tolist() == nodes and captured.counts.tolist() == kept
 
 
+def test_a_refused_call_writes_no_rows(device):
+    case = Case([4000], [6], 8, 2, 128, BF16, parents=trees([6]))
+    q, k, v, _, step = case.place(device)
+    tree = ops.pack_tree(step, flat(case.parents).to(device))
+    assert tree._plan.num_partial_rows > 0
+    tree._workspace_bytes = 0
+    was = k.clone(), v.clone()
+    rows = torch.ones((6, 2, 128), dtype=BF16, device=device)
+    with pytest.raises(RuntimeError, match="workspace of"):
+        ops.tree_attention(q, k, v, 1, step, tree, 1.0, new_key=rows, new_value=rows)
+    for x, y in zip(was, (k, v)):
+        assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+
+
 def test_refusals(device):
     case = Case([40, 9], [6, 3], 8, 2, 128, BF16, parents=trees([6, 3]))
     q, k, v, _, step = case.place(device)
