@@ -298,13 +298,14 @@ struct Trees {
 //  * a unit costs 8.4 us beside its stages, a stage 1.5 us of its workgroup, and the
 //    caches' rows, read once for all tiles of a sequence, come at 5.5 TB/s (3.06 us a
 //    stage of every resident workgroup);
+//  * a workgroup of four waves takes 0.6 us a stage and 1.2 us more a unit;
 //  * units that do not all fit the chip at once share its workgroups, and the last
 //    ones leave part of it idle;
 //  * tiles in several runs are joined by a launch of its own.
-// Of 15 splits of nine steps each (four of 32/8 and 32/32 heads of 128; 16-bit heads of
-// 64 and 256; 8-bit and fp32 caches) the pick was the fastest or within 2 % of it in
-// six, within 9 % in the others; one run a tile took up to 11 times as long, one stage
-// a run up to four times.
+// Of 12 to 15 splits of 13 steps each (32/8 and 32/32 heads of 128; 16-bit heads of 64,
+// 80 and 256; 8-bit and fp32 caches) the pick was the fastest or within 3 % of it in
+// eight, within 8 % in the others; one run a tile took up to 11 times as long, one stage
+// a run up to five times.
 struct TreeCost {
   double unit, stage, bytes;  // us
   int slots;                  // workgroups resident on a CU
@@ -319,7 +320,8 @@ TreeCost tree_cost(int dtype, int head_dim) {
 int32_t choose_split(const Trees& t, const PaTreeDims& d) {
   const int64_t heads = d.num_kv_heads * static_cast<int64_t>(pa::decode_sub_groups(d.num_query_heads / d.num_kv_heads));
   const TreeCost c = tree_cost(d.dtype, d.head_dim);
-  const int64_t slots = static_cast<int64_t>(c.slots) * (d.compute_units > 0 ? d.compute_units : 256);
+  const int64_t cus = d.compute_units > 0 ? d.compute_units : 256;
+  const int64_t slots = c.slots * cus;
   int64_t longest = 1, all = 0, unique = 0;
   int64_t num_tiles = 0;
   for (int32_t i = 0; i < d.num_seqs; ++i) {
@@ -345,8 +347,10 @@ int32_t choose_split(const Trees& t, const PaTreeDims& d) {
       runs = cut.runs > runs ? cut.runs : runs;
     }
     const double units = static_cast<double>(items * heads);
-    double chain = run * c.stage;
-    double bytes = unique * heads * c.bytes / slots + 0.2 * run * c.bytes;
+    // (no more units than CUs: workgroups of four waves, tree_attention.hip)
+    const bool four = c.slots > 1 && units <= static_cast<double>(cus);
+    double chain = run * c.stage * (four ? 0.4 : 1.0) + (four ? 1.2 : 0.0);
+    double bytes = unique * heads * c.bytes / slots + 0.2 * run * c.bytes * (four ? 0.4 : 1.0);
     if (units > slots) {
       chain = (units * c.unit + all * heads * c.stage) / slots + 0.5 * chain;
       bytes += units * c.unit / slots;

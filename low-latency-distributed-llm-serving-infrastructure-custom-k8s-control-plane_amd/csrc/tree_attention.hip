@@ -5,10 +5,10 @@
 // stages of one tile of a sequence's nodes, and its record holds all that a unit
 // has to know of its sequence.  The tile has 64 query rows, node after node, the
 // query heads of the KV head (or sub-group) side by side: two blocks of 32, of which
-// a small tree fills one.  Wave w takes tiles w, w + 2, ... of 32 context tokens of
-// the run for all rows, with flash-style online softmax in fp32, and keeps its own K
-// and V in its own part of LDS, two tiles deep: no wave waits for another until they
-// are joined at the end.
+// a small tree fills one.  A workgroup has two or four waves (kWaves); wave w takes
+// tiles w, w + kWaves, ... of 32 context tokens of the run for all rows, with
+// flash-style online softmax in fp32, and keeps its own K and V in its own part of
+// LDS, two tiles deep: no wave waits for another until they are joined at the end.
 //   S^T[kv][row] = sum_d K[kv][d] Q[row][d]
 //   O^T[d][row] += sum_kv V^T[d][kv] P^T[kv][row]     (v_mfma_f32_32x32x16)
 // with the layouts, the swizzled LDS rows, the direct global -> LDS copies, the
@@ -18,12 +18,12 @@
 //
 // What bounds it is the cache's bytes, read once for a tile's rows (32 trees of 9-17
 // nodes after 100-8000 tokens, 32/8 heads of 128: 108 us and 9 for the join, 5.0 TB/s;
-// 8 of 64 nodes after 1000-4000, 32/32 heads: 67 and 5.5, 5.1 TB/s); for trees whose
-// tiles share a short context the one wave a SIMD, whose products and softmax follow
-// each other (2 of 40-60 nodes under a window of 8192: 35 and 5.5 us, 310 TFLOP/s); for
+// 8 of 64 nodes after 1000-4000, 32/32 heads: 70 us, 4.9 TB/s); for trees whose tiles
+// share a short context the one wave a SIMD, whose products and softmax follow each
+// other (2 of 40-60 nodes under a window of 8192: 34 and 5 us, 330 TFLOP/s); for
 // short runs the chain of round trips at a unit's start (record; block ids, query and
-// masks; K and V: one of 26 nodes after 3000, 16 and 4 us).  The causal prefill's tiles,
-// shared by eight waves, took 145, 95, and 28 us where this now takes 118, 73 and 19.6.
+// masks; K and V: one of 26 nodes after 3000, 14 and 4 us).  The causal prefill's tiles,
+// shared by eight waves, took 145, 95, and 28 us where this now takes 118, 73 and 18.
 // V's operands read behind the softmax, and the accumulators copied out of the matrix
 // registers at each tile: 133, 91 and 21 us.
 //
@@ -40,17 +40,16 @@ namespace pa {
 
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kWaves = kThreads / kWave;
 constexpr int kRows = kTreeRows;
 constexpr int kSlots = 2;  // tiles of K and of V a wave holds
 
 // D: the head dim of the LDS rows and MFMA tiles, DM in memory (80 and 96 run on
 // rows of 128 whose pieces past DM are zero).
-template <typename T, int D, int DM>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D > 64 ? 1 : 2))) void
+template <typename T, int D, int DM, int kWaves>
+__global__ __launch_bounds__(kWaves * kWave) __attribute__((amdgpu_waves_per_eu(D > 64 ? 1 : 2))) void
 tree_attention_kernel(PrefillArgs a) {
   static_assert(Elem<T>::kBytes == 2, "16-bit caches (bf16 or fp16)");
+  constexpr int kThreads = kWaves * kWave;
   constexpr bool MASKD = DM < D;
   constexpr int KS = D / 16;       // QK k-steps
   constexpr int DB = D / 32;       // output d blocks
@@ -416,16 +415,30 @@ tree_attention_kernel(PrefillArgs a) {
     attend(std::integral_constant<int, 2>());
 }
 
+// No more units than CUs: four waves each, which halve a unit's chain where a second
+// workgroup would not share its CU (us, four and two waves: one tree of 26 nodes after
+// 3000, 32/8 heads of 128, 24 items 17.8 and 20.1, 4 items 29.7 and 48.3; 8 trees of 64,
+// 32/32 heads, 8 items 71 and 104).  More units: two, of which a CU holds two or three (2
+// trees under a window of 8192, 54 items 48.8 and 41.4; 64 trees of 9-17 nodes, 9/3 heads
+// of 64, 251 items 52 and 41).
+template <typename T, int D, int DM>
+hipError_t launch_d(const PrefillArgs& a, dim3 grid, hipStream_t s) {
+  if (static_cast<int>(grid.x) <= device_compute_units())
+    hipLaunchKernelGGL((tree_attention_kernel<T, D, DM, 4>), grid, dim3(4 * kWave), 0, s, a);
+  else
+    hipLaunchKernelGGL((tree_attention_kernel<T, D, DM, 2>), grid, dim3(2 * kWave), 0, s, a);
+  return hipGetLastError();
+}
+
 template <typename T>
 hipError_t launch_t(const PrefillArgs& a, int head_dim, dim3 grid, hipStream_t s) {
   switch (head_dim) {
-    case 64: hipLaunchKernelGGL((tree_attention_kernel<T, 64, 64>), grid, dim3(kThreads), 0, s, a); break;
-    case 80: hipLaunchKernelGGL((tree_attention_kernel<T, 128, 80>), grid, dim3(kThreads), 0, s, a); break;
-    case 96: hipLaunchKernelGGL((tree_attention_kernel<T, 128, 96>), grid, dim3(kThreads), 0, s, a); break;
-    case 128: hipLaunchKernelGGL((tree_attention_kernel<T, 128, 128>), grid, dim3(kThreads), 0, s, a); break;
+    case 64: return launch_d<T, 64, 64>(a, grid, s);
+    case 80: return launch_d<T, 128, 80>(a, grid, s);
+    case 96: return launch_d<T, 128, 96>(a, grid, s);
+    case 128: return launch_d<T, 128, 128>(a, grid, s);
     default: return hipErrorNotSupported;
   }
-  return hipGetLastError();
 }
 
 }  // namespace

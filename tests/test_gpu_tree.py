@@ -66,6 +66,18 @@ def test_other_steps(device, starts, counts, heads, kv_heads, dim, dtype):
     case.check(ops.tree_attention(q, k, v, 1, step, tree, case.scaling))
 
 
+@pytest.mark.parametrize("window,sinks", [(None, 0), (150, 5)])
+@pytest.mark.parametrize("dim,dtype", [(64, FP16), (80, BF16), (96, FP16), (128, BF16), (256, BF16)])
+def test_more_units_than_compute_units(device, dim, dtype, window, sinks):
+    counts = [1 + (37 * i) % 90 for i in range(20)]
+    case = Case([13 * i * i for i in range(20)], counts, 32, 16, dim, dtype, parents=trees(counts), window=window,
+                sinks=sinks, seed=dim)
+    q, k, v, _, step = case.place(device)
+    tree = ops.pack_tree(step, flat(case.parents).to(device), window=window, sinks=sinks)
+    assert tree._plan.num_items * 16 > 256
+    case.check(ops.tree_attention(q, k, v, 1, step, tree, case.scaling))
+
+
 def test_a_chain_is_causal_attention_and_roots_see_the_context_alone(device):
     starts, counts = [300, 20], [50, 9]
     chain = [list(range(-1, n - 1)) for n in counts]
