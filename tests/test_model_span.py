@@ -21,13 +21,14 @@ BLOCK_SIZE = 16
 
 
 def tiny_model(kind, device, dtype=torch.float32, window=None, layers=2, heads=8, kv_heads=2, head_dim=64):
-    config = {"llama": transformers.LlamaConfig, "mistral": transformers.MistralConfig}[kind]
-    extra = {"sliding_window": window} if kind == "mistral" else {}
+    config = {"llama": transformers.LlamaConfig, "qwen2": transformers.Qwen2Config}[kind]
+    extra = {"sliding_window": window, "use_sliding_window": True,
+             "layer_types": ["sliding_attention"] * layers} if kind == "qwen2" else {"head_dim": head_dim}
     cfg = config(vocab_size=256, hidden_size=heads * head_dim, intermediate_size=256, num_hidden_layers=layers,
-                 num_attention_heads=heads, num_key_value_heads=kv_heads, head_dim=head_dim,
+                 num_attention_heads=heads, num_key_value_heads=kv_heads,
                  max_position_embeddings=2048, initializer_range=0.08, **extra)
     torch.manual_seed(0)
-    cls = {"llama": transformers.LlamaForCausalLM, "mistral": transformers.MistralForCausalLM}[kind]
+    cls = {"llama": transformers.LlamaForCausalLM, "qwen2": transformers.Qwen2ForCausalLM}[kind]
     model = cls(cfg).to(device=device, dtype=dtype)
     return model.eval()
 
@@ -103,16 +104,16 @@ def check_windows(device, kind, layer_window, window, sinks, tol):
     assert worst <= tol, worst
 
 
-@pytest.mark.parametrize("kind,layer_window,window,sinks", [("mistral", 24, None, 0), ("llama", None, 17, 5),
-                                                           ("mistral", 40, 64, 3)])
+@pytest.mark.parametrize("kind,layer_window,window,sinks", [("qwen2", 24, None, 0), ("llama", None, 17, 5),
+                                                           ("qwen2", 40, 64, 3)])
 def test_cpu_windows_match_the_models_forward(monkeypatch, kind, layer_window, window, sinks):
     monkeypatch.setattr(paged_attention, "_BACKEND", None)
     check_windows("cpu", kind, layer_window, window, sinks, 1e-3)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("kind,layer_window,window,sinks", [("mistral", 24, None, 0), ("llama", None, 17, 5),
-                                                           ("mistral", 40, 64, 3), ("mistral", 4096, None, 0)])
+@pytest.mark.parametrize("kind,layer_window,window,sinks", [("qwen2", 24, None, 0), ("llama", None, 17, 5),
+                                                           ("qwen2", 40, 64, 3), ("qwen2", 4096, None, 0)])
 def test_gpu_windows_match_the_models_forward(device, kind, layer_window, window, sinks):
     check_windows("cuda", kind, layer_window, window, sinks, 2e-3)
 
