@@ -1711,6 +1711,12 @@ def _window_step(step: PackedStep, window: int, sinks: int, num_kv_heads: int, n
     return sub
 
 
+def _output_shape(query, q):
+    """Shape of the output for ``query`` checked as ``q``; None: like the query (whose
+    empty_like takes 1.3 us, a new_empty of a shape 2.2)."""
+    return None if query.shape == q.shape and query.is_contiguous() else tuple(q.shape)
+
+
 def _attention_window(query, key_cache, value_cache, layer_idx, step, scaling, out, new_key, new_value, key_scales,
                       value_scales, window, sinks) -> torch.Tensor:
     """:func:`attention` under a window as one library call; checks and shared
@@ -1745,13 +1751,14 @@ def _attention_window(query, key_cache, value_cache, layer_idx, step, scaling, o
                 setattr(call, name, getattr(lists, name))
             call.dims.partition_size = sub.partition_size
         # (the steps' workspaces of other head counts stay alive with the call)
-        cached = (ctypes.byref(call), _native.PaWindow(*limits), tuple(q.shape), strides, step._extra_ws, sub._extra_ws)
+        cached = (ctypes.byref(call), _native.PaWindow(*limits), _output_shape(query, q), strides, step._extra_ws,
+                  sub._extra_ws)
         if len(calls) >= 64:
             calls.clear()
         calls[key] = cached
     call_ref, limits, shape, strides, _, _ = cached
     if out is None:
-        rows_out = query.new_empty(shape)
+        rows_out = torch.empty_like(query) if shape is None else query.new_empty(shape)
     else:
         rows_out = _output_for(_query_view(query), key_cache, out)
     if step.num_decode_items == 0 and step.num_prefill_items == 0:
@@ -1974,11 +1981,11 @@ def tree_attention(
             positions=tree.position_ids.data_ptr(), items=tree._items, merge_items=tree._merge_items,
             workspace=tree._workspace, workspace_bytes=tree._workspace_bytes, plan=tree._plan,
             window=_native.PaWindow(tree.window, tree.sinks))
-        cached = (key, ctypes.byref(call), tuple(q.shape), strides)
+        cached = (key, ctypes.byref(call), _output_shape(query, q), strides)
         tree.__dict__["_layer_call"] = cached
     _, call_ref, shape, strides = cached
     if out is None:
-        rows_out = query.new_empty(shape)
+        rows_out = torch.empty_like(query) if shape is None else query.new_empty(shape)
     else:
         rows_out = _output_for(_query_view(query), key_cache, out)
     rows = None
