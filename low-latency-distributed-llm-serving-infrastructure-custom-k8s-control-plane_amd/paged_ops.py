@@ -1700,10 +1700,21 @@ def _window_step(step: PackedStep, window: int, sinks: int, num_kv_heads: int, n
         partition = int(_plan(shorter, counts, step.block_size, step.prefill_tile, given, num_kv_heads, num_query_heads,
                               per_item, per_cu, _compute_units(device), None,
                               cache_dtype_code(cache_dtype) if per_cu else -1, head_dim).partition_size)
-        longest = int((shorter + 1)[counts == 1].max())
+        contexts = (shorter + 1)[counts == 1]
+        longest = int(contexts.max())
         if longest > partition and not given:
-            # (as many partitions of one size: the windows' length is no power of two)
-            partition = (-(-longest // -(-longest // partition)) + 31) // 32 * 32
+            # As many partitions of one size, since the windows' length is no power of two
+            # (8 sequences, window 2048, 32/8 heads of 128: 416 tokens 19.7 us, 512 20.7; 256
+            # of 32-32768, window 4096: 2080 298 us, 4096 319).  But for a launch that gives
+            # every CU one whole partition, beside short rests: there the even ones would be
+            # more than the CUs (16 sequences, window 4096: 832 60.7 us, 1024 51.5; window
+            # 1024: 224 19.5, 256 17.5).
+            even = (-(-longest // -(-longest // partition)) + 31) // 32 * 32
+            cus = _compute_units(device)
+            whole, raw, evened = (per_item * int(n.sum()) for n in (
+                contexts // partition, -(-contexts // partition), -(-contexts // even)))
+            if evened <= cus or whole > cus or raw > 2 * cus:
+                partition = even
         sub = pack_step(step._source_table, shorter, counts, step.block_size, prefill_tile=step.prefill_tile,
                         partition_size=partition, num_kv_heads=num_kv_heads,
                         num_query_heads=num_query_heads, head_dim=head_dim, dtype=cache_dtype, rows=rows)
