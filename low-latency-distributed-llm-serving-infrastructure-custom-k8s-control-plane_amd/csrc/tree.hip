@@ -164,7 +164,9 @@ __global__ __launch_bounds__(kTreeThreads) void pack_tree_kernel(PackTreeArgs a)
 // the loads of a batch go out together and a node's heads spread over workgroups
 // (26 nodes of 32 heads of 128 in 16 runs: 3.9 us; one workgroup a node, eight partials
 // a trip: 13.2).  Up to four runs go in a batch of four (8 trees of 64 nodes, 32 heads
-// of 128, two runs each: 5.4 us; sixteen slots, most of them the last run again: 9.2).
+// of 128, two runs each: 5.4 us; sixteen slots, most of them the last run again: 9.2),
+// up to eight in one of eight (2 trees of 40-60 nodes in 5 runs, with their attention:
+// 37.0 us, in sixteen slots 38.2).
 constexpr int kMergeRuns = 16;
 constexpr int kFewRuns = 4;
 template <typename T, int D>
@@ -216,6 +218,7 @@ __global__ __launch_bounds__(kTreeThreads) void merge_tree_kernel(MergeTreeArgs 
     }
   };
   if (item.z <= kFewRuns) join(std::integral_constant<int, kFewRuns>());
+  else if (item.z <= 2 * kFewRuns) join(std::integral_constant<int, 2 * kFewRuns>());
   else join(std::integral_constant<int, kMergeRuns>());
   // (a sum of zero is a row that attends nothing, whose result is zero; a NaN stays)
   T* out = reinterpret_cast<T*>(a.output) + (first + t0 + tok) * hq * D + static_cast<int64_t>(r) * 4;

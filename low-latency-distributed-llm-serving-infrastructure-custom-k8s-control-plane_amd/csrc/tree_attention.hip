@@ -17,7 +17,7 @@
 // depend on each other.
 //
 // What bounds it is the cache's bytes, read once for a tile's rows (32 trees of 9-17
-// nodes after 100-8000 tokens, 32/8 heads of 128: 108 us and 9 for the join, 5.0 TB/s;
+// nodes after 100-8000 tokens, 32/8 heads of 128: 108 us and 7.5 for the join, 5.0 TB/s;
 // 8 of 64 nodes after 1000-4000, 32/32 heads: 70 us, 4.9 TB/s); for trees whose tiles
 // share a short context the one wave a SIMD, whose products and softmax follow each
 // other (2 of 40-60 nodes under a window of 8192: 34 and 5 us, 330 TFLOP/s); for
