@@ -124,6 +124,25 @@ __device__ __forceinline__ void hide(f32x16& s, uint32_t seen) {
   }
 }
 
+// Eight of a lane's probabilities (half c of its 16) as the product's operand, in two
+// terms of the type: themselves rounded, and what the rounding left, so that a weight is
+// off by 2^-16 (bf16) of itself at most.  Their sums, of both terms, go to sum0 and sum1.
+template <typename T>
+__device__ __forceinline__ void split_weights(const f32x16& s, int c, uint4& term, uint4& rest, float& sum0,
+                                              float& sum1) {
+  constexpr uint32_t kOnes = Elem<T>::kDtype == PA_DTYPE_BF16 ? 0x3F803F80u : 0x3C003C00u;
+  auto split = [&](int i, uint32_t& w, uint32_t& r, float& sum) {
+    const float x = s[8 * c + i], y = s[8 * c + i + 1];
+    w = pack_half2<T>(x, y);
+    r = pack_half2<T>(x - half_lo<T>(w), y - half_hi<T>(w));
+    sum = dot2_half<T>(r, kOnes, dot2_half<T>(w, kOnes, sum));
+  };
+  split(0, term.x, rest.x, sum0);
+  split(2, term.y, rest.y, sum1);
+  split(4, term.z, rest.z, sum0);
+  split(6, term.w, rest.w, sum1);
+}
+
 constexpr float kLazyRescale = 8.f;  // log2 headroom before a row maximum moves
 
 }  // namespace pa

@@ -44,6 +44,9 @@ constexpr int kIdAhead = 8;      // stages between an id slot's copy and the sta
 template <typename T, int D, int DM, bool LANE_IDS, bool APPEND, bool CODES = false, int SPAN = kSpanAll>
 __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a) {
   constexpr bool TREE = SPAN == kSpanTree;
+  // Terms of a probability in the product with V: a tree's nodes answer as the decode of
+  // their tokens would (prefill_tree.hip), prompts take one (prefill.hip).
+  constexpr int TERMS = TREE ? 2 : 1;
   constexpr int kItemInts = TREE ? kTreeItemInts : 2;
   static_assert(SPAN == kSpanAll || !APPEND, "their rows are written before");
   static_assert(Elem<T>::kBytes == 2, "16-bit rows (bf16 or fp16)");
@@ -797,6 +800,7 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
         for (int i = 0; i < 16; ++i) sn[i] = 0.f;
         uint4 va[2][DB];
         uint4 pb[2];
+        [[maybe_unused]] uint4 rest[2];
         float rsum0 = 0.f, rsum1 = 0.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -804,17 +808,21 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
 #pragma unroll
           for (int j = ks * kPerQk; j < (ks + 1) * kPerQk; ++j) s_cur[j] = fast_exp2(fmaf(s_cur[j], scale, -msc));
 #pragma unroll
-          for (int r = ks * (kVReads / KS); r < (ks + 1) * (kVReads / KS); ++r) read_vt(slot, r, va);
+          for (int r = ks * (kVReads / TERMS / KS); r < (ks + 1) * (kVReads / TERMS / KS); ++r) read_vt(slot, r, va);
           if (((ks + 1) * kPerQk) % 8 == 0) {
             const int c = (ks + 1) * kPerQk / 8 - 1;
-            pb[c].x = pack_half2<T>(s_cur[8 * c + 0], s_cur[8 * c + 1]);
-            pb[c].y = pack_half2<T>(s_cur[8 * c + 2], s_cur[8 * c + 3]);
-            pb[c].z = pack_half2<T>(s_cur[8 * c + 4], s_cur[8 * c + 5]);
-            pb[c].w = pack_half2<T>(s_cur[8 * c + 6], s_cur[8 * c + 7]);
-            rsum0 = dot2_half<T>(pb[c].x, kOnes, rsum0);
-            rsum1 = dot2_half<T>(pb[c].y, kOnes, rsum1);
-            rsum0 = dot2_half<T>(pb[c].z, kOnes, rsum0);
-            rsum1 = dot2_half<T>(pb[c].w, kOnes, rsum1);
+            if constexpr (TERMS == 2) {
+              split_weights<T>(s_cur, c, pb[c], rest[c], rsum0, rsum1);
+            } else {
+              pb[c].x = pack_half2<T>(s_cur[8 * c + 0], s_cur[8 * c + 1]);
+              pb[c].y = pack_half2<T>(s_cur[8 * c + 2], s_cur[8 * c + 3]);
+              pb[c].z = pack_half2<T>(s_cur[8 * c + 4], s_cur[8 * c + 5]);
+              pb[c].w = pack_half2<T>(s_cur[8 * c + 6], s_cur[8 * c + 7]);
+              rsum0 = dot2_half<T>(pb[c].x, kOnes, rsum0);
+              rsum1 = dot2_half<T>(pb[c].y, kOnes, rsum1);
+              rsum0 = dot2_half<T>(pb[c].z, kOnes, rsum0);
+              rsum1 = dot2_half<T>(pb[c].w, kOnes, rsum1);
+            }
           }
         }
         // (8-bit rows: the conversions ahead of A leave the scheduler one region
@@ -824,9 +832,18 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
         if constexpr (CODES) __builtin_amdgcn_sched_barrier(0);
         // ---- B: O^T += V^T P^T | row maxima of S_next | K reads of stage st+2
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+        for (int kk = 0; kk < 2; ++kk) {
+          if (TERMS == 2 && kk == 1) {  // (not ahead with the others: registers)
+#pragma unroll
+            for (int r = kVReads / 2; r < kVReads; ++r) read_vt(slot, r, va);
+          }
 #pragma unroll
           for (int db = 0; db < DB; ++db) acc[db] = mfma32<T>(va[kk][db], pb[kk], acc[db]);
+          if constexpr (TERMS == 2) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[db] = mfma32<T>(va[kk][db], rest[kk], acc[db]);
+          }
+        }
         read_k((slot + 2) & (kKBufs - 1), ka);
         prefetch_ids(st + 1);
         if constexpr (MASKED) mask_tile(2 * (st + 1) + kh, sn);
@@ -835,13 +852,13 @@ __global__ __launch_bounds__(kPrefillThreads) void prefill_kernel(PrefillArgs a)
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kVReads / KS, 0);
-          __builtin_amdgcn_sched_group_barrier(kSchedValu, 6 * 8 / KS, 0);
+          __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kVReads / TERMS / KS, 0);
+          __builtin_amdgcn_sched_group_barrier(kSchedValu, (TERMS == 2 ? 10 : 6) * 8 / KS, 0);
         }
 #pragma unroll
         for (int i = 0; i < 2 * DB; ++i) {
-          __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(kSchedDsRead, (KS + 2) / (2 * DB), 0);
+          __builtin_amdgcn_sched_group_barrier(kSchedMfma, TERMS, 0);
+          __builtin_amdgcn_sched_group_barrier(kSchedDsRead, (KS + 2 + (TERMS == 2 ? kVReads / 2 : 0)) / (2 * DB), 0);
           __builtin_amdgcn_sched_group_barrier(kSchedValu, 2, 0);
         }
         if (MASKED && bad_ids) {

@@ -8,11 +8,14 @@
 // [32 w, 32 w + 32), and the context goes by in steps of 32 tokens.  (Waves without
 // a live row only copy.)  The rings have four slots each of K and V, filled three
 // steps ahead: K of step st+5 goes out in step st, when K of st+1 is in registers
-// already, and V of st+3.  Items, masks and partial results as there.
+// already, and V of st+3.  Items, masks, partial results and a probability's two terms
+// as there.
 //
-// 16 trees of 9-17 nodes after 100-6000 tokens, 16/4 heads: 58 us, 3.5 TB/s (a unit's
+// 16 trees of 9-17 nodes after 100-6000 tokens, 16/4 heads: 60 us, 3.4 TB/s (a unit's
 // start, its steps' chain between barriers, and the join); 66 us while the compiler
-// moved the accumulators at each step and waited for the query in the loop.
+// moved the accumulators at each step and waited for the query in the loop.  With a
+// probability in one term 55-56 us, off 64 bits by 2.2e-3 (2-norm) where two terms are
+// by 1.65e-3.
 #include <type_traits>
 
 #include "tree_common.hpp"
@@ -254,7 +257,6 @@ __global__ __launch_bounds__(kThreads) void tree_attention256_kernel(PrefillArgs
     stage_barrier();
     if (ntiles > 4) copy_k(4, 0);
   }
-  constexpr uint32_t kOnes = Elem<T>::kDtype == PA_DTYPE_BF16 ? 0x3F803F80u : 0x3C003C00u;
 
   auto step = [&](int st, f32x16& s_cur, f32x16& s_nxt, auto masked, auto slot_c) {
     constexpr bool MASKED = decltype(masked)::value;
@@ -268,7 +270,7 @@ __global__ __launch_bounds__(kThreads) void tree_attention256_kernel(PrefillArgs
       f32x16 sn;
 #pragma unroll
       for (int i = 0; i < 16; ++i) sn[i] = 0.f;
-      uint4 pb[2];
+      uint4 pb[2], rest[2];
       float rsum0 = 0.f, rsum1 = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -277,21 +279,18 @@ __global__ __launch_bounds__(kThreads) void tree_attention256_kernel(PrefillArgs
         for (int j = ks * kPerQk; j < (ks + 1) * kPerQk; ++j) s_cur[j] = fast_exp2(fmaf(s_cur[j], scale, -msc));
         if (((ks + 1) * kPerQk) % 8 == 0) {
           const int c = (ks + 1) * kPerQk / 8 - 1;
-          pb[c].x = pack_half2<T>(s_cur[8 * c + 0], s_cur[8 * c + 1]);
-          pb[c].y = pack_half2<T>(s_cur[8 * c + 2], s_cur[8 * c + 3]);
-          pb[c].z = pack_half2<T>(s_cur[8 * c + 4], s_cur[8 * c + 5]);
-          pb[c].w = pack_half2<T>(s_cur[8 * c + 6], s_cur[8 * c + 7]);
-          rsum0 = dot2_half<T>(pb[c].x, kOnes, rsum0);
-          rsum1 = dot2_half<T>(pb[c].y, kOnes, rsum1);
-          rsum0 = dot2_half<T>(pb[c].z, kOnes, rsum0);
-          rsum1 = dot2_half<T>(pb[c].w, kOnes, rsum1);
+          split_weights<T>(s_cur, c, pb[c], rest[c], rsum0, rsum1);
         }
       }
       // ---- B: O^T += V^T P^T | row maxima of S_next | K reads of step st+2
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) acc[db] = mfma32<T>(read_vt(SLOT, kk, db), pb[kk], acc[db]);
+        for (int kk = 0; kk < 2; ++kk) {
+          const uint4 v = read_vt(SLOT, kk, db);
+          acc[db] = mfma32<T>(v, pb[kk], acc[db]);
+          acc[db] = mfma32<T>(v, rest[kk], acc[db]);
+        }
       read_k((SLOT + 2) & (kBufs - 1), ka);
       if constexpr (MASKED) mask_tile(st + 1, sn);
       l += rsum0 + rsum1;
@@ -299,12 +298,12 @@ __global__ __launch_bounds__(kThreads) void tree_attention256_kernel(PrefillArgs
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(kSchedValu, 6 * 8 / KS, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedValu, 10 * 8 / KS, 0);
       }
 #pragma unroll
       for (int i = 0; i < 2 * DB; ++i) {
         __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 2, 0);
         __builtin_amdgcn_sched_group_barrier(kSchedDsRead, (KS + 2 * DB - 1) / (2 * DB), 0);
         __builtin_amdgcn_sched_group_barrier(kSchedValu, 2, 0);
       }
