@@ -278,6 +278,7 @@ class PackedStep:
         self._windows = {}  # decode work lists of layers with a window (see _window_step)
         self._packs = 0  # repacks so far
         self._partition_given = False
+        self._lists_only = False  # another step's lists of a window (see _window_step)
 
     # -- addresses and views ---------------------------------------------------
     def ptr(self, name: str) -> int:
@@ -651,7 +652,7 @@ def _run_pack(step: PackedStep, with_gather: bool = False, updates: Optional[np.
     if staging is not None:
         staging.done(slot, device, stream)
     _native.check(status, "pa_pack")
-    if fresh and pooled:
+    if fresh and pooled and not step._lists_only:  # (a step's lists of a window are no later step)
         table._pa_pack_generation = _pack_generation(table) + 1
         step._generation = table._pa_pack_generation
     return gather
@@ -674,6 +675,7 @@ def pack_step(
     updates: Optional[np.ndarray] = None,
     allocated_tokens=None,
     step_table: bool = False,
+    _lists_only: bool = False,
 ) -> PackedStep:
     """Plan a step on the host, upload its description once, and run the GPU
     packing kernels.
@@ -763,6 +765,7 @@ def pack_step(
                       head_shape, (starts, counts, rows_arr))
     step._merge_state_bytes = state_bytes  # cleared by every pa_pack of the step
     step._partition_given = partition_size is not None
+    step._lists_only = _lists_only
     step._heads = (int(num_kv_heads), hq, None if head_dim is None else int(head_dim), dtype)
     upd = None if not n_upd else np.ascontiguousarray(updates, dtype=np.int32)
     gather = _run_pack(step, with_gather=with_gather, updates=upd, fresh=True)
@@ -1717,7 +1720,8 @@ def _window_step(step: PackedStep, window: int, sinks: int, num_kv_heads: int, n
                 partition = even
         sub = pack_step(step._source_table, shorter, counts, step.block_size, prefill_tile=step.prefill_tile,
                         partition_size=partition, num_kv_heads=num_kv_heads,
-                        num_query_heads=num_query_heads, head_dim=head_dim, dtype=cache_dtype, rows=rows)
+                        num_query_heads=num_query_heads, head_dim=head_dim, dtype=cache_dtype, rows=rows,
+                        _lists_only=True)
     step._windows[key] = sub
     return sub
 

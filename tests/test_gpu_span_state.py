@@ -1,0 +1,63 @@
+"""What a step under a window, or of trees, keeps from one call to the next, and what a
+call leaves as it was."""
+
+import numpy as np
+import pytest
+import torch
+
+from helpers import pkg
+from span_oracle import CODE, Case, ancestors, random_tree
+from test_gpu_tree import plain_accept
+
+pytestmark = pytest.mark.gpu
+
+ops = pkg("paged_ops")
+manager_mod = pkg("memory.manager")
+request_mod = pkg("engine.request")
+paged_attention = pkg("model.paged_attention")
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def store_of(device, lengths, kv_heads=2, head_dim=64, query_heads=8, blocks=600):
+    m = manager_mod.PagedKVCacheManager(total_blocks=blocks, block_size=16, num_heads=kv_heads, head_dim=head_dim,
+                                        dtype=BF16, num_layers=1, device=device)
+    m.num_query_heads = query_heads
+    seqs = [request_mod.Request(i + 1, list(range(n))) for i, n in enumerate(lengths)]
+    for seq in seqs:
+        m.allocate_prefix_blocks(seq)
+    return m, seqs
+
+
+def slots_of(m, seqs, lengths):
+    out = []
+    for seq, n in zip(seqs, lengths):
+        blocks = np.asarray(seq.block_table.get_physical_blocks(), np.int64)
+        out.append(blocks[np.arange(n) // 16] * 16 + np.arange(n) % 16)
+    return np.concatenate(out)
+
+
+def attend(m, step, window, query_heads=8):
+    q = torch.randn((step.num_query_tokens, query_heads, m.head_dim), dtype=BF16, device=m.device)
+    return ops.attention(q, m.key_cache, m.value_cache, 0, step, 0.1, window=window, sinks=4)
+
+
+def test_gather_slots_are_there_after_a_windowed_call(device):
+    """The lists of a window are no later step on the pool: slots first read behind it
+    (and behind a repack with it) are the step's, and it makes no other step stale."""
+    lengths = [200, 330]
+    m, seqs = store_of(device, lengths)
+    want = slots_of(m, seqs, lengths)
+    context = paged_attention.PagedStepContext(m, seqs, [n - 1 for n in lengths], [1, 1])
+    attend(m, context.packed, 48)
+    assert len(context.packed._windows) == 1 and all(s is not context.packed for s in context.packed._windows.values())
+    assert np.array_equal(context.gather_slots.cpu().numpy(), want)
+    older = m.pack_step(seqs, [n - 1 for n in lengths], [1, 1])
+    newer = m.pack_step(seqs, [n - 1 for n in lengths], [1, 1])
+    attend(m, older, 48)
+    assert np.array_equal(newer.gather_slots.cpu().numpy(), want)
+    attend(m, newer, 48)
+    newer.repack([n - 2 for n in lengths], [1, 1])
+    assert np.array_equal(newer.gather_slots.cpu().numpy(), slots_of(m, seqs, [n - 1 for n in lengths]))
+    with pytest.raises(RuntimeError, match="earlier step"):
+        older.gather_slots
