@@ -275,7 +275,7 @@ class PackedStep:
         self._generation = 0  # the pool's pack count when this step was packed
         self._merge_state_bytes = 0  # merge records at the end of the decode workspace
         self._heads = None  # (H_kv, H_q, D, cache dtype) the step was packed for, as far as given
-        self._windows = {}  # decode work lists of layers with a window (see _window_step)
+        self._windows = {}  # decode work lists of layers with a window (see _window_step); None: this step's
         self._packs = 0  # repacks so far
         self._partition_given = False
         self._lists_only = False  # another step's lists of a window (see _window_step)
@@ -352,7 +352,7 @@ class PackedStep:
         if self.table_width and plan.max_blocks > self.table_width:
             raise ValueError("repack: a context grew past the step's block table")
         windows = [(sub, _window_starts(starts, counts, self.block_size, key[0], key[1]))
-                   for key, sub in self._windows.items() if sub is not self]
+                   for key, sub in self._windows.items() if sub is not None]
         for sub, shorter in windows:
             p = _plan(shorter, counts, self.block_size, self.prefill_tile, sub.partition_size, 1, 1, 1, 1, 1)
             if (p.num_decode_items, p.num_merge_items) != (sub.num_decode_items, sub.num_merge_items):
@@ -375,7 +375,7 @@ class PackedStep:
         replays."""
         _run_pack(self)
         for sub in self._windows.values():
-            if sub is not self:
+            if sub is not None:
                 _run_pack(sub)
 
     @property
@@ -1685,13 +1685,12 @@ def _window_step(step: PackedStep, window: int, sinks: int, num_kv_heads: int, n
     lists stay while contexts grow.  ``step`` itself where no context is shorter
     (its lists serve shorter contexts as well)."""
     key = (window, sinks, num_kv_heads, num_query_heads, head_dim, cache_dtype)
-    sub = step._windows.get(key)
-    if sub is not None:
-        return sub
+    if key in step._windows:
+        return step._windows[key] or step
     starts, counts, rows = step._inputs
     shorter = _window_starts(starts, counts, step.block_size, window, sinks)
     if step.num_decode_items == 0 or bool((shorter == starts).all()):
-        sub = step
+        sub = None  # (the step itself here would keep it alive until the garbage collector ran)
     else:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the first attention of a step under a window packs its work lists, which a graph "
@@ -1723,7 +1722,7 @@ def _window_step(step: PackedStep, window: int, sinks: int, num_kv_heads: int, n
                         num_query_heads=num_query_heads, head_dim=head_dim, dtype=cache_dtype, rows=rows,
                         _lists_only=True)
     step._windows[key] = sub
-    return sub
+    return sub or step
 
 
 def _output_shape(query, q):

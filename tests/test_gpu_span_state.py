@@ -1,6 +1,9 @@
 """What a step under a window, or of trees, keeps from one call to the next, and what a
 call leaves as it was."""
 
+import gc
+import weakref
+
 import numpy as np
 import pytest
 import torch
@@ -50,7 +53,7 @@ def test_gather_slots_are_there_after_a_windowed_call(device):
     want = slots_of(m, seqs, lengths)
     context = paged_attention.PagedStepContext(m, seqs, [n - 1 for n in lengths], [1, 1])
     attend(m, context.packed, 48)
-    assert len(context.packed._windows) == 1 and all(s is not context.packed for s in context.packed._windows.values())
+    assert [s is not None for s in context.packed._windows.values()] == [True]
     assert np.array_equal(context.gather_slots.cpu().numpy(), want)
     older = m.pack_step(seqs, [n - 1 for n in lengths], [1, 1])
     newer = m.pack_step(seqs, [n - 1 for n in lengths], [1, 1])
@@ -61,3 +64,19 @@ def test_gather_slots_are_there_after_a_windowed_call(device):
     assert np.array_equal(newer.gather_slots.cpu().numpy(), slots_of(m, seqs, [n - 1 for n in lengths]))
     with pytest.raises(RuntimeError, match="earlier step"):
         older.gather_slots
+
+
+@pytest.mark.parametrize("window", [48, 4096])
+def test_a_step_goes_with_its_last_reference(device, window):
+    """Under a window that its contexts reach past, and under one that they do not: its
+    device memory does not wait for the garbage collector."""
+    m, seqs = store_of(device, [200, 330])
+    step = m.pack_step(seqs, [199, 329], [1, 1])
+    attend(m, step, window)
+    gone = weakref.ref(step)
+    gc.disable()
+    try:
+        del step
+        assert gone() is None
+    finally:
+        gc.enable()
