@@ -497,6 +497,7 @@ namespace {
 
 // pa_decode_phases with the split-K partials in `workspace`, or, when
 // `use_scratch`, in this device's `scratch` array (workspace ignored).
+// check_only: every check, no launch.
 int decode_phases(const char* who, bool use_scratch, int32_t phases, const void* query,
                   const void* key_cache, const void* value_cache, int32_t layer_idx,
                   PaStepDims dims, const int32_t* block_tables, const int32_t* context_lens,
@@ -504,7 +505,7 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
                   int64_t num_decode_items, const int32_t* merge_items, int64_t num_merge_items,
                   float scaling, void* output, void* workspace, size_t workspace_bytes,
                   void* stream, const PaNewRows* new_rows = nullptr, const PaCacheScales* scales = nullptr,
-                  PaWindow window = {0, 0}) {
+                  PaWindow window = {0, 0}, bool check_only = false) {
   if (phases <= 0 || (phases & ~(PA_DECODE_PHASE_PARTITIONS | PA_DECODE_PHASE_MERGE)) != 0)
     return fail(PA_ERR_INVALID_ARGUMENT, "%s: phases must be a non-empty mask of "
                 "PA_DECODE_PHASE_PARTITIONS and PA_DECODE_PHASE_MERGE, got %d", who, phases);
@@ -584,6 +585,7 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
                     workspace_bytes);
       if (wl.state > 0) merge_state = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + wl.acc + wl.ml);
     }
+    if (check_only) return PA_OK;
     pa::DecodeArgs a{};
     a.query = query;
     a.q_token_stride = dims.q_token_stride;
@@ -635,7 +637,7 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
                 dims.head_dim, dims.dtype);
   // The generic kernel finishes every row in one pass: it is the partition
   // phase, and the merge phase has nothing to do.
-  if (!(phases & PA_DECODE_PHASE_PARTITIONS)) return PA_OK;
+  if (check_only || !(phases & PA_DECODE_PHASE_PARTITIONS)) return PA_OK;
   pa::GenericArgs a{};
   a.query = query;
   a.q_token_stride = dims.q_token_stride;
@@ -715,13 +717,14 @@ int pa_decode_no_alloc(const void* query, const void* key_cache, const void* val
 
 namespace {
 
-// pa_prefill, and with new_rows pa_prefill_append (the fast path only).
+// pa_prefill, and with new_rows pa_prefill_append (the fast path only).  check_only: every
+// check, no launch.
 int prefill_impl(const char* who, const void* query, const void* key_cache, const void* value_cache,
                  int32_t layer_idx, PaStepDims dims, const int32_t* block_tables,
                  const int32_t* context_lens, const int64_t* cu_seqlens, const int32_t* prefill_items,
                  int64_t num_prefill_items, int32_t prefill_tile, float scaling, void* output,
                  void* stream, const PaNewRows* new_rows, const PaCacheScales* scales = nullptr,
-                 PaWindow window = {0, 0}) {
+                 PaWindow window = {0, 0}, bool check_only = false) {
   int rc = check_step(dims, who);
   if (rc != PA_OK) return rc;
   if (layer_idx < 0 || layer_idx >= dims.num_layers)
@@ -763,6 +766,7 @@ int prefill_impl(const char* who, const void* query, const void* key_cache, cons
       return fail(PA_ERR_UNSUPPORTED, "%s: shape or alignment not taken by the fused write "
                   "(write the rows with pa_reshape_and_cache, then call pa_prefill)", who);
   }
+  if (check_only && (fast || pa::generic_supported(dims.dtype, dims.head_dim))) return PA_OK;
   if (fast) {
     pa::PrefillArgs a{};
     a.query = query;
@@ -1191,23 +1195,30 @@ int pa_attention_window(const PaStepCall* call, PaWindow window, const void* que
                        window);
     if (rc != PA_ERR_UNSUPPORTED) return rc;
   }
-  if (new_rows != nullptr) {
-    rc = write_rows(c.dims, *new_rows, key_cache, value_cache, key_scales, value_scales, c.scatter_slots, layer_idx,
-                    stream);
-    if (rc != PA_OK) return rc;
-  }
-  if (c.num_prefill_items > 0) {
-    rc = prefill_impl(who, query, key_cache, value_cache, layer_idx, c.dims, c.block_tables, c.context_lens,
-                      c.cu_seqlens, c.prefill_items, c.num_prefill_items, c.prefill_tile, scaling, output, stream,
-                      nullptr, sp, window);
-    if (rc != PA_OK) return rc;
-  }
-  if (c.num_decode_items > 0)
+  auto prompts = [&](bool check_only) {
+    if (c.num_prefill_items <= 0) return static_cast<int>(PA_OK);
+    return prefill_impl(who, query, key_cache, value_cache, layer_idx, c.dims, c.block_tables, c.context_lens,
+                        c.cu_seqlens, c.prefill_items, c.num_prefill_items, c.prefill_tile, scaling, output, stream,
+                        nullptr, sp, window, check_only);
+  };
+  auto decodes = [&](bool check_only) {
+    if (c.num_decode_items <= 0) return static_cast<int>(PA_OK);
     return decode_phases(who, false, phases, query, key_cache, value_cache, layer_idx, c.dims, c.block_tables,
                          c.context_lens, c.cu_seqlens, c.decode_items, c.num_decode_items, c.merge_items,
                          c.num_merge_items, scaling, output, c.workspace, c.workspace_bytes, stream, nullptr, sp,
-                         window);
-  return PA_OK;
+                         window, check_only);
+  };
+  if (new_rows != nullptr) {
+    // (behind every check, so that a refused call writes nothing)
+    rc = prompts(true);
+    if (rc == PA_OK) rc = decodes(true);
+    if (rc == PA_OK)
+      rc = write_rows(c.dims, *new_rows, key_cache, value_cache, key_scales, value_scales, c.scatter_slots, layer_idx,
+                      stream);
+    if (rc != PA_OK) return rc;
+  }
+  rc = prompts(false);
+  return rc == PA_OK ? decodes(false) : rc;
 }
 
 int pa_pack_tree(const int32_t* parents, const int32_t* context_lens, const int64_t* cu_seqlens,

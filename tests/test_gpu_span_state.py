@@ -80,3 +80,25 @@ def test_a_step_goes_with_its_last_reference(device, window):
         assert gone() is None
     finally:
         gc.enable()
+
+
+@pytest.mark.parametrize("starts,counts", [([40, 300, 700], [1, 33, 1]), ([40, 700], [1, 1])])
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype,cache_dtype", [
+    (8, 2, 128, BF16, BF16), (4, 2, 64, FP32, FP32), (8, 2, 128, BF16, CODE)])
+def test_a_refused_windowed_call_writes_no_rows(device, heads, kv_heads, dim, dtype, cache_dtype, starts, counts):
+    case = Case(starts, counts, heads, kv_heads, dim, dtype, cache_dtype, window=50, sinks=3)
+    q, k, v, scales, step = case.place(device)
+    rows = torch.full((sum(counts), kv_heads, dim), 300.0, dtype=dtype, device=device)
+
+    def call():
+        ops.attention(q, k, v, 1, step, case.scaling, new_key=rows, new_value=rows, window=50, sinks=3, **scales)
+
+    call()
+    for cached in step._window_calls.values():
+        cached[0]._obj.workspace_bytes = 8
+    rows.mul_(1.5)
+    was = [x.clone() for x in (k, v, *scales.values())]
+    with pytest.raises(RuntimeError, match="workspace of"):
+        call()
+    for x, y in zip(was, (k, v, *scales.values())):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
