@@ -806,7 +806,10 @@ typedef struct {
  * No counterpart in the reference, whose mask is causal alone.  One layer of a
  * packed step under a window (at least 1): pa_attention_step, or with scales
  * (of an 8-bit cache; NULL otherwise) pa_attention_step_8bit, over what the
- * window and the sinks leave; new_rows may be NULL.  Block-table entries of
+ * window and the sinks leave; new_rows may be NULL.  Of pa_attention_step's flags
+ * there are none: the decode launch of a step of single tokens writes their rows
+ * where it can, every other step's are written by pa_reshape_and_cache (_8bit)
+ * ahead of the attention.  A refused call writes nothing.  Block-table entries of
  * positions that no query of the step sees are not read, and neither are their
  * rows.
  *

@@ -1622,11 +1622,14 @@ def attention(
     sees is not read, and its table entries may be -1.  The first call of a step
     with a window packs the decode's work lists for it, which later layers and
     :meth:`PackedStep.rerun` reuse: make one before a graph is captured.  New rows
-    are written ahead of the attention on a step with prompts.
+    are written ahead of the attention on a step with prompts
+    (``fused_prefill_write=True`` is refused there).
     """
     if (new_key is None) != (new_value is None):
         raise ValueError("new_key and new_value are given together")
     if window is not None:
+        if fused_prefill_write and new_key is not None and step.num_prefill_items > 0:
+            raise ValueError("fused_prefill_write: under a window a step's prompts are written ahead of the attention")
         return _attention_window(query, key_cache, value_cache, layer_idx, step, scaling, out, new_key, new_value,
                                  key_scales, value_scales, window, sinks)
     if sinks:

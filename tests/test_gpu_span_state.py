@@ -102,3 +102,12 @@ def test_a_refused_windowed_call_writes_no_rows(device, heads, kv_heads, dim, dt
         call()
     for x, y in zip(was, (k, v, *scales.values())):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+def test_a_windowed_step_refuses_a_write_inside_the_prefill(device):
+    case = Case([40, 0], [1, 33], 8, 2, 128, BF16, window=50)
+    q, k, v, _, step = case.place(device)
+    rows = torch.zeros((34, 2, 128), dtype=BF16, device=device)
+    with pytest.raises(ValueError, match="fused_prefill_write"):
+        ops.attention(q, k, v, 1, step, 1.0, new_key=rows, new_value=rows, fused_prefill_write=True, window=50)
+    ops.attention(q, k, v, 1, step, 1.0, new_key=rows, new_value=rows, fused_prefill_write=False, window=50)
