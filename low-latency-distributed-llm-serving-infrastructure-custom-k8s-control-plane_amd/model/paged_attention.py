@@ -167,9 +167,11 @@ class PagedStepContext:
             raise RuntimeError("this step is not on a GPU store")
         tile = paged_ops.prefill_tile_for(num_query_heads, self.store.num_heads)
         if self.packed.prefill_tile != tile:
+            first = self.packed
             self.packed = self.store.pack_rows(self._rows, self._starts, self._counts,
-                                               num_query_heads=num_query_heads,
-                                               partition_size=self.packed.partition_size)
+                                               num_query_heads=num_query_heads, partition_size=first.partition_size)
+            # (the first one's choice, which is none of a caller's: windows choose their own)
+            self.packed._partition_given = first._partition_given
         return self.packed
 
     def window_of(self, sliding_window: Optional[int]) -> Optional[int]:

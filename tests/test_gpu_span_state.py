@@ -82,6 +82,25 @@ def test_a_step_goes_with_its_last_reference(device, window):
         gc.enable()
 
 
+def test_a_step_packed_again_for_its_heads_splits_a_window_as_a_new_one(device):
+    """A store that does not know its model's heads packs a step again for them, with
+    the partition that it had: which is none that a caller asked for."""
+    lengths = [6000, 5000, 7000]
+    m, seqs = store_of(device, lengths, query_heads=None, blocks=1200)
+    starts = [n - 1 for n in lengths]
+    context = paged_attention.PagedStepContext(m, seqs, starts, [1] * 3)
+    first = context.packed
+    step = context.packed_for(8)
+    assert step is not first and step.partition_size == first.partition_size
+    m.num_query_heads = 8
+    fresh = m.pack_step(seqs, starts, [1] * 3)
+    for window in (256, 1024, 3000):
+        got, want = (ops._window_step(s, window, 4, 2, 8, 64, BF16).partition_size for s in (step, fresh))
+        assert got == want
+    given = m.pack_rows(context._rows, context._starts, context._counts, num_query_heads=8, partition_size=512)
+    assert ops._window_step(given, 1024, 4, 2, 8, 64, BF16).partition_size == 512
+
+
 @pytest.mark.parametrize("starts,counts", [([40, 300, 700], [1, 33, 1]), ([40, 700], [1, 1])])
 @pytest.mark.parametrize("heads,kv_heads,dim,dtype,cache_dtype", [
     (8, 2, 128, BF16, BF16), (4, 2, 64, FP32, FP32), (8, 2, 128, BF16, CODE)])
