@@ -846,6 +846,7 @@ typedef struct {
     int32_t compute_units;    /* of the device (0: 256) */
     int32_t split_stages;     /* > 0: use it; 0: choose */
     PaWindow window;
+    int32_t *packed_parents;  /* pa_pack_tree: where to leave the parents it read */
 } PaTreeDims;
 
 typedef struct {
@@ -876,7 +877,9 @@ int pa_plan_tree(const int64_t *start_positions, const int64_t *node_counts,
  * node itself or an ancestor), positions int64 [T] (the start plus the node's
  * depth) and, for a plan with a tile, the attention's work lists: items int32
  * [num_items, 8], merge_items int32 [num_merge_items, 4] (16-byte aligned).
- * block_table_rows: as in PaStepDims of the attention.
+ * block_table_rows: as in PaStepDims of the attention.  dims.packed_parents (int32
+ * [T], or NULL) gets the parents that the masks are of, for pa_accept_tree:
+ * `parents` may then change before it runs.
  * Entries past a size in the plan are dropped, entries left over are marked.
  */
 int pa_pack_tree(const int32_t *parents, const int32_t *context_lens,

@@ -15,7 +15,7 @@ import threading
 from pathlib import Path
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libpaged_attention_amd.so"
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 PA_OK = 0
 PA_ERR_INVALID_ARGUMENT = 1
@@ -230,6 +230,7 @@ class PaTreeDims(ctypes.Structure):
         ("compute_units", ctypes.c_int32),
         ("split_stages", ctypes.c_int32),
         ("window", PaWindow),
+        ("packed_parents", ctypes.c_void_p),
     ]
 
 

@@ -150,7 +150,7 @@ int scratch_address(void** out, const char* who) {
 
 extern "C" {
 
-int pa_abi_version(void) { return 14; }
+int pa_abi_version(void) { return 15; }
 
 const char* pa_error_string(int code) {
   switch (code) {
@@ -1247,6 +1247,7 @@ int pa_pack_tree(const int32_t* parents, const int32_t* context_lens, const int6
   a.rows = block_table_rows;
   a.masks = masks;
   a.positions = positions;
+  a.packed_parents = dims.packed_parents;
   a.items = plan.tile > 0 ? reinterpret_cast<int4*>(items) : nullptr;
   a.merge_items = reinterpret_cast<int4*>(merge_items);
   a.max_items = plan.num_items;

@@ -297,6 +297,7 @@ struct PackTreeArgs {
   const int64_t* cu_seqlens;
   uint32_t* masks;              // [T, mask_words]
   int64_t* positions;           // [T]
+  int32_t* packed_parents;      // [T]: the parents that the masks are of, or null
   const int32_t* rows;          // row of the block table per sequence, or null (row = seq)
   int4* items;                  // kTreeItemInts each, or null
   int4* merge_items;            // (sequence, tile, splits, first partial row)

@@ -78,7 +78,11 @@ __global__ __launch_bounds__(kTreeThreads) void pack_tree_kernel(PackTreeArgs a)
   const int seq = blockIdx.x;
   const TreeSeq s = tree_seq(a.cu_seqlens, seq, a.num_query_tokens);
   const int start = a.context_lens[seq] - s.count;
-  for (int i = tid; i < s.count; i += kTreeThreads) s_parent[i] = parent_of(a.parents, s.first, i);
+  for (int i = tid; i < s.count; i += kTreeThreads) {
+    const int p = parent_of(a.parents, s.first, i);
+    s_parent[i] = p;
+    if (a.packed_parents != nullptr) a.packed_parents[s.first + i] = p;
+  }
   int64_t items = 0, merges = 0, rows = 0;
   if (a.items != nullptr) {
     for (int j = tid; j < seq; j += kTreeThreads) {

@@ -1801,8 +1801,9 @@ class TreeStep:
     ``masks`` int32 [T, words]: bit j % 32 of word j // 32 of a node's row is set
     where node j of its sequence is the node itself or one of its ancestors.
     ``position_ids`` int64 [T]: the sequence's start plus the node's depth.  The
-    masks, the attention's work lists and the workspace of its partial results are kept
-    in one buffer; calls that share a tree must not overlap in time.
+    masks, the parents that they are of (``parents`` is the caller's and may change),
+    the attention's work lists and the workspace of its partial results are kept in one
+    buffer; calls that share a tree must not overlap in time.
     """
 
     def __init__(self, step: PackedStep, parents: torch.Tensor, dims, plan, heads, limits, position_ids, buffer,
@@ -1814,7 +1815,9 @@ class TreeStep:
         self._dims, self._plan, self._heads = dims, plan, heads
         self._buffer = buffer
         base = buffer.data_ptr()
-        self._masks, self._items, self._merge_items, self._workspace = (base + at for at in offsets)
+        self._masks, self._packed_parents, self._items, self._merge_items, self._workspace = (
+            base + at for at in offsets)
+        dims.packed_parents = self._packed_parents
         self._workspace_bytes = workspace_bytes
         self._packs = -1
 
@@ -1837,7 +1840,8 @@ class TreeStep:
 
     def repack(self, parents=None) -> None:
         """Pack the trees anew after :meth:`PackedStep.repack`, or with other
-        ``parents``, every output at its address.  ValueError where the step now
+        ``parents`` (written into the tensor that the tree was packed from: trees that
+        share it read them at their own next run), every output at its address.  ValueError where the step now
         needs longer work lists than this tree has: pack a new one."""
         plan = _plan_tree(self.step, self._dims, self._plan.split_stages)
         had = self._plan
@@ -1920,15 +1924,16 @@ def pack_tree(
         _compute_units(device), 0, _native.PaWindow(*limits))
     plan = _plan_tree(step, dims, 0)
     parents = _parents(step, parents)
-    # masks | items | merge items | workspace
-    items = _align(4 * tokens * plan.mask_words)
+    # masks | parents | items | merge items | workspace
+    packed = _align(4 * tokens * plan.mask_words)
+    items = packed + _align(4 * tokens)
     merge_items = items + _align(32 * plan.num_items)
     workspace = merge_items + _align(16 * plan.num_merge_items)
     workspace_bytes = decode_workspace_bytes(plan.num_partial_rows, hq, dim)
     buffer = torch.empty(workspace + workspace_bytes, dtype=torch.uint8, device=device)
     position_ids = torch.empty(tokens, dtype=torch.int64, device=device)
     tree = TreeStep(step, parents, dims, plan, (hkv, hq, dim) if dim else None, limits, position_ids, buffer,
-                    (0, items, merge_items, workspace), workspace_bytes)
+                    (0, packed, items, merge_items, workspace), workspace_bytes)
     tree.rerun()
     tree._packs = step._packs
     return tree
@@ -2030,8 +2035,8 @@ def accept_tree(step: PackedStep, tree: TreeStep, drafted: torch.Tensor, predict
     """The path of each tree whose tokens the model itself would have chosen: from
     node 0 (the sequence's last known token) on, the first child whose ``drafted``
     token is the one ``predicted`` at its parent, until there is none.  Both int64
-    [T]: the nodes' own tokens, and the model's choice after each.  All on the
-    device: nothing is read back."""
+    [T]: the nodes' own tokens, and the model's choice after each.  The parents are those
+    of the tree's last packing, as its masks.  All on the device: nothing is read back."""
     _check_tree(step, tree)
     device = step.buffer.device
     t, b = step.num_query_tokens, step.num_seqs
@@ -2047,7 +2052,7 @@ def accept_tree(step: PackedStep, tree: TreeStep, drafted: torch.Tensor, predict
     next_tokens = torch.empty(b, dtype=torch.int64, device=device)
     with _current(device):
         status = _native.load_library().pa_accept_tree(
-            tree.parents.data_ptr(), step.ptr("cu_seqlens"), drafted.data_ptr(), predicted.data_ptr(), b, t,
+            tree._packed_parents, step.ptr("cu_seqlens"), drafted.data_ptr(), predicted.data_ptr(), b, t,
             nodes.data_ptr(), counts.data_ptr(), next_tokens.data_ptr(), _stream(device))
     _native.check(status, "pa_accept_tree")
     return AcceptedPath(nodes, counts, next_tokens)

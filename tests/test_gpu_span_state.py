@@ -101,6 +101,47 @@ def test_a_step_packed_again_for_its_heads_splits_a_window_as_a_new_one(device):
     assert ops._window_step(given, 1024, 4, 2, 8, 64, BF16).partition_size == 512
 
 
+def flat(parents, device):
+    return torch.tensor([p for t in parents for p in t], dtype=torch.int32, device=device)
+
+
+def check_tree(step, tree, parents, drafted, predicted):
+    masks, first = tree.masks.cpu().numpy().view(np.uint32), 0
+    for up in parents:
+        n = len(up)
+        bits = ((masks[first:first + n, :, None] >> np.arange(32, dtype=np.uint32)) & 1).reshape(n, -1)
+        assert np.array_equal(bits[:, :n], ancestors(up))
+        first += n
+    path = ops.accept_tree(step, tree, drafted, predicted)
+    nodes, kept, nexts = plain_accept(parents, drafted.tolist(), predicted.tolist())
+    assert path.nodes.tolist() == nodes and path.counts.tolist() == kept and path.next_tokens.tolist() == nexts
+
+
+def test_trees_of_one_tensor_of_parents(device):
+    """A tree accepts the paths of the parents that its masks are of, whatever another
+    tree of the same tensor, or its owner, has put there since."""
+    counts = [30, 1, 45]
+    rng = np.random.Generator(np.random.PCG64(3))
+    old, new, last = ([random_tree(rng, n) for n in counts] for _ in range(3))
+    case = Case([100, 7, 300], counts, 8, 2, 128, BF16, parents=old)
+    q, k, v, _, step = case.place(device)
+    drafted, predicted = (torch.from_numpy(rng.integers(0, 2, sum(counts))).to(device) for _ in range(2))
+    shared = flat(old, device)
+    one, two = ops.pack_tree(step, shared), ops.pack_tree(step, shared, window=64, sinks=3)
+    paths = [plain_accept(p, drafted.tolist(), predicted.tolist()) for p in (old, new, last)]
+    assert paths[0] != paths[1] and paths[1] != paths[2]
+    one.repack(flat(new, device))
+    check_tree(step, one, new, drafted, predicted)
+    check_tree(step, two, old, drafted, predicted)
+    two.repack()  # (reads the tensor as it is)
+    check_tree(step, two, new, drafted, predicted)
+    shared.copy_(flat(last, device))
+    check_tree(step, one, new, drafted, predicted)
+    one.rerun()
+    check_tree(step, one, last, drafted, predicted)
+    check_tree(step, two, new, drafted, predicted)
+
+
 @pytest.mark.parametrize("starts,counts", [([40, 300, 700], [1, 33, 1]), ([40, 700], [1, 1])])
 @pytest.mark.parametrize("heads,kv_heads,dim,dtype,cache_dtype", [
     (8, 2, 128, BF16, BF16), (4, 2, 64, FP32, FP32), (8, 2, 128, BF16, CODE)])
