@@ -142,6 +142,60 @@ def test_trees_of_one_tensor_of_parents(device):
     check_tree(step, two, new, drafted, predicted)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype,cache_dtype", [
+    (8, 2, 128, BF16, BF16), (9, 3, 64, FP16, FP16), (4, 2, 256, BF16, BF16), (4, 2, 64, FP32, FP32),
+    (8, 2, 128, BF16, CODE)])
+def test_a_graph_of_trees_whose_runs_change(device, heads, kv_heads, dim, dtype, cache_dtype):
+    """A captured layer of trees whose contexts shrink and grow again, so that tiles are
+    split in other runs, or in none, at other places of the lists."""
+    counts = [20, 90, 9]
+    rng = np.random.Generator(np.random.PCG64(dim))
+    places = [[3000, 2500, 2900], [40, 2400, 700], [2900, 0, 130], [70, 64, 1], [2999, 2222, 1111]]
+    cases = [Case(starts, counts, heads, kv_heads, dim, dtype, cache_dtype, poison=False, drop=False, seed=4,
+                  parents=[random_tree(rng, n) for n in counts]) for starts in places]
+    q, k, v, scales, _ = cases[0].place(device)
+    table = torch.zeros(cases[0].table.shape, dtype=torch.int32, device=device)
+
+    def fill(c):
+        table.fill_(-1)
+        table[:, :c.full_table.shape[1]] = torch.from_numpy(c.full_table).to(device)
+        for cache, x in ((k, c.keys), (v, c.vals)):
+            cache.view(torch.uint8)[1, :x.shape[0]] = x.view(torch.uint8).to(device)
+        for name, s in c.scales.items():
+            scales[name][1, :s.shape[0]] = s.to(device)
+        q.copy_(c.query)
+
+    fill(cases[0])
+    step = ops.pack_step(table, cases[0].starts, counts, 16, num_kv_heads=kv_heads, num_query_heads=heads,
+                         head_dim=dim, dtype=cache_dtype)
+    tree = ops.pack_tree(step, flat(cases[0].parents, device))
+    out = torch.zeros_like(q)
+
+    def layer():
+        step.rerun()
+        tree.rerun()
+        ops.tree_attention(q, k, v, 1, step, tree, cases[0].scaling, out=out, **scales)
+
+    layer()
+    cases[0].check(out)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        layer()
+    sizes = set()
+    for c in cases + cases[::-1]:
+        fill(c)
+        step.repack(c.starts, counts)
+        tree.repack(flat(c.parents, device))
+        plan = ops._plan_tree(step, tree._dims, tree._plan.split_stages)
+        sizes.add((plan.num_items, plan.num_merge_items))
+        out.zero_()
+        graph.replay()
+        c.check(out)
+        c.check(ops.tree_attention(q, k, v, 1, step, tree, c.scaling, **scales))
+    assert len(sizes) > 2
+
+
 @pytest.mark.parametrize("starts,counts", [([40, 300, 700], [1, 33, 1]), ([40, 700], [1, 1])])
 @pytest.mark.parametrize("heads,kv_heads,dim,dtype,cache_dtype", [
     (8, 2, 128, BF16, BF16), (4, 2, 64, FP32, FP32), (8, 2, 128, BF16, CODE)])
