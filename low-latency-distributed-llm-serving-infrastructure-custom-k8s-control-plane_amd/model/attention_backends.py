@@ -54,8 +54,12 @@ class AttentionBackend(ABC):
 
     @abstractmethod
     def attend(self, query: torch.Tensor, store: "PagedKVCacheManager", layer_idx: int,
-               context: "PagedStepContext", scaling: float, dropout: float) -> torch.Tensor:
-        ...
+               context: "PagedStepContext", scaling: float, dropout: float,
+               window: Optional[int] = None) -> torch.Tensor:
+        """``window``: given (by name) for a layer that sees less than its contexts, whose
+        query at position p sees the positions q <= p with p - q < window or q <
+        ``context.sinks``.  A backend without it serves the other layers alone: such a
+        call is a TypeError."""
 
 
 def dense_sdpa(query, store, layer_idx, context, scaling, dropout, window=None) -> torch.Tensor:

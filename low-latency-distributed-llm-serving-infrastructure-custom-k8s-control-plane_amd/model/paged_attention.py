@@ -180,6 +180,13 @@ class PagedStepContext:
             return self.window if sliding_window is None else int(sliding_window)
         return min(int(sliding_window), self.window)
 
+    def within(self, window: int) -> bool:
+        """Whether no context of the step reaches past ``window``, so that it limits nothing
+        (never in a launch that a graph captures, which may serve longer contexts)."""
+        if self.packed is None:
+            return max(self.context_lens, default=0) <= window
+        return self.packed.max_context <= window and not torch.cuda.is_current_stream_capturing()
+
     def tree_for(self, num_query_heads: int, window: Optional[int] = None) -> paged_ops.TreeStep:
         """The step's packed trees for layers of ``num_query_heads`` under ``window``."""
         step = self.packed_for(num_query_heads)
@@ -291,7 +298,8 @@ def paged_attention_forward(
 
     ``sliding_window``, which transformers hands over for layers that have one,
     limits the layer to that window (the context's ``window`` limits every layer,
-    and its ``sinks`` stay visible in both)."""
+    and its ``sinks`` stay visible in both).  A window that some context reaches past
+    goes to the backend's ``attend`` as ``window``."""
     context: PagedStepContext = module.paged_context
     store = context.store
     layer_idx = module.layer_idx
@@ -299,7 +307,7 @@ def paged_attention_forward(
     new_key, new_value = key[0].transpose(0, 1), value[0].transpose(0, 1)
     scale = module.scaling if scaling is None else scaling
     window = context.window_of(kwargs.get("sliding_window"))
-    limits = {} if window is None else {"window": window}
+    limits = {} if window is None or context.within(window) else {"window": window}
     backend = _BACKEND if _BACKEND is not None else _default_backend(store)
     if store.on_gpu:
         from .attention_backends import NativePagedBackend
