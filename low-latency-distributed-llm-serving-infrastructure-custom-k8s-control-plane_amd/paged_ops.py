@@ -1676,8 +1676,8 @@ def _window_of(window, sinks) -> Tuple[int, int]:
 
 def _window_starts(starts: np.ndarray, counts: np.ndarray, block_size: int, window: int, sinks: int) -> np.ndarray:
     """Starts that give each single-token sequence the longest shorter context it
-    can have under the window (pa_window_context)."""
-    most = -(-sinks // block_size) * block_size + window + block_size - 1
+    can have under the window."""
+    most = _native.load_library().pa_window_context(_INT32_MAX, _native.PaWindow(window, sinks), block_size)
     return np.where(counts == 1, np.minimum(starts, most - 1), starts)
 
 
