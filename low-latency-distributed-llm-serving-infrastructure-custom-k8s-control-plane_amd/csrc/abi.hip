@@ -612,7 +612,7 @@ int decode_phases(const char* who, bool use_scratch, int32_t phases, const void*
     a.scale_log2e = scaling * pa::kLog2e;
     a.group = group;
     a.sub_groups = pa::decode_workgroups_per_head(dims.dtype, dims.head_dim, group);
-    // A record's fields hold counts and items below 65535.
+    // (a record's fields: 16 bits of a sequence's partitions, 24 of 1 + an item)
     a.merge_state = records_fit ? merge_state : nullptr;
     a.window = window.window;
     a.sinks = window.sinks;

@@ -100,8 +100,9 @@ __device__ __forceinline__ void merge_partials(const float* ml, const float* acc
 // arrivals, bits 16-39 hold 1 + the item of the partial last partition
 // (added by that workgroup) and bits 40-63 1 + the item of partition 0,
 // the first of the sequence's full partitions, which pa_pack lists as
-// consecutive items (added by that workgroup; the host passes records
-// only for fewer than 65535 items, so every field fits).  The workgroup
+// consecutive items (added by that workgroup; the host passes records only
+// where every field fits: fewer than 65535 items, or, under a window, fewer than
+// 2^24 - 1 and of no sequence more than 65535).  The workgroup
 // whose addition brings the count to nparts has every field in the value
 // the atomic returns; it resets the record for the next launch (the
 // records start at zero and every launch leaves them at zero) and merges

@@ -52,8 +52,8 @@ struct DecodeArgs {
   // Merge records of the in-launch split-K merge, 8 bytes per (sequence,
   // unit, sub-group): arrivals, first full-partition item, partial item.
   // Zero before the launch and left zero by it; null (always for 65535 or
-  // more items): the partition phase stores partials only and the merge
-  // kernel combines them.
+  // more items without a window): the partition phase stores partials only and
+  // the merge kernel combines them.
   int32_t* merge_state;
   int32_t num_seqs;  // sequences the records cover
   // The matrix-core launch's: (2^32 - 1) / d of the two divisors that map its

@@ -294,7 +294,9 @@ struct Trees {
 };
 
 // Stages per item, by the modelled time of the candidates.  Measured on 32/8 heads
-// of 128 with 47 to 2026 stages of 64 tokens a KV head (a unit is an item's KV head):
+// of 128 with 47 to 2026 stages of 64 tokens a KV head (a unit is an item's KV head), one
+// term a probability (with two a stage takes up to a seventh longer, which moves no pick
+// far: see below):
 //  * a unit costs 8.4 us beside its stages, a stage 1.5 us of its workgroup, and the
 //    caches' rows, read once for all tiles of a sequence, come at 5.5 TB/s (3.06 us a
 //    stage of every resident workgroup);
@@ -302,9 +304,9 @@ struct Trees {
 //  * units that do not all fit the chip at once share its workgroups, and the last
 //    ones leave part of it idle;
 //  * tiles in several runs are joined by a launch of its own.
-// Of 12 to 15 splits of 13 steps each (32/8 and 32/32 heads of 128; 16-bit heads of 64,
+// Of 12 to 16 splits of 13 steps each (32/8 and 32/32 heads of 128; 16-bit heads of 64,
 // 80 and 256; 8-bit and fp32 caches) the pick was the fastest or within 3 % of it in
-// eight, within 8 % in the others; one run a tile took up to 11 times as long, one stage
+// nine, within 7 % in the others; one run a tile took up to 9 times as long, one stage
 // a run up to five times.
 struct TreeCost {
   double unit, stage, bytes;  // us

@@ -56,7 +56,8 @@ constexpr int kIdAhead = 8;
 constexpr int kLdsBytes = kIdBase + kIdSlots * kIdSlotBytes;
 
 // WINDOW: a window with sinks, as in prefill_kernel.hpp (4 prompts of 2048 tokens at 0
-// to 12288, 16/4 heads, window 2048, 4 sinks: 397 us, 607 TFLOP/s).
+// to 12288, 16/4 heads, window 2048, 4 sinks: 397 us, 607 TFLOP/s; one term a probability,
+// as without a window: prefill_window.hip).
 template <typename T, bool LANE_IDS, bool WINDOW>
 __global__ __launch_bounds__(kThreads) void prefill256_kernel(PrefillArgs a) {
   static_assert(Elem<T>::kBytes == 2, "16-bit caches (bf16 or fp16)");

@@ -74,9 +74,8 @@ PA_HOST_DEVICE StageSpan tree_span(int start, int nodes, int window, int sinks, 
   return stage_span(window_start(start, window), start + nodes, sinks, stage);
 }
 
-// Whether the matrix-core kernels of trees (tree_attention.hip; over 8-bit and fp32
-// caches prefill.hip and prefill_f32.hip) serve the shape: (dtype: the cache's; 8-bit codes
-// under 16-bit queries); its tiles walk stages of kTreeStage positions.
+// Positions of a stage, in which the tiles of every matrix-core kernel of trees walk
+// their context.
 constexpr int kTreeStage = 64;
 // Query rows of a tile over 16-bit caches, heads of up to 128; nodes of a tile of
 // any shape (dtype: the cache's).
@@ -103,6 +102,9 @@ PA_HOST_DEVICE int tree_max_stages(int block_size) {
   const long long n = static_cast<long long>(kTreeIds - 8) * block_size / kTreeStage;
   return n < (1 << 24) ? static_cast<int>(n) : 1 << 24;
 }
+// Whether a matrix-core kernel of trees serves the shape (dtype: the cache's, 8-bit codes
+// under 16-bit queries): tree_attention.hip, for heads of 256 tree_attention256.hip, over
+// 8-bit caches prefill_tree.hip, over fp32 ones prefill_f32.hip.
 bool tree_fast_path_supported(int dtype, int head_dim, int group, int block_size);
 
 }  // namespace pa

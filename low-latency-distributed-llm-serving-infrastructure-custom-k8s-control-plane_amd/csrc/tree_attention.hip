@@ -17,15 +17,15 @@
 // depend on each other.
 //
 // What bounds it is the cache's bytes, read once for a tile's rows (32 trees of 9-17
-// nodes after 100-8000 tokens, 32/8 heads of 128: 108 us and 7.5 for the join, 5.0 TB/s;
-// 8 of 64 nodes after 1000-4000, 32/32 heads: 70 us, 4.9 TB/s); for trees whose tiles
+// nodes after 100-8000 tokens, 32/8 heads of 128: 114 us and 7.5 for the join, 4.7 TB/s;
+// 8 of 64 nodes after 1000-4000, 32/32 heads: 77 us, 4.5 TB/s); for trees whose tiles
 // share a short context the one wave a SIMD, whose products and softmax follow each
-// other (2 of 40-60 nodes under a window of 8192: 34 and 5 us, 330 TFLOP/s); for
-// short runs the chain of round trips at a unit's start (record; block ids, query and
-// masks; K and V: one of 26 nodes after 3000, 14 and 4 us).  The causal prefill's tiles,
-// shared by eight waves, took 145, 95, and 28 us where this now takes 118, 73 and 18.
-// V's operands read behind the softmax, and the accumulators copied out of the matrix
-// registers at each tile: 133, 91 and 21 us.
+// other (2 of 40-60 nodes under a window of 8192: 38 and 4.5 us); for short runs the
+// chain of round trips at a unit's start (record; block ids, query and masks; K and V:
+// one of 26 nodes after 3000, 15 and 4 us).  With one term a probability (below) the
+// causal prefill's tiles, shared by eight waves, took 145, 95, and 28 us where this took
+// 118, 73 and 18; V's operands read behind the softmax, and the accumulators copied out
+// of the matrix registers at each tile: 133, 91 and 21 us.
 //
 // A probability goes into the product as two terms of the type (split_weights()), as the
 // decode's does: a node that verifies a token answers as the decode of that token would,

@@ -96,7 +96,8 @@ struct TreeRun {
 
 // Around the only vector instructions on accumulators, a rescale's: without it the
 // compiler copies all of them out of the matrix registers at each tile, for the case of
-// a rescale (32 trees of 9-17 nodes, 32/8 heads of 128: 132 us, with it 122).
+// a rescale (32 trees of 9-17 nodes, 32/8 heads of 128, one term a probability: 132 us,
+// with it 122).
 __device__ __forceinline__ void in_matrix_registers(f32x16& x) { asm("" : "+a"(x)); }
 
 // s_waitcnt's immediate for vmcnt(0) alone.

@@ -1713,7 +1713,12 @@ def _window_step(step: PackedStep, window: int, sinks: int, num_kv_heads: int, n
             # of 32-32768, window 4096: 2080 298 us, 4096 319).  But for a launch that gives
             # every CU one whole partition, beside short rests: there the even ones would be
             # more than the CUs (16 sequences, window 4096: 832 60.7 us, 1024 51.5; window
-            # 1024: 224 19.5, 256 17.5).
+            # 1024: 224 19.5, 256 17.5).  With rests that make it more than two a CU the
+            # whole ones do not run alone, and even ones share the chip better: over 16-bit
+            # caches 3-12 % (256 of 16-16000 tokens, window 4096, 32/8 heads: 4096 257 us,
+            # 2080 248; 16/4 of 80: 108 and 96); over fp32 ones 17-24 % where whole ones
+            # leave CUs without (80 of 16-16000: 190 and 158), and up to 11 % less where
+            # they do not (window 1500: 82.7 and 92.5).
             even = (-(-longest // -(-longest // partition)) + 31) // 32 * 32
             cus = _compute_units(device)
             whole, raw, evened = (per_item * int(n.sum()) for n in (
