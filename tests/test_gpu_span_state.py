@@ -225,3 +225,59 @@ def test_a_windowed_step_refuses_a_write_inside_the_prefill(device):
     with pytest.raises(ValueError, match="fused_prefill_write"):
         ops.attention(q, k, v, 1, step, 1.0, new_key=rows, new_value=rows, fused_prefill_write=True, window=50)
     ops.attention(q, k, v, 1, step, 1.0, new_key=rows, new_value=rows, fused_prefill_write=False, window=50)
+
+
+def test_trees_of_other_sizes_after_a_repack(device):
+    """The same number of nodes, dealt otherwise to the sequences."""
+    starts, counts, others = [700, 90, 0], [40, 16, 8], [8, 16, 40]
+    rng = np.random.Generator(np.random.PCG64(9))
+    parents, drawn = ([random_tree(rng, n) for n in c] for c in (counts, others))
+    ends = [s + max(a, b) for s, a, b in zip(starts, counts, others)]
+    table, at = np.full((3, -(-max(ends) // 16)), -1, np.int32), 0
+    cases = [Case(starts, c, 8, 2, 128, BF16, parents=p, seed=9, poison=False, drop=False)
+             for c, p in ((counts, parents), (others, drawn))]
+    blocks = sum(-(-e // 16) for e in ends)
+    k, v = (torch.zeros((2, blocks, 16, 2, 128), dtype=BF16, device=device) for _ in range(2))
+    for i, e in enumerate(ends):
+        n = -(-e // 16)
+        table[i, :n] = np.arange(at, at + n)
+        at += n
+    q = torch.zeros((64, 8, 128), dtype=BF16, device=device)
+
+    def fill(c):
+        for i, (s, n) in enumerate(zip(c.starts, c.counts)):
+            pos = np.arange(s + n)
+            mine, here = (torch.from_numpy(t[i, pos // 16].astype(np.int64) * 16 + pos % 16)
+                          for t in (c.full_table, table))
+            for cache, x in ((k, c.keys), (v, c.vals)):
+                cache[1].view(-1, 2, 128)[here.to(device)] = x.view(-1, 2, 128)[mine].to(device)
+        q.copy_(c.query)
+
+    fill(cases[0])
+    step = ops.pack_step(torch.from_numpy(table).to(device), starts, counts, 16, num_kv_heads=2, num_query_heads=8,
+                         head_dim=128, dtype=BF16)
+    tree = ops.pack_tree(step, flat(parents, device))
+    for c in cases + cases[:1]:
+        fill(c)
+        step.repack(starts, c.counts)
+        tree.repack(flat(c.parents, device))
+        c.check(ops.tree_attention(q, k, v, 1, step, tree, c.scaling))
+
+
+def test_refusals_of_trees_and_windows_that_outgrow_their_lists(device, monkeypatch):
+    case = Case([3000], [26], 8, 2, 128, BF16, parents=[list(range(-1, 25))], drop=False)
+    q, k, v, _, _ = case.place(device)
+    step = ops.pack_step(torch.from_numpy(case.table).to(device), [40], [26], 16, num_kv_heads=2, num_query_heads=8,
+                         head_dim=128, dtype=BF16)
+    tree = ops.pack_tree(step, flat(case.parents, device))
+    step.repack([3000], [26])
+    with pytest.raises(ValueError, match="longer work lists"):
+        tree.repack()
+    with pytest.raises(RuntimeError, match="repack its tree"):
+        ops.tree_attention(q, k, v, 1, step, tree, case.scaling)
+    case.check(ops.tree_attention(q, k, v, 1, step, ops.pack_tree(step, tree.parents), case.scaling))
+    decode = ops.pack_step(torch.from_numpy(case.table).to(device), [3000], [1], 16, num_kv_heads=2,
+                           num_query_heads=8, head_dim=128, dtype=BF16)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="a graph cannot capture"):
+        ops.attention(q[:1], k, v, 1, decode, 1.0, window=64)
